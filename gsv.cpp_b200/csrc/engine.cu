@@ -10,6 +10,7 @@
 #include "../../include/gsvcu.h"
 #include "gguf_reader.h"
 #include "kernels.h"
+#include "paged.h"
 
 using namespace gsvcu;
 
@@ -426,9 +427,14 @@ struct gsvcu_ctx {
     size_t op_part_n = 0;
     void* op_a16 = nullptr;   // scratch of gsvcu_op_q8_gemm_tc (bytes)
     size_t op_a16_n = 0;
+    float* op_split = nullptr;        // split results of gsvcu_op_chunk_attention
+    size_t op_split_n = 0;
+    int32_t* op_arrived = nullptr;    // its arrival counters, zero between launches
+    size_t op_arrived_n = 0;
     // set when a bounded wait in a kernel gave up: [0] decode attention in the decode steps (read and
     // cleared with the slot state), [1] gsvcu_op_decode_attention (read and cleared by gsvcu_sync),
-    // [2] the tcgen05 prefill GEMM (read and cleared at the end of each prefill pass)
+    // [2] the tcgen05 prefill GEMM (read and cleared at the end of each prefill pass),
+    // [3] the paged-cache operators' status bits (read and cleared by gsvcu_sync)
     int32_t* att_err = nullptr;
     // test-only fault injection (gsvcu_set_wait_fault): extra bytes each K/V page wait expects, poll limit
     uint32_t fault_extra_tx = 0, fault_poll_limit = 0;
@@ -498,6 +504,8 @@ gsvcu_ctx::~gsvcu_ctx() {
     for (void* p : wallocs) cudaFree(p);
     if (op_part) cudaFree(op_part);
     if (op_a16) cudaFree(op_a16);
+    if (op_split) cudaFree(op_split);
+    if (op_arrived) cudaFree(op_arrived);
     if (att_err) cudaFree(att_err);
     for (cudaStream_t gs : gstream)
         if (gs) cudaStreamDestroy(gs);
@@ -1363,7 +1371,8 @@ int gsvcu_create(int device, gsvcu_ctx** out) {
     bool dense_usable = false;
     if (gemm_q8_init_device() != cudaSuccess || gemm_tc_init_device() != cudaSuccess ||
         gemm_fx_init_device() != cudaSuccess || attention_init_device() != cudaSuccess ||
-        logits_init_device() != cudaSuccess || dense_init_device(&dense_usable) != cudaSuccess) {
+        logits_init_device() != cudaSuccess || chunk_attention_init_device() != cudaSuccess ||
+        dense_init_device(&dense_usable) != cudaSuccess) {
         cudaGetLastError();
         return GSVCU_ERR_CUDA;
     }
@@ -1371,8 +1380,8 @@ int gsvcu_create(int device, gsvcu_ctx** out) {
     c->device = device;
     c->dense_ok = dense_usable;
     if (cudaStreamCreateWithFlags(&c->stream, cudaStreamNonBlocking) != cudaSuccess ||
-        cudaMalloc((void**)&c->att_err, 3 * sizeof(int32_t)) != cudaSuccess ||
-        cudaMemset(c->att_err, 0, 3 * sizeof(int32_t)) != cudaSuccess ||
+        cudaMalloc((void**)&c->att_err, 4 * sizeof(int32_t)) != cudaSuccess ||
+        cudaMemset(c->att_err, 0, 4 * sizeof(int32_t)) != cudaSuccess ||
         cudaStreamCreateWithFlags(&c->gstream[0], cudaStreamNonBlocking) != cudaSuccess ||
         cudaStreamCreateWithFlags(&c->gstream[1], cudaStreamNonBlocking) != cudaSuccess ||
         cudaEventCreateWithFlags(&c->gevent[0], cudaEventDisableTiming) != cudaSuccess ||
@@ -1824,6 +1833,126 @@ int gsvcu_op_prefill_attention(gsvcu_ctx* ctx, const float* qkv_dev, int32_t n_s
     return GSVCU_OK;
 }
 
+// The cache and batch descriptions of the paged-cache operators, checked on the host.
+static int paged_views(gsvcu_ctx* ctx, const gsvcu_paged_kv* kv, const gsvcu_chunk_batch* b, int32_t layer,
+                       int32_t n_q_head, PagedView& pv, ChunkView& cv) {
+    if (!kv || !b) return ctx->fail(GSVCU_ERR_ARG, "paged cache: null cache or batch");
+    if (kv->kv_dtype != GSVCU_KV_F16 && kv->kv_dtype != GSVCU_KV_F32 && kv->kv_dtype != GSVCU_KV_BF16)
+        return ctx->fail(GSVCU_ERR_ARG, "paged cache: kv_dtype must be F16, F32 or BF16");
+    if (!kv->pool_dev || ((uintptr_t)kv->pool_dev & 15))
+        return ctx->fail(GSVCU_ERR_ARG, "paged cache: pool_dev must be 16-byte aligned device memory");
+    if (kv->n_page <= 0 || kv->n_layer <= 0 || kv->n_kv_head <= 0)
+        return ctx->fail(GSVCU_ERR_ARG, "paged cache: n_page, n_layer and n_kv_head must be positive");
+    if (kv->head_dim != 32 && kv->head_dim != 64 && kv->head_dim != 128)
+        return ctx->fail(GSVCU_ERR_ARG, "paged cache: head_dim must be 32, 64 or 128");
+    if (layer < 0 || layer >= kv->n_layer) return ctx->fail(GSVCU_ERR_ARG, "paged cache: layer out of range");
+    if (n_q_head < 0 || n_q_head % kv->n_kv_head)
+        return ctx->fail(GSVCU_ERR_ARG, "paged cache: n_q_head must be a multiple of n_kv_head");
+    if (!b->row_start_dev || !b->kv_len_dev || !b->block_table_dev)
+        return ctx->fail(GSVCU_ERR_ARG, "chunk batch: null row_start, kv_len or block_table");
+    if (b->n_seq < 0 || b->max_pages <= 0 || b->max_pages > INT32_MAX / PAGE || b->n_rows < 0 || b->max_chunk < 0 ||
+        b->max_chunk > b->n_rows || (b->n_rows > 0 && b->max_chunk == 0) || b->max_kv < 0)
+        return ctx->fail(GSVCU_ERR_ARG, "chunk batch: sizes out of range");
+    pv.pool = kv->pool_dev; pv.kv_dtype = kv->kv_dtype; pv.n_page = kv->n_page; pv.n_layer = kv->n_layer;
+    pv.layer = layer; pv.n_head = kv->n_kv_head; pv.head_dim = kv->head_dim;
+    cv.row_start = b->row_start_dev; cv.kv_len = b->kv_len_dev; cv.table = b->block_table_dev;
+    cv.n_seq = b->n_seq; cv.max_pages = b->max_pages; cv.n_rows = b->n_rows; cv.max_chunk = b->max_chunk;
+    cv.max_kv = b->max_kv > 0 ? std::min(b->max_kv, b->max_pages * PAGE) : b->max_pages * PAGE;
+    return GSVCU_OK;
+}
+
+static bool aligned_to(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
+
+int gsvcu_op_kv_append(gsvcu_ctx* ctx, const gsvcu_paged_kv* kv, const gsvcu_chunk_batch* batch, int32_t layer,
+                       int32_t row_dtype, int32_t n_q_head, const void* q_dev, int64_t q_stride, const void* k_dev,
+                       int64_t k_stride, const void* v_dev, int64_t v_stride, const float* cos_dev,
+                       const float* sin_dev, int32_t n_pos, int32_t rot_dim, int32_t rot_pairs, const int32_t* pos_dev,
+                       void* q_out_dev, int64_t q_out_stride) {
+    if (!ctx) return GSVCU_ERR_ARG;
+    KvAppendParams p;
+    TRY(paged_views(ctx, kv, batch, layer, n_q_head, p.kv, p.batch));
+    if (row_dtype != GSVCU_KV_F32 && row_dtype != kv->kv_dtype)
+        return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_kv_append: rows must be F32 or the cache's type");
+    if (batch->n_rows > 0 && (!k_dev || !v_dev || (n_q_head > 0 && (!q_dev || !q_out_dev))))
+        return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_kv_append: null rows");
+    const int64_t D = kv->head_dim;
+    if (k_stride < kv->n_kv_head * D || v_stride < kv->n_kv_head * D ||
+        (n_q_head > 0 && (q_stride < n_q_head * D || q_out_stride < n_q_head * D)))
+        return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_kv_append: row stride shorter than its heads");
+    const size_t rs = row_dtype == GSVCU_KV_F32 ? 4 : 2, ks = kv->kv_dtype == GSVCU_KV_F32 ? 4 : 2;
+    if (!aligned_to(q_dev, rs) || !aligned_to(k_dev, rs) || !aligned_to(v_dev, rs) || !aligned_to(q_out_dev, ks))
+        return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_kv_append: rows not aligned to their element");
+    if (rot_dim < 0 || rot_dim > D || rot_dim % 2 || (rot_dim > 0 && (!cos_dev || !sin_dev || n_pos <= 0)) ||
+        rot_pairs < 0 || rot_pairs > 1)
+        return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_kv_append: rot_dim must be even, at most head_dim, with its cos / sin table");
+    p.row_dtype = row_dtype; p.n_q_head = n_q_head; p.q = q_dev; p.q_stride = q_stride; p.k = k_dev;
+    p.k_stride = k_stride; p.v = v_dev; p.v_stride = v_stride; p.cos = cos_dev; p.sin = sin_dev; p.n_pos = n_pos;
+    p.rot = rot_dim; p.pairs = rot_pairs; p.pos = pos_dev; p.q_out = q_out_dev; p.q_out_stride = q_out_stride;
+    p.err = ctx->att_err + 3;
+    if (batch->n_rows == 0 || batch->n_seq == 0) return GSVCU_OK;
+    DeviceGuard g(ctx->device);
+    launch_kv_append(p, ctx->stream);
+    CKC(ctx, cudaGetLastError());
+    ctx->launches++;
+    return GSVCU_OK;
+}
+
+int gsvcu_op_chunk_attention(gsvcu_ctx* ctx, const gsvcu_paged_kv* kv, const gsvcu_chunk_batch* batch, int32_t layer,
+                             int32_t n_q_head, const void* q_dev, int64_t q_stride, float scale, int32_t window,
+                             const int32_t* prefix_dev, void* out_dev, int64_t out_stride, float* lse_dev) {
+    if (!ctx) return GSVCU_ERR_ARG;
+    ChunkAttnParams p;
+    TRY(paged_views(ctx, kv, batch, layer, n_q_head, p.kv, p.batch));
+    if (n_q_head <= 0 || (batch->n_rows > 0 && (!q_dev || !out_dev)))
+        return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_chunk_attention: null rows");
+    const int64_t D = kv->head_dim;
+    if (q_stride < n_q_head * D || out_stride < n_q_head * D)
+        return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_chunk_attention: row stride shorter than its heads");
+    const size_t ks = kv->kv_dtype == GSVCU_KV_F32 ? 4 : 2;
+    if (!aligned_to(q_dev, ks) || !aligned_to(out_dev, ks) || !aligned_to(lse_dev, 4))
+        return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_chunk_attention: rows not aligned to their element");
+    if (window < 0 || !std::isfinite(scale))
+        return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_chunk_attention: window must be >= 0 and scale finite");
+    p.n_q_head = n_q_head; p.q = q_dev; p.q_stride = q_stride; p.scale = scale; p.window = window;
+    p.prefix = prefix_dev; p.out = out_dev; p.out_stride = out_stride; p.lse = lse_dev; p.err = ctx->att_err + 3;
+    if (batch->n_rows == 0 || batch->n_seq == 0) return GSVCU_OK;
+    const ChunkAttnPlan plan = chunk_attention_plan(p);
+    if ((int64_t)batch->n_seq * plan.tiles * kv->n_kv_head * plan.n_split > INT32_MAX)
+        return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_chunk_attention: batch too large for one launch");
+    DeviceGuard g(ctx->device);
+    if (plan.part_floats > ctx->op_split_n) {
+        CKC(ctx, cudaStreamSynchronize(ctx->stream));
+        if (ctx->op_split) cudaFree(ctx->op_split);
+        ctx->op_split = nullptr;
+        ctx->op_split_n = 0;
+        if (cudaMalloc((void**)&ctx->op_split, plan.part_floats * 4) != cudaSuccess) {
+            cudaGetLastError();
+            ctx->op_split = nullptr;
+            return ctx->fail(GSVCU_ERR_OOM, "gsvcu_op_chunk_attention: no memory for the split results");
+        }
+        ctx->op_split_n = plan.part_floats;
+    }
+    if (plan.arrivals > ctx->op_arrived_n) {
+        CKC(ctx, cudaStreamSynchronize(ctx->stream));
+        if (ctx->op_arrived) cudaFree(ctx->op_arrived);
+        ctx->op_arrived = nullptr;
+        ctx->op_arrived_n = 0;
+        if (cudaMalloc((void**)&ctx->op_arrived, plan.arrivals * sizeof(int32_t)) != cudaSuccess) {
+            cudaGetLastError();
+            ctx->op_arrived = nullptr;
+            return ctx->fail(GSVCU_ERR_OOM, "gsvcu_op_chunk_attention: no memory for the arrival counters");
+        }
+        ctx->op_arrived_n = plan.arrivals;
+        CKC(ctx, cudaMemsetAsync(ctx->op_arrived, 0, plan.arrivals * sizeof(int32_t), ctx->stream));
+    }
+    p.part = ctx->op_split;
+    p.arrived = ctx->op_arrived;
+    launch_chunk_attention(p, plan, ctx->stream);
+    CKC(ctx, cudaGetLastError());
+    ctx->launches++;
+    return GSVCU_OK;
+}
+
 int gsvcu_op_sample(gsvcu_ctx* ctx, const float* logits_dev, int32_t B, int32_t V, int32_t eos,
                     const gsvcu_sampler_cfg* cfg, const int32_t* prev_host, const int32_t* n_prev_host,
                     int32_t prev_stride, const int32_t* step_host, uint64_t* rng_host, int32_t* tokens_host) {
@@ -1967,14 +2096,27 @@ int gsvcu_fused_decode(const gsvcu_ctx* ctx) {
 int gsvcu_sync(gsvcu_ctx* ctx) {
     if (!ctx) return GSVCU_ERR_ARG;
     DeviceGuard g(ctx->device);
-    int32_t oerr = 0;
-    CKC(ctx, cudaMemcpyAsync(&oerr, ctx->att_err + 1, sizeof(oerr), cudaMemcpyDeviceToHost, ctx->stream));
+    int32_t word[3] = {0, 0, 0};   // status words [1] to [3]
+    CKC(ctx, cudaMemcpyAsync(word, ctx->att_err + 1, sizeof(word), cudaMemcpyDeviceToHost, ctx->stream));
     CKC(ctx, cudaStreamSynchronize(ctx->stream));
+    const int32_t oerr = word[0], perr = word[2];
+    if (perr) {
+        CKC(ctx, cudaMemsetAsync(ctx->att_err + 3, 0, sizeof(int32_t), ctx->stream));
+        CKC(ctx, cudaStreamSynchronize(ctx->stream));
+    }
     if (oerr) {
         CKC(ctx, cudaMemsetAsync(ctx->att_err + 1, 0, sizeof(int32_t), ctx->stream));
         CKC(ctx, cudaStreamSynchronize(ctx->stream));
         return ctx->fail(GSVCU_ERR_CUDA, "gsvcu_op_decode_attention: staged K/V never arrived (bounded wait gave up)");
     }
+    if (perr & PAGED_WAIT)
+        return ctx->fail(GSVCU_ERR_CUDA, "gsvcu_op_chunk_attention: a bounded wait gave up");
+    if (perr & PAGED_BAD_PAGE)
+        return ctx->fail(GSVCU_ERR_ARG, "paged cache: the block table names a page outside the pool");
+    if (perr & PAGED_BAD_LENGTH)
+        return ctx->fail(GSVCU_ERR_ARG, "chunk batch: row_start or kv_len outside the sizes given to the call");
+    if (perr & PAGED_BAD_POSITION)
+        return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_kv_append: a row's position is outside the cos / sin table");
     return GSVCU_OK;
 }
 

@@ -1,0 +1,625 @@
+// paged_attention.cu -- attention of a chunk of new tokens over the paged KV cache, split over the keys.
+//
+// A query row at position p (its chunk's rows are the last of the sequence's kv_len keys) sees key j when
+//   j < prefix,  or  j <= p and (no window or j > p - window).
+// out = sum_j w_j v_j / sum_j w_j with w_j = exp(scale q.k_j - m), lse = m + log(sum_j w_j); a row that sees
+// nothing gives 0 and -infinity. The g query heads that share a kv head are rows of one tile (packed row
+// r = token * g + head in the group), so K and V are read once for all of them.
+//
+// k_chunk_attn: one CTA per (sequence, row tile, kv head, key split). Its four warps take the split's key
+// tiles in turn, each with its own cp.async ring, running maximum, sum and output (in registers), so no
+// barrier stands inside the loop; they are joined at the end in warp order. With several splits the CTA that
+// arrives last joins the splits' results in split order (a fixed order: results do not depend on timing).
+// F16 / BF16 products run on mma.m16n8k16 with the weights split into two 16-bit parts (w = hi + lo), so
+// rounding them costs nothing against the output's own rounding; F32 ones on mma.m16n8k8.tf32 with both
+// operands in two parts (three products), which leaves an error near 2^-22. Sums, maxima and outputs are f32.
+// Keys past kv_len are never read (zero-filled), keys that a row must not see get weight 0.
+#include <cuda_bf16.h>
+
+#include "kernels.h"
+#include "paged.h"
+
+namespace gsvcu {
+namespace {
+
+constexpr float NEG_INF = -__builtin_huge_valf();
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr int NW = 4;   // warps per CTA
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool in) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t a, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(a)
+                 : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t a, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(a)
+                 : "memory");
+}
+__device__ __forceinline__ float lds(uint32_t a) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+    return v;
+}
+
+// d += a b, the type's tensor-core product.
+__device__ __forceinline__ void mma16(__half, float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma16(__nv_bfloat16, float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma8(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Two 16-bit values of the type, x in the low half, and what their rounding left over.
+__device__ __forceinline__ uint32_t pack_split(__half, float x, float y, uint32_t& rest) {
+    const __half2 h = __floats2half2_rn(x, y);
+    const __half2 r = __floats2half2_rn(x - __low2float(h), y - __high2float(h));
+    rest = *(const uint32_t*)&r;
+    return *(const uint32_t*)&h;
+}
+__device__ __forceinline__ uint32_t pack_split(__nv_bfloat16, float x, float y, uint32_t& rest) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    const __nv_bfloat162 r = __floats2bfloat162_rn(x - __low2float(h), y - __high2float(h));
+    rest = *(const uint32_t*)&r;
+    return *(const uint32_t*)&h;
+}
+// x = hi + lo to about 22 bits: both carry the 10 fraction bits that the tensor core reads. The low part of
+// an infinite or NaN value is set to 0, so it stays what it is.
+__device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
+    const float rest = x - __uint_as_float(hi);
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(rest));
+    if (!(fabsf(rest) < __builtin_huge_valf())) lo = 0;
+}
+
+// Key tile of one warp's ring stage: KT keys of K, then of V, rows of RB bytes in 16-byte pieces; piece c of
+// row r lies at c ^ swz(r), so the 8 rows of a matrix fragment fall into different banks.
+template <typename T, int D, int MT>
+struct Cfg {
+    static constexpr int RB = D * (int)sizeof(T);
+    static constexpr int PIECES = RB / 16;
+    static constexpr int KT = sizeof(T) == 4 ? (D == 32 ? 32 : 16) : 2048 / D;
+    static constexpr int STAGES = RB > 256 ? 2 : 3;
+    static constexpr int ROWS = 16 * MT;
+    static constexpr int TILE = KT * RB;   // bytes of K (or V)
+    static constexpr int QPLANES = sizeof(T) == 4 ? 2 : 1;   // F32: high and low parts
+    static constexpr size_t RING = (size_t)NW * STAGES * 2 * TILE;
+    static constexpr size_t JOIN = (size_t)NW * ROWS * D * 4;   // reuses the ring
+    static constexpr size_t OFF_Q = RING > JOIN ? RING : JOIN;
+    static constexpr size_t OFF_ML = OFF_Q + (size_t)QPLANES * ROWS * RB;
+    static constexpr size_t SMEM = OFF_ML + (size_t)NW * ROWS * 8 + 16;
+};
+template <int RB>
+__device__ __forceinline__ uint32_t at(int row, int piece) {
+    const int swz = RB == 64 ? (row >> 1) & 3 : row & 7;
+    return (uint32_t)(row * RB + ((piece ^ swz) << 4));
+}
+
+template <typename T> __device__ __forceinline__ T narrow(float x);
+template <> __device__ __forceinline__ float narrow<float>(float x) { return x; }
+template <> __device__ __forceinline__ __half narrow<__half>(float x) { return __float2half_rn(x); }
+template <> __device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+struct SplitArgs {
+    ChunkAttnParams p;
+    int group, tiles, n_split, split_tiles;
+    float c;          // scale * log2(e)
+    bool vec_q, vec_out;
+};
+
+// Four consecutive outputs of one packed row.
+template <typename T>
+__device__ __forceinline__ void store_out(const SplitArgs& a, int64_t row, int head, int d, const float (&o)[4], int D) {
+    T* dst = (T*)a.p.out + row * a.p.out_stride + (int64_t)head * D + d;
+    if (a.vec_out) {
+        T v[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = narrow<T>(o[i]);
+        if constexpr (sizeof(T) == 4) *(float4*)dst = make_float4(v[0], v[1], v[2], v[3]);
+        else *(uint2*)dst = *(const uint2*)v;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) dst[i] = narrow<T>(o[i]);
+    }
+}
+
+template <typename T, int D, int MT>
+__global__ void __launch_bounds__(NW * 32) k_chunk_attn(SplitArgs a) {
+    using C = Cfg<T, D, MT>;
+    constexpr int KT = C::KT, RB = C::RB, ROWS = C::ROWS, ST = C::STAGES;
+    constexpr bool F32 = sizeof(T) == 4;
+    extern __shared__ __align__(128) uint8_t sm[];
+    const ChunkAttnParams& p = a.p;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    int id = blockIdx.x;
+    const int sp = id % a.n_split;
+    id /= a.n_split;
+    const int h = id % p.kv.n_head;
+    id /= p.kv.n_head;
+    const int tile = id % a.tiles, s = id / a.tiles;
+    griddep_wait();
+    griddep_launch();
+
+    // the sequence: rows [row0, row0 + n), keys [0, len); what is out of bounds is cut off and reported
+    int row0 = p.batch.row_start[s], n = p.batch.row_start[s + 1] - row0, len = p.batch.kv_len[s];
+    const int cap = min(p.batch.max_kv, p.batch.max_pages * PAGE);
+    if (tid == 0 && sp == 0 && h == 0 && tile == 0 &&
+        (row0 < 0 || n < 0 || row0 + n > p.batch.n_rows || len < 0 || len > cap || n > p.batch.max_chunk))
+        atomicOr(p.err, PAGED_BAD_LENGTH);
+    const int total = len;   // positions count from the true length
+    len = max(0, min(len, cap));
+    if (row0 < 0 || row0 > p.batch.n_rows) return;
+    n = min(n, p.batch.n_rows - row0);
+    const int r0 = tile * ROWS, rows = min(ROWS, n * a.group - r0);   // packed rows of this tile
+    if (rows <= 0) return;
+
+    // keys that some row of the tile sees: [0, np) and [lo, hi)
+    const int p0 = total - n + r0 / a.group, p1 = total - n + (r0 + rows - 1) / a.group;
+    const int np = p.prefix ? max(0, min(p.prefix[s], len)) : 0;
+    int hi = max(0, min(len, p1 + 1)), lo = p.window ? max(0, p0 - p.window + 1) : 0;
+    if (hi <= lo) lo = hi = 0;
+    int t_lo, t_hi, n1;
+    if (np >= lo) {
+        t_lo = n1 = 0;
+        t_hi = (max(np, hi) + KT - 1) / KT;
+    } else {
+        t_lo = lo / KT;
+        t_hi = (hi + KT - 1) / KT;
+        n1 = min((np + KT - 1) / KT, t_lo);
+    }
+    const int n_tiles = n1 + t_hi - t_lo;
+    const int n_act = max(1, (n_tiles + a.split_tiles - 1) / a.split_tiles);
+    if (sp >= n_act) return;
+    const int v0 = sp * a.split_tiles, v1 = min(n_tiles, v0 + a.split_tiles);
+    const int mine = v0 + warp < v1 ? (v1 - v0 - warp + NW - 1) / NW : 0;
+    auto key0 = [&](int i) {
+        const int v = v0 + warp + i * NW;
+        return (v < n1 ? v : v - n1 + t_lo) * KT;
+    };
+
+    // queries into shared memory, zero past the tile's rows
+    uint8_t* sq = sm + C::OFF_Q;
+    for (int i = tid; i < ROWS * C::PIECES; i += NW * 32) {
+        const int r = i / C::PIECES, c = i % C::PIECES;
+        uint4 u = make_uint4(0, 0, 0, 0);
+        if (r < rows) {
+            const int tok = (r0 + r) / a.group, j = (r0 + r) % a.group;
+            const T* src = (const T*)p.q + (int64_t)(row0 + tok) * p.q_stride + (int64_t)(h * a.group + j) * D + c * (16 / (int)sizeof(T));
+            if (a.vec_q) {
+                u = *(const uint4*)src;
+            } else {
+                T* x = (T*)&u;
+#pragma unroll
+                for (int k = 0; k < 16 / (int)sizeof(T); k++) x[k] = src[k];
+            }
+        }
+        if constexpr (F32) {
+            uint4 w;
+            uint32_t* x = (uint32_t*)&u;
+            uint32_t* y = (uint32_t*)&w;
+#pragma unroll
+            for (int k = 0; k < 4; k++) split_tf32(__uint_as_float(x[k]), x[k], y[k]);
+            *(uint4*)(sq + ROWS * RB + at<RB>(r, c)) = w;
+        }
+        *(uint4*)(sq + at<RB>(r, c)) = u;
+    }
+
+    // ring: the page numbers of 32 tiles ahead sit in the warp's lanes
+    const uint32_t ring = smem_addr(sm) + (uint32_t)(warp * ST * 2 * C::TILE);
+    const int32_t* tab = p.batch.table + (int64_t)s * p.batch.max_pages;
+    const int64_t block = (int64_t)PAGE * D;   // elements of one (page, layer, K or V, head)
+    int pages = 0;
+    bool bad = false;
+    auto fetch = [&](int i) {
+        if (i < mine) {
+            if ((i & 31) == 0) pages = i + lane < mine ? tab[key0(i + lane) / PAGE] : 0;
+            const int k0 = key0(i);
+            const int page = __shfl_sync(0xffffffffu, pages, i & 31);
+            const bool held = page >= 0 && page < p.kv.n_page;
+            bad |= !held;
+            const T* kp = (const T*)p.kv.pool;
+            if (held) kp += (((int64_t)page * p.kv.n_layer + p.kv.layer) * 2 * p.kv.n_head + h) * block + (k0 % PAGE) * D;
+            const T* vp = held ? kp + p.kv.n_head * block : kp;
+            const uint32_t dst = ring + (uint32_t)((i % ST) * 2 * C::TILE);
+            const int keys = held ? len - k0 : 0;
+#pragma unroll
+            for (int j = 0; j < KT * C::PIECES / 32; j++) {
+                const int x = j * 32 + lane, r = x / C::PIECES, c = x % C::PIECES;
+                const bool in = r < keys;
+                cp16(dst + at<RB>(r, c), in ? (const uint8_t*)kp + x * 16 : (const uint8_t*)p.kv.pool, in);
+                cp16(dst + C::TILE + at<RB>(r, c), in ? (const uint8_t*)vp + x * 16 : (const uint8_t*)p.kv.pool, in);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int i = 0; i < ST - 1; i++) fetch(i);
+    __syncthreads();   // queries
+
+    // this lane's rows: 2 MT of them (fragment rows lane / 4 and + 8)
+    int see_lo[MT][2], see_hi[MT][2];
+#pragma unroll
+    for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const int pos = total - n + (r0 + min(rows - 1, mt * 16 + lane / 4 + 8 * e)) / a.group;
+            see_hi[mt][e] = min(len, pos + 1);
+            see_lo[mt][e] = p.window ? pos - p.window + 1 : 0;
+        }
+    float m[MT][2], l[MT][2], o[MT][D / 8][4];
+#pragma unroll
+    for (int mt = 0; mt < MT; mt++) {
+        m[mt][0] = m[mt][1] = NEG_INF;
+        l[mt][0] = l[mt][1] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < D / 8; d++) o[mt][d][0] = o[mt][d][1] = o[mt][d][2] = o[mt][d][3] = 0.0f;
+    }
+    const uint32_t sqa = smem_addr(sq);
+
+    for (int i = 0; i < mine; i++) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(ST - 2) : "memory");
+        __syncwarp();
+        const uint32_t kt = ring + (uint32_t)((i % ST) * 2 * C::TILE), vt = kt + C::TILE;
+        float sc[MT][KT / 8][4];
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+            for (int j = 0; j < KT / 8; j++) sc[mt][j][0] = sc[mt][j][1] = sc[mt][j][2] = sc[mt][j][3] = 0.0f;
+        if constexpr (!F32) {
+#pragma unroll
+            for (int kk = 0; kk < D / 16; kk++) {
+                uint32_t qa[MT][4];
+#pragma unroll
+                for (int mt = 0; mt < MT; mt++) ldsm4(sqa + at<RB>(mt * 16 + (lane & 15), kk * 2 + (lane >> 4)), qa[mt]);
+#pragma unroll
+                for (int j = 0; j < KT / 16; j++) {
+                    uint32_t kb[4];
+                    ldsm4(kt + at<RB>(j * 16 + (lane & 7) + ((lane >> 4) << 3), kk * 2 + ((lane >> 3) & 1)), kb);
+#pragma unroll
+                    for (int mt = 0; mt < MT; mt++) {
+                        mma16(T(), sc[mt][2 * j], qa[mt], kb[0], kb[1]);
+                        mma16(T(), sc[mt][2 * j + 1], qa[mt], kb[2], kb[3]);
+                    }
+                }
+            }
+        } else {
+            const uint32_t w4 = (lane & 3) * 4;
+            float low[MT][KT / 8][4];   // the two products with a low part, added at the end
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                for (int j = 0; j < KT / 8; j++) low[mt][j][0] = low[mt][j][1] = low[mt][j][2] = low[mt][j][3] = 0.0f;
+#pragma unroll
+            for (int kk = 0; kk < D / 8; kk++) {
+                uint32_t qh[MT][4], ql[MT][4];
+#pragma unroll
+                for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const uint32_t x = at<RB>(mt * 16 + lane / 4 + 8 * (e & 1), kk * 2 + (e >> 1)) + w4;
+                        qh[mt][e] = __float_as_uint(lds(sqa + x));
+                        ql[mt][e] = __float_as_uint(lds(sqa + ROWS * RB + x));
+                    }
+#pragma unroll
+                for (int j = 0; j < KT / 8; j++) {
+                    uint32_t bh[2], bl[2];
+#pragma unroll
+                    for (int e = 0; e < 2; e++)
+                        split_tf32(lds(kt + at<RB>(j * 8 + lane / 4, kk * 2 + e) + w4), bh[e], bl[e]);
+#pragma unroll
+                    for (int mt = 0; mt < MT; mt++) {
+                        mma8(low[mt][j], ql[mt], bh[0], bh[1]);
+                        mma8(low[mt][j], qh[mt], bl[0], bl[1]);
+                        mma8(sc[mt][j], qh[mt], bh[0], bh[1]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                for (int j = 0; j < KT / 8; j++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) sc[mt][j][e] += low[mt][j][e];
+        }
+        // scores in log2 units; keys that a row must not see to -infinity
+        const int k0 = key0(i);
+        const bool whole = k0 + KT <= np || (k0 + KT <= min(len, p0 + 1) && (!p.window || k0 > p1 - p.window));
+        float mx[MT][2];
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++) {
+            mx[mt][0] = mx[mt][1] = NEG_INF;
+#pragma unroll
+            for (int j = 0; j < KT / 8; j++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    float x = sc[mt][j][e] * a.c;
+                    if (!whole) {
+                        const int key = k0 + j * 8 + (lane & 3) * 2 + (e & 1);
+                        if (!(key < np || (key < see_hi[mt][e >> 1] && key >= see_lo[mt][e >> 1]))) x = NEG_INF;
+                    }
+                    sc[mt][j][e] = x;
+                    mx[mt][e >> 1] = fmaxf(mx[mt][e >> 1], x);
+                }
+        }
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                float x = mx[mt][e];
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+                const float top = fmaxf(m[mt][e], x);
+                if (top > m[mt][e]) {
+                    const float f = ex2(m[mt][e] - top);
+                    l[mt][e] *= f;
+#pragma unroll
+                    for (int d = 0; d < D / 8; d++) {
+                        o[mt][d][2 * e] *= f;
+                        o[mt][d][2 * e + 1] *= f;
+                    }
+                    m[mt][e] = top;
+                }
+                const float ref = top == NEG_INF ? 0.0f : top;
+#pragma unroll
+                for (int j = 0; j < KT / 8; j++)
+#pragma unroll
+                    for (int g = 0; g < 2; g++) {
+                        const float w = ex2(sc[mt][j][2 * e + g] - ref);
+                        sc[mt][j][2 * e + g] = w;
+                        l[mt][e] += w;
+                    }
+            }
+        if constexpr (!F32) {
+#pragma unroll
+            for (int kk = 0; kk < KT / 16; kk++) {
+                uint32_t wh[MT][4], wl[MT][4];
+#pragma unroll
+                for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        wh[mt][e] = pack_split(T(), sc[mt][2 * kk + (e >> 1)][2 * (e & 1)], sc[mt][2 * kk + (e >> 1)][2 * (e & 1) + 1], wl[mt][e]);
+#pragma unroll
+                for (int d = 0; d < D / 16; d++) {
+                    uint32_t vb[4];
+                    ldsm4t(vt + at<RB>(kk * 16 + (lane & 15), d * 2 + (lane >> 4)), vb);
+#pragma unroll
+                    for (int mt = 0; mt < MT; mt++) {
+                        mma16(T(), o[mt][2 * d], wl[mt], vb[0], vb[1]);
+                        mma16(T(), o[mt][2 * d], wh[mt], vb[0], vb[1]);
+                        mma16(T(), o[mt][2 * d + 1], wl[mt], vb[2], vb[3]);
+                        mma16(T(), o[mt][2 * d + 1], wh[mt], vb[2], vb[3]);
+                    }
+                }
+            }
+        } else {
+            // the fragment's k index is a key: index lane % 4 takes key 2 (lane % 4), lane % 4 + 4 the next one,
+            // as the score fragment holds them. A tile's products are summed by themselves and then added to o
+            // (the tensor core's additions truncate: over a long cache that would drift, rounded ones do not).
+            uint32_t wh[KT / 8][MT][4], wl[KT / 8][MT][4];
+#pragma unroll
+            for (int j = 0; j < KT / 8; j++)
+#pragma unroll
+                for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) split_tf32(sc[mt][j][2 * (e & 1) + (e >> 1)], wh[j][mt][e], wl[j][mt][e]);
+#pragma unroll
+            for (int d = 0; d < D / 8; d++) {
+                float x[MT][4];
+#pragma unroll
+                for (int mt = 0; mt < MT; mt++) x[mt][0] = x[mt][1] = x[mt][2] = x[mt][3] = 0.0f;
+#pragma unroll
+                for (int j = 0; j < KT / 8; j++) {
+                    uint32_t bh[2], bl[2];
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const int dim = d * 8 + lane / 4;
+                        split_tf32(lds(vt + at<RB>(j * 8 + (lane & 3) * 2 + e, dim / 4) + (dim & 3) * 4), bh[e], bl[e]);
+                    }
+#pragma unroll
+                    for (int mt = 0; mt < MT; mt++) {
+                        mma8(x[mt], wl[j][mt], bh[0], bh[1]);
+                        mma8(x[mt], wh[j][mt], bl[0], bl[1]);
+                        mma8(x[mt], wh[j][mt], bh[0], bh[1]);
+                    }
+                }
+#pragma unroll
+                for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) o[mt][d][e] += x[mt][e];
+            }
+        }
+        __syncwarp();   // every lane is done with the stage that the next fetch overwrites
+        fetch(i + ST - 1);
+    }
+    if (bad && lane == 0) atomicOr(p.err, PAGED_BAD_PAGE);
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+
+    // join the warps
+    float* ml = (float*)(sm + C::OFF_ML);   // [NW][ROWS] {m, l}
+    float* so = (float*)sm;                 // [NW][ROWS][D]
+    __syncthreads();
+#pragma unroll
+    for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            float x = l[mt][e];
+            x += __shfl_xor_sync(0xffffffffu, x, 1);
+            x += __shfl_xor_sync(0xffffffffu, x, 2);
+            const int r = mt * 16 + lane / 4 + 8 * e;
+            if ((lane & 3) == 0) {
+                ml[2 * (warp * ROWS + r)] = m[mt][e];
+                ml[2 * (warp * ROWS + r) + 1] = x;
+            }
+#pragma unroll
+            for (int d = 0; d < D / 8; d++)
+                *(float2*)(so + (size_t)(warp * ROWS + r) * D + d * 8 + (lane & 3) * 2) =
+                    make_float2(o[mt][d][2 * e], o[mt][d][2 * e + 1]);
+        }
+    __syncthreads();
+    const int64_t unit = ((int64_t)s * a.tiles + tile) * p.kv.n_head + h;
+    float* part_o = p.part + unit * a.n_split * (ROWS * (D + 2));   // [split][ROWS][D], then [split][ROWS] {m, l}
+    float* part_ml = part_o + (int64_t)a.n_split * ROWS * D;
+    for (int i = tid; i < rows * (D / 4); i += NW * 32) {
+        const int r = i / (D / 4), d = i % (D / 4) * 4;
+        float top = NEG_INF;
+#pragma unroll
+        for (int w = 0; w < NW; w++) top = fmaxf(top, ml[2 * (w * ROWS + r)]);
+        const float ref = top == NEG_INF ? 0.0f : top;
+        float sum = 0.0f, x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < NW; w++) {
+            const float f = ex2(ml[2 * (w * ROWS + r)] - ref);
+            sum = fmaf(f, ml[2 * (w * ROWS + r) + 1], sum);
+            const float4 v = *(const float4*)(so + (size_t)(w * ROWS + r) * D + d);
+            x[0] = fmaf(f, v.x, x[0]); x[1] = fmaf(f, v.y, x[1]);
+            x[2] = fmaf(f, v.z, x[2]); x[3] = fmaf(f, v.w, x[3]);
+        }
+        if (n_act == 1) {
+            const int tok = (r0 + r) / a.group, head = h * a.group + (r0 + r) % a.group;
+            if (top != NEG_INF) {
+#pragma unroll
+                for (int k = 0; k < 4; k++) x[k] = x[k] / sum;
+            }
+            store_out<T>(a, row0 + tok, head, d, x, D);
+            if (p.lse && d == 0)
+                p.lse[(int64_t)(row0 + tok) * p.n_q_head + head] = top == NEG_INF ? NEG_INF : (top + log2f(sum)) * LN2;
+        } else {
+            *(float4*)(part_o + ((int64_t)sp * ROWS + r) * D + d) = make_float4(x[0], x[1], x[2], x[3]);
+            if (d == 0) *(float2*)(part_ml + 2 * ((int64_t)sp * ROWS + r)) = make_float2(top, sum);
+        }
+    }
+    if (n_act == 1) return;
+
+    // the CTA that arrives last joins the splits
+    int* last = (int*)(sm + C::OFF_ML + (size_t)NW * ROWS * 8);
+    __threadfence();
+    __syncthreads();
+    if (tid == 0) *last = atomicAdd(p.arrived + unit, 1) == n_act - 1;
+    __syncthreads();
+    if (!*last) return;
+    __threadfence();
+    if (tid == 0) p.arrived[unit] = 0;
+    for (int i = tid; i < rows * (D / 4); i += NW * 32) {
+        const int r = i / (D / 4), d = i % (D / 4) * 4;
+        float top = NEG_INF;
+        for (int w = 0; w < n_act; w++) top = fmaxf(top, __ldcg(part_ml + 2 * ((int64_t)w * ROWS + r)));
+        const float ref = top == NEG_INF ? 0.0f : top;
+        float sum = 0.0f, x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+        for (int w = 0; w < n_act; w++) {
+            const float2 e = __ldcg((const float2*)(part_ml + 2 * ((int64_t)w * ROWS + r)));
+            const float f = ex2(e.x - ref);
+            sum = fmaf(f, e.y, sum);
+            const float4 v = __ldcg((const float4*)(part_o + ((int64_t)w * ROWS + r) * D + d));
+            x[0] = fmaf(f, v.x, x[0]); x[1] = fmaf(f, v.y, x[1]);
+            x[2] = fmaf(f, v.z, x[2]); x[3] = fmaf(f, v.w, x[3]);
+        }
+        const int tok = (r0 + r) / a.group, head = h * a.group + (r0 + r) % a.group;
+        if (top != NEG_INF) {
+#pragma unroll
+            for (int k = 0; k < 4; k++) x[k] = x[k] / sum;
+        }
+        store_out<T>(a, row0 + tok, head, d, x, D);
+        if (p.lse && d == 0)
+            p.lse[(int64_t)(row0 + tok) * p.n_q_head + head] = top == NEG_INF ? NEG_INF : (top + log2f(sum)) * LN2;
+    }
+}
+
+// Calls f with the kernel's compile-time variant for (type, head dim, row tile).
+template <typename T, int D, typename F>
+void pick_rows(int row_tile, F f) {
+    if (row_tile == 16) f(k_chunk_attn<T, D, 1>, Cfg<T, D, 1>::SMEM);
+    else f(k_chunk_attn<T, D, 2>, Cfg<T, D, 2>::SMEM);
+}
+template <typename T, typename F>
+void pick_dim(int dim, int row_tile, F f) {
+    if (dim == 32) pick_rows<T, 32>(row_tile, f);
+    else if (dim == 64) pick_rows<T, 64>(row_tile, f);
+    else pick_rows<T, 128>(row_tile, f);
+}
+template <typename F>
+void pick(int dtype, int dim, int row_tile, F f) {
+    if (dtype == GSVCU_KV_F32) pick_dim<float>(dim, row_tile, f);
+    else if (dtype == GSVCU_KV_F16) pick_dim<__half>(dim, row_tile, f);
+    else pick_dim<__nv_bfloat16>(dim, row_tile, f);
+}
+
+}  // namespace
+
+cudaError_t chunk_attention_init_device() {
+    cudaError_t e = cudaSuccess;
+    for (int ty : {GSVCU_KV_F16, GSVCU_KV_F32, GSVCU_KV_BF16})
+        for (int dim : {32, 64, 128})
+            for (int rows : {16, 32})
+                pick(ty, dim, rows, [&](auto k, size_t smem) {
+                    const cudaError_t r = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+                    if (e == cudaSuccess) e = r;
+                });
+    return e;
+}
+
+ChunkAttnPlan chunk_attention_plan(const ChunkAttnParams& p) {
+    const int D = p.kv.head_dim, size = p.kv.kv_dtype == GSVCU_KV_F32 ? 4 : 2;
+    const int kt = size == 4 ? (D == 32 ? 32 : 16) : 2048 / D;
+    const int64_t packed = (int64_t)p.batch.max_chunk * (p.n_q_head / p.kv.n_head);
+    ChunkAttnPlan c;
+    c.row_tile = packed <= 16 ? 16 : 32;
+    c.tiles = (int)((packed + c.row_tile - 1) / c.row_tile);
+    const int64_t units = (int64_t)p.batch.n_seq * c.tiles * p.kv.n_head;
+    const int max_tiles = (p.batch.max_kv + kt - 1) / kt;
+    // Enough CTAs for the 148 SMs x 2; a split keeps at least 4 tiles for each warp.
+    const int64_t want = (2 * 148 + units - 1) / units;
+    const int least = 4 * NW;
+    int n = (int)(want < 1 ? 1 : want);
+    if (n > (max_tiles + least - 1) / least) n = (max_tiles + least - 1) / least;
+    if (n < 1) n = 1;
+    c.split_tiles = (max_tiles + n - 1) / n;
+    c.split_tiles = (c.split_tiles + NW - 1) / NW * NW;
+    if (c.split_tiles < NW) c.split_tiles = NW;
+    c.n_split = (max_tiles + c.split_tiles - 1) / c.split_tiles;
+    if (c.n_split < 1) c.n_split = 1;
+    if (c.n_split > 1) {
+        c.part_floats = (size_t)units * c.n_split * c.row_tile * (D + 2);
+        c.arrivals = (size_t)units;
+    }
+    return c;
+}
+
+void launch_chunk_attention(const ChunkAttnParams& p, const ChunkAttnPlan& plan, cudaStream_t s) {
+    const size_t size = p.kv.kv_dtype == GSVCU_KV_F32 ? 4 : 2;
+    SplitArgs a;
+    a.p = p;
+    a.group = p.n_q_head / p.kv.n_head;
+    a.tiles = plan.tiles;
+    a.n_split = plan.n_split;
+    a.split_tiles = plan.split_tiles;
+    a.c = p.scale * LOG2E;
+    a.vec_q = ((uintptr_t)p.q & 15) == 0 && (p.q_stride * (int64_t)size) % 16 == 0;
+    a.vec_out = ((uintptr_t)p.out & 15) == 0 && (p.out_stride * (int64_t)size) % 16 == 0;
+    const int64_t ctas = (int64_t)p.batch.n_seq * plan.tiles * p.kv.n_head * plan.n_split;
+    if (ctas <= 0) return;
+    pick(p.kv.kv_dtype, p.kv.head_dim, plan.row_tile, [&](auto k, size_t smem) {
+        launch_pdl(k, dim3((unsigned)ctas), dim3(NW * 32), smem, s, a);
+    });
+}
+
+}  // namespace gsvcu

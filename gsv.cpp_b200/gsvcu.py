@@ -18,7 +18,7 @@ HEADER = os.path.join(os.path.dirname(HERE), "include", "gsvcu.h")
 
 OK = 0
 ERR = {-1: "ARG", -2: "CUDA", -3: "OOM", -4: "IO", -5: "FORMAT", -6: "STATE", -7: "DEVICE"}
-KV_F16, KV_F32 = 0, 1
+KV_F16, KV_F32, KV_BF16 = 0, 1, 2
 EPI_BIAS, EPI_RESID, EPI_RELU_Q8 = 0, 1, 2
 
 
@@ -49,9 +49,18 @@ class Finished(C.Structure):
                 ("n_tokens", C.c_int32)]
 
 
+class PagedKVDesc(C.Structure):
+    _fields_ = [("pool", C.c_void_p)] + [(n, C.c_int32) for n in ("kv_dtype", "n_page", "n_layer", "n_kv_head", "head_dim")]
+
+
+class ChunkBatchDesc(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("row_start", "kv_len", "block_table")] + \
+               [(n, C.c_int32) for n in ("n_seq", "max_pages", "n_rows", "max_chunk", "max_kv")]
+
+
 PROGRESS_FN = C.CFUNCTYPE(None, C.c_void_p, C.c_int32)
 
-_P, _I, _U64 = C.c_void_p, C.c_int32, C.c_uint64
+_P, _I, _I64, _U64 = C.c_void_p, C.c_int32, C.c_int64, C.c_uint64
 # exported C entry points and their ctypes signatures
 SIGNATURES = {
     "gsvcu_create": ([C.c_int, C.POINTER(C.c_void_p)], C.c_int),
@@ -91,6 +100,10 @@ SIGNATURES = {
     "gsvcu_set_wait_fault": ([_P, _I], C.c_int),
     "gsvcu_set_prefill_gemm": ([_P, _I], C.c_int),
     "gsvcu_op_q8_gemm_tc": ([_P, _P, _P, _I, _P, _P, _I, _I, _P, _P, _I, _P, _P, _P], C.c_int),
+    "gsvcu_op_kv_append": ([_P, C.POINTER(PagedKVDesc), C.POINTER(ChunkBatchDesc), _I, _I, _I, _P, _I64, _P, _I64, _P,
+                            _I64, _P, _P, _I, _I, _I, _P, _P, _I64], C.c_int),
+    "gsvcu_op_chunk_attention": ([_P, C.POINTER(PagedKVDesc), C.POINTER(ChunkBatchDesc), _I, _I, _P, _I64, C.c_float, _I,
+                                  _P, _P, _I64, _P], C.c_int),
     "gsvcu_op_pack_q8_0_f16": ([_P, _P, _I, _I, _P], C.c_int),
 }
 
@@ -179,6 +192,78 @@ def _ptr(a):
     if hasattr(a, "data_ptr"):
         return C.c_void_p(a.data_ptr())
     return a.ctypes.data_as(C.c_void_p)
+
+
+_KV_TYPES = {"torch.float16": KV_F16, "torch.float32": KV_F32, "torch.bfloat16": KV_BF16}
+_KV_TYPE_OF = {}   # the same by dtype object, filled as they are met (this module does not import torch)
+
+
+def _kv_type(dtype, what):
+    ty = _KV_TYPE_OF.get(dtype)
+    if ty is None:
+        ty = _KV_TYPES.get(str(dtype))
+        if ty is None:
+            raise ValueError(f"{what}: float16, float32 or bfloat16 expected, got {dtype}")
+        _KV_TYPE_OF[dtype] = ty
+    return ty
+
+
+def _ints(t, shape, what):
+    """Device address of a contiguous int32 tensor of this shape."""
+    if t.shape != shape or not t.is_contiguous() or str(t.dtype) != "torch.int32":
+        raise ValueError(f"{what}: contiguous int32 {list(shape)} expected, got {t.dtype} {list(t.shape)}")
+    return t.data_ptr()
+
+
+def _floats(t, shape, what):
+    """Device address of a contiguous float32 tensor of this shape."""
+    if t.shape != shape or not t.is_contiguous() or _kv_type(t.dtype, what) != KV_F32:
+        raise ValueError(f"{what}: contiguous float32 {list(shape)} expected, got {t.dtype} {list(t.shape)}")
+    return t.data_ptr()
+
+
+def _rows(t, n_rows, heads, head_dim, what):
+    """Stride between the rows of a [rows][heads][head_dim] device tensor whose heads lie side by side."""
+    if t.shape != (n_rows, heads, head_dim):
+        raise ValueError(f"{what}: [{n_rows}][{heads}][{head_dim}] expected, got {list(t.shape)}")
+    row, head, one = t.stride()
+    if one != 1 or (head != head_dim and heads > 1):
+        raise ValueError(f"{what}: each row's heads must be contiguous")
+    if n_rows <= 1:
+        return heads * head_dim
+    if row < heads * head_dim:
+        raise ValueError(f"{what}: rows overlap")
+    return row
+
+
+class PagedKV:
+    """A paged KV cache (gsvcu_paged_kv) over a device tensor [page][layer][2][kv head][64][head dim]."""
+
+    def __init__(self, pool):
+        if pool.dim() != 6 or pool.shape[2] != 2 or pool.shape[4] != 64 or not pool.is_contiguous():
+            raise ValueError(f"pool: contiguous [page][layer][2][kv head][64][head dim] expected, got {list(pool.shape)}")
+        self.pool, self.dtype = pool, pool.dtype
+        self.n_kv_head, self.head_dim = pool.shape[3], pool.shape[5]
+        self.desc = PagedKVDesc(pool.data_ptr(), _kv_type(pool.dtype, "pool"), pool.shape[0], pool.shape[1],
+                                pool.shape[3], pool.shape[5])
+        self.ref = C.byref(self.desc)
+
+
+class ChunkBatch:
+    """A ragged batch over a paged cache (gsvcu_chunk_batch): int32 device tensors row_start [n_seq + 1], kv_len
+    [n_seq], block_table [n_seq][max_pages]; n_rows packed rows, max_chunk >= the longest chunk, max_kv >= the
+    longest kv_len (0: what the table holds). The tensors may be updated in place between calls."""
+
+    def __init__(self, row_start, kv_len, block_table, n_rows, max_chunk, max_kv=0):
+        n_seq = kv_len.shape[0]
+        if block_table.dim() != 2:
+            raise ValueError("block_table: [n_seq][max_pages] expected")
+        self.keep = (row_start, kv_len, block_table)
+        self.n_seq, self.n_rows = n_seq, n_rows
+        self.desc = ChunkBatchDesc(_ints(row_start, (n_seq + 1,), "row_start"), _ints(kv_len, (n_seq,), "kv_len"),
+                                   _ints(block_table, (n_seq, block_table.shape[1]), "block_table"), n_seq,
+                                   block_table.shape[1], n_rows, max_chunk, max_kv)
+        self.ref = C.byref(self.desc)
 
 
 class _Reqs:
@@ -393,6 +478,45 @@ class Context:
         tl = np.ascontiguousarray(text_len, np.int32)
         self._check(self.lib.gsvcu_op_prefill_attention(self.h, _ptr(qkv), ss.size, _ptr(ss), _ptr(sl), _ptr(tl),
                                                         _ptr(out_q), _ptr(out_d), _ptr(out_f32)))
+
+    def op_kv_append(self, cache: PagedKV, chunks: ChunkBatch, layer, q, k, v, q_out, cos=None, sin=None, pos=None,
+                     pairs=False):
+        """Append k, v rows [n_rows][kv heads][head dim] to the paged cache and rotate q into q_out (both may be
+        None); cos / sin: f32 [positions][rotated / 2], pos: int32 [n_rows] (None: the cache positions).
+        gsvcu_op_kv_append."""
+        n, D, H = chunks.n_rows, cache.head_dim, cache.n_kv_head
+        ty = k.dtype
+        ks, vs = _rows(k, n, H, D, "k"), _rows(v, n, H, D, "v")
+        nq = qp = qs = op = os_ = 0
+        if q is not None:
+            nq, qp, op = q.shape[1], q.data_ptr(), q_out.data_ptr()
+            qs, os_ = _rows(q, n, nq, D, "q"), _rows(q_out, n, nq, D, "q_out")
+            if q_out.dtype != cache.dtype:
+                raise ValueError("q_out must have the cache's type")
+        if v.dtype != ty or (q is not None and q.dtype != ty):
+            raise ValueError("q, k and v must have one type")
+        n_pos = rot = cp = sp = 0
+        if cos is not None:
+            shape = cos.shape
+            n_pos, rot = shape[0], 2 * shape[1]
+            cp, sp = _floats(cos, shape, "cos"), _floats(sin, shape, "sin")
+        self._check(self.lib.gsvcu_op_kv_append(
+            self.h, cache.ref, chunks.ref, layer, _kv_type(ty, "k"), nq, qp, qs, k.data_ptr(), ks, v.data_ptr(), vs, cp, sp,
+            n_pos, rot, 1 if pairs else 0, None if pos is None else _ints(pos, (n,), "pos"), op, os_))
+
+    def op_chunk_attention(self, cache: PagedKV, chunks: ChunkBatch, layer, q, out, scale=None, prefix=None, window=0,
+                           lse=None):
+        """Attention of the batch's rows q [n_rows][heads][head dim] over the paged cache into out; scale None: 1 /
+        sqrt(head dim); prefix: int32 [n_seq] keys that every row sees; window: keys a row looks back on (0: all);
+        lse: f32 [n_rows][heads]. gsvcu_op_chunk_attention."""
+        n, D, nq = chunks.n_rows, cache.head_dim, q.shape[1]
+        qs, os_ = _rows(q, n, nq, D, "q"), _rows(out, n, nq, D, "out")
+        if q.dtype != cache.dtype or out.dtype != cache.dtype:
+            raise ValueError("q and out must have the cache's type")
+        self._check(self.lib.gsvcu_op_chunk_attention(
+            self.h, cache.ref, chunks.ref, layer, nq, q.data_ptr(), qs, D ** -0.5 if scale is None else scale, window,
+            None if prefix is None else _ints(prefix, (chunks.n_seq,), "prefix"), out.data_ptr(), os_,
+            None if lse is None else _floats(lse, (n, nq), "lse")))
 
     def op_sample(self, logits, V, eos, steps, rng_states, prev=None, top_k=15, top_p=1.0, temperature=1.0, rep=1.35):
         """logits: torch CUDA [B][V]; prev: list of int arrays (repetition windows). Returns (tokens, new states)."""

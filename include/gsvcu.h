@@ -33,7 +33,9 @@ enum {
     GSVCU_ERR_DEVICE = -7    /* device is not an sm_100 GPU or does not exist */
 };
 
-enum { GSVCU_KV_F16 = 0, GSVCU_KV_F32 = 1 };
+/* Element types of a KV cache. BF16 is for the paged-cache operators (gsvcu_op_kv_append,
+ * gsvcu_op_chunk_attention); the AR model's own cache is F16 or F32. */
+enum { GSVCU_KV_F16 = 0, GSVCU_KV_F32 = 1, GSVCU_KV_BF16 = 2 };
 
 typedef struct gsvcu_ctx gsvcu_ctx;
 
@@ -263,6 +265,56 @@ int gsvcu_op_prefill_attention(gsvcu_ctx* ctx, const float* qkv_dev, int32_t n_s
                                const int32_t* seq_len, const int32_t* text_len, int8_t* out_q_dev,
                                uint16_t* out_d_dev, float* out_f32_dev);
 
+/* ---- Paged-cache operators (no counterpart in the reference): appending rows to a paged KV cache and
+ * attention of a chunk of new tokens over it, for decoders of any head layout: prompts in chunks, a few
+ * drafted tokens at once, single tokens. Both run on the context's stream, read the batch from device
+ * memory and allocate nothing after a first call of the same sizes, so they can be captured in a graph. */
+
+/* The cache: pages [page][n_layer][K, V][n_kv_head][64 tokens][head_dim] of kv_dtype elements in pool_dev
+ * (16-byte aligned); head_dim 32, 64 or 128. */
+typedef struct {
+    void* pool_dev;
+    int32_t kv_dtype, n_page, n_layer, n_kv_head, head_dim;
+} gsvcu_paged_kv;
+
+/* The batch (device arrays): sequence s owns the packed rows row_start[s] .. row_start[s + 1] - 1
+ * (row_start [n_seq + 1], ascending), holds kv_len[s] keys with these rows and keeps key c in page
+ * block_table[s][c / 64], slot c % 64 (block_table [n_seq][max_pages]; entries past its keys are not read).
+ * Row i of n is the token at cache position kv_len[s] - n + i. Host sizes: n_rows packed rows, max_chunk at
+ * least the longest chunk, max_kv at least the longest kv_len (0: max_pages * 64); the closer these are, the
+ * better the work is cut up. A page outside the pool, or lengths outside these sizes, touch no memory
+ * outside the arrays; the rows they concern are undefined, and the next gsvcu_sync returns GSVCU_ERR_ARG. */
+typedef struct {
+    const int32_t *row_start_dev, *kv_len_dev, *block_table_dev;
+    int32_t n_seq, max_pages, n_rows, max_chunk, max_kv;
+} gsvcu_chunk_batch;
+
+/* Append: k and v rows [n_rows][n_kv_head][head_dim] (strides in elements between rows) go to their cache
+ * positions at `layer`, q rows [n_rows][n_q_head][head_dim] to q_out_dev (n_q_head 0: no q). The first rot_dim
+ * elements of every q and k head are rotated first: a' = a cos - b sin, b' = a sin + b cos with a, b =
+ * elements i and i + rot_dim / 2 (rot_pairs 0) or 2 i and 2 i + 1 (rot_pairs 1) and cos / sin [n_pos][rot_dim
+ * / 2] at the row's position: pos_dev[row], or its cache position when pos_dev is null. rot_dim 0: no
+ * rotation. Rows are F32 or the cache's type (row_dtype); sums in F32, one rounding to the cache's type.
+ * q_out_dev has the cache's type and may be q_dev itself (same type and stride). Rows whose cache position is
+ * negative (a chunk longer than its kv_len) are not stored. A position outside the table is reported by the
+ * next gsvcu_sync (GSVCU_ERR_ARG). */
+int gsvcu_op_kv_append(gsvcu_ctx* ctx, const gsvcu_paged_kv* kv, const gsvcu_chunk_batch* batch, int32_t layer,
+                       int32_t row_dtype, int32_t n_q_head, const void* q_dev, int64_t q_stride, const void* k_dev,
+                       int64_t k_stride, const void* v_dev, int64_t v_stride, const float* cos_dev,
+                       const float* sin_dev, int32_t n_pos, int32_t rot_dim, int32_t rot_pairs, const int32_t* pos_dev,
+                       void* q_out_dev, int64_t q_out_stride);
+
+/* Attention of the batch's rows over the cache at `layer`. Query head h reads kv head h / (n_q_head /
+ * n_kv_head). The row at position p sees key j < kv_len when j < prefix[s], or j <= p and (window 0 or j >
+ * p - window): causal with a prefix that all rows see (prefix_dev null: none; the whole length: no mask) and a
+ * sliding window. q and out rows have the cache's type (strides in elements, out not overlapping q);
+ * lse_dev (may be null) [n_rows][n_q_head] gets the natural logarithm of each row's sum of exp(scale q.k).
+ * A row that sees no key gives 0 and -infinity. Scores, softmax and sums are F32. Keys from kv_len on are
+ * never read; keys below it must be finite where any row of the chunk may see them. */
+int gsvcu_op_chunk_attention(gsvcu_ctx* ctx, const gsvcu_paged_kv* kv, const gsvcu_chunk_batch* batch, int32_t layer,
+                             int32_t n_q_head, const void* q_dev, int64_t q_stride, float scale, int32_t window,
+                             const int32_t* prefix_dev, void* out_dev, int64_t out_stride, float* lse_dev);
+
 /* One sampling step per row (gsv_logits_to_probs + gsv_sample, reference src/gsv_sampler.cpp:8-89,
  * with the step < 11 EOS mask of src/gsv_ar.cpp:768): logits_dev [B][V] f32; prev_host [B][prev_stride]
  * repetition windows of n_prev_host[b] tokens (NULL = none); step_host [B] step index; rng_host [B]
@@ -417,8 +469,9 @@ int64_t gsvcu_kernel_launches(const gsvcu_ctx* ctx);
  * it with events. */
 void* gsvcu_stream(const gsvcu_ctx* ctx);
 
-/* Synchronise the context's stream. Also reports (GSVCU_ERR_CUDA, once) a bounded wait of
- * gsvcu_op_decode_attention that gave up since the last call. */
+/* Synchronise the context's stream. Also reports, once, what the kernels found since the last call: a bounded
+ * wait of gsvcu_op_decode_attention or gsvcu_op_chunk_attention that gave up (GSVCU_ERR_CUDA), pages, lengths
+ * or positions outside their arrays in gsvcu_op_kv_append / gsvcu_op_chunk_attention (GSVCU_ERR_ARG). */
 int gsvcu_sync(gsvcu_ctx* ctx);
 
 /* Failure-path testing (no counterpart in the reference, whose KV allocation failure exits the process,

@@ -174,3 +174,32 @@ def test_bench_weight_bytes_per_format(tmp_path):
         t = {x.name: int(x.n_bytes) for x in gguf.GGUFReader(path).tensors}
         layer = sum(v for k, v in t.items() if k.startswith("transformer.block0."))
         assert 24 * layer + t["ar.predict"] == nbytes, name
+
+
+def test_paged_operators_null_arguments_are_rejected():
+    """The paged-cache operators refuse a null context before any device work."""
+    lib = gsvcu.load_library()
+    kv, batch = gsvcu.PagedKVDesc(), gsvcu.ChunkBatchDesc()
+    assert lib.gsvcu_op_kv_append(None, C.byref(kv), C.byref(batch), 0, 0, 0, None, 0, None, 0, None, 0, None, None, 0,
+                                  0, 0, None, None, 0) == -1
+    assert lib.gsvcu_op_chunk_attention(None, C.byref(kv), C.byref(batch), 0, 1, None, 0, 1.0, 0, None, None, 0, None) == -1
+
+
+def test_paged_cache_and_batch_objects_check_their_tensors():
+    """PagedKV and ChunkBatch take only what the C structs can describe (no device work)."""
+    torch = pytest.importorskip("torch")
+    pool = torch.zeros(3, 2, 2, 4, 64, 32, dtype=torch.bfloat16)
+    kv = gsvcu.PagedKV(pool)
+    d = kv.desc
+    assert (d.pool, d.kv_dtype, d.n_page, d.n_layer, d.n_kv_head, d.head_dim) == (pool.data_ptr(), 2, 3, 2, 4, 32)
+    for bad in (pool[:, :, :1], pool.transpose(3, 4), pool[..., :16], pool.double(), pool[:, :, :, :, :32].contiguous()):
+        with pytest.raises(ValueError):
+            gsvcu.PagedKV(bad)
+    i32 = dict(dtype=torch.int32)
+    start, lens, table = torch.tensor([0, 2, 3], **i32), torch.tensor([70, 1], **i32), torch.zeros(2, 5, **i32)
+    b = gsvcu.ChunkBatch(start, lens, table, 3, 2, 70).desc
+    assert (b.n_seq, b.max_pages, b.n_rows, b.max_chunk, b.max_kv) == (2, 5, 3, 2, 70)
+    for bad in ((start[:2], lens, table), (start, lens.long(), table), (start, lens, table[:1]), (start, lens, table[0]),
+                (start, lens, table.T.contiguous().T)):
+        with pytest.raises(ValueError):
+            gsvcu.ChunkBatch(*bad, 3, 2)
