@@ -1845,6 +1845,8 @@ static int paged_views(gsvcu_ctx* ctx, const gsvcu_paged_kv* kv, const gsvcu_chu
         return ctx->fail(GSVCU_ERR_ARG, "paged cache: n_page, n_layer and n_kv_head must be positive");
     if (kv->head_dim != 32 && kv->head_dim != 64 && kv->head_dim != 128)
         return ctx->fail(GSVCU_ERR_ARG, "paged cache: head_dim must be 32, 64 or 128");
+    if ((int64_t)kv->n_page * kv->n_layer > INT32_MAX / 2 / kv->n_kv_head)
+        return ctx->fail(GSVCU_ERR_ARG, "paged cache: more than 2^31 (page, layer, head) blocks");
     if (layer < 0 || layer >= kv->n_layer) return ctx->fail(GSVCU_ERR_ARG, "paged cache: layer out of range");
     if (n_q_head < 0 || n_q_head % kv->n_kv_head)
         return ctx->fail(GSVCU_ERR_ARG, "paged cache: n_q_head must be a multiple of n_kv_head");
@@ -1947,7 +1949,8 @@ int gsvcu_op_chunk_attention(gsvcu_ctx* ctx, const gsvcu_paged_kv* kv, const gsv
     }
     p.part = ctx->op_split;
     p.arrived = ctx->op_arrived;
-    launch_chunk_attention(p, plan, ctx->stream);
+    if (!launch_chunk_attention(p, plan, ctx->stream))
+        return ctx->fail(GSVCU_ERR_CUDA, "gsvcu_op_chunk_attention: tensor map encoding failed");
     CKC(ctx, cudaGetLastError());
     ctx->launches++;
     return GSVCU_OK;

@@ -60,6 +60,7 @@ struct ChunkAttnParams {
 };
 // How one call is cut up, from the sizes alone; scratch it needs.
 struct ChunkAttnPlan {
+    bool tensor = false;   // the tcgen05 kernel (paged_attention_tc.cu)
     int row_tile = 0;      // packed rows (token x query head of one kv head) of a CTA
     int tiles = 0;         // row tiles per sequence (bound)
     int n_split = 0;       // key splits (bound)
@@ -67,7 +68,10 @@ struct ChunkAttnPlan {
     size_t part_floats = 0, arrivals = 0;
 };
 ChunkAttnPlan chunk_attention_plan(const ChunkAttnParams& p);
-void launch_chunk_attention(const ChunkAttnParams& p, const ChunkAttnPlan& plan, cudaStream_t s);
+// False: not launched (no tensor map).
+bool launch_chunk_attention(const ChunkAttnParams& p, const ChunkAttnPlan& plan, cudaStream_t s);
+bool launch_chunk_attention_tc(const ChunkAttnParams& p, const ChunkAttnPlan& plan, cudaStream_t s);
 cudaError_t chunk_attention_init_device();   // dynamic shared-memory limits on the current device
+cudaError_t chunk_attention_tc_init_device();
 
 }  // namespace gsvcu

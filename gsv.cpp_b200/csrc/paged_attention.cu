@@ -18,20 +18,14 @@
 
 #include "kernels.h"
 #include "paged.h"
+#include "paged_join.cuh"
 
 namespace gsvcu {
 namespace {
 
-constexpr float NEG_INF = -__builtin_huge_valf();
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr int NW = 4;   // warps per CTA
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool in) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
 }
@@ -114,33 +108,12 @@ __device__ __forceinline__ uint32_t at(int row, int piece) {
     return (uint32_t)(row * RB + ((piece ^ swz) << 4));
 }
 
-template <typename T> __device__ __forceinline__ T narrow(float x);
-template <> __device__ __forceinline__ float narrow<float>(float x) { return x; }
-template <> __device__ __forceinline__ __half narrow<__half>(float x) { return __float2half_rn(x); }
-template <> __device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
-
 struct SplitArgs {
     ChunkAttnParams p;
     int group, tiles, n_split, split_tiles;
     float c;          // scale * log2(e)
     bool vec_q, vec_out;
 };
-
-// Four consecutive outputs of one packed row.
-template <typename T>
-__device__ __forceinline__ void store_out(const SplitArgs& a, int64_t row, int head, int d, const float (&o)[4], int D) {
-    T* dst = (T*)a.p.out + row * a.p.out_stride + (int64_t)head * D + d;
-    if (a.vec_out) {
-        T v[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) v[i] = narrow<T>(o[i]);
-        if constexpr (sizeof(T) == 4) *(float4*)dst = make_float4(v[0], v[1], v[2], v[3]);
-        else *(uint2*)dst = *(const uint2*)v;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; i++) dst[i] = narrow<T>(o[i]);
-    }
-}
 
 template <typename T, int D, int MT>
 __global__ void __launch_bounds__(NW * 32) k_chunk_attn(SplitArgs a) {
@@ -159,51 +132,24 @@ __global__ void __launch_bounds__(NW * 32) k_chunk_attn(SplitArgs a) {
     griddep_wait();
     griddep_launch();
 
-    // the sequence: rows [row0, row0 + n), keys [0, len); what is out of bounds is cut off and reported
-    int row0 = p.batch.row_start[s], n = p.batch.row_start[s + 1] - row0, len = p.batch.kv_len[s];
-    const int cap = min(p.batch.max_kv, p.batch.max_pages * PAGE);
-    if (tid == 0 && sp == 0 && h == 0 && tile == 0 &&
-        (row0 < 0 || n < 0 || row0 + n > p.batch.n_rows || len < 0 || len > cap || n > p.batch.max_chunk))
-        atomicOr(p.err, PAGED_BAD_LENGTH);
-    const int total = len;   // positions count from the true length
-    len = max(0, min(len, cap));
-    if (row0 < 0 || row0 > p.batch.n_rows) return;
-    n = min(n, p.batch.n_rows - row0);
-    const int r0 = tile * ROWS, rows = min(ROWS, n * a.group - r0);   // packed rows of this tile
-    if (rows <= 0) return;
-
-    // keys that some row of the tile sees: [0, np) and [lo, hi)
-    const int p0 = total - n + r0 / a.group, p1 = total - n + (r0 + rows - 1) / a.group;
-    const int np = p.prefix ? max(0, min(p.prefix[s], len)) : 0;
-    int hi = max(0, min(len, p1 + 1)), lo = p.window ? max(0, p0 - p.window + 1) : 0;
-    if (hi <= lo) lo = hi = 0;
-    int t_lo, t_hi, n1;
-    if (np >= lo) {
-        t_lo = n1 = 0;
-        t_hi = (max(np, hi) + KT - 1) / KT;
-    } else {
-        t_lo = lo / KT;
-        t_hi = (hi + KT - 1) / KT;
-        n1 = min((np + KT - 1) / KT, t_lo);
-    }
-    const int n_tiles = n1 + t_hi - t_lo;
+    ChunkRange c;
+    if (!chunk_range(p, s, tile, a.group, ROWS, KT, tid == 0 && sp == 0 && h == 0 && tile == 0, c)) return;
+    const int row0 = c.row0, n = c.n, total = c.total, len = c.len, r0 = c.r0, rows = c.rows, p0 = c.p0, p1 = c.p1, np = c.np;
+    const int n_tiles = c.n_tiles;
     const int n_act = max(1, (n_tiles + a.split_tiles - 1) / a.split_tiles);
     if (sp >= n_act) return;
     const int v0 = sp * a.split_tiles, v1 = min(n_tiles, v0 + a.split_tiles);
     const int mine = v0 + warp < v1 ? (v1 - v0 - warp + NW - 1) / NW : 0;
-    auto key0 = [&](int i) {
-        const int v = v0 + warp + i * NW;
-        return (v < n1 ? v : v - n1 + t_lo) * KT;
-    };
+    auto key0 = [&](int i) { return c.tile_of(v0 + warp + i * NW) * KT; };
 
     // queries into shared memory, zero past the tile's rows
     uint8_t* sq = sm + C::OFF_Q;
     for (int i = tid; i < ROWS * C::PIECES; i += NW * 32) {
-        const int r = i / C::PIECES, c = i % C::PIECES;
+        const int r = i / C::PIECES, pc = i % C::PIECES;
         uint4 u = make_uint4(0, 0, 0, 0);
         if (r < rows) {
             const int tok = (r0 + r) / a.group, j = (r0 + r) % a.group;
-            const T* src = (const T*)p.q + (int64_t)(row0 + tok) * p.q_stride + (int64_t)(h * a.group + j) * D + c * (16 / (int)sizeof(T));
+            const T* src = (const T*)p.q + (int64_t)(row0 + tok) * p.q_stride + (int64_t)(h * a.group + j) * D + pc * (16 / (int)sizeof(T));
             if (a.vec_q) {
                 u = *(const uint4*)src;
             } else {
@@ -218,9 +164,9 @@ __global__ void __launch_bounds__(NW * 32) k_chunk_attn(SplitArgs a) {
             uint32_t* y = (uint32_t*)&w;
 #pragma unroll
             for (int k = 0; k < 4; k++) split_tf32(__uint_as_float(x[k]), x[k], y[k]);
-            *(uint4*)(sq + ROWS * RB + at<RB>(r, c)) = w;
+            *(uint4*)(sq + ROWS * RB + at<RB>(r, pc)) = w;
         }
-        *(uint4*)(sq + at<RB>(r, c)) = u;
+        *(uint4*)(sq + at<RB>(r, pc)) = u;
     }
 
     // ring: the page numbers of 32 tiles ahead sit in the warp's lanes
@@ -243,10 +189,10 @@ __global__ void __launch_bounds__(NW * 32) k_chunk_attn(SplitArgs a) {
             const int keys = held ? len - k0 : 0;
 #pragma unroll
             for (int j = 0; j < KT * C::PIECES / 32; j++) {
-                const int x = j * 32 + lane, r = x / C::PIECES, c = x % C::PIECES;
+                const int x = j * 32 + lane, r = x / C::PIECES, pc = x % C::PIECES;
                 const bool in = r < keys;
-                cp16(dst + at<RB>(r, c), in ? (const uint8_t*)kp + x * 16 : (const uint8_t*)p.kv.pool, in);
-                cp16(dst + C::TILE + at<RB>(r, c), in ? (const uint8_t*)vp + x * 16 : (const uint8_t*)p.kv.pool, in);
+                cp16(dst + at<RB>(r, pc), in ? (const uint8_t*)kp + x * 16 : (const uint8_t*)p.kv.pool, in);
+                cp16(dst + C::TILE + at<RB>(r, pc), in ? (const uint8_t*)vp + x * 16 : (const uint8_t*)p.kv.pool, in);
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
@@ -499,7 +445,7 @@ __global__ void __launch_bounds__(NW * 32) k_chunk_attn(SplitArgs a) {
 #pragma unroll
                 for (int k = 0; k < 4; k++) x[k] = x[k] / sum;
             }
-            store_out<T>(a, row0 + tok, head, d, x, D);
+            store_out<T, D>(p, a.vec_out, row0 + tok, head, d, x);
             if (p.lse && d == 0)
                 p.lse[(int64_t)(row0 + tok) * p.n_q_head + head] = top == NEG_INF ? NEG_INF : (top + log2f(sum)) * LN2;
         } else {
@@ -509,39 +455,8 @@ __global__ void __launch_bounds__(NW * 32) k_chunk_attn(SplitArgs a) {
     }
     if (n_act == 1) return;
 
-    // the CTA that arrives last joins the splits
-    int* last = (int*)(sm + C::OFF_ML + (size_t)NW * ROWS * 8);
-    __threadfence();
-    __syncthreads();
-    if (tid == 0) *last = atomicAdd(p.arrived + unit, 1) == n_act - 1;
-    __syncthreads();
-    if (!*last) return;
-    __threadfence();
-    if (tid == 0) p.arrived[unit] = 0;
-    for (int i = tid; i < rows * (D / 4); i += NW * 32) {
-        const int r = i / (D / 4), d = i % (D / 4) * 4;
-        float top = NEG_INF;
-        for (int w = 0; w < n_act; w++) top = fmaxf(top, __ldcg(part_ml + 2 * ((int64_t)w * ROWS + r)));
-        const float ref = top == NEG_INF ? 0.0f : top;
-        float sum = 0.0f, x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-        for (int w = 0; w < n_act; w++) {
-            const float2 e = __ldcg((const float2*)(part_ml + 2 * ((int64_t)w * ROWS + r)));
-            const float f = ex2(e.x - ref);
-            sum = fmaf(f, e.y, sum);
-            const float4 v = __ldcg((const float4*)(part_o + ((int64_t)w * ROWS + r) * D + d));
-            x[0] = fmaf(f, v.x, x[0]); x[1] = fmaf(f, v.y, x[1]);
-            x[2] = fmaf(f, v.z, x[2]); x[3] = fmaf(f, v.w, x[3]);
-        }
-        const int tok = (r0 + r) / a.group, head = h * a.group + (r0 + r) % a.group;
-        if (top != NEG_INF) {
-#pragma unroll
-            for (int k = 0; k < 4; k++) x[k] = x[k] / sum;
-        }
-        store_out<T>(a, row0 + tok, head, d, x, D);
-        if (p.lse && d == 0)
-            p.lse[(int64_t)(row0 + tok) * p.n_q_head + head] = top == NEG_INF ? NEG_INF : (top + log2f(sum)) * LN2;
-    }
+    join_splits<T, D, ROWS, NW * 32>(p, c, s, tile, h, a.group, a.tiles, a.n_split, n_act, a.vec_out,
+                                     (int*)(sm + C::OFF_ML + (size_t)NW * ROWS * 8));
 }
 
 // Calls f with the kernel's compile-time variant for (type, head dim, row tile).
@@ -574,7 +489,8 @@ cudaError_t chunk_attention_init_device() {
                     const cudaError_t r = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
                     if (e == cudaSuccess) e = r;
                 });
-    return e;
+    const cudaError_t r = chunk_attention_tc_init_device();
+    return e == cudaSuccess ? r : e;
 }
 
 ChunkAttnPlan chunk_attention_plan(const ChunkAttnParams& p) {
@@ -582,6 +498,25 @@ ChunkAttnPlan chunk_attention_plan(const ChunkAttnParams& p) {
     const int kt = size == 4 ? (D == 32 ? 32 : 16) : 2048 / D;
     const int64_t packed = (int64_t)p.batch.max_chunk * (p.n_q_head / p.kv.n_head);
     ChunkAttnPlan c;
+    if (size == 2 && packed > 32 && p.scale != 0.0f) {
+        // Many rows of 16-bit types: the tcgen05 kernel (a zero scale would multiply masked -infinities by 0 there).
+        // Splits only while there are fewer CTAs than SMs, and of 4 tiles at least.
+        c.tensor = true;
+        c.row_tile = 256;
+        c.tiles = (int)((packed + 255) / 256);
+        const int64_t units = (int64_t)p.batch.n_seq * c.tiles * p.kv.n_head;
+        const int max_tiles = (p.batch.max_kv + 127) / 128;
+        int n = (int)(148 / units > 1 ? 148 / units : 1);
+        if (n > max_tiles / 4) n = max_tiles / 4;
+        if (n < 1) n = 1;
+        c.split_tiles = (max_tiles + n - 1) / n;
+        c.n_split = (max_tiles + c.split_tiles - 1) / c.split_tiles;
+        if (c.n_split > 1) {
+            c.part_floats = (size_t)units * c.n_split * c.row_tile * (D + 2);
+            c.arrivals = (size_t)units;
+        }
+        return c;
+    }
     c.row_tile = packed <= 16 ? 16 : 32;
     c.tiles = (int)((packed + c.row_tile - 1) / c.row_tile);
     const int64_t units = (int64_t)p.batch.n_seq * c.tiles * p.kv.n_head;
@@ -604,7 +539,8 @@ ChunkAttnPlan chunk_attention_plan(const ChunkAttnParams& p) {
     return c;
 }
 
-void launch_chunk_attention(const ChunkAttnParams& p, const ChunkAttnPlan& plan, cudaStream_t s) {
+bool launch_chunk_attention(const ChunkAttnParams& p, const ChunkAttnPlan& plan, cudaStream_t s) {
+    if (plan.tensor) return launch_chunk_attention_tc(p, plan, s);
     const size_t size = p.kv.kv_dtype == GSVCU_KV_F32 ? 4 : 2;
     SplitArgs a;
     a.p = p;
@@ -616,10 +552,10 @@ void launch_chunk_attention(const ChunkAttnParams& p, const ChunkAttnPlan& plan,
     a.vec_q = ((uintptr_t)p.q & 15) == 0 && (p.q_stride * (int64_t)size) % 16 == 0;
     a.vec_out = ((uintptr_t)p.out & 15) == 0 && (p.out_stride * (int64_t)size) % 16 == 0;
     const int64_t ctas = (int64_t)p.batch.n_seq * plan.tiles * p.kv.n_head * plan.n_split;
-    if (ctas <= 0) return;
     pick(p.kv.kv_dtype, p.kv.head_dim, plan.row_tile, [&](auto k, size_t smem) {
         launch_pdl(k, dim3((unsigned)ctas), dim3(NW * 32), smem, s, a);
     });
+    return true;
 }
 
 }  // namespace gsvcu
