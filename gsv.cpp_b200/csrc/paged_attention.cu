@@ -455,7 +455,7 @@ __global__ void __launch_bounds__(NW * 32) k_chunk_attn(SplitArgs a) {
     }
     if (n_act == 1) return;
 
-    join_splits<T, D, ROWS, NW * 32>(p, c, s, tile, h, a.group, a.tiles, a.n_split, n_act, a.vec_out,
+    join_splits<T, D, ROWS, NW * 32>(p, c, s, tile, h, a.group, a.tiles, a.n_split, n_act, a.vec_out, tid,
                                      (int*)(sm + C::OFF_ML + (size_t)NW * ROWS * 8));
 }
 

@@ -3,10 +3,11 @@
 //
 // k_chunk_attn_tc: one CTA per (sequence, 256 packed rows, kv head, key split), as two row tiles of 128 rows
 // (packed row r = token * g + query head of the group). Key tiles are 128 keys = two pages, each page's
-// [64][head dim] block fetched by TMA into a ring that K and V tiles take in turn (K0 V0 K1 V1 ...).
+// [64][head dim] block fetched by TMA into a ring of pairs (V of one tile, K of the next).
 //   warp 0     page numbers (32 per load) and TMA
 //   warp 1     MMA: S = Q K^T (both operands in shared memory), O += P V (P in tensor memory, V in shared
 //              memory as it lies in the page: the MN-major operand, so nothing is transposed)
+//   warp 2     clears what the last page holds past the last key
 //   warps 4-7  softmax of row tile 0, one thread per row (TMEM lane); warps 8-11 of row tile 1
 // The MMAs of one row tile run under the other's softmax: S0 S1 | PV0 S0' PV1 S1' | ... Each thread takes its
 // 128 scores into registers, writes the weights P over them in tensor memory as 16-bit pairs, and keeps the
@@ -17,6 +18,8 @@
 // V rows past kv_len in the last tile are zeroed in shared memory before its product, absent pages are
 // zero-filled by TMA (a block index past the pool), masked keys get weight 0.
 #include <cuda_bf16.h>
+
+#include <type_traits>
 
 #include "paged.h"
 #include "paged_join.cuh"
@@ -38,10 +41,10 @@ struct Smem {
     static constexpr int RB = D >= 64 ? 128 : 2 * D;              // bytes of a swizzled row
     static constexpr int ATOMS = D >= 64 ? D / 64 : 1;            // 64-dim column blocks of a tile
     static constexpr int ENTRY = KT * D * 2;                      // bytes of a K or V tile
-    static constexpr int NE = D == 128 ? 4 : 8;                   // ring entries
+    static constexpr int NP = 2;                                  // ring pairs (even)
     static constexpr size_t OFF_RING = (size_t)ROWS * D * 2;      // after Q
-    static constexpr size_t OFF_BAR = OFF_RING + (size_t)NE * ENTRY;
-    static constexpr int NBAR = 2 * NE + 7;                       // full, empty, S full [2], P full [2], O done [2], drain
+    static constexpr size_t OFF_BAR = OFF_RING + (size_t)NP * 2 * ENTRY;
+    static constexpr int NBAR = 2 * NP + 11;   // full, empty, S full [2], P full [2][2], O done [2], V landed, V cleared, drain
     static constexpr size_t SMEM = OFF_BAR + NBAR * 8 + 16 + 1024;
 };
 
@@ -54,25 +57,53 @@ struct TcArgs {
     bool vec_q, vec_out;
 };
 
-// Shared-memory operand descriptor: address and strides in 16-byte units, version 1, swizzle of RB-byte rows.
+// Shared-memory operand descriptors, low word: address and column-block stride lbo in 16-byte units (addresses
+// stay below 2^18, so a descriptor moves by adding 16-byte units); high word: 8-row groups at 8 * RB bytes,
+// version 1, 128- or 64-byte swizzle of RB-byte rows.
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t lbo) { return (addr >> 4) | ((lbo >> 4) << 16); }
 template <int RB>
-__device__ __forceinline__ uint64_t op_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
-    constexpr uint64_t mode = RB == 128 ? 2 : 4;   // 128- or 64-byte swizzle
-    return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(sbo >> 4) << 32) |
-           ((uint64_t)1 << 46) | (mode << 61);
-}
+constexpr uint32_t DESC_HI = (8 * RB >> 4) | (1u << 14) | ((RB == 128 ? 2u : 4u) << 29);
 // Instruction descriptor: f32 accumulator, 16-bit operands (0 F16, 1 BF16), B MN-major when `tb`.
 __host__ __device__ constexpr uint32_t instr(int type, int tb, int n) {
     return (1u << 4) | ((uint32_t)type << 7) | ((uint32_t)type << 10) | ((uint32_t)tb << 16) | ((uint32_t)(n >> 3) << 17) |
            ((uint32_t)(128 >> 4) << 24);
 }
-// D (tensor memory) (+)= A (tensor memory, 16-bit pairs) x B (shared memory).
-__device__ __forceinline__ void mma_ta(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// The MMA warp runs its loop as a whole and one elected lane issues: operands then stay in uniform registers.
+// (Under a branch on the lane every operand was moved there for each MMA, 60 cycles apiece.)
+// D (tensor memory) (+)= A (shared memory) x B (shared memory); descriptors as low words and one high word.
+template <uint32_t HI, uint32_t ID, bool ADD>
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b) {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        "{\n .reg .pred p, q;\n .reg .b64 a, b;\n elect.sync _|q, 0xffffffff;\n setp.ne.b32 p, %5, 0;\n"
+        " mov.b64 a, {%1, %3};\n mov.b64 b, {%2, %3};\n"
+        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n}\n" ::"r"(d),
+        "r"(a), "r"(b), "n"(HI), "n"(ID), "n"((int)ADD)
         : "memory");
+}
+// D (tensor memory) (+)= A (tensor memory, 16-bit pairs) x B (shared memory).
+template <uint32_t HI, uint32_t ID>
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t add) {
+    asm volatile(
+        "{\n .reg .pred p, q;\n .reg .b64 b;\n elect.sync _|q, 0xffffffff;\n setp.ne.b32 p, %5, 0;\n"
+        " mov.b64 b, {%2, %3};\n"
+        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n}\n" ::"r"(d),
+        "r"(a), "r"(b), "n"(HI), "n"(ID), "r"(add)
+        : "memory");
+}
+// The barrier completes a phase when every MMA that the elected lane issued before is done.
+__device__ __forceinline__ void commit(uint32_t bar) {
+    asm volatile(
+        "{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n"
+        " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(bar)
+        : "memory");
+}
+// Bounded wait of a converged warp, with a warp-uniform result.
+__device__ __forceinline__ bool wait_warp(uint32_t b, uint32_t parity, volatile int* abort_flag) {
+    for (uint32_t it = 0; it < TC_SPIN_LIMIT; it++) {
+        if (__any_sync(0xffffffffu, bar_try_short(b, parity))) return true;
+        if (__any_sync(0xffffffffu, *abort_flag)) return false;
+    }
+    return false;
 }
 #define R8(x, i) "+r"(x[i]), "+r"(x[i + 1]), "+r"(x[i + 2]), "+r"(x[i + 3]), "+r"(x[i + 4]), "+r"(x[i + 5]), "+r"(x[i + 6]), "+r"(x[i + 7])
 #define R32(x) R8(x, 0), R8(x, 8), R8(x, 16), R8(x, 24)
@@ -102,6 +133,11 @@ __device__ __forceinline__ void tmem_st16u(uint32_t a, const uint32_t (&r)[16]) 
         : "memory");
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float y;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
 template <typename T> __device__ __forceinline__ uint32_t pack2(float x, float y);
 template <> __device__ __forceinline__ uint32_t pack2<__half>(float x, float y) {
     const __half2 h = __floats2half2_rn(x, y);
@@ -110,6 +146,34 @@ template <> __device__ __forceinline__ uint32_t pack2<__half>(float x, float y) 
 template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float x, float y) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
     return *(const uint32_t*)&h;
+}
+
+// One pair of weights in EVERY takes its exponentials on the FMA pipe: the special-function unit (16 per cycle
+// and SM) would need 2048 cycles for two row tiles of 128 keys, as many as their products at head dim 128.
+constexpr int EVERY = 4;
+// 2^x of two values on the FMA pipe: x = n + f with n the nearest integer (by the 1.5 * 2^23 addend) and
+// |f| <= 1/2, 2^f by its relative minimax polynomial (least squares with Lawson's weights: degree 3 for BF16,
+// relative error 7.5e-5; degree 4 for F16, 2.6e-6), n added to the exponent. Below 2^-126: 2^-126.
+template <typename T>
+__device__ __forceinline__ uint64_t ex2_pair(uint64_t x) {
+    x = f2pack(fmaxf(f2lo(x), -126.0f), fmaxf(f2hi(x), -126.0f));
+    const uint64_t big = f2pack(12582912.0f, 12582912.0f), nbig = f2pack(-12582912.0f, -12582912.0f);
+    const uint64_t n = fadd2(x, big);
+    const uint64_t f = ffma2(fadd2(n, nbig), f2pack(-1.0f, -1.0f), x);
+    auto k = [](float v) { return f2pack(v, v); };
+    uint64_t y;
+    if constexpr (__is_same(T, __half)) {
+        y = ffma2(f, k(0x1.3997d6p-7f), k(0x1.ca1440p-5f));
+        y = ffma2(f, y, k(0x1.ec06dap-3f));
+        y = ffma2(f, y, k(0x1.62e0dcp-1f));
+        y = ffma2(f, y, k(0x1.ffffe8p-1f));
+    } else {
+        y = ffma2(f, k(0x1.c3f760p-5f), k(0x1.f0de1ap-3f));
+        y = ffma2(f, y, k(0x1.62f31ap-1f));
+        y = ffma2(f, y, k(0x1.fff692p-1f));
+    }
+    return f2pack(__int_as_float(__float_as_int(f2lo(y)) + (__float_as_int(f2lo(n)) << 23)),
+                  __int_as_float(__float_as_int(f2hi(y)) + (__float_as_int(f2hi(n)) << 23)));
 }
 
 template <typename T, int D>
@@ -123,11 +187,11 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t bar0 = su32(sm + L::OFF_BAR);
     auto full = [&](int e) { return bar0 + 8u * e; };
-    auto empty = [&](int e) { return bar0 + 8u * (L::NE + e); };
-    auto sfull = [&](int t) { return bar0 + 8u * (2 * L::NE + t); };
-    auto pfull = [&](int t) { return bar0 + 8u * (2 * L::NE + 2 + t); };
-    auto odone = [&](int t) { return bar0 + 8u * (2 * L::NE + 4 + t); };
-    const uint32_t drain = bar0 + 8u * (2 * L::NE + 6);
+    auto empty = [&](int e) { return bar0 + 8u * (L::NP + e); };
+    auto sfull = [&](int t) { return bar0 + 8u * (2 * L::NP + t); };
+    auto pfull = [&](int t, int half) { return bar0 + 8u * (2 * L::NP + 2 + 2 * t + half); };
+    auto odone = [&](int t) { return bar0 + 8u * (2 * L::NP + 6 + t); };
+    const uint32_t vhere = bar0 + 8u * (2 * L::NP + 8), vclear = vhere + 8, drain = vhere + 16;
     uint32_t* tmem_slot = (uint32_t*)(sm + L::OFF_BAR + L::NBAR * 8);
     volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
     int* last_slot = (int*)(tmem_slot + 2);
@@ -150,8 +214,10 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
     auto key0 = [&](int j) { return c.tile_of(v0 + j) * KT; };
 
     if (tid == 0) {
-        for (int e = 0; e < L::NE; e++) { bar_init(full(e), 1); bar_init(empty(e), 1); }
-        for (int t = 0; t < 2; t++) { bar_init(sfull(t), 1); bar_init(pfull(t), 128); bar_init(odone(t), 1); }
+        for (int e = 0; e < L::NP; e++) { bar_init(full(e), 1); bar_init(empty(e), 1); }
+        for (int t = 0; t < 2; t++) { bar_init(sfull(t), 1); bar_init(pfull(t, 0), 4); bar_init(pfull(t, 1), 4); bar_init(odone(t), 1); }
+        bar_init(vhere, 1);
+        bar_init(vclear, 32);
         bar_init(drain, 1);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -188,250 +254,302 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
 
-    if (warp == 0) {
-        // ring entry g: K (even) or V (odd) of tile g / 2
-        const int32_t* tab = p.batch.table + (int64_t)s * p.batch.max_pages;
-        int blk = 0;
-        bool ok = true, bad = false;
-        int g = 0;
-        for (; g < 2 * nt && ok; g++) {
-            const int j = g >> 1, e = g % L::NE;
-            if ((g & 1) == 0 && (j & 15) == 0) {   // the blocks of 16 tiles: lane = (tile, page)
-                const int jj = j + (lane >> 1);
-                blk = a.n_blocks;                   // past the pool: zero fill
-                if (jj < nt) {
-                    const int key = key0(jj) + PAGE * (lane & 1);
-                    if (key < c.len) {
-                        const int page = tab[key / PAGE];
-                        if (page >= 0 && page < p.kv.n_page) blk = ((page * p.kv.n_layer + p.kv.layer) * 2) * p.kv.n_head + h;
-                        else bad = true;
+    // Registers move from the TMA / MMA warps to the softmax: 128 x 104 + 256 x 200 = 384 x 168, the launch's own.
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+        if (warp == 0) {
+            // pair i: V of tile i - 1, then K of tile i (what the MMA warp needs together)
+            const int32_t* tab = p.batch.table + (int64_t)s * p.batch.max_pages;
+            int blk = 0;
+            bool ok = true, bad = false;
+            int i = 0;
+            uint32_t v0b = 0, v1b = 0;   // K blocks of the tile before (its V follows one pair later)
+            for (; i <= nt && nt > 0 && ok; i++) {
+                const int e = i % L::NP;
+                if ((i & 15) == 0) {   // the blocks of 16 tiles: lane = (tile, page)
+                    const int jj = i + (lane >> 1);
+                    blk = a.n_blocks;   // past the pool: zero fill
+                    if (jj < nt) {
+                        const int key = key0(jj) + PAGE * (lane & 1);
+                        if (key < c.len) {
+                            const int page = tab[key / PAGE];
+                            if (page >= 0 && page < p.kv.n_page) blk = ((page * p.kv.n_layer + p.kv.layer) * 2) * p.kv.n_head + h;
+                            else bad = true;
+                        }
                     }
                 }
+                const uint32_t k0b = __shfl_sync(0xffffffffu, blk, (i & 15) * 2), k1b = __shfl_sync(0xffffffffu, blk, (i & 15) * 2 + 1);
+                if (lane == 0) {
+                    ok = bar_wait_short(empty(e), ((uint32_t)(i / L::NP) & 1u) ^ 1u, abort_flag);
+                    if (ok) {
+                        bar_expect_tx(full(e), (i > 0 && i < nt ? 2 : 1) * L::ENTRY);
+                        const uint32_t dst = su32(sm + L::OFF_RING + (size_t)e * 2 * L::ENTRY);
+                        auto load = [&](uint32_t to, uint32_t b0, uint32_t b1) {
+#pragma unroll
+                            for (int at = 0; at < L::ATOMS; at++) {
+                                tma_load_3d(to + at * KT * L::RB, &a.map, at * 64, 0, (int)b0, full(e));
+                                tma_load_3d(to + at * KT * L::RB + PAGE * L::RB, &a.map, at * 64, 0, (int)b1, full(e));
+                            }
+                        };
+                        const uint32_t none = a.n_blocks;
+                        if (i > 0) load(dst, v0b == none ? none : v0b + p.kv.n_head, v1b == none ? none : v1b + p.kv.n_head);
+                        if (i < nt) load(dst + L::ENTRY, k0b, k1b);
+                    }
+                }
+                v0b = k0b;
+                v1b = k1b;
+                ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
             }
-            const int b0 = __shfl_sync(0xffffffffu, blk, (j & 15) * 2), b1 = __shfl_sync(0xffffffffu, blk, (j & 15) * 2 + 1);
+            if (bad) atomicOr(p.err, PAGED_BAD_PAGE);
             if (lane == 0) {
-                ok = bar_wait_short(empty(e), ((uint32_t)(g / L::NE) & 1u) ^ 1u, abort_flag);
-                if (ok) {
-                    bar_expect_tx(full(e), L::ENTRY);
-                    const uint32_t dst = su32(sm + L::OFF_RING + (size_t)e * L::ENTRY);
-                    const int dv = (g & 1) ? p.kv.n_head : 0;
+                if (!ok) {
+                    atomicOr(p.err, PAGED_WAIT);
+                    *abort_flag = 1;
+                    i--;   // its copies were not issued
+                }
+                // every copy has landed before the CTA may end
+                for (int k = i - 1; k >= 0 && k >= i - L::NP; k--)
+                    for (uint32_t it = 0; it < TC_POLL_LIMIT; it++)
+                        if (bar_try(full(k % L::NP), (uint32_t)(k / L::NP) & 1u)) break;
+            }
+        } else if (warp == 1) {
+            constexpr uint32_t HI = DESC_HI<L::RB>;
+            const uint32_t tm = __reduce_or_sync(0xffffffffu, tmem);   // (into a uniform register)
+            const uint32_t sq = su32(sm), ring = su32(sm + L::OFF_RING);
+            const bool cut = nt > 0 && key0(nt - 1) + KT > c.len;
+            // The loop is unrolled over the ring, so addresses and most phases are constants: this warp shares its
+            // scheduler with two softmax warps, and every instruction between two products is idle tensor time.
+            auto scores = [&](int t, int e) {   // S_t = Q_t K^T with the K of pair e
+                const uint32_t qd = desc_lo(sq + (uint32_t)t * 128 * D * 2, 16);
+                const uint32_t kd = desc_lo(ring + (uint32_t)(2 * e + 1) * L::ENTRY, 16);
+                const uint32_t st = tm + (uint32_t)t * KT;
+                mma_ss<HI, ID_S, false>(st, qd, kd);
 #pragma unroll
-                    for (int at = 0; at < L::ATOMS; at++) {
-                        tma_load_3d(dst + at * KT * L::RB, &a.map, at * 64, 0, b0 < a.n_blocks ? b0 + dv : b0, full(e));
-                        tma_load_3d(dst + at * KT * L::RB + PAGE * L::RB, &a.map, at * 64, 0, b1 < a.n_blocks ? b1 + dv : b1, full(e));
+                for (int kk = 1; kk < D / 16; kk++) {
+                    const uint32_t off = (kk / 4 * 128 * L::RB + 32 * (kk % 4)) >> 4;   // 64-dim block, 16 dims in it
+                    mma_ss<HI, ID_S, true>(st, qd + off, kd + off);
+                }
+                commit(sfull(t));
+            };
+            auto values = [&](int t, int e, uint32_t add, uint32_t parity) -> bool {   // O_t += P_t V, 64 keys at a time
+                const uint32_t vd = desc_lo(ring + (uint32_t)(2 * e) * L::ENTRY, KT * L::RB);
+                const uint32_t ot = tm + TM_O + (uint32_t)t * 128, pt = tm + (uint32_t)t * KT;
+#pragma unroll
+                for (int half = 0; half < 2; half++) {
+                    if (!wait_warp(pfull(t, half), parity, abort_flag)) return false;
+                    tc_fence_after();
+#pragma unroll
+                    for (int kk = half * KT / 32; kk < (half + 1) * KT / 32; kk++)
+                        mma_ts<HI, ID_O>(ot, pt + 8u * kk, vd + ((kk * 16 * L::RB) >> 4), kk == 0 ? add : 1u);
+                }
+                return true;
+            };
+            bool ok = nt == 0 || wait_warp(full(0), 0, abort_flag);
+            if (ok && nt > 0) {
+                scores(0, 0);
+                if (halves == 2) scores(1, 0);
+                commit(empty(0));
+            }
+            uint32_t ring_phase = 0;
+            for (int j0 = 0; j0 < nt && ok; j0 += L::NP, ring_phase ^= 1u) {
+#pragma unroll
+                for (int u = 0; u < L::NP; u++) {
+                    const int j = j0 + u, e = (u + 1) % L::NP;   // tile j's V and tile j + 1's K are pair j + 1
+                    if (j >= nt || !ok) break;
+                    ok = wait_warp(full(e), u == L::NP - 1 ? ring_phase ^ 1u : ring_phase, abort_flag);
+                    const bool more = j + 1 < nt;
+                    if (!more && cut && ok) {
+                        if (lane == 0) bar_arrive(vhere);
+                        ok = wait_warp(vclear, 0, abort_flag);
                     }
+                    ok = ok && values(0, e, (uint32_t)j, u & 1);
+                    if (!ok) break;
+                    if (more) scores(0, e);
+                    if (halves == 2) {
+                        ok = values(1, e, (uint32_t)j, u & 1);
+                        if (!ok) break;
+                        if (more) scores(1, e);
+                    }
+                    if (more) commit(empty(e));
                 }
             }
-            ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
-        }
-        if (bad) atomicOr(p.err, PAGED_BAD_PAGE);
-        if (lane == 0) {
+            if (ok && nt > 0) {
+                commit(odone(0));
+                if (halves == 2) commit(odone(1));
+            }
             if (!ok) {
-                atomicOr(p.err, PAGED_WAIT);
-                *abort_flag = 1;
-                g--;   // its copies were not issued
-            }
-            // every copy has landed before the CTA may end
-            for (int k = g - 1; k >= 0 && k >= g - L::NE; k--)
+                if (lane == 0) {
+                    atomicOr(p.err, PAGED_WAIT);
+                    *abort_flag = 1;
+                }
+                commit(drain);   // what was issued ends before the tensor memory is freed
                 for (uint32_t it = 0; it < TC_POLL_LIMIT; it++)
-                    if (bar_try(full(k % L::NE), (uint32_t)(k / L::NE) & 1u)) break;
-        }
-    } else if (warp == 1) {
-        const uint32_t sq = su32(sm), ring = su32(sm + L::OFF_RING);
-        bool ok = true;
-        auto wait_entry = [&](int g) { return bar_wait_short_warp(full(g % L::NE), (uint32_t)(g / L::NE) & 1u, abort_flag); };
-        auto scores = [&](int t, int j) {   // S_t = Q_t K_j^T
-            if (lane != 0) return;
-            const uint32_t k = ring + (uint32_t)((2 * j) % L::NE) * L::ENTRY, q = sq + (uint32_t)t * 128 * D * 2;
-#pragma unroll
-            for (int kk = 0; kk < D / 16; kk++) {
-                const uint32_t off = (uint32_t)(kk / 4) * 128 * L::RB + 32u * (kk % 4);   // 64-dim block, 16 dims in it
-                umma_f16(tmem + (uint32_t)t * KT, op_desc<L::RB>(q + off, 16, 8 * L::RB), op_desc<L::RB>(k + off, 16, 8 * L::RB),
-                         ID_S, (uint32_t)kk);
+                    if (__any_sync(0xffffffffu, bar_try(drain, 0))) break;
             }
-            umma_commit(sfull(t));
-            if (t == halves - 1) umma_commit(empty((2 * j) % L::NE));
-        };
-        auto values = [&](int t, int j) {   // O_t += P_t V_j
-            if (lane != 0) return;
-            const uint32_t v = ring + (uint32_t)((2 * j + 1) % L::NE) * L::ENTRY;
-#pragma unroll
-            for (int kk = 0; kk < KT / 16; kk++)
-                mma_ta(tmem + TM_O + (uint32_t)t * 128, tmem + (uint32_t)t * KT + 8u * kk,
-                       op_desc<L::RB>(v + (uint32_t)kk * 16 * L::RB, KT * L::RB, 8 * L::RB), ID_O, (uint32_t)(j | kk));
-            if (j == nt - 1) umma_commit(odone(t));
-            if (t == halves - 1) umma_commit(empty((2 * j + 1) % L::NE));
-        };
-        if (nt > 0) {
-            ok = wait_entry(0);
-            if (ok)
-                for (int t = 0; t < halves; t++) scores(t, 0);
-        }
-        for (int j = 0; j < nt && ok; j++) {
-            ok = wait_entry(2 * j + 1);
-            if (!ok) break;
-            const int k0 = key0(j);
-            if (k0 + KT > c.len) {   // V rows past the last key: whatever the page holds there, 0 here
-                uint8_t* v = sm + L::OFF_RING + (size_t)((2 * j + 1) % L::NE) * L::ENTRY;
-                const int r0 = c.len - k0, n16 = L::RB / 16;
+            __syncwarp();
+        } else if (warp == 2 && nt > 0 && key0(nt - 1) + KT > c.len) {
+            // V rows past the last key: whatever the page holds there becomes 0
+            const int e = nt % L::NP, n16 = L::RB / 16;
+            if (wait_warp(vhere, 0, abort_flag) && wait_warp(full(e), (uint32_t)(nt / L::NP) & 1u, abort_flag)) {
+                uint8_t* v = sm + L::OFF_RING + (size_t)e * 2 * L::ENTRY;
                 for (int at = 0; at < L::ATOMS; at++)
-                    for (int i = r0 * n16 + lane; i < KT * n16; i += 32)
+                    for (int i = (c.len - key0(nt - 1)) * n16 + lane; i < KT * n16; i += 32)
                         *(uint4*)(v + (size_t)at * KT * L::RB + i * 16) = make_uint4(0, 0, 0, 0);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-            }
-            for (int t = 0; t < halves && ok; t++) {
-                ok = bar_wait_short_warp(pfull(t), (uint32_t)j & 1u, abort_flag);
-                if (!ok) break;
-                tc_fence_after();
-                values(t, j);
-                if (j + 1 < nt) {
-                    if (t == 0) ok = wait_entry(2 * j + 2);
-                    if (ok) scores(t, j + 1);
-                }
+                bar_arrive(vclear);
             }
         }
-        if (lane == 0 && !ok) {
-            atomicOr(p.err, PAGED_WAIT);
-            *abort_flag = 1;
-            umma_commit(drain);   // what was issued ends before the tensor memory is freed
-            for (uint32_t it = 0; it < TC_POLL_LIMIT; it++)
-                if (bar_try(drain, 0)) break;
-        }
-    } else if (warp >= 4 && (warp - 4) / 4 < halves) {
-        const int t = (warp - 4) / 4, q = warp & 3, r = 128 * t + 32 * q + lane;
-        const uint32_t tl = tmem + ((uint32_t)(32 * q) << 16), ts = tl + (uint32_t)t * KT, to = tl + TM_O + (uint32_t)t * 128;
-        const int pos = c.total - c.n + (c.r0 + min(r, c.rows - 1)) / a.group;
-        const int see_hi = min(c.len, pos + 1), see_lo = p.window ? pos - p.window + 1 : 0;
-        float mref = NEG_INF, l = 0.0f;
-        bool ok = true;
-        for (int j = 0; j < nt && ok; j++) {
-            if (!bar_wait_short_warp(sfull(t), (uint32_t)j & 1u, abort_flag)) { ok = false; break; }
+        tc_fence_before();
+        __syncthreads();
+        if (warp == 1) {
             tc_fence_after();
-            uint32_t x[4][32];
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+        if ((warp - 4) / 4 < halves) {
+            const int t = (warp - 4) / 4, q = warp & 3, r = 128 * t + 32 * q + lane;
+            const uint32_t tl = tmem + ((uint32_t)(32 * q) << 16), ts = tl + (uint32_t)t * KT, to = tl + TM_O + (uint32_t)t * 128;
+            const int pos = c.total - c.n + (c.r0 + min(r, c.rows - 1)) / a.group;
+            const int see_hi = min(c.len, pos + 1), see_lo = p.window ? pos - p.window + 1 : 0;
+            float mref = NEG_INF, l = 0.0f;
+            bool ok = true;
+            for (int j = 0; j < nt && ok; j++) {
+                if (!bar_wait_short_warp(sfull(t), (uint32_t)j & 1u, abort_flag)) { ok = false; break; }
+                tc_fence_after();
+                uint32_t x[4][32];
 #pragma unroll
-            for (int k = 0; k < 4; k++) tmem_ld32(ts + 32u * k, x[k]);
-            tmem_wait_ld();
+                for (int k = 0; k < 4; k++) tmem_ld32(ts + 32u * k, x[k]);
+                tmem_wait_ld();
 #pragma unroll
-            for (int k = 0; k < 4; k++) bind32(x[k]);
-            const int k0 = key0(j);
-            if (!(k0 + KT <= c.np || (k0 + KT <= min(c.len, c.p0 + 1) && (!p.window || k0 > c.p1 - p.window)))) {
+                for (int k = 0; k < 4; k++) bind32(x[k]);
+                const int k0 = key0(j);
+                const bool whole = k0 + KT <= c.np || (k0 + KT <= min(c.len, c.p0 + 1) && (!p.window || k0 > c.p1 - p.window));
+                if (!whole) {
 #pragma unroll
-                for (int i = 0; i < KT; i++) {
-                    const int key = k0 + i;
-                    if (!(key < c.np || (key < see_hi && key >= see_lo))) x[i / 32][i % 32] = __float_as_uint(NEG_INF);
+                    for (int i = 0; i < KT; i++) {
+                        const int key = k0 + i;
+                        if (!(key < c.np || (key < see_hi && key >= see_lo))) x[i / 32][i % 32] = __float_as_uint(NEG_INF);
+                    }
+                    asm volatile("" ::: "memory");   // keeps the tests out of the tiles that need none
                 }
-            }
-            float mx[4];
+                float mx[4];
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                mx[k] = __uint_as_float(x[k][0]);
+                for (int k = 0; k < 4; k++) {
+                    mx[k] = __uint_as_float(x[k][0]);
 #pragma unroll
-                for (int i = 1; i < 32; i++) mx[k] = fmaxf(mx[k], __uint_as_float(x[k][i]));
-            }
-            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.c;
-            // raise the reference maximum of the warp's rows when one of them needs it
-            if (__any_sync(0xffffffffu, top > mref + TAU)) {
-                const float up = fmaxf(mref, top);
-                if (j > 0) {   // (O is at rest: S of this tile was committed after the PV before it)
-                    const float f = up == NEG_INF ? 1.0f : ex2(mref - up);
-                    l *= f;
+                    for (int i = 1; i < 31; i += 2) mx[k] = max3(mx[k], __uint_as_float(x[k][i]), __uint_as_float(x[k][i + 1]));
+                    mx[k] = fmaxf(mx[k], __uint_as_float(x[k][31]));
+                }
+                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.c;
+                // raise the reference maximum of the warp's rows when one of them needs it
+                if (__any_sync(0xffffffffu, top > mref + TAU)) {
+                    const float up = fmaxf(mref, top);
+                    if (j > 0) {   // (O is at rest: S of this tile was committed after the PV before it)
+                        const float f = up == NEG_INF ? 1.0f : ex2(mref - up);
+                        l *= f;
 #pragma unroll 1
-                    for (int d = 0; d < D; d += 32) {
-                        uint32_t o[32];
+                        for (int d = 0; d < D; d += 32) {
+                            uint32_t o[32];
+                            tmem_ld32(to + (uint32_t)d, o);
+                            tmem_wait_ld();
+                            bind32(o);
+#pragma unroll
+                            for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                            tmem_st32(to + (uint32_t)d, o);
+                        }
+                        tmem_wait_st();
+                    }
+                    mref = up;
+                }
+                const float ref = mref == NEG_INF ? 0.0f : -mref;
+                const uint64_t c2 = f2pack(a.c, a.c), ref2 = f2pack(ref, ref);
+                uint64_t sum = 0;   // two partial sums
+                auto weights = [&](auto tested) {
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        uint32_t w[16];
+#pragma unroll
+                        for (int i = 0; i < 16; i++) {
+                            uint64_t e = ffma2(f2pack(__uint_as_float(x[k][2 * i]), __uint_as_float(x[k][2 * i + 1])), c2, ref2);
+                            if (!decltype(tested)::value && i % EVERY == EVERY - 1) e = ex2_pair<T>(e);
+                            else e = f2pack(ex2(f2lo(e)), ex2(f2hi(e)));
+                            sum = fadd2(sum, e);
+                            w[i] = pack2<T>(f2lo(e), f2hi(e));
+                        }
+                        tmem_st16u(ts + 16u * k, w);
+                        if (k & 1) {   // half of the tile's weights: their product may start
+                            tmem_wait_st();
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) bar_arrive(pfull(t, k >> 1));
+                        }
+                    }
+                };
+                if (whole) weights(std::false_type{});
+                else weights(std::true_type{});
+                l += f2lo(sum) + f2hi(sum);
+            }
+            if (ok && nt > 0) ok = bar_wait_short_warp(odone(t), 0, abort_flag);
+            tc_fence_after();
+            const bool mine = r < c.rows;
+            const int tok = (c.r0 + r) / a.group, head = h * a.group + (c.r0 + r) % a.group;
+            const int64_t row = c.row0 + tok;
+            const int64_t unit = ((int64_t)s * a.tiles + tile) * p.kv.n_head + h;
+            float* part = p.part + unit * a.n_split * (ROWS * (D + 2));
+            const float il = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+            if (ok) {
+#pragma unroll 1
+                for (int d = 0; d < D; d += 32) {
+                    uint32_t o[32];
+                    if (nt > 0) {
                         tmem_ld32(to + (uint32_t)d, o);
                         tmem_wait_ld();
                         bind32(o);
+                    } else {
 #pragma unroll
-                        for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                        tmem_st32(to + (uint32_t)d, o);
+                        for (int i = 0; i < 32; i++) o[i] = 0;
                     }
-                    tmem_wait_st();
-                }
-                mref = up;
-            }
-            const float ref = mref == NEG_INF ? 0.0f : -mref;
-            float sum[2] = {0.0f, 0.0f};
+                    if (!mine) continue;
+                    if (n_act == 1) {
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                uint32_t w[16];
+                        for (int i = 0; i < 32; i += 8) {
+                            float y[8];
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const float w0 = ex2(fmaf(__uint_as_float(x[k][2 * i]), a.c, ref));
-                    const float w1 = ex2(fmaf(__uint_as_float(x[k][2 * i + 1]), a.c, ref));
-                    sum[0] += w0;
-                    sum[1] += w1;
-                    w[i] = pack2<T>(w0, w1);
-                }
-                tmem_st16u(ts + 16u * k, w);
-            }
-            l += sum[0] + sum[1];
-            tmem_wait_st();
-            tc_fence_before();
-            bar_arrive(pfull(t));
-        }
-        if (ok && nt > 0) ok = bar_wait_short_warp(odone(t), 0, abort_flag);
-        tc_fence_after();
-        const bool mine = r < c.rows;
-        const int tok = (c.r0 + r) / a.group, head = h * a.group + (c.r0 + r) % a.group;
-        const int64_t row = c.row0 + tok;
-        const int64_t unit = ((int64_t)s * a.tiles + tile) * p.kv.n_head + h;
-        float* part = p.part + unit * a.n_split * (ROWS * (D + 2));
-        const float il = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-        if (ok) {
-#pragma unroll 1
-            for (int d = 0; d < D; d += 32) {
-                uint32_t o[32];
-                if (nt > 0) {
-                    tmem_ld32(to + (uint32_t)d, o);
-                    tmem_wait_ld();
-                    bind32(o);
-                } else {
+                            for (int k = 0; k < 8; k++) y[k] = __uint_as_float(o[i + k]) * il;
+                            T* dst = (T*)p.out + row * p.out_stride + (int64_t)head * D + d + i;
+                            const uint4 u = make_uint4(pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]), pack2<T>(y[4], y[5]), pack2<T>(y[6], y[7]));
+                            if (a.vec_out) {
+                                *(uint4*)dst = u;
+                            } else {
+                                const T* e = (const T*)&u;
 #pragma unroll
-                    for (int i = 0; i < 32; i++) o[i] = 0;
-                }
-                if (!mine) continue;
-                if (n_act == 1) {
-#pragma unroll
-                    for (int i = 0; i < 32; i += 8) {
-                        float y[8];
-#pragma unroll
-                        for (int k = 0; k < 8; k++) y[k] = __uint_as_float(o[i + k]) * il;
-                        T* dst = (T*)p.out + row * p.out_stride + (int64_t)head * D + d + i;
-                        const uint4 u = make_uint4(pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]), pack2<T>(y[4], y[5]), pack2<T>(y[6], y[7]));
-                        if (a.vec_out) {
-                            *(uint4*)dst = u;
-                        } else {
-                            const T* e = (const T*)&u;
-#pragma unroll
-                            for (int k = 0; k < 8; k++) dst[k] = e[k];
+                                for (int k = 0; k < 8; k++) dst[k] = e[k];
+                            }
                         }
-                    }
-                } else {
-                    float* dst = part + ((int64_t)sp * ROWS + r) * D + d;
+                    } else {
+                        float* dst = part + ((int64_t)sp * ROWS + r) * D + d;
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4)
-                        *(uint4*)(dst + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                        for (int i = 0; i < 32; i += 4)
+                            *(uint4*)(dst + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                    }
                 }
+                if (mine) {
+                    if (n_act > 1)
+                        *(float2*)(part + (int64_t)a.n_split * ROWS * D + 2 * ((int64_t)sp * ROWS + r)) = make_float2(mref, l);
+                    else if (p.lse)
+                        p.lse[row * p.n_q_head + head] = mref == NEG_INF ? NEG_INF : (mref + log2f(l)) * LN2;
+                }
+            } else if (lane == 0) {
+                atomicOr(p.err, PAGED_WAIT);
+                *abort_flag = 1;
             }
-            if (mine) {
-                if (n_act > 1)
-                    *(float2*)(part + (int64_t)a.n_split * ROWS * D + 2 * ((int64_t)sp * ROWS + r)) = make_float2(mref, l);
-                else if (p.lse)
-                    p.lse[row * p.n_q_head + head] = mref == NEG_INF ? NEG_INF : (mref + log2f(l)) * LN2;
-            }
-        } else if (lane == 0) {
-            atomicOr(p.err, PAGED_WAIT);
-            *abort_flag = 1;
         }
+        tc_fence_before();
+        __syncthreads();
+    if (n_act > 1)
+        join_splits<T, D, ROWS, 256>(p, c, s, tile, h, a.group, a.tiles, a.n_split, n_act, a.vec_out, tid - 128, last_slot);
     }
-    tc_fence_before();
-    __syncthreads();
-    if (warp == 1) {
-        tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
-    }
-    if (n_act > 1) join_splits<T, D, ROWS, THREADS>(p, c, s, tile, h, a.group, a.tiles, a.n_split, n_act, a.vec_out, last_slot);
 }
 
 template <typename F>

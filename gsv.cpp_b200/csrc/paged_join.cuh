@@ -82,20 +82,19 @@ __device__ __forceinline__ void store_out(const ChunkAttnParams& p, bool vec, in
     }
 }
 
-// The whole CTA, after its split's results are in p.part ([split][ROWS][D] unnormalised outputs, then
+// THREADS threads of the CTA (tid among them; barrier 1), after their split's results are in p.part ([split][ROWS][D] unnormalised outputs, then
 // [split][ROWS] {maximum (log2 units), sum}): the CTA that arrives last joins the n_act splits in their order,
 // so the result does not depend on the arrival order, and clears the counter.
 template <typename T, int D, int ROWS, int THREADS>
 __device__ __forceinline__ void join_splits(const ChunkAttnParams& p, const ChunkRange& c, int s, int tile, int h, int group,
-                                            int tiles, int n_split, int n_act, bool vec, int* last) {
+                                            int tiles, int n_split, int n_act, bool vec, int tid, int* last) {
     const int64_t unit = ((int64_t)s * tiles + tile) * p.kv.n_head + h;
     const float* part_o = p.part + unit * n_split * (ROWS * (D + 2));
     const float* part_ml = part_o + (int64_t)n_split * ROWS * D;
-    const int tid = threadIdx.x;
     __threadfence();
-    __syncthreads();
+    asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory");
     if (tid == 0) *last = atomicAdd(p.arrived + unit, 1) == n_act - 1;
-    __syncthreads();
+    asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory");
     if (!*last) return;
     __threadfence();
     if (tid == 0) p.arrived[unit] = 0;
