@@ -10,6 +10,8 @@
 // tiles in turn, each with its own cp.async ring, running maximum, sum and output (in registers), so no
 // barrier stands inside the loop; they are joined at the end in warp order. With several splits the CTA that
 // arrives last joins the splits' results in split order (a fixed order: results do not depend on timing).
+// Everything is transposed: S^T = K Q^T with 16 keys and 8 query rows per product, O^T = V^T P^T, because few
+// rows are the rule here (one decoding token of one head is one row) and 8 is the smaller side of mma.sync.
 // F16 / BF16 products run on mma.m16n8k16 with the weights split into two 16-bit parts (w = hi + lo), so
 // rounding them costs nothing against the output's own rounding; F32 ones on mma.m16n8k8.tf32 with both
 // operands in two parts (three products), which leaves an error near 2^-22. Sums, maxima and outputs are f32.
@@ -24,6 +26,8 @@ namespace gsvcu {
 namespace {
 
 constexpr int NW = 4;   // warps per CTA
+// Keys of one warp's tile: 8 KB of K and V (16 KB for wide F32 rows), at least the 16 of one product.
+__host__ __device__ constexpr int key_tile(int dim, int size) { return size == 2 ? 2048 / dim : dim == 32 ? 32 : 16; }
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool in) {
@@ -85,19 +89,34 @@ __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) 
     if (!(fabsf(rest) < __builtin_huge_valf())) lo = 0;
 }
 
+// [keys][rows] 8 x 8 block of 16-bit values, as a product leaves it, to [rows][keys], as the next one reads it.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+// The same for a pair of f32 values per lane: high and low halves apart.
+__device__ __forceinline__ void transpose8(float& x, float& y) {
+    const uint32_t a = __float_as_uint(x), b = __float_as_uint(y);
+    const uint32_t hi = transpose8(__byte_perm(a, b, 0x7632)), lo = transpose8(__byte_perm(a, b, 0x5410));
+    x = __uint_as_float(__byte_perm(lo, hi, 0x5410));
+    y = __uint_as_float(__byte_perm(lo, hi, 0x7632));
+}
+
 // Key tile of one warp's ring stage: KT keys of K, then of V, rows of RB bytes in 16-byte pieces; piece c of
 // row r lies at c ^ swz(r), so the 8 rows of a matrix fragment fall into different banks.
-template <typename T, int D, int MT>
+template <typename T, int D, int NT>
 struct Cfg {
     static constexpr int RB = D * (int)sizeof(T);
     static constexpr int PIECES = RB / 16;
-    static constexpr int KT = sizeof(T) == 4 ? (D == 32 ? 32 : 16) : 2048 / D;
+    static constexpr int KT = key_tile(D, (int)sizeof(T));
     static constexpr int STAGES = RB > 256 ? 2 : 3;
-    static constexpr int ROWS = 16 * MT;
+    static constexpr int ROWS = 8 * NT;
     static constexpr int TILE = KT * RB;   // bytes of K (or V)
     static constexpr int QPLANES = sizeof(T) == 4 ? 2 : 1;   // F32: high and low parts
+    static constexpr int OSTR = D + 4;     // row stride of the outputs to be joined: lanes on different banks
     static constexpr size_t RING = (size_t)NW * STAGES * 2 * TILE;
-    static constexpr size_t JOIN = (size_t)NW * ROWS * D * 4;   // reuses the ring
+    static constexpr size_t JOIN = (size_t)NW * ROWS * OSTR * 4;   // reuses the ring
     static constexpr size_t OFF_Q = RING > JOIN ? RING : JOIN;
     static constexpr size_t OFF_ML = OFF_Q + (size_t)QPLANES * ROWS * RB;
     static constexpr size_t SMEM = OFF_ML + (size_t)NW * ROWS * 8 + 16;
@@ -115,9 +134,9 @@ struct SplitArgs {
     bool vec_q, vec_out;
 };
 
-template <typename T, int D, int MT>
+template <typename T, int D, int NT>
 __global__ void __launch_bounds__(NW * 32) k_chunk_attn(SplitArgs a) {
-    using C = Cfg<T, D, MT>;
+    using C = Cfg<T, D, NT>;
     constexpr int KT = C::KT, RB = C::RB, ROWS = C::ROWS, ST = C::STAGES;
     constexpr bool F32 = sizeof(T) == 4;
     extern __shared__ __align__(128) uint8_t sm[];
@@ -201,196 +220,227 @@ __global__ void __launch_bounds__(NW * 32) k_chunk_attn(SplitArgs a) {
     for (int i = 0; i < ST - 1; i++) fetch(i);
     __syncthreads();   // queries
 
-    // this lane's rows: 2 MT of them (fragment rows lane / 4 and + 8)
-    int see_lo[MT][2], see_hi[MT][2];
+    // this lane's rows: 2 of every 8 (fragment columns 2 (lane % 4) and the next)
+    const int col = (lane & 3) * 2, kr = lane >> 2;   // kr: the lane's key (or dim) in a fragment, and + 8
+    int see_lo[NT][2], see_hi[NT][2];
 #pragma unroll
-    for (int mt = 0; mt < MT; mt++)
+    for (int b = 0; b < NT; b++)
 #pragma unroll
         for (int e = 0; e < 2; e++) {
-            const int pos = total - n + (r0 + min(rows - 1, mt * 16 + lane / 4 + 8 * e)) / a.group;
-            see_hi[mt][e] = min(len, pos + 1);
-            see_lo[mt][e] = p.window ? pos - p.window + 1 : 0;
+            const int pos = total - n + (r0 + min(rows - 1, b * 8 + col + e)) / a.group;
+            see_hi[b][e] = min(len, pos + 1);
+            see_lo[b][e] = p.window ? pos - p.window + 1 : 0;
         }
-    float m[MT][2], l[MT][2], o[MT][D / 8][4];
+    float m[NT][2], l[NT][2], o[NT][D / 16][4];
 #pragma unroll
-    for (int mt = 0; mt < MT; mt++) {
-        m[mt][0] = m[mt][1] = NEG_INF;
-        l[mt][0] = l[mt][1] = 0.0f;
+    for (int b = 0; b < NT; b++) {
+        m[b][0] = m[b][1] = NEG_INF;
+        l[b][0] = l[b][1] = 0.0f;
 #pragma unroll
-        for (int d = 0; d < D / 8; d++) o[mt][d][0] = o[mt][d][1] = o[mt][d][2] = o[mt][d][3] = 0.0f;
+        for (int d = 0; d < D / 16; d++) o[b][d][0] = o[b][d][1] = o[b][d][2] = o[b][d][3] = 0.0f;
     }
     const uint32_t sqa = smem_addr(sq);
+    // F16 / BF16 query fragments: in registers where they are few, else read again for every tile
+    constexpr bool QREG = !F32 && NT * D <= 256;
+    uint32_t qr[QREG ? NT : 1][QREG ? D / 16 : 1][2];
+    auto query = [&](int b, int kk, uint32_t (&q)[4]) {   // dims 16 kk .. 16 kk + 31 of rows 8 b .. 8 b + 7
+        ldsm4(sqa + at<RB>(b * 8 + (lane & 7), kk * 2 + (lane >> 3)), q);
+    };
+    if constexpr (QREG) {
+#pragma unroll
+        for (int b = 0; b < NT; b++)
+#pragma unroll
+            for (int kk = 0; kk < D / 16; kk += 2) {
+                uint32_t q[4];
+                query(b, kk, q);
+                qr[b][kk][0] = q[0]; qr[b][kk][1] = q[1];
+                qr[b][kk + 1][0] = q[2]; qr[b][kk + 1][1] = q[3];
+            }
+    }
 
     for (int i = 0; i < mine; i++) {
         asm volatile("cp.async.wait_group %0;" ::"n"(ST - 2) : "memory");
         __syncwarp();
         const uint32_t kt = ring + (uint32_t)((i % ST) * 2 * C::TILE), vt = kt + C::TILE;
-        float sc[MT][KT / 8][4];
+        float sc[NT][KT / 16][4];   // [key kr, + 8][row col, + 1]
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++)
+        for (int b = 0; b < NT; b++)
 #pragma unroll
-            for (int j = 0; j < KT / 8; j++) sc[mt][j][0] = sc[mt][j][1] = sc[mt][j][2] = sc[mt][j][3] = 0.0f;
+            for (int j = 0; j < KT / 16; j++) sc[b][j][0] = sc[b][j][1] = sc[b][j][2] = sc[b][j][3] = 0.0f;
         if constexpr (!F32) {
 #pragma unroll
-            for (int kk = 0; kk < D / 16; kk++) {
-                uint32_t qa[MT][4];
+            for (int kk = 0; kk < D / 16; kk += 2) {
+                uint32_t qa[NT][4];
 #pragma unroll
-                for (int mt = 0; mt < MT; mt++) ldsm4(sqa + at<RB>(mt * 16 + (lane & 15), kk * 2 + (lane >> 4)), qa[mt]);
-#pragma unroll
-                for (int j = 0; j < KT / 16; j++) {
-                    uint32_t kb[4];
-                    ldsm4(kt + at<RB>(j * 16 + (lane & 7) + ((lane >> 4) << 3), kk * 2 + ((lane >> 3) & 1)), kb);
-#pragma unroll
-                    for (int mt = 0; mt < MT; mt++) {
-                        mma16(T(), sc[mt][2 * j], qa[mt], kb[0], kb[1]);
-                        mma16(T(), sc[mt][2 * j + 1], qa[mt], kb[2], kb[3]);
+                for (int b = 0; b < NT; b++) {
+                    if constexpr (QREG) {
+                        qa[b][0] = qr[b][kk][0]; qa[b][1] = qr[b][kk][1];
+                        qa[b][2] = qr[b][kk + 1][0]; qa[b][3] = qr[b][kk + 1][1];
+                    } else {
+                        query(b, kk, qa[b]);
                     }
                 }
+#pragma unroll
+                for (int j = 0; j < KT / 16; j++)
+#pragma unroll
+                    for (int k2 = 0; k2 < 2; k2++) {
+                        uint32_t ka[4];
+                        ldsm4(kt + at<RB>(j * 16 + (lane & 15), (kk + k2) * 2 + (lane >> 4)), ka);
+#pragma unroll
+                        for (int b = 0; b < NT; b++) mma16(T(), sc[b][j], ka, qa[b][2 * k2], qa[b][2 * k2 + 1]);
+                    }
             }
         } else {
             const uint32_t w4 = (lane & 3) * 4;
-            float low[MT][KT / 8][4];   // the two products with a low part, added at the end
+            float low[NT][KT / 16][4];   // the two products with a low part, added at the end
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++)
+            for (int b = 0; b < NT; b++)
 #pragma unroll
-                for (int j = 0; j < KT / 8; j++) low[mt][j][0] = low[mt][j][1] = low[mt][j][2] = low[mt][j][3] = 0.0f;
+                for (int j = 0; j < KT / 16; j++) low[b][j][0] = low[b][j][1] = low[b][j][2] = low[b][j][3] = 0.0f;
 #pragma unroll
             for (int kk = 0; kk < D / 8; kk++) {
-                uint32_t qh[MT][4], ql[MT][4];
+                uint32_t qh[NT][2], ql[NT][2];
 #pragma unroll
-                for (int mt = 0; mt < MT; mt++)
+                for (int b = 0; b < NT; b++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const uint32_t x = at<RB>(mt * 16 + lane / 4 + 8 * (e & 1), kk * 2 + (e >> 1)) + w4;
-                        qh[mt][e] = __float_as_uint(lds(sqa + x));
-                        ql[mt][e] = __float_as_uint(lds(sqa + ROWS * RB + x));
+                    for (int e = 0; e < 2; e++) {
+                        const uint32_t x = at<RB>(b * 8 + kr, kk * 2 + e) + w4;
+                        qh[b][e] = __float_as_uint(lds(sqa + x));
+                        ql[b][e] = __float_as_uint(lds(sqa + ROWS * RB + x));
                     }
 #pragma unroll
-                for (int j = 0; j < KT / 8; j++) {
-                    uint32_t bh[2], bl[2];
+                for (int j = 0; j < KT / 16; j++) {
+                    uint32_t kh[4], kl[4];
 #pragma unroll
-                    for (int e = 0; e < 2; e++)
-                        split_tf32(lds(kt + at<RB>(j * 8 + lane / 4, kk * 2 + e) + w4), bh[e], bl[e]);
+                    for (int e = 0; e < 4; e++)
+                        split_tf32(lds(kt + at<RB>(j * 16 + kr + 8 * (e & 1), kk * 2 + (e >> 1)) + w4), kh[e], kl[e]);
 #pragma unroll
-                    for (int mt = 0; mt < MT; mt++) {
-                        mma8(low[mt][j], ql[mt], bh[0], bh[1]);
-                        mma8(low[mt][j], qh[mt], bl[0], bl[1]);
-                        mma8(sc[mt][j], qh[mt], bh[0], bh[1]);
+                    for (int b = 0; b < NT; b++) {
+                        mma8(low[b][j], kl, qh[b][0], qh[b][1]);
+                        mma8(low[b][j], kh, ql[b][0], ql[b][1]);
+                        mma8(sc[b][j], kh, qh[b][0], qh[b][1]);
                     }
                 }
             }
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++)
+            for (int b = 0; b < NT; b++)
 #pragma unroll
-                for (int j = 0; j < KT / 8; j++)
+                for (int j = 0; j < KT / 16; j++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) sc[mt][j][e] += low[mt][j][e];
+                    for (int e = 0; e < 4; e++) sc[b][j][e] += low[b][j][e];
         }
         // scores in log2 units; keys that a row must not see to -infinity
         const int k0 = key0(i);
         const bool whole = k0 + KT <= np || (k0 + KT <= min(len, p0 + 1) && (!p.window || k0 > p1 - p.window));
-        float mx[MT][2];
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++) {
-            mx[mt][0] = mx[mt][1] = NEG_INF;
+        for (int b = 0; b < NT; b++)
 #pragma unroll
-            for (int j = 0; j < KT / 8; j++)
+            for (int j = 0; j < KT / 16; j++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    float x = sc[mt][j][e] * a.c;
-                    if (!whole) {
-                        const int key = k0 + j * 8 + (lane & 3) * 2 + (e & 1);
-                        if (!(key < np || (key < see_hi[mt][e >> 1] && key >= see_lo[mt][e >> 1]))) x = NEG_INF;
+                for (int e = 0; e < 4; e++) sc[b][j][e] *= a.c;
+        if (!whole) {
+#pragma unroll
+            for (int b = 0; b < NT; b++)
+#pragma unroll
+                for (int j = 0; j < KT / 16; j++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int key = k0 + j * 16 + kr + 8 * (e >> 1);
+                        if (!(key < np || (key < see_hi[b][e & 1] && key >= see_lo[b][e & 1]))) sc[b][j][e] = NEG_INF;
                     }
-                    sc[mt][j][e] = x;
-                    mx[mt][e >> 1] = fmaxf(mx[mt][e >> 1], x);
-                }
+            asm volatile("" ::: "memory");   // keeps the tests out of the tiles that need none
         }
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++)
+        for (int b = 0; b < NT; b++)
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-                float x = mx[mt][e];
-                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-                const float top = fmaxf(m[mt][e], x);
-                if (top > m[mt][e]) {
-                    const float f = ex2(m[mt][e] - top);
-                    l[mt][e] *= f;
+                float top = fmaxf(sc[b][0][e], sc[b][0][e + 2]);
 #pragma unroll
-                    for (int d = 0; d < D / 8; d++) {
-                        o[mt][d][2 * e] *= f;
-                        o[mt][d][2 * e + 1] *= f;
+                for (int j = 1; j < KT / 16; j++) top = fmaxf(top, fmaxf(sc[b][j][e], sc[b][j][e + 2]));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                if (top > m[b][e]) {
+                    const float f = ex2(m[b][e] - top);
+                    l[b][e] *= f;
+#pragma unroll
+                    for (int d = 0; d < D / 16; d++) {
+                        o[b][d][e] *= f;
+                        o[b][d][e + 2] *= f;
                     }
-                    m[mt][e] = top;
+                    m[b][e] = top;
                 }
-                const float ref = top == NEG_INF ? 0.0f : top;
+                const float ref = m[b][e] == NEG_INF ? 0.0f : m[b][e];
 #pragma unroll
-                for (int j = 0; j < KT / 8; j++)
+                for (int j = 0; j < KT / 16; j++)
 #pragma unroll
                     for (int g = 0; g < 2; g++) {
-                        const float w = ex2(sc[mt][j][2 * e + g] - ref);
-                        sc[mt][j][2 * e + g] = w;
-                        l[mt][e] += w;
+                        const float w = ex2(sc[b][j][e + 2 * g] - ref);
+                        sc[b][j][e + 2 * g] = w;
+                        l[b][e] += w;
                     }
             }
         if constexpr (!F32) {
 #pragma unroll
-            for (int kk = 0; kk < KT / 16; kk++) {
-                uint32_t wh[MT][4], wl[MT][4];
+            for (int j = 0; j < KT / 16; j++) {
+                uint32_t wh[NT][2], wl[NT][2];
 #pragma unroll
-                for (int mt = 0; mt < MT; mt++)
+                for (int b = 0; b < NT; b++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        wh[mt][e] = pack_split(T(), sc[mt][2 * kk + (e >> 1)][2 * (e & 1)], sc[mt][2 * kk + (e >> 1)][2 * (e & 1) + 1], wl[mt][e]);
+                    for (int g = 0; g < 2; g++) {
+                        uint32_t rest;
+                        wh[b][g] = transpose8(pack_split(T(), sc[b][j][2 * g], sc[b][j][2 * g + 1], rest));
+                        wl[b][g] = transpose8(rest);
+                    }
 #pragma unroll
                 for (int d = 0; d < D / 16; d++) {
-                    uint32_t vb[4];
-                    ldsm4t(vt + at<RB>(kk * 16 + (lane & 15), d * 2 + (lane >> 4)), vb);
+                    uint32_t va[4];
+                    ldsm4t(vt + at<RB>(j * 16 + (lane & 7) + ((lane >> 4) << 3), d * 2 + ((lane >> 3) & 1)), va);
 #pragma unroll
-                    for (int mt = 0; mt < MT; mt++) {
-                        mma16(T(), o[mt][2 * d], wl[mt], vb[0], vb[1]);
-                        mma16(T(), o[mt][2 * d], wh[mt], vb[0], vb[1]);
-                        mma16(T(), o[mt][2 * d + 1], wl[mt], vb[2], vb[3]);
-                        mma16(T(), o[mt][2 * d + 1], wh[mt], vb[2], vb[3]);
+                    for (int b = 0; b < NT; b++) {
+                        mma16(T(), o[b][d], va, wl[b][0], wl[b][1]);
+                        mma16(T(), o[b][d], va, wh[b][0], wh[b][1]);
                     }
                 }
             }
         } else {
-            // the fragment's k index is a key: index lane % 4 takes key 2 (lane % 4), lane % 4 + 4 the next one,
-            // as the score fragment holds them. A tile's products are summed by themselves and then added to o
-            // (the tensor core's additions truncate: over a long cache that would drift, rounded ones do not).
-            uint32_t wh[KT / 8][MT][4], wl[KT / 8][MT][4];
+            // the fragment's k index is a key: index lane % 4 takes key 2 (lane % 4), lane % 4 + 4 the next one, as the
+            // transposed weights lie. A tile's products are summed by themselves and then added to o (the tensor
+            // core's additions truncate: over a long cache that would drift, rounded ones do not).
+            uint32_t wh[NT][KT / 8][2], wl[NT][KT / 8][2];
 #pragma unroll
-            for (int j = 0; j < KT / 8; j++)
-#pragma unroll
-                for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) split_tf32(sc[mt][j][2 * (e & 1) + (e >> 1)], wh[j][mt][e], wl[j][mt][e]);
-#pragma unroll
-            for (int d = 0; d < D / 8; d++) {
-                float x[MT][4];
-#pragma unroll
-                for (int mt = 0; mt < MT; mt++) x[mt][0] = x[mt][1] = x[mt][2] = x[mt][3] = 0.0f;
+            for (int b = 0; b < NT; b++)
 #pragma unroll
                 for (int j = 0; j < KT / 8; j++) {
-                    uint32_t bh[2], bl[2];
+                    float x = sc[b][j / 2][2 * (j & 1)], y = sc[b][j / 2][2 * (j & 1) + 1];
+                    transpose8(x, y);
+                    split_tf32(x, wh[b][j][0], wl[b][j][0]);
+                    split_tf32(y, wh[b][j][1], wl[b][j][1]);
+                }
 #pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        const int dim = d * 8 + lane / 4;
-                        split_tf32(lds(vt + at<RB>(j * 8 + (lane & 3) * 2 + e, dim / 4) + (dim & 3) * 4), bh[e], bl[e]);
+            for (int d = 0; d < D / 16; d++) {
+                float x[NT][4];
+#pragma unroll
+                for (int b = 0; b < NT; b++) x[b][0] = x[b][1] = x[b][2] = x[b][3] = 0.0f;
+#pragma unroll
+                for (int j = 0; j < KT / 8; j++) {
+                    uint32_t vh[4], vl[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int dim = d * 16 + kr + 8 * (e & 1);
+                        split_tf32(lds(vt + at<RB>(j * 8 + col + (e >> 1), dim / 4) + (dim & 3) * 4), vh[e], vl[e]);
                     }
 #pragma unroll
-                    for (int mt = 0; mt < MT; mt++) {
-                        mma8(x[mt], wl[j][mt], bh[0], bh[1]);
-                        mma8(x[mt], wh[j][mt], bl[0], bl[1]);
-                        mma8(x[mt], wh[j][mt], bh[0], bh[1]);
+                    for (int b = 0; b < NT; b++) {
+                        mma8(x[b], vl, wh[b][j][0], wh[b][j][1]);
+                        mma8(x[b], vh, wl[b][j][0], wl[b][j][1]);
+                        mma8(x[b], vh, wh[b][j][0], wh[b][j][1]);
                     }
                 }
 #pragma unroll
-                for (int mt = 0; mt < MT; mt++)
+                for (int b = 0; b < NT; b++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) o[mt][d][e] += x[mt][e];
+                    for (int e = 0; e < 4; e++) o[b][d][e] += x[b][e];
             }
         }
         __syncwarp();   // every lane is done with the stage that the next fetch overwrites
@@ -401,24 +451,26 @@ __global__ void __launch_bounds__(NW * 32) k_chunk_attn(SplitArgs a) {
 
     // join the warps
     float* ml = (float*)(sm + C::OFF_ML);   // [NW][ROWS] {m, l}
-    float* so = (float*)sm;                 // [NW][ROWS][D]
+    float* so = (float*)sm;                 // [NW][ROWS][OSTR]
     __syncthreads();
 #pragma unroll
-    for (int mt = 0; mt < MT; mt++)
+    for (int b = 0; b < NT; b++)
 #pragma unroll
         for (int e = 0; e < 2; e++) {
-            float x = l[mt][e];
-            x += __shfl_xor_sync(0xffffffffu, x, 1);
-            x += __shfl_xor_sync(0xffffffffu, x, 2);
-            const int r = mt * 16 + lane / 4 + 8 * e;
-            if ((lane & 3) == 0) {
-                ml[2 * (warp * ROWS + r)] = m[mt][e];
-                ml[2 * (warp * ROWS + r) + 1] = x;
+            float x = l[b][e];
+            x += __shfl_xor_sync(0xffffffffu, x, 4);
+            x += __shfl_xor_sync(0xffffffffu, x, 8);
+            x += __shfl_xor_sync(0xffffffffu, x, 16);
+            const int r = warp * ROWS + b * 8 + col + e;
+            if (lane < 4) {
+                ml[2 * r] = m[b][e];
+                ml[2 * r + 1] = x;
             }
 #pragma unroll
-            for (int d = 0; d < D / 8; d++)
-                *(float2*)(so + (size_t)(warp * ROWS + r) * D + d * 8 + (lane & 3) * 2) =
-                    make_float2(o[mt][d][2 * e], o[mt][d][2 * e + 1]);
+            for (int d = 0; d < D / 16; d++) {
+                so[r * C::OSTR + d * 16 + kr] = o[b][d][e];
+                so[r * C::OSTR + d * 16 + kr + 8] = o[b][d][e + 2];
+            }
         }
     __syncthreads();
     const int64_t unit = ((int64_t)s * a.tiles + tile) * p.kv.n_head + h;
@@ -435,7 +487,7 @@ __global__ void __launch_bounds__(NW * 32) k_chunk_attn(SplitArgs a) {
         for (int w = 0; w < NW; w++) {
             const float f = ex2(ml[2 * (w * ROWS + r)] - ref);
             sum = fmaf(f, ml[2 * (w * ROWS + r) + 1], sum);
-            const float4 v = *(const float4*)(so + (size_t)(w * ROWS + r) * D + d);
+            const float4 v = *(const float4*)(so + (w * ROWS + r) * C::OSTR + d);
             x[0] = fmaf(f, v.x, x[0]); x[1] = fmaf(f, v.y, x[1]);
             x[2] = fmaf(f, v.z, x[2]); x[3] = fmaf(f, v.w, x[3]);
         }
@@ -462,8 +514,10 @@ __global__ void __launch_bounds__(NW * 32) k_chunk_attn(SplitArgs a) {
 // Calls f with the kernel's compile-time variant for (type, head dim, row tile).
 template <typename T, int D, typename F>
 void pick_rows(int row_tile, F f) {
-    if (row_tile == 16) f(k_chunk_attn<T, D, 1>, Cfg<T, D, 1>::SMEM);
-    else f(k_chunk_attn<T, D, 2>, Cfg<T, D, 2>::SMEM);
+    if (row_tile == 8) f(k_chunk_attn<T, D, 1>, Cfg<T, D, 1>::SMEM);
+    else if (row_tile == 16) f(k_chunk_attn<T, D, 2>, Cfg<T, D, 2>::SMEM);
+    else if (row_tile == 24) f(k_chunk_attn<T, D, 3>, Cfg<T, D, 3>::SMEM);
+    else f(k_chunk_attn<T, D, 4>, Cfg<T, D, 4>::SMEM);
 }
 template <typename T, typename F>
 void pick_dim(int dim, int row_tile, F f) {
@@ -484,7 +538,7 @@ cudaError_t chunk_attention_init_device() {
     cudaError_t e = cudaSuccess;
     for (int ty : {GSVCU_KV_F16, GSVCU_KV_F32, GSVCU_KV_BF16})
         for (int dim : {32, 64, 128})
-            for (int rows : {16, 32})
+            for (int rows : {8, 16, 24, 32})
                 pick(ty, dim, rows, [&](auto k, size_t smem) {
                     const cudaError_t r = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
                     if (e == cudaSuccess) e = r;
@@ -495,7 +549,7 @@ cudaError_t chunk_attention_init_device() {
 
 ChunkAttnPlan chunk_attention_plan(const ChunkAttnParams& p) {
     const int D = p.kv.head_dim, size = p.kv.kv_dtype == GSVCU_KV_F32 ? 4 : 2;
-    const int kt = size == 4 ? (D == 32 ? 32 : 16) : 2048 / D;
+    const int kt = key_tile(D, size);
     const int64_t packed = (int64_t)p.batch.max_chunk * (p.n_q_head / p.kv.n_head);
     ChunkAttnPlan c;
     if (size == 2 && packed > 32 && p.scale != 0.0f) {
@@ -517,7 +571,7 @@ ChunkAttnPlan chunk_attention_plan(const ChunkAttnParams& p) {
         }
         return c;
     }
-    c.row_tile = packed <= 16 ? 16 : 32;
+    c.row_tile = packed >= 32 ? 32 : (int)(packed + 7) / 8 * 8;
     c.tiles = (int)((packed + c.row_tile - 1) / c.row_tile);
     const int64_t units = (int64_t)p.batch.n_seq * c.tiles * p.kv.n_head;
     const int max_tiles = (p.batch.max_kv + kt - 1) / kt;
