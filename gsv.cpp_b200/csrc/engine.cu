@@ -1852,7 +1852,7 @@ static int paged_views(gsvcu_ctx* ctx, const gsvcu_paged_kv* kv, const gsvcu_chu
         return ctx->fail(GSVCU_ERR_ARG, "paged cache: n_q_head must be a multiple of n_kv_head");
     if (!b->row_start_dev || !b->kv_len_dev || !b->block_table_dev)
         return ctx->fail(GSVCU_ERR_ARG, "chunk batch: null row_start, kv_len or block_table");
-    if (b->n_seq < 0 || b->max_pages <= 0 || b->max_pages > INT32_MAX / PAGE || b->n_rows < 0 || b->max_chunk < 0 ||
+    if (b->n_seq < 0 || b->max_pages <= 0 || b->max_pages > (1 << 24) || b->n_rows < 0 || b->max_chunk < 0 ||
         b->max_chunk > b->n_rows || (b->n_rows > 0 && b->max_chunk == 0) || b->max_kv < 0)
         return ctx->fail(GSVCU_ERR_ARG, "chunk batch: sizes out of range");
     pv.pool = kv->pool_dev; pv.kv_dtype = kv->kv_dtype; pv.n_page = kv->n_page; pv.n_layer = kv->n_layer;
@@ -1915,7 +1915,10 @@ int gsvcu_op_chunk_attention(gsvcu_ctx* ctx, const gsvcu_paged_kv* kv, const gsv
         return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_chunk_attention: rows not aligned to their element");
     if (window < 0 || !std::isfinite(scale))
         return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_chunk_attention: window must be >= 0 and scale finite");
-    p.n_q_head = n_q_head; p.q = q_dev; p.q_stride = q_stride; p.scale = scale; p.window = window;
+    if ((int64_t)batch->n_rows * n_q_head > (1 << 30))
+        return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_chunk_attention: more than 2^30 (row, head) pairs");
+    p.n_q_head = n_q_head; p.q = q_dev; p.q_stride = q_stride; p.scale = scale;
+    p.window = window < (1 << 30) ? window : 0;   // (wider than any cache)
     p.prefix = prefix_dev; p.out = out_dev; p.out_stride = out_stride; p.lse = lse_dev; p.err = ctx->att_err + 3;
     if (batch->n_rows == 0 || batch->n_seq == 0) return GSVCU_OK;
     const ChunkAttnPlan plan = chunk_attention_plan(p);

@@ -26,8 +26,11 @@ namespace gsvcu {
 namespace {
 
 constexpr int NW = 4;   // warps per CTA
-// Keys of one warp's tile: 8 KB of K and V (16 KB for wide F32 rows), at least the 16 of one product.
-__host__ __device__ constexpr int key_tile(int dim, int size) { return size == 2 ? 2048 / dim : dim == 32 ? 32 : 16; }
+// Keys of one warp's tile: 8 KB of K and V, 16 KB for wide F32 rows (a product takes 16 keys at least), 4 KB for
+// F16 / BF16 heads of 32, where the CTAs are short and four of them fit an SM (64 slots: 36.9 us against 38.4).
+__host__ __device__ constexpr int key_tile(int dim, int size) {
+    return dim == 32 ? 32 : size == 2 ? 2048 / dim : 16;
+}
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool in) {
@@ -151,17 +154,51 @@ __global__ void __launch_bounds__(NW * 32) k_chunk_attn(SplitArgs a) {
     griddep_wait();
     griddep_launch();
 
+    // Without a window this warp's tiles are known before the sequence's length: the first page numbers are fetched
+    // beside it (entries past the sequence are not used).
+    const int32_t* tab = p.batch.table + (int64_t)s * p.batch.max_pages;
+    const int v0 = sp * a.split_tiles;
+    int pages = 0;
+    if (!p.window) pages = tab[min((v0 + warp + lane * NW) / (PAGE / KT), p.batch.max_pages - 1)];
     ChunkRange c;
     if (!chunk_range(p, s, tile, a.group, ROWS, KT, tid == 0 && sp == 0 && h == 0 && tile == 0, c)) return;
     const int row0 = c.row0, n = c.n, total = c.total, len = c.len, r0 = c.r0, rows = c.rows, p0 = c.p0, p1 = c.p1, np = c.np;
     const int n_tiles = c.n_tiles;
     const int n_act = max(1, (n_tiles + a.split_tiles - 1) / a.split_tiles);
     if (sp >= n_act) return;
-    const int v0 = sp * a.split_tiles, v1 = min(n_tiles, v0 + a.split_tiles);
+    const int v1 = min(n_tiles, v0 + a.split_tiles);
     const int mine = v0 + warp < v1 ? (v1 - v0 - warp + NW - 1) / NW : 0;
     auto key0 = [&](int i) { return c.tile_of(v0 + warp + i * NW) * KT; };
 
-    // queries into shared memory, zero past the tile's rows
+    // ring: the page numbers of 32 tiles ahead sit in the warp's lanes
+    const uint32_t ring = smem_addr(sm) + (uint32_t)(warp * ST * 2 * C::TILE);
+    const int64_t block = (int64_t)PAGE * D;   // elements of one (page, layer, K or V, head)
+    bool bad = false;
+    auto fetch = [&](int i) {
+        if (i < mine) {
+            if ((i & 31) == 0 && (i || p.window)) pages = i + lane < mine ? tab[key0(i + lane) / PAGE] : 0;
+            const int k0 = key0(i);
+            const int page = __shfl_sync(0xffffffffu, pages, i & 31);
+            const bool held = page >= 0 && page < p.kv.n_page;
+            bad |= !held;
+            const T* kp = (const T*)p.kv.pool;
+            if (held) kp += (((int64_t)page * p.kv.n_layer + p.kv.layer) * 2 * p.kv.n_head + h) * block + (k0 % PAGE) * D;
+            const T* vp = held ? kp + p.kv.n_head * block : kp;
+            const uint32_t dst = ring + (uint32_t)((i % ST) * 2 * C::TILE);
+            const int keys = held ? len - k0 : 0;
+#pragma unroll
+            for (int j = 0; j < KT * C::PIECES / 32; j++) {
+                const int x = j * 32 + lane, r = x / C::PIECES, pc = x % C::PIECES;
+                const bool in = r < keys;
+                cp16(dst + at<RB>(r, pc), in ? (const uint8_t*)kp + x * 16 : (const uint8_t*)p.kv.pool, in);
+                cp16(dst + C::TILE + at<RB>(r, pc), in ? (const uint8_t*)vp + x * 16 : (const uint8_t*)p.kv.pool, in);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int i = 0; i < ST - 1; i++) fetch(i);
+    // queries into shared memory, zero past the tile's rows (after the first copies are under way)
     uint8_t* sq = sm + C::OFF_Q;
     for (int i = tid; i < ROWS * C::PIECES; i += NW * 32) {
         const int r = i / C::PIECES, pc = i % C::PIECES;
@@ -188,36 +225,6 @@ __global__ void __launch_bounds__(NW * 32) k_chunk_attn(SplitArgs a) {
         *(uint4*)(sq + at<RB>(r, pc)) = u;
     }
 
-    // ring: the page numbers of 32 tiles ahead sit in the warp's lanes
-    const uint32_t ring = smem_addr(sm) + (uint32_t)(warp * ST * 2 * C::TILE);
-    const int32_t* tab = p.batch.table + (int64_t)s * p.batch.max_pages;
-    const int64_t block = (int64_t)PAGE * D;   // elements of one (page, layer, K or V, head)
-    int pages = 0;
-    bool bad = false;
-    auto fetch = [&](int i) {
-        if (i < mine) {
-            if ((i & 31) == 0) pages = i + lane < mine ? tab[key0(i + lane) / PAGE] : 0;
-            const int k0 = key0(i);
-            const int page = __shfl_sync(0xffffffffu, pages, i & 31);
-            const bool held = page >= 0 && page < p.kv.n_page;
-            bad |= !held;
-            const T* kp = (const T*)p.kv.pool;
-            if (held) kp += (((int64_t)page * p.kv.n_layer + p.kv.layer) * 2 * p.kv.n_head + h) * block + (k0 % PAGE) * D;
-            const T* vp = held ? kp + p.kv.n_head * block : kp;
-            const uint32_t dst = ring + (uint32_t)((i % ST) * 2 * C::TILE);
-            const int keys = held ? len - k0 : 0;
-#pragma unroll
-            for (int j = 0; j < KT * C::PIECES / 32; j++) {
-                const int x = j * 32 + lane, r = x / C::PIECES, pc = x % C::PIECES;
-                const bool in = r < keys;
-                cp16(dst + at<RB>(r, pc), in ? (const uint8_t*)kp + x * 16 : (const uint8_t*)p.kv.pool, in);
-                cp16(dst + C::TILE + at<RB>(r, pc), in ? (const uint8_t*)vp + x * 16 : (const uint8_t*)p.kv.pool, in);
-            }
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-#pragma unroll
-    for (int i = 0; i < ST - 1; i++) fetch(i);
     __syncthreads();   // queries
 
     // this lane's rows: 2 of every 8 (fragment columns 2 (lane % 4) and the next)
@@ -492,14 +499,7 @@ __global__ void __launch_bounds__(NW * 32) k_chunk_attn(SplitArgs a) {
             x[2] = fmaf(f, v.z, x[2]); x[3] = fmaf(f, v.w, x[3]);
         }
         if (n_act == 1) {
-            const int tok = (r0 + r) / a.group, head = h * a.group + (r0 + r) % a.group;
-            if (top != NEG_INF) {
-#pragma unroll
-                for (int k = 0; k < 4; k++) x[k] = x[k] / sum;
-            }
-            store_out<T, D>(p, a.vec_out, row0 + tok, head, d, x);
-            if (p.lse && d == 0)
-                p.lse[(int64_t)(row0 + tok) * p.n_q_head + head] = top == NEG_INF ? NEG_INF : (top + log2f(sum)) * LN2;
+            finish<T, D>(p, c, a.vec_out, a.group, h, r, d, top, sum, x);
         } else {
             *(float4*)(part_o + ((int64_t)sp * ROWS + r) * D + d) = make_float4(x[0], x[1], x[2], x[3]);
             if (d == 0) *(float2*)(part_ml + 2 * ((int64_t)sp * ROWS + r)) = make_float2(top, sum);
@@ -508,7 +508,7 @@ __global__ void __launch_bounds__(NW * 32) k_chunk_attn(SplitArgs a) {
     if (n_act == 1) return;
 
     join_splits<T, D, ROWS, NW * 32>(p, c, s, tile, h, a.group, a.tiles, a.n_split, n_act, a.vec_out, tid,
-                                     (int*)(sm + C::OFF_ML + (size_t)NW * ROWS * 8));
+                                     (int*)(sm + C::OFF_ML + (size_t)NW * ROWS * 8), (float*)sm);
 }
 
 // Calls f with the kernel's compile-time variant for (type, head dim, row tile).
@@ -575,13 +575,22 @@ ChunkAttnPlan chunk_attention_plan(const ChunkAttnParams& p) {
     c.tiles = (int)((packed + c.row_tile - 1) / c.row_tile);
     const int64_t units = (int64_t)p.batch.n_seq * c.tiles * p.kv.n_head;
     const int max_tiles = (p.batch.max_kv + kt - 1) / kt;
-    // Enough CTAs for the 148 SMs x 2; a split keeps at least 4 tiles for each warp.
-    const int64_t want = (2 * 148 + units - 1) / units;
+    // Splits, measured on 148 SMs. Few units: one wave of CTAs (one sequence of 131072 keys: 88 us, 100 with two
+    // waves). Several sequences: up to four waves, so that lengths even out (32 sequences of 1000 to 9000 keys: 134 us
+    // with two splits, 119 with four), while a split still streams 1 MB (64 sequences of 2100 keys at head dim 32: 37 us
+    // whole, 48 in two). A split keeps 4 tiles for each warp.
+    size_t smem = 0;
+    pick(p.kv.kv_dtype, D, c.row_tile, [&](auto, size_t bytes) { smem = bytes; });
+    const int64_t slots = 148 * (int64_t)(232448 / (smem + 1024));
+    int64_t n = (slots + units / 2) / units;
+    if (p.batch.n_seq > 1) {
+        const int64_t even = (4 * slots + units - 1) / units, whole = ((int64_t)p.batch.max_kv * 2 * D * size) >> 20;
+        if (n < (even < whole ? even : whole)) n = even < whole ? even : whole;
+    }
     const int least = 4 * NW;
-    int n = (int)(want < 1 ? 1 : want);
     if (n > (max_tiles + least - 1) / least) n = (max_tiles + least - 1) / least;
     if (n < 1) n = 1;
-    c.split_tiles = (max_tiles + n - 1) / n;
+    c.split_tiles = (int)((max_tiles + n - 1) / n);
     c.split_tiles = (c.split_tiles + NW - 1) / NW * NW;
     if (c.split_tiles < NW) c.split_tiles = NW;
     c.n_split = (max_tiles + c.split_tiles - 1) / c.split_tiles;

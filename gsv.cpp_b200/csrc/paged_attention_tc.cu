@@ -548,7 +548,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
         tc_fence_before();
         __syncthreads();
     if (n_act > 1)
-        join_splits<T, D, ROWS, 256>(p, c, s, tile, h, a.group, a.tiles, a.n_split, n_act, a.vec_out, tid - 128, last_slot);
+        join_splits<T, D, ROWS, 256>(p, c, s, tile, h, a.group, a.tiles, a.n_split, n_act, a.vec_out, tid - 128, last_slot,
+                                            (float*)sm);
     }
 }
 

@@ -82,45 +82,98 @@ __device__ __forceinline__ void store_out(const ChunkAttnParams& p, bool vec, in
     }
 }
 
-// THREADS threads of the CTA (tid among them; barrier 1), after their split's results are in p.part ([split][ROWS][D] unnormalised outputs, then
-// [split][ROWS] {maximum (log2 units), sum}): the CTA that arrives last joins the n_act splits in their order,
-// so the result does not depend on the arrival order, and clears the counter.
+// Four outputs (and the log-sum-exp) of row r of the tile from their unnormalised sums.
+template <typename T, int D>
+__device__ __forceinline__ void finish(const ChunkAttnParams& p, const ChunkRange& c, bool vec, int group, int h, int r, int d,
+                                       float top, float sum, float (&x)[4]) {
+    const int tok = (c.r0 + r) / group, head = h * group + (c.r0 + r) % group;
+    if (top != NEG_INF) {
+#pragma unroll
+        for (int k = 0; k < 4; k++) x[k] = x[k] / sum;
+    }
+    store_out<T, D>(p, vec, c.row0 + tok, head, d, x);
+    if (p.lse && d == 0)
+        p.lse[(int64_t)(c.row0 + tok) * p.n_q_head + head] = top == NEG_INF ? NEG_INF : (top + log2f(sum)) * LN2;
+}
+
+// THREADS threads of the CTA (tid among them; barrier 1), after their split's results are in p.part ([split][ROWS][D]
+// unnormalised outputs, then [split][ROWS] {maximum (log2 units), sum}): the CTA that arrives last joins the
+// n_act splits and clears the counter. Every sum runs in an order that the sizes alone decide, so the result does
+// not depend on the arrival order. buf: shared memory, 8 * THREADS floats.
 template <typename T, int D, int ROWS, int THREADS>
 __device__ __forceinline__ void join_splits(const ChunkAttnParams& p, const ChunkRange& c, int s, int tile, int h, int group,
-                                            int tiles, int n_split, int n_act, bool vec, int tid, int* last) {
+                                            int tiles, int n_split, int n_act, bool vec, int tid, int* last, float* buf) {
+    auto sync = [] { asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory"); };
     const int64_t unit = ((int64_t)s * tiles + tile) * p.kv.n_head + h;
     const float* part_o = p.part + unit * n_split * (ROWS * (D + 2));
     const float* part_ml = part_o + (int64_t)n_split * ROWS * D;
     __threadfence();
-    asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory");
+    sync();
     if (tid == 0) *last = atomicAdd(p.arrived + unit, 1) == n_act - 1;
-    asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory");
+    sync();
     if (!*last) return;
     __threadfence();
     if (tid == 0) p.arrived[unit] = 0;
-    for (int i = tid; i < c.rows * (D / 4); i += THREADS) {
-        const int r = i / (D / 4), d = i % (D / 4) * 4;
-        float top = NEG_INF;
-        for (int w = 0; w < n_act; w++) top = fmaxf(top, __ldcg(part_ml + 2 * ((int64_t)w * ROWS + r)));
-        const float ref = top == NEG_INF ? 0.0f : top;
-        float sum = 0.0f, x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-        for (int w = 0; w < n_act; w++) {
-            const float2 e = __ldcg((const float2*)(part_ml + 2 * ((int64_t)w * ROWS + r)));
-            const float f = ex2(e.x - ref);
-            sum = fmaf(f, e.y, sum);
-            const float4 v = __ldcg((const float4*)(part_o + ((int64_t)w * ROWS + r) * D + d));
-            x[0] = fmaf(f, v.x, x[0]); x[1] = fmaf(f, v.y, x[1]);
-            x[2] = fmaf(f, v.z, x[2]); x[3] = fmaf(f, v.w, x[3]);
-        }
-        const int tok = (c.r0 + r) / group, head = h * group + (c.r0 + r) % group;
-        if (top != NEG_INF) {
+    // thread = four outputs of a row over every per-th split; where rows and outputs are fewer than the threads,
+    // per of them share a row's splits
+    const int items = c.rows * (D / 4);
+    int per = 1;
+    while (per * 2 * items <= THREADS && per * 2 <= n_act) per *= 2;
+    for (int i = tid; i < items * per; i += THREADS) {
+        const int item = per > 1 ? i % items : i, g = per > 1 ? i / items : 0, r = item / (D / 4), d = item % (D / 4) * 4;
+        const int mine = (n_act - g + per - 1) / per;   // splits g, g + per, ...
+        const int64_t step_ml = 2 * (int64_t)per * ROWS, step_o = (int64_t)per * ROWS * D;
+        const float* ml = part_ml + 2 * (g * ROWS + r);
+        const float* po = part_o + ((int64_t)g * ROWS + r) * D + d;
+        float top = NEG_INF, sum = 0.0f, x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        // 8 and 4 loads in flight whatever the count
+        for (int w0 = 0; w0 < mine; w0 += 8) {
+            float m[8];
 #pragma unroll
-            for (int k = 0; k < 4; k++) x[k] = x[k] / sum;
+            for (int k = 0; k < 8; k++) m[k] = w0 + k < mine ? __ldcg(ml + (w0 + k) * step_ml) : NEG_INF;
+#pragma unroll
+            for (int k = 0; k < 8; k++) top = fmaxf(top, m[k]);
         }
-        store_out<T, D>(p, vec, c.row0 + tok, head, d, x);
-        if (p.lse && d == 0)
-            p.lse[(int64_t)(c.row0 + tok) * p.n_q_head + head] = top == NEG_INF ? NEG_INF : (top + log2f(sum)) * LN2;
+        const float ref = top == NEG_INF ? 0.0f : top;
+        for (int w0 = 0; w0 < mine; w0 += 4) {
+            float2 e[4];
+            float4 v[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const bool in = w0 + k < mine;
+                e[k] = in ? __ldcg((const float2*)(ml + (w0 + k) * step_ml)) : make_float2(NEG_INF, 0.0f);
+                v[k] = in ? __ldcg((const float4*)(po + (w0 + k) * step_o)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const float f = ex2(e[k].x - ref);
+                sum = fmaf(f, e[k].y, sum);
+                x[0] = fmaf(f, v[k].x, x[0]); x[1] = fmaf(f, v[k].y, x[1]);
+                x[2] = fmaf(f, v[k].z, x[2]); x[3] = fmaf(f, v[k].w, x[3]);
+            }
+        }
+        if (per > 1) {
+            *(float4*)(buf + 8 * i) = make_float4(x[0], x[1], x[2], x[3]);
+            *(float2*)(buf + 8 * i + 4) = make_float2(top, sum);
+        } else {
+            finish<T, D>(p, c, vec, group, h, r, d, top, sum, x);
+        }
+    }
+    if (per > 1) {   // (items * per <= THREADS)
+        sync();
+        if (tid < items) {
+            float top = NEG_INF, sum = 0.0f, x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int g = 0; g < per; g++) top = fmaxf(top, buf[8 * (g * items + tid) + 4]);
+            const float ref = top == NEG_INF ? 0.0f : top;
+            for (int g = 0; g < per; g++) {
+                const float* y = buf + 8 * (g * items + tid);
+                const float f = ex2(y[4] - ref);
+                sum = fmaf(f, y[5], sum);
+#pragma unroll
+                for (int k = 0; k < 4; k++) x[k] = fmaf(f, y[k], x[k]);
+            }
+            finish<T, D>(p, c, vec, group, h, tid / (D / 4), tid % (D / 4) * 4, top, sum, x);
+        }
     }
 }
 

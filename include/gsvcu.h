@@ -279,7 +279,7 @@ typedef struct {
 
 /* The batch (device arrays): sequence s owns the packed rows row_start[s] .. row_start[s + 1] - 1
  * (row_start [n_seq + 1], ascending), holds kv_len[s] keys with these rows and keeps key c in page
- * block_table[s][c / 64], slot c % 64 (block_table [n_seq][max_pages]; entries past its keys are not read).
+ * block_table[s][c / 64], slot c % 64 (block_table [n_seq][max_pages], max_pages <= 2^24; entries past its keys are not used).
  * Row i of n is the token at cache position kv_len[s] - n + i. Host sizes: n_rows packed rows, max_chunk at
  * least the longest chunk, max_kv at least the longest kv_len (0: max_pages * 64); the closer these are, the
  * better the work is cut up. A page outside the pool, or lengths outside these sizes, touch no memory
