@@ -204,8 +204,12 @@ void launch(const KvAppendParams& p, cudaStream_t s) {
         launch_pdl(k_kv_append_any<TI, T, D>, dim3((p.batch.n_rows + 3) / 4), dim3(128), 0, s, p);
         return;
     }
-    const int head_lanes = 256 / (D / 16);
-    launch_pdl(k_kv_append<TI, T, D>, dim3(p.batch.n_rows), dim3(256), 0, s, p, head_lanes);
+    // Threads per row: a warp when rows alone fill the GPU (31k rows of 48 heads x 128: 130 us, 170 with 256 threads a
+    // row, whose angles then serve one head instead of twelve), up to 256 when there are few and latency counts.
+    int per_row = 256;
+    while (per_row > 32 && (int64_t)per_row * p.batch.n_rows > 148 * 2048) per_row /= 2;
+    const int rows = 256 / per_row;
+    launch_pdl(k_kv_append<TI, T, D>, dim3((p.batch.n_rows + rows - 1) / rows), dim3(256), 0, s, p, per_row / (D / 16));
 }
 template <typename TI, typename T>
 void launch_d(const KvAppendParams& p, cudaStream_t s) {
