@@ -1952,10 +1952,10 @@ int gsvcu_op_chunk_attention(gsvcu_ctx* ctx, const gsvcu_paged_kv* kv, const gsv
     }
     p.part = ctx->op_split;
     p.arrived = ctx->op_arrived;
-    if (!launch_chunk_attention(p, plan, ctx->stream))
-        return ctx->fail(GSVCU_ERR_CUDA, "gsvcu_op_chunk_attention: tensor map encoding failed");
+    const int kernels = launch_chunk_attention(p, plan, ctx->stream);
+    if (kernels == 0) return ctx->fail(GSVCU_ERR_CUDA, "gsvcu_op_chunk_attention: tensor map encoding failed");
     CKC(ctx, cudaGetLastError());
-    ctx->launches++;
+    ctx->launches += kernels;
     return GSVCU_OK;
 }
 

@@ -64,12 +64,14 @@ struct ChunkAttnPlan {
     int row_tile = 0;      // packed rows (token x query head of one kv head) of a CTA
     int tiles = 0;         // row tiles per sequence (bound)
     int n_split = 0;       // key splits (bound)
+    int key_tile = 0;      // keys of a tile
     int split_tiles = 0;   // key tiles of a split
+    bool join_apart = false;   // the splits are joined by a kernel of its own, not by the last CTA
     size_t part_floats = 0, arrivals = 0;
 };
 ChunkAttnPlan chunk_attention_plan(const ChunkAttnParams& p);
-// False: not launched (no tensor map).
-bool launch_chunk_attention(const ChunkAttnParams& p, const ChunkAttnPlan& plan, cudaStream_t s);
+// Kernels launched; 0: none (no tensor map).
+int launch_chunk_attention(const ChunkAttnParams& p, const ChunkAttnPlan& plan, cudaStream_t s);
 bool launch_chunk_attention_tc(const ChunkAttnParams& p, const ChunkAttnPlan& plan, cudaStream_t s);
 cudaError_t chunk_attention_init_device();   // dynamic shared-memory limits on the current device
 cudaError_t chunk_attention_tc_init_device();

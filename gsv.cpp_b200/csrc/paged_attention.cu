@@ -133,7 +133,7 @@ struct SplitArgs {
     ChunkAttnParams p;
     int group, tiles, n_split, split_tiles;
     float c;          // scale * log2(e)
-    bool vec_q, vec_out;
+    bool vec_q, vec_out, join_apart;
 };
 
 template <typename T, int D, int NT>
@@ -504,7 +504,7 @@ __global__ void __launch_bounds__(NW * 32) k_chunk_attn(SplitArgs a) {
             if (d == 0) *(float2*)(part_ml + 2 * ((int64_t)sp * ROWS + r)) = make_float2(top, sum);
         }
     }
-    if (n_act == 1) return;
+    if (n_act == 1 || a.join_apart) return;
 
     join_splits<T, D, ROWS, NW * 32>(p, c, s, tile, h, a.group, a.tiles, a.n_split, n_act, a.vec_out, tid,
                                      (int*)(sm + C::OFF_ML + (size_t)NW * ROWS * 8), (float*)sm);
@@ -564,10 +564,9 @@ ChunkAttnPlan chunk_attention_plan(const ChunkAttnParams& p) {
         if (n < 1) n = 1;
         c.split_tiles = (max_tiles + n - 1) / n;
         c.n_split = (max_tiles + c.split_tiles - 1) / c.split_tiles;
-        if (c.n_split > 1) {
-            c.part_floats = (size_t)units * c.n_split * c.row_tile * (D + 2);
-            c.arrivals = (size_t)units;
-        }
+        c.key_tile = 128;
+        c.join_apart = c.n_split > 1;
+        if (c.n_split > 1) c.part_floats = (size_t)units * c.n_split * c.row_tile * (D + 2);
         return c;
     }
     c.row_tile = packed >= 32 ? 32 : (int)(packed + 7) / 8 * 8;
@@ -594,30 +593,63 @@ ChunkAttnPlan chunk_attention_plan(const ChunkAttnParams& p) {
     if (c.split_tiles < NW) c.split_tiles = NW;
     c.n_split = (max_tiles + c.split_tiles - 1) / c.split_tiles;
     if (c.n_split < 1) c.n_split = 1;
+    c.key_tile = kt;
     if (c.n_split > 1) {
+        // Joined by the last CTA while a unit has 8 rows (one sequence of 131072 keys: 89 us, 101 with a second kernel),
+        // by a kernel over the whole GPU when it has more (drafts of 5: 18.3 us, 19.5).
+        c.join_apart = c.row_tile > 8;
         c.part_floats = (size_t)units * c.n_split * c.row_tile * (D + 2);
-        c.arrivals = (size_t)units;
+        c.arrivals = c.join_apart ? 0 : (size_t)units;
     }
     return c;
 }
 
-bool launch_chunk_attention(const ChunkAttnParams& p, const ChunkAttnPlan& plan, cudaStream_t s) {
-    if (plan.tensor) return launch_chunk_attention_tc(p, plan, s);
+template <typename T, int D>
+static void launch_join_rows(const ChunkAttnParams& p, const ChunkAttnPlan& c, bool vec, cudaStream_t s) {
+    const int group = p.n_q_head / p.kv.n_head, rows = 1024 / D;
+    const int64_t ctas = (int64_t)p.batch.n_seq * c.tiles * p.kv.n_head * ((c.row_tile + rows - 1) / rows);
+    auto go = [&](auto k) {
+        launch_pdl(k, dim3((unsigned)ctas), dim3(256), 0, s, p, group, c.tiles, c.n_split, c.split_tiles, c.key_tile, vec);
+    };
+    if (c.row_tile == 8) go(k_chunk_join<T, D, 8>);
+    else if (c.row_tile == 16) go(k_chunk_join<T, D, 16>);
+    else if (c.row_tile == 24) go(k_chunk_join<T, D, 24>);
+    else if (c.row_tile == 32) go(k_chunk_join<T, D, 32>);
+    else if constexpr (sizeof(T) == 2) go(k_chunk_join<T, D, 256>);
+}
+template <typename T>
+static void launch_join(const ChunkAttnParams& p, const ChunkAttnPlan& c, bool vec, cudaStream_t s) {
+    if (p.kv.head_dim == 32) launch_join_rows<T, 32>(p, c, vec, s);
+    else if (p.kv.head_dim == 64) launch_join_rows<T, 64>(p, c, vec, s);
+    else launch_join_rows<T, 128>(p, c, vec, s);
+}
+
+int launch_chunk_attention(const ChunkAttnParams& p, const ChunkAttnPlan& plan, cudaStream_t s) {
     const size_t size = p.kv.kv_dtype == GSVCU_KV_F32 ? 4 : 2;
-    SplitArgs a;
-    a.p = p;
-    a.group = p.n_q_head / p.kv.n_head;
-    a.tiles = plan.tiles;
-    a.n_split = plan.n_split;
-    a.split_tiles = plan.split_tiles;
-    a.c = p.scale * LOG2E;
-    a.vec_q = ((uintptr_t)p.q & 15) == 0 && (p.q_stride * (int64_t)size) % 16 == 0;
-    a.vec_out = ((uintptr_t)p.out & 15) == 0 && (p.out_stride * (int64_t)size) % 16 == 0;
-    const int64_t ctas = (int64_t)p.batch.n_seq * plan.tiles * p.kv.n_head * plan.n_split;
-    pick(p.kv.kv_dtype, p.kv.head_dim, plan.row_tile, [&](auto k, size_t smem) {
-        launch_pdl(k, dim3((unsigned)ctas), dim3(NW * 32), smem, s, a);
-    });
-    return true;
+    const bool vec_out = ((uintptr_t)p.out & 15) == 0 && (p.out_stride * (int64_t)size) % 16 == 0;
+    if (plan.tensor) {
+        if (!launch_chunk_attention_tc(p, plan, s)) return 0;
+    } else {
+        SplitArgs a;
+        a.p = p;
+        a.group = p.n_q_head / p.kv.n_head;
+        a.tiles = plan.tiles;
+        a.n_split = plan.n_split;
+        a.split_tiles = plan.split_tiles;
+        a.c = p.scale * LOG2E;
+        a.vec_q = ((uintptr_t)p.q & 15) == 0 && (p.q_stride * (int64_t)size) % 16 == 0;
+        a.vec_out = vec_out;
+        a.join_apart = plan.join_apart;
+        const int64_t ctas = (int64_t)p.batch.n_seq * plan.tiles * p.kv.n_head * plan.n_split;
+        pick(p.kv.kv_dtype, p.kv.head_dim, plan.row_tile, [&](auto k, size_t smem) {
+            launch_pdl(k, dim3((unsigned)ctas), dim3(NW * 32), smem, s, a);
+        });
+    }
+    if (!plan.join_apart) return 1;
+    if (p.kv.kv_dtype == GSVCU_KV_F32) launch_join<float>(p, plan, vec_out, s);
+    else if (p.kv.kv_dtype == GSVCU_KV_F16) launch_join<__half>(p, plan, vec_out, s);
+    else launch_join<__nv_bfloat16>(p, plan, vec_out, s);
+    return 2;
 }
 
 }  // namespace gsvcu

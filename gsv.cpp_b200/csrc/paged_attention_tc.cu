@@ -133,6 +133,8 @@ __device__ __forceinline__ void tmem_st16u(uint32_t a, const uint32_t (&r)[16]) 
         : "memory");
 }
 
+// The lowest n bits (n cut to 0 .. 32).
+__device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : 0xffffffffu >> (32 - min(n, 32)); }
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float y;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
@@ -194,7 +196,6 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
     const uint32_t vhere = bar0 + 8u * (2 * L::NP + 8), vclear = vhere + 8, drain = vhere + 16;
     uint32_t* tmem_slot = (uint32_t*)(sm + L::OFF_BAR + L::NBAR * 8);
     volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
-    int* last_slot = (int*)(tmem_slot + 2);
 
     int id = blockIdx.x;
     const int sp = id % a.n_split;
@@ -202,14 +203,21 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
     const int h = id % p.kv.n_head;
     id /= p.kv.n_head;
     const int s = id % p.batch.n_seq, tile = a.tiles - 1 - id / p.batch.n_seq;   // the last rows see most keys: first
+    if (tid == 0) asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&a.map) : "memory");
     griddep_wait();
     griddep_launch();
 
+    // Without a window the key tiles are known before the sequence's length: warp 0 fetches the first page numbers
+    // beside it (lane = tile, page; entries past the sequence are not used).
+    const int v0 = sp * a.split_tiles;
+    const int32_t* tab = p.batch.table + (int64_t)s * p.batch.max_pages;
+    int first_page = 0;
+    if (warp == 0 && !p.window) first_page = tab[min(v0 * 2 + lane, p.batch.max_pages - 1)];
     ChunkRange c;
     if (!chunk_range(p, s, tile, a.group, ROWS, KT, tid == 0 && sp == 0 && h == 0 && tile == 0, c)) return;
     const int n_act = max(1, (c.n_tiles + a.split_tiles - 1) / a.split_tiles);
     if (sp >= n_act) return;
-    const int v0 = sp * a.split_tiles, nt = min(c.n_tiles, v0 + a.split_tiles) - v0;   // this CTA's key tiles
+    const int nt = min(c.n_tiles, v0 + a.split_tiles) - v0;   // this CTA's key tiles
     const int halves = c.rows > 128 ? 2 : 1;
     auto key0 = [&](int j) { return c.tile_of(v0 + j) * KT; };
 
@@ -222,31 +230,87 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    // Warp 0's work: pair i is V of tile i - 1, then K of tile i (what the MMA warp needs together).
+    int blk = 0;
+    bool bad = false;
+    uint32_t v0b = 0, v1b = 0;   // blocks of the tile before (its V follows one pair later)
+    auto load_pair = [&](int i) -> bool {
+        const int e = i % L::NP;
+        if ((i & 15) == 0) {   // the blocks of 16 tiles: lane = (tile, page)
+            const int jj = i + (lane >> 1);
+            blk = a.n_blocks;   // past the pool: zero fill
+            if (jj < nt) {
+                const int key = key0(jj) + PAGE * (lane & 1);
+                if (key < c.len) {
+                    const int page = i == 0 && !p.window ? first_page : tab[key / PAGE];
+                    if (page >= 0 && page < p.kv.n_page) blk = ((page * p.kv.n_layer + p.kv.layer) * 2) * p.kv.n_head + h;
+                    else bad = true;
+                }
+            }
+        }
+        const uint32_t k0b = __shfl_sync(0xffffffffu, blk, (i & 15) * 2), k1b = __shfl_sync(0xffffffffu, blk, (i & 15) * 2 + 1);
+        bool ok = true;
+        if (lane == 0) {
+            ok = bar_wait_short(empty(e), ((uint32_t)(i / L::NP) & 1u) ^ 1u, abort_flag);
+            if (ok) {
+                bar_expect_tx(full(e), (i > 0 && i < nt ? 2 : 1) * L::ENTRY);
+                const uint32_t dst = su32(sm + L::OFF_RING + (size_t)e * 2 * L::ENTRY);
+                auto load = [&](uint32_t to, uint32_t b0, uint32_t b1) {
+#pragma unroll
+                    for (int at = 0; at < L::ATOMS; at++) {
+                        tma_load_3d(to + at * KT * L::RB, &a.map, at * 64, 0, (int)b0, full(e));
+                        tma_load_3d(to + at * KT * L::RB + PAGE * L::RB, &a.map, at * 64, 0, (int)b1, full(e));
+                    }
+                };
+                const uint32_t none = a.n_blocks;
+                if (i > 0) load(dst, v0b == none ? none : v0b + p.kv.n_head, v1b == none ? none : v1b + p.kv.n_head);
+                if (i < nt) load(dst + L::ENTRY, k0b, k1b);
+            }
+        }
+        v0b = k0b;
+        v1b = k1b;
+        return __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+    };
+    const int pairs = nt > 0 ? nt + 1 : 0, early = min(pairs, L::NP);   // the first ones find the ring empty
+    if (warp == 0) {
+        __syncwarp();
+        for (int i = 0; i < early; i++) load_pair(i);
+    }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(su32(tmem_slot)), "r"(512)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    // Q, swizzled as the MMA reads it ([tile][64-dim block][128 rows][RB bytes]), zero past the CTA's rows
-    for (int i = tid; i < ROWS * (D / 8); i += THREADS) {
-        const int r = i / (D / 8), pc = i % (D / 8);
-        if (r >= 128 * halves) break;
-        uint4 u = make_uint4(0, 0, 0, 0);
-        if (r < c.rows) {
-            const int tok = (c.r0 + r) / a.group, j = (c.r0 + r) % a.group;
-            const T* src = (const T*)p.q + (int64_t)(c.row0 + tok) * p.q_stride + (int64_t)(h * a.group + j) * D + pc * 8;
-            if (a.vec_q) {
-                u = *(const uint4*)src;
-            } else {
-                T* x = (T*)&u;
+    // Q, swizzled as the MMA reads it ([tile][64-dim block][128 rows][RB bytes]), zero past the CTA's rows; four loads
+    // in flight per thread (one at a time this was a third of a short call)
+    constexpr int STEP = THREADS - 32;
+    for (int i0 = tid - 32; warp > 0 && i0 < 128 * halves * (D / 8); i0 += 4 * STEP) {
+        uint4 u[4];
 #pragma unroll
-                for (int k = 0; k < 8; k++) x[k] = src[k];
+        for (int m = 0; m < 4; m++) {
+            const int i = i0 + m * STEP, r = i / (D / 8), pc = i % (D / 8);
+            u[m] = make_uint4(0, 0, 0, 0);
+            if (r < c.rows) {
+                const int tok = (c.r0 + r) / a.group, j = (c.r0 + r) % a.group;
+                const T* src = (const T*)p.q + (int64_t)(c.row0 + tok) * p.q_stride + (int64_t)(h * a.group + j) * D + pc * 8;
+                if (a.vec_q) {
+                    u[m] = *(const uint4*)src;
+                } else {
+                    T* x = (T*)&u[m];
+#pragma unroll
+                    for (int k = 0; k < 8; k++) x[k] = src[k];
+                }
             }
-            if (a.negate) { u.x ^= 0x80008000u; u.y ^= 0x80008000u; u.z ^= 0x80008000u; u.w ^= 0x80008000u; }
         }
-        const int rt = r & 127, atom = D >= 64 ? pc / 8 : 0, ch = D >= 64 ? pc % 8 : pc;
-        const int swz = L::RB == 128 ? rt & 7 : (rt >> 1) & 3;
-        *(uint4*)(sm + (size_t)(r >> 7) * 128 * D * 2 + (size_t)atom * 128 * L::RB + rt * L::RB + ((ch ^ swz) << 4)) = u;
+#pragma unroll
+        for (int m = 0; m < 4; m++) {
+            const int i = i0 + m * STEP, r = i / (D / 8), pc = i % (D / 8);
+            if (r >= 128 * halves) break;
+            if (a.negate) { u[m].x ^= 0x80008000u; u[m].y ^= 0x80008000u; u[m].z ^= 0x80008000u; u[m].w ^= 0x80008000u; }
+            const int rt = r & 127, atom = D >= 64 ? pc / 8 : 0, ch = D >= 64 ? pc % 8 : pc;
+            const int swz = L::RB == 128 ? rt & 7 : (rt >> 1) & 3;
+            *(uint4*)(sm + (size_t)(r >> 7) * 128 * D * 2 + (size_t)atom * 128 * L::RB + rt * L::RB + ((ch ^ swz) << 4)) = u[m];
+        }
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     tc_fence_before();
@@ -258,48 +322,9 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
         if (warp == 0) {
-            // pair i: V of tile i - 1, then K of tile i (what the MMA warp needs together)
-            const int32_t* tab = p.batch.table + (int64_t)s * p.batch.max_pages;
-            int blk = 0;
-            bool ok = true, bad = false;
-            int i = 0;
-            uint32_t v0b = 0, v1b = 0;   // K blocks of the tile before (its V follows one pair later)
-            for (; i <= nt && nt > 0 && ok; i++) {
-                const int e = i % L::NP;
-                if ((i & 15) == 0) {   // the blocks of 16 tiles: lane = (tile, page)
-                    const int jj = i + (lane >> 1);
-                    blk = a.n_blocks;   // past the pool: zero fill
-                    if (jj < nt) {
-                        const int key = key0(jj) + PAGE * (lane & 1);
-                        if (key < c.len) {
-                            const int page = tab[key / PAGE];
-                            if (page >= 0 && page < p.kv.n_page) blk = ((page * p.kv.n_layer + p.kv.layer) * 2) * p.kv.n_head + h;
-                            else bad = true;
-                        }
-                    }
-                }
-                const uint32_t k0b = __shfl_sync(0xffffffffu, blk, (i & 15) * 2), k1b = __shfl_sync(0xffffffffu, blk, (i & 15) * 2 + 1);
-                if (lane == 0) {
-                    ok = bar_wait_short(empty(e), ((uint32_t)(i / L::NP) & 1u) ^ 1u, abort_flag);
-                    if (ok) {
-                        bar_expect_tx(full(e), (i > 0 && i < nt ? 2 : 1) * L::ENTRY);
-                        const uint32_t dst = su32(sm + L::OFF_RING + (size_t)e * 2 * L::ENTRY);
-                        auto load = [&](uint32_t to, uint32_t b0, uint32_t b1) {
-#pragma unroll
-                            for (int at = 0; at < L::ATOMS; at++) {
-                                tma_load_3d(to + at * KT * L::RB, &a.map, at * 64, 0, (int)b0, full(e));
-                                tma_load_3d(to + at * KT * L::RB + PAGE * L::RB, &a.map, at * 64, 0, (int)b1, full(e));
-                            }
-                        };
-                        const uint32_t none = a.n_blocks;
-                        if (i > 0) load(dst, v0b == none ? none : v0b + p.kv.n_head, v1b == none ? none : v1b + p.kv.n_head);
-                        if (i < nt) load(dst + L::ENTRY, k0b, k1b);
-                    }
-                }
-                v0b = k0b;
-                v1b = k1b;
-                ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
-            }
+            int i = early;
+            bool ok = true;
+            for (; i < pairs && ok; i++) ok = load_pair(i);
             if (bad) atomicOr(p.err, PAGED_BAD_PAGE);
             if (lane == 0) {
                 if (!ok) {
@@ -427,9 +452,14 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
                 const bool whole = k0 + KT <= c.np || (k0 + KT <= min(c.len, c.p0 + 1) && (!p.window || k0 > c.p1 - p.window));
                 if (!whole) {
 #pragma unroll
-                    for (int i = 0; i < KT; i++) {
-                        const int key = k0 + i;
-                        if (!(key < c.np || (key < see_hi && key >= see_lo))) x[i / 32][i % 32] = __float_as_uint(NEG_INF);
+                    for (int k = 0; k < 4; k++) {
+                        const int at = k0 + 32 * k;   // bit i: the row sees key at + i
+                        const uint32_t seen = (below(see_hi - at) & ~below(see_lo - at)) | below(c.np - at);
+                        if (seen != 0xffffffffu) {
+#pragma unroll
+                            for (int i = 0; i < 32; i++)
+                                if (!(seen >> i & 1u)) x[k][i] = __float_as_uint(NEG_INF);
+                        }
                     }
                     asm volatile("" ::: "memory");   // keeps the tests out of the tiles that need none
                 }
@@ -547,9 +577,6 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
         }
         tc_fence_before();
         __syncthreads();
-    if (n_act > 1)
-        join_splits<T, D, ROWS, 256>(p, c, s, tile, h, a.group, a.tiles, a.n_split, n_act, a.vec_out, tid - 128, last_slot,
-                                            (float*)sm);
     }
 }
 

@@ -96,6 +96,63 @@ __device__ __forceinline__ void finish(const ChunkAttnParams& p, const ChunkRang
         p.lse[(int64_t)(c.row0 + tok) * p.n_q_head + head] = top == NEG_INF ? NEG_INF : (top + log2f(sum)) * LN2;
 }
 
+// Splits g, g + per, ... of n_act added up for four outputs of row r; 8 loads in flight whatever the count.
+template <int D, int ROWS>
+__device__ __forceinline__ void sum_splits(const float* part_o, const float* part_ml, int n_act, int g, int per, int r, int d,
+                                           float& top, float& sum, float (&x)[4]) {
+    const int mine = (n_act - g + per - 1) / per;
+    const int64_t step_ml = 2 * (int64_t)per * ROWS, step_o = (int64_t)per * ROWS * D;
+    const float* ml = part_ml + 2 * (g * ROWS + r);
+    const float* po = part_o + ((int64_t)g * ROWS + r) * D + d;
+    top = NEG_INF;
+    sum = x[0] = x[1] = x[2] = x[3] = 0.0f;
+    for (int w0 = 0; w0 < mine; w0 += 8) {
+        float m[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) m[k] = w0 + k < mine ? __ldcg(ml + (w0 + k) * step_ml) : NEG_INF;
+#pragma unroll
+        for (int k = 0; k < 8; k++) top = fmaxf(top, m[k]);
+    }
+    const float ref = top == NEG_INF ? 0.0f : top;
+    for (int w0 = 0; w0 < mine; w0 += 8) {
+        float2 e[8];
+        float4 v[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const bool in = w0 + k < mine;
+            e[k] = in ? __ldcg((const float2*)(ml + (w0 + k) * step_ml)) : make_float2(NEG_INF, 0.0f);
+            v[k] = in ? __ldcg((const float4*)(po + (w0 + k) * step_o)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const float f = ex2(e[k].x - ref);
+            sum = fmaf(f, e[k].y, sum);
+            x[0] = fmaf(f, v[k].x, x[0]); x[1] = fmaf(f, v[k].y, x[1]);
+            x[2] = fmaf(f, v[k].z, x[2]); x[3] = fmaf(f, v[k].w, x[3]);
+        }
+    }
+}
+
+// Joining as a kernel of its own: a CTA per (unit, 1024 outputs).
+template <typename T, int D, int ROWS>
+__global__ void __launch_bounds__(256) k_chunk_join(ChunkAttnParams p, int group, int tiles, int n_split, int split_tiles,
+                                                    int key_tile, bool vec) {
+    constexpr int R = 1024 / D;   // rows of a CTA
+    griddep_wait();
+    griddep_launch();
+    const int64_t unit = blockIdx.x / ((ROWS + R - 1) / R);
+    const int r = blockIdx.x % ((ROWS + R - 1) / R) * R + threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4;
+    const int h = (int)(unit % p.kv.n_head), tile = (int)(unit / p.kv.n_head % tiles), s = (int)(unit / p.kv.n_head / tiles);
+    ChunkRange c;
+    if (!chunk_range(p, s, tile, group, ROWS, key_tile, false, c) || r >= c.rows) return;
+    const int n_act = (c.n_tiles + split_tiles - 1) / split_tiles;
+    if (n_act <= 1) return;   // (written by the only split)
+    const float* part_o = p.part + unit * n_split * (ROWS * (D + 2));
+    float top, sum, x[4];
+    sum_splits<D, ROWS>(part_o, part_o + (int64_t)n_split * ROWS * D, n_act, 0, 1, r, d, top, sum, x);
+    finish<T, D>(p, c, vec, group, h, r, d, top, sum, x);
+}
+
 // THREADS threads of the CTA (tid among them; barrier 1), after their split's results are in p.part ([split][ROWS][D]
 // unnormalised outputs, then [split][ROWS] {maximum (log2 units), sum}): the CTA that arrives last joins the
 // n_act splits and clears the counter. Every sum runs in an order that the sizes alone decide, so the result does
@@ -121,37 +178,8 @@ __device__ __forceinline__ void join_splits(const ChunkAttnParams& p, const Chun
     while (per * 2 * items <= THREADS && per * 2 <= n_act) per *= 2;
     for (int i = tid; i < items * per; i += THREADS) {
         const int item = per > 1 ? i % items : i, g = per > 1 ? i / items : 0, r = item / (D / 4), d = item % (D / 4) * 4;
-        const int mine = (n_act - g + per - 1) / per;   // splits g, g + per, ...
-        const int64_t step_ml = 2 * (int64_t)per * ROWS, step_o = (int64_t)per * ROWS * D;
-        const float* ml = part_ml + 2 * (g * ROWS + r);
-        const float* po = part_o + ((int64_t)g * ROWS + r) * D + d;
-        float top = NEG_INF, sum = 0.0f, x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        // 8 and 4 loads in flight whatever the count
-        for (int w0 = 0; w0 < mine; w0 += 8) {
-            float m[8];
-#pragma unroll
-            for (int k = 0; k < 8; k++) m[k] = w0 + k < mine ? __ldcg(ml + (w0 + k) * step_ml) : NEG_INF;
-#pragma unroll
-            for (int k = 0; k < 8; k++) top = fmaxf(top, m[k]);
-        }
-        const float ref = top == NEG_INF ? 0.0f : top;
-        for (int w0 = 0; w0 < mine; w0 += 4) {
-            float2 e[4];
-            float4 v[4];
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const bool in = w0 + k < mine;
-                e[k] = in ? __ldcg((const float2*)(ml + (w0 + k) * step_ml)) : make_float2(NEG_INF, 0.0f);
-                v[k] = in ? __ldcg((const float4*)(po + (w0 + k) * step_o)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            }
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const float f = ex2(e[k].x - ref);
-                sum = fmaf(f, e[k].y, sum);
-                x[0] = fmaf(f, v[k].x, x[0]); x[1] = fmaf(f, v[k].y, x[1]);
-                x[2] = fmaf(f, v[k].z, x[2]); x[3] = fmaf(f, v[k].w, x[3]);
-            }
-        }
+        float top, sum, x[4];
+        sum_splits<D, ROWS>(part_o, part_ml, n_act, g, per, r, d, top, sum, x);
         if (per > 1) {
             *(float4*)(buf + 8 * i) = make_float4(x[0], x[1], x[2], x[3]);
             *(float2*)(buf + 8 * i + 4) = make_float2(top, sum);
