@@ -34,17 +34,20 @@ constexpr int KT = 128;                 // keys per tile
 constexpr int ROWS = 256;               // packed rows per CTA
 constexpr int THREADS = 384;
 constexpr float TAU = 8.0f;             // log2 headroom of P above the row's reference maximum
-constexpr uint32_t TM_O = 256;          // tensor-memory column of O0
 
 template <int D>
 struct Smem {
     static constexpr int RB = D >= 64 ? 128 : 2 * D;              // bytes of a swizzled row
     static constexpr int ATOMS = D >= 64 ? D / 64 : 1;            // 64-dim column blocks of a tile
     static constexpr int ENTRY = KT * D * 2;                      // bytes of a K or V tile
-    static constexpr int NP = 2;                                  // ring pairs (even)
+    static constexpr int NP = 2;                                  // ring pairs: V of tile i - 1, K of tile i
+    // Tensor memory: two score buffers (one per row tile; for tiles in turn when there is one row tile), P over the
+    // first half of its scores, then O.
+    static constexpr uint32_t TM_O = 2 * KT;
     static constexpr size_t OFF_RING = (size_t)ROWS * D * 2;      // after Q
     static constexpr size_t OFF_BAR = OFF_RING + (size_t)NP * 2 * ENTRY;
-    static constexpr int NBAR = 2 * NP + 11;   // full, empty, S full [2], P full [2][2], O done [2], V landed, V cleared, drain
+    // full, empty [NP], S full [2], P full [2][2 halves], PV done [2], V landed, V cleared, drain
+    static constexpr int NBAR = 2 * NP + 11;
     static constexpr size_t SMEM = OFF_BAR + NBAR * 8 + 16 + 1024;
 };
 
@@ -190,10 +193,10 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
     const uint32_t bar0 = su32(sm + L::OFF_BAR);
     auto full = [&](int e) { return bar0 + 8u * e; };
     auto empty = [&](int e) { return bar0 + 8u * (L::NP + e); };
-    auto sfull = [&](int t) { return bar0 + 8u * (2 * L::NP + t); };
-    auto pfull = [&](int t, int half) { return bar0 + 8u * (2 * L::NP + 2 + 2 * t + half); };
-    auto odone = [&](int t) { return bar0 + 8u * (2 * L::NP + 6 + t); };
-    const uint32_t vhere = bar0 + 8u * (2 * L::NP + 8), vclear = vhere + 8, drain = vhere + 16;
+    auto sfull = [&](int b) { return bar0 + 8u * (2 * L::NP + b); };
+    auto pfull = [&](int b, int half) { return bar0 + 8u * (2 * L::NP + 2 + 2 * b + half); };
+    auto pvdone = [&](int t) { return bar0 + 8u * (2 * L::NP + 6 + t); };
+    const uint32_t vhere = pvdone(2), vclear = vhere + 8, drain = vhere + 16;
     uint32_t* tmem_slot = (uint32_t*)(sm + L::OFF_BAR + L::NBAR * 8);
     volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
 
@@ -223,7 +226,12 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
 
     if (tid == 0) {
         for (int e = 0; e < L::NP; e++) { bar_init(full(e), 1); bar_init(empty(e), 1); }
-        for (int t = 0; t < 2; t++) { bar_init(sfull(t), 1); bar_init(pfull(t, 0), 4); bar_init(pfull(t, 1), 4); bar_init(odone(t), 1); }
+        for (int b = 0; b < 2; b++) {
+            bar_init(sfull(b), 1);
+            bar_init(pfull(b, 0), 4);
+            bar_init(pfull(b, 1), 4);
+            bar_init(pvdone(b), 1);
+        }
         bar_init(vhere, 1);
         bar_init(vclear, 32);
         bar_init(drain, 1);
@@ -233,7 +241,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
     // Warp 0's work: pair i is V of tile i - 1, then K of tile i (what the MMA warp needs together).
     int blk = 0;
     bool bad = false;
-    uint32_t v0b = 0, v1b = 0;   // blocks of the tile before (its V follows one pair later)
+    uint32_t v0b = 0, v1b = 0;   // K blocks of the tile before (its V follows one pair later)
     auto load_pair = [&](int i) -> bool {
         const int e = i % L::NP;
         if ((i & 15) == 0) {   // the blocks of 16 tiles: lane = (tile, page)
@@ -253,7 +261,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
         if (lane == 0) {
             ok = bar_wait_short(empty(e), ((uint32_t)(i / L::NP) & 1u) ^ 1u, abort_flag);
             if (ok) {
-                bar_expect_tx(full(e), (i > 0 && i < nt ? 2 : 1) * L::ENTRY);
+                const bool has_v = i > 0, has_k = i < nt;
+                bar_expect_tx(full(e), ((int)has_v + (int)has_k) * L::ENTRY);
                 const uint32_t dst = su32(sm + L::OFF_RING + (size_t)e * 2 * L::ENTRY);
                 auto load = [&](uint32_t to, uint32_t b0, uint32_t b1) {
 #pragma unroll
@@ -263,8 +272,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
                     }
                 };
                 const uint32_t none = a.n_blocks;
-                if (i > 0) load(dst, v0b == none ? none : v0b + p.kv.n_head, v1b == none ? none : v1b + p.kv.n_head);
-                if (i < nt) load(dst + L::ENTRY, k0b, k1b);
+                if (has_v) load(dst, v0b == none ? none : v0b + p.kv.n_head, v1b == none ? none : v1b + p.kv.n_head);
+                if (has_k) load(dst + L::ENTRY, k0b, k1b);
             }
         }
         v0b = k0b;
@@ -344,24 +353,25 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
             const bool cut = nt > 0 && key0(nt - 1) + KT > c.len;
             // The loop is unrolled over the ring, so addresses and most phases are constants: this warp shares its
             // scheduler with two softmax warps, and every instruction between two products is idle tensor time.
-            auto scores = [&](int t, int e) {   // S_t = Q_t K^T with the K of pair e
+            auto scores = [&](int t, int b, int e) {   // S buffer b = Q_t K^T with the K of pair e
                 const uint32_t qd = desc_lo(sq + (uint32_t)t * 128 * D * 2, 16);
                 const uint32_t kd = desc_lo(ring + (uint32_t)(2 * e + 1) * L::ENTRY, 16);
-                const uint32_t st = tm + (uint32_t)t * KT;
+                const uint32_t st = tm + (uint32_t)b * KT;
                 mma_ss<HI, ID_S, false>(st, qd, kd);
 #pragma unroll
                 for (int kk = 1; kk < D / 16; kk++) {
                     const uint32_t off = (kk / 4 * 128 * L::RB + 32 * (kk % 4)) >> 4;   // 64-dim block, 16 dims in it
                     mma_ss<HI, ID_S, true>(st, qd + off, kd + off);
                 }
-                commit(sfull(t));
+                commit(sfull(b));
             };
-            auto values = [&](int t, int e, uint32_t add, uint32_t parity) -> bool {   // O_t += P_t V, 64 keys at a time
+            // O_t += P V with the V of pair e, 64 keys at a time
+            auto values = [&](int t, int b, int e, uint32_t add, uint32_t parity) -> bool {
                 const uint32_t vd = desc_lo(ring + (uint32_t)(2 * e) * L::ENTRY, KT * L::RB);
-                const uint32_t ot = tm + TM_O + (uint32_t)t * 128, pt = tm + (uint32_t)t * KT;
+                const uint32_t ot = tm + L::TM_O + (uint32_t)t * 128, pt = tm + (uint32_t)b * KT;
 #pragma unroll
                 for (int half = 0; half < 2; half++) {
-                    if (!wait_warp(pfull(t, half), parity, abort_flag)) return false;
+                    if (!wait_warp(pfull(b, half), parity, abort_flag)) return false;
                     tc_fence_after();
 #pragma unroll
                     for (int kk = half * KT / 32; kk < (half + 1) * KT / 32; kk++)
@@ -371,36 +381,51 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
             };
             bool ok = nt == 0 || wait_warp(full(0), 0, abort_flag);
             if (ok && nt > 0) {
-                scores(0, 0);
-                if (halves == 2) scores(1, 0);
+                scores(0, 0, 0);
+                if (halves == 2) scores(1, 1, 0);
                 commit(empty(0));
             }
-            uint32_t ring_phase = 0;
-            for (int j0 = 0; j0 < nt && ok; j0 += L::NP, ring_phase ^= 1u) {
+            // V of tile j and K of tile j + 1 are pair j + 1; at the last tile V has to be cleared first
+            auto wait_pair = [&](int j, int e, uint32_t parity) -> bool {
+                if (!wait_warp(full(e), parity, abort_flag)) return false;
+                if (j + 1 < nt || !cut) return true;
+                if (lane == 0) bar_arrive(vhere);
+                return wait_warp(vclear, 0, abort_flag);
+            };
+            uint32_t turn = 0;   // parity of how often the ring went round
+            if (halves == 2) {
+                for (int j0 = 0; j0 < nt && ok; j0 += L::NP, turn ^= 1u) {
 #pragma unroll
-                for (int u = 0; u < L::NP; u++) {
-                    const int j = j0 + u, e = (u + 1) % L::NP;   // tile j's V and tile j + 1's K are pair j + 1
-                    if (j >= nt || !ok) break;
-                    ok = wait_warp(full(e), u == L::NP - 1 ? ring_phase ^ 1u : ring_phase, abort_flag);
-                    const bool more = j + 1 < nt;
-                    if (!more && cut && ok) {
-                        if (lane == 0) bar_arrive(vhere);
-                        ok = wait_warp(vclear, 0, abort_flag);
-                    }
-                    ok = ok && values(0, e, (uint32_t)j, u & 1);
-                    if (!ok) break;
-                    if (more) scores(0, e);
-                    if (halves == 2) {
-                        ok = values(1, e, (uint32_t)j, u & 1);
+                    for (int u = 0; u < L::NP; u++) {
+                        const int j = j0 + u, e = u ^ 1;
+                        if (j >= nt) break;
+                        const bool more = j + 1 < nt;
+                        ok = wait_pair(j, e, turn ^ (uint32_t)u) && values(0, 0, e, (uint32_t)j, u);
                         if (!ok) break;
-                        if (more) scores(1, e);
+                        if (more) scores(0, 0, e);
+                        ok = values(1, 1, e, (uint32_t)j, u);
+                        if (!ok) break;
+                        if (more) scores(1, 1, e);
+                        commit(empty(e));
                     }
-                    if (more) commit(empty(e));
                 }
-            }
-            if (ok && nt > 0) {
-                commit(odone(0));
-                if (halves == 2) commit(odone(1));
+                commit(pvdone(0));
+                commit(pvdone(1));
+            } else {   // one row tile: the next scores go to the other buffer, before this tile's product
+                for (int j0 = 0; j0 < nt && ok; j0 += L::NP, turn ^= 1u) {
+#pragma unroll
+                    for (int u = 0; u < L::NP; u++) {
+                        const int j = j0 + u, e = u ^ 1;
+                        if (j >= nt) break;
+                        ok = wait_pair(j, e, turn ^ (uint32_t)u);
+                        if (!ok) break;
+                        if (j + 1 < nt) scores(0, e, e);
+                        ok = values(0, u, e, (uint32_t)j, turn);
+                        if (!ok) break;
+                        commit(pvdone(0));
+                        commit(empty(e));
+                    }
+                }
             }
             if (!ok) {
                 if (lane == 0) {
@@ -418,8 +443,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
             if (wait_warp(vhere, 0, abort_flag) && wait_warp(full(e), (uint32_t)(nt / L::NP) & 1u, abort_flag)) {
                 uint8_t* v = sm + L::OFF_RING + (size_t)e * 2 * L::ENTRY;
                 for (int at = 0; at < L::ATOMS; at++)
-                    for (int i = (c.len - key0(nt - 1)) * n16 + lane; i < KT * n16; i += 32)
-                        *(uint4*)(v + (size_t)at * KT * L::RB + i * 16) = make_uint4(0, 0, 0, 0);
+                    for (int k = (c.len - key0(nt - 1)) * n16 + lane; k < KT * n16; k += 32)
+                        *(uint4*)(v + (size_t)at * KT * L::RB + k * 16) = make_uint4(0, 0, 0, 0);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 bar_arrive(vclear);
             }
@@ -434,13 +459,15 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
         asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
         if ((warp - 4) / 4 < halves) {
             const int t = (warp - 4) / 4, q = warp & 3, r = 128 * t + 32 * q + lane;
-            const uint32_t tl = tmem + ((uint32_t)(32 * q) << 16), ts = tl + (uint32_t)t * KT, to = tl + TM_O + (uint32_t)t * 128;
+            const uint32_t tl = tmem + ((uint32_t)(32 * q) << 16), to = tl + L::TM_O + (uint32_t)t * 128;
             const int pos = c.total - c.n + (c.r0 + min(r, c.rows - 1)) / a.group;
             const int see_hi = min(c.len, pos + 1), see_lo = p.window ? pos - p.window + 1 : 0;
             float mref = NEG_INF, l = 0.0f;
             bool ok = true;
             for (int j = 0; j < nt && ok; j++) {
-                if (!bar_wait_short_warp(sfull(t), (uint32_t)j & 1u, abort_flag)) { ok = false; break; }
+                const int n = halves * j + t, b = n & 1;   // the scores' number, their buffer
+                const uint32_t ts = tl + (uint32_t)b * KT;
+                if (!bar_wait_short_warp(sfull(b), (uint32_t)n >> 1 & 1u, abort_flag)) { ok = false; break; }
                 tc_fence_after();
                 uint32_t x[4][32];
 #pragma unroll
@@ -475,7 +502,12 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
                 // raise the reference maximum of the warp's rows when one of them needs it
                 if (__any_sync(0xffffffffu, top > mref + TAU)) {
                     const float up = fmaxf(mref, top);
-                    if (j > 0) {   // (O is at rest: S of this tile was committed after the PV before it)
+                    if (j > 0) {
+                        // O must be at rest. With two row tiles it is: these scores were issued after the product before
+                        if (halves == 1) {
+                            if (!bar_wait_short_warp(pvdone(t), (uint32_t)(j - 1) & 1u, abort_flag)) { ok = false; break; }
+                            tc_fence_after();
+                        }
                         const float f = up == NEG_INF ? 1.0f : ex2(mref - up);
                         l *= f;
 #pragma unroll 1
@@ -512,7 +544,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
                             tmem_wait_st();
                             tc_fence_before();
                             __syncwarp();
-                            if (lane == 0) bar_arrive(pfull(t, k >> 1));
+                            if (lane == 0) bar_arrive(pfull(b, k >> 1));
                         }
                     }
                 };
@@ -520,7 +552,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
                 else weights(std::true_type{});
                 l += f2lo(sum) + f2hi(sum);
             }
-            if (ok && nt > 0) ok = bar_wait_short_warp(odone(t), 0, abort_flag);
+            if (ok && nt > 0) ok = bar_wait_short_warp(pvdone(t), halves == 2 ? 0u : (uint32_t)(nt - 1) & 1u, abort_flag);
             tc_fence_after();
             const bool mine = r < c.rows;
             const int tok = (c.r0 + r) / a.group, head = h * a.group + (c.r0 + r) % a.group;
