@@ -541,3 +541,15 @@ def test_bad_device_arrays_are_reported(ctx, ty, q):
     order(ctx).op_kv_append(cache, chunks, 1, x, kv, kv, qo, cos=ang, sin=ang)
     expect("position")
     attend(ctx, Case(ty, [q], [q + 7], 4, 2, 64))
+
+
+def test_example_of_streaming_requests():
+    """examples/chunked_decoder.py: prompts in pieces beside single tokens against the same prompts whole. Two BF16
+    layers: the paths round the same sums in another order, 2^-8 each time, over 2 layers' products and residuals."""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.abspath(__file__)), "..", "examples", "chunked_decoder.py")
+    spec = importlib.util.spec_from_file_location("chunked_decoder", path)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    assert mod.main(lengths=(130, 9, 65), pieces=(50, 1, 64)) < 4 * 2.0 ** -8
