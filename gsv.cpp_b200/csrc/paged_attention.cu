@@ -553,15 +553,31 @@ ChunkAttnPlan chunk_attention_plan(const ChunkAttnParams& p) {
     ChunkAttnPlan c;
     if (size == 2 && packed > 32 && p.scale != 0.0f) {
         // Many rows of 16-bit types: the tcgen05 kernel (a zero scale would multiply masked -infinities by 0 there).
-        // Splits only while there are fewer CTAs than SMs, and of 4 tiles at least.
+        // Row tiles per CTA and key splits by the shortest estimate, in units of 100 cycles: a key tile of 128 takes 29 for
+        // two row tiles and 20 for one, splitting and joining 150, CTAs run in waves of one per SM. Measured: 4 chunks
+        // of up to 570 rows over 1200 keys, 4 heads of 64: 16.4 us with one row tile, 23.9 with two in two splits; 512
+        // tokens over 8192 keys (16/4 x 128): 54 us with one row tile in two splits, 48 with two in four.
         c.tensor = true;
-        c.row_tile = 256;
-        c.tiles = (int)((packed + 255) / 256);
-        const int64_t units = (int64_t)p.batch.n_seq * c.tiles * p.kv.n_head;
         const int max_tiles = (p.batch.max_kv + 127) / 128;
-        int n = (int)(148 / units > 1 ? 148 / units : 1);
-        if (n > max_tiles / 4) n = max_tiles / 4;
-        if (n < 1) n = 1;
+        int64_t best = INT64_MAX;
+        int n = 1;
+        for (int rows = 256; rows >= 128; rows /= 2) {
+            if (rows == 128 && packed <= 128) break;   // (one row tile already)
+            const int64_t tiles = (packed + rows - 1) / rows, units = p.batch.n_seq * tiles * p.kv.n_head;
+            const int64_t fit = 148 / units < max_tiles ? 148 / units : max_tiles;
+            for (int64_t m : {(int64_t)1, fit}) {
+                if (m < 1) continue;
+                const int64_t waves = (units * m + 147) / 148, per = (max_tiles + m - 1) / m;
+                const int64_t cost = waves * per * (rows == 256 && packed > 128 ? 29 : 20) + (m > 1 ? 150 : 0);
+                if (cost < best) {
+                    best = cost;
+                    n = (int)m;
+                    c.row_tile = rows;
+                    c.tiles = (int)tiles;
+                }
+            }
+        }
+        const int64_t units = (int64_t)p.batch.n_seq * c.tiles * p.kv.n_head;
         c.split_tiles = (max_tiles + n - 1) / n;
         c.n_split = (max_tiles + c.split_tiles - 1) / c.split_tiles;
         c.key_tile = 128;
@@ -615,7 +631,10 @@ static void launch_join_rows(const ChunkAttnParams& p, const ChunkAttnPlan& c, b
     else if (c.row_tile == 16) go(k_chunk_join<T, D, 16>);
     else if (c.row_tile == 24) go(k_chunk_join<T, D, 24>);
     else if (c.row_tile == 32) go(k_chunk_join<T, D, 32>);
-    else if constexpr (sizeof(T) == 2) go(k_chunk_join<T, D, 256>);
+    else if constexpr (sizeof(T) == 2) {
+        if (c.row_tile == 128) go(k_chunk_join<T, D, 128>);
+        else go(k_chunk_join<T, D, 256>);
+    }
 }
 template <typename T>
 static void launch_join(const ChunkAttnParams& p, const ChunkAttnPlan& c, bool vec, cudaStream_t s) {

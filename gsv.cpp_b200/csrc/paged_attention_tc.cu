@@ -31,7 +31,7 @@ namespace {
 using namespace tc;
 
 constexpr int KT = 128;                 // keys per tile
-constexpr int ROWS = 256;               // packed rows per CTA
+constexpr int ROWS = 256;               // packed rows per CTA, two row tiles (one of 128 when the call has few CTAs)
 constexpr int THREADS = 384;
 constexpr float TAU = 8.0f;             // log2 headroom of P above the row's reference maximum
 
@@ -54,7 +54,7 @@ struct Smem {
 struct TcArgs {
     ChunkAttnParams p;
     CUtensorMap map;   // pool as [block][64][D], box [1][64][min(D, 64)]
-    int group, tiles, n_split, split_tiles, n_blocks;
+    int group, row_tile, tiles, n_split, split_tiles, n_blocks;
     float c;           // |scale| * log2(e)
     bool negate;       // scale < 0: Q enters negated
     bool vec_q, vec_out;
@@ -217,7 +217,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
     int first_page = 0;
     if (warp == 0 && !p.window) first_page = tab[min(v0 * 2 + lane, p.batch.max_pages - 1)];
     ChunkRange c;
-    if (!chunk_range(p, s, tile, a.group, ROWS, KT, tid == 0 && sp == 0 && h == 0 && tile == 0, c)) return;
+    if (!chunk_range(p, s, tile, a.group, a.row_tile, KT, tid == 0 && sp == 0 && h == 0 && tile == 0, c)) return;
     const int n_act = max(1, (c.n_tiles + a.split_tiles - 1) / a.split_tiles);
     if (sp >= n_act) return;
     const int nt = min(c.n_tiles, v0 + a.split_tiles) - v0;   // this CTA's key tiles
@@ -293,6 +293,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
     // Q, swizzled as the MMA reads it ([tile][64-dim block][128 rows][RB bytes]), zero past the CTA's rows; four loads
     // in flight per thread (one at a time this was a third of a short call)
     constexpr int STEP = THREADS - 32;
+    const int tok0 = c.r0 / a.group, rem0 = c.r0 % a.group;
+    const float inv = 1.0f / (float)a.group;   // (x + 1/2) / group is far enough from whole numbers for x < 2^20
     for (int i0 = tid - 32; warp > 0 && i0 < 128 * halves * (D / 8); i0 += 4 * STEP) {
         uint4 u[4];
 #pragma unroll
@@ -300,8 +302,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
             const int i = i0 + m * STEP, r = i / (D / 8), pc = i % (D / 8);
             u[m] = make_uint4(0, 0, 0, 0);
             if (r < c.rows) {
-                const int tok = (c.r0 + r) / a.group, j = (c.r0 + r) % a.group;
-                const T* src = (const T*)p.q + (int64_t)(c.row0 + tok) * p.q_stride + (int64_t)(h * a.group + j) * D + pc * 8;
+                const int up = (int)(((float)(rem0 + r) + 0.5f) * inv), j = rem0 + r - up * a.group;
+                const T* src = (const T*)p.q + (int64_t)(c.row0 + tok0 + up) * p.q_stride + (int64_t)(h * a.group + j) * D + pc * 8;
                 if (a.vec_q) {
                     u[m] = *(const uint4*)src;
                 } else {
@@ -558,7 +560,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
             const int tok = (c.r0 + r) / a.group, head = h * a.group + (c.r0 + r) % a.group;
             const int64_t row = c.row0 + tok;
             const int64_t unit = ((int64_t)s * a.tiles + tile) * p.kv.n_head + h;
-            float* part = p.part + unit * a.n_split * (ROWS * (D + 2));
+            float* part = p.part + unit * a.n_split * (a.row_tile * (D + 2));
             const float il = l > 0.0f || l != l ? 1.0f / l : 0.0f;
             if (ok) {
 #pragma unroll 1
@@ -590,7 +592,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
                             }
                         }
                     } else {
-                        float* dst = part + ((int64_t)sp * ROWS + r) * D + d;
+                        float* dst = part + ((int64_t)sp * a.row_tile + r) * D + d;
 #pragma unroll
                         for (int i = 0; i < 32; i += 4)
                             *(uint4*)(dst + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
@@ -598,7 +600,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
                 }
                 if (mine) {
                     if (n_act > 1)
-                        *(float2*)(part + (int64_t)a.n_split * ROWS * D + 2 * ((int64_t)sp * ROWS + r)) = make_float2(mref, l);
+                        *(float2*)(part + (int64_t)a.n_split * a.row_tile * D + 2 * ((int64_t)sp * a.row_tile + r)) = make_float2(mref, l);
                     else if (p.lse)
                         p.lse[row * p.n_q_head + head] = mref == NEG_INF ? NEG_INF : (mref + log2f(l)) * LN2;
                 }
@@ -642,6 +644,7 @@ bool launch_chunk_attention_tc(const ChunkAttnParams& p, const ChunkAttnPlan& pl
     TcArgs a;
     a.p = p;
     a.group = p.n_q_head / p.kv.n_head;
+    a.row_tile = plan.row_tile;
     a.tiles = plan.tiles;
     a.n_split = plan.n_split;
     a.split_tiles = plan.split_tiles;

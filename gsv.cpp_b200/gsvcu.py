@@ -208,9 +208,19 @@ def _kv_type(dtype, what):
     return ty
 
 
+_INT32 = set()   # torch.int32, once met
+
+
+def _is_int32(dtype):
+    if str(dtype) == "torch.int32":
+        _INT32.add(dtype)
+        return True
+    return False
+
+
 def _ints(t, shape, what):
     """Device address of a contiguous int32 tensor of this shape."""
-    if t.shape != shape or not t.is_contiguous() or str(t.dtype) != "torch.int32":
+    if t.shape != shape or not t.is_contiguous() or not (t.dtype in _INT32 or _is_int32(t.dtype)):
         raise ValueError(f"{what}: contiguous int32 {list(shape)} expected, got {t.dtype} {list(t.shape)}")
     return t.data_ptr()
 
@@ -222,11 +232,12 @@ def _floats(t, shape, what):
     return t.data_ptr()
 
 
-def _rows(t, n_rows, heads, head_dim, what):
-    """Stride between the rows of a [rows][heads][head_dim] device tensor whose heads lie side by side."""
-    if t.shape != (n_rows, heads, head_dim):
-        raise ValueError(f"{what}: [{n_rows}][{heads}][{head_dim}] expected, got {list(t.shape)}")
+def _row_stride(t, shape, what):
+    """Stride between the rows of a device tensor of this [rows][heads][head_dim] shape, heads side by side."""
+    if t.shape != shape:
+        raise ValueError(f"{what}: {list(shape)} expected, got {list(t.shape)}")
     row, head, one = t.stride()
+    n_rows, heads, head_dim = shape
     if one != 1 or (head != head_dim and heads > 1):
         raise ValueError(f"{what}: each row's heads must be contiguous")
     if n_rows <= 1:
@@ -485,12 +496,13 @@ class Context:
         None); cos / sin: f32 [positions][rotated / 2], pos: int32 [n_rows] (None: the cache positions).
         gsvcu_op_kv_append."""
         n, D, H = chunks.n_rows, cache.head_dim, cache.n_kv_head
-        ty = k.dtype
-        ks, vs = _rows(k, n, H, D, "k"), _rows(v, n, H, D, "v")
+        ty, shape = k.dtype, (n, H, D)
+        ks, vs = _row_stride(k, shape, "k"), _row_stride(v, shape, "v")
         nq = qp = qs = op = os_ = 0
         if q is not None:
             nq, qp, op = q.shape[1], q.data_ptr(), q_out.data_ptr()
-            qs, os_ = _rows(q, n, nq, D, "q"), _rows(q_out, n, nq, D, "q_out")
+            shape = (n, nq, D)
+            qs, os_ = _row_stride(q, shape, "q"), _row_stride(q_out, shape, "q_out")
             if q_out.dtype != cache.dtype:
                 raise ValueError("q_out must have the cache's type")
         if v.dtype != ty or (q is not None and q.dtype != ty):
@@ -510,7 +522,8 @@ class Context:
         sqrt(head dim); prefix: int32 [n_seq] keys that every row sees; window: keys a row looks back on (0: all);
         lse: f32 [n_rows][heads]. gsvcu_op_chunk_attention."""
         n, D, nq = chunks.n_rows, cache.head_dim, q.shape[1]
-        qs, os_ = _rows(q, n, nq, D, "q"), _rows(out, n, nq, D, "out")
+        shape = (n, nq, D)
+        qs, os_ = _row_stride(q, shape, "q"), _row_stride(out, shape, "out")
         if q.dtype != cache.dtype or out.dtype != cache.dtype:
             raise ValueError("q and out must have the cache's type")
         self._check(self.lib.gsvcu_op_chunk_attention(
