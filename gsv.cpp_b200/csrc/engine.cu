@@ -1925,30 +1925,25 @@ int gsvcu_op_chunk_attention(gsvcu_ctx* ctx, const gsvcu_paged_kv* kv, const gsv
     if ((int64_t)batch->n_seq * plan.tiles * kv->n_kv_head * plan.n_split > INT32_MAX)
         return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_chunk_attention: batch too large for one launch");
     DeviceGuard g(ctx->device);
-    if (plan.part_floats > ctx->op_split_n) {
-        CKC(ctx, cudaStreamSynchronize(ctx->stream));
-        if (ctx->op_split) cudaFree(ctx->op_split);
-        ctx->op_split = nullptr;
-        ctx->op_split_n = 0;
-        if (cudaMalloc((void**)&ctx->op_split, plan.part_floats * 4) != cudaSuccess) {
+    // Scratch at least doubles when it grows, and what it replaces stays until the context ends: captured graphs
+    // may hold its address.
+    auto grow = [&](void** at, size_t* have, size_t need) -> int {
+        if (need <= *have) return GSVCU_OK;
+        const size_t n = std::max(need, 2 * *have);
+        void* fresh = nullptr;
+        if (cudaMalloc(&fresh, n * 4) != cudaSuccess) {
             cudaGetLastError();
-            ctx->op_split = nullptr;
             return ctx->fail(GSVCU_ERR_OOM, "gsvcu_op_chunk_attention: no memory for the split results");
         }
-        ctx->op_split_n = plan.part_floats;
-    }
+        if (*at) ctx->wallocs.push_back(*at);
+        *at = fresh;
+        *have = n;
+        return GSVCU_OK;
+    };
+    TRY(grow((void**)&ctx->op_split, &ctx->op_split_n, plan.part_floats));
     if (plan.arrivals > ctx->op_arrived_n) {
-        CKC(ctx, cudaStreamSynchronize(ctx->stream));
-        if (ctx->op_arrived) cudaFree(ctx->op_arrived);
-        ctx->op_arrived = nullptr;
-        ctx->op_arrived_n = 0;
-        if (cudaMalloc((void**)&ctx->op_arrived, plan.arrivals * sizeof(int32_t)) != cudaSuccess) {
-            cudaGetLastError();
-            ctx->op_arrived = nullptr;
-            return ctx->fail(GSVCU_ERR_OOM, "gsvcu_op_chunk_attention: no memory for the arrival counters");
-        }
-        ctx->op_arrived_n = plan.arrivals;
-        CKC(ctx, cudaMemsetAsync(ctx->op_arrived, 0, plan.arrivals * sizeof(int32_t), ctx->stream));
+        TRY(grow((void**)&ctx->op_arrived, &ctx->op_arrived_n, plan.arrivals));
+        CKC(ctx, cudaMemsetAsync(ctx->op_arrived, 0, ctx->op_arrived_n * sizeof(int32_t), ctx->stream));
     }
     p.part = ctx->op_split;
     p.arrived = ctx->op_arrived;
@@ -2106,14 +2101,14 @@ int gsvcu_sync(gsvcu_ctx* ctx) {
     CKC(ctx, cudaMemcpyAsync(word, ctx->att_err + 1, sizeof(word), cudaMemcpyDeviceToHost, ctx->stream));
     CKC(ctx, cudaStreamSynchronize(ctx->stream));
     const int32_t oerr = word[0], perr = word[2];
-    if (perr) {
-        CKC(ctx, cudaMemsetAsync(ctx->att_err + 3, 0, sizeof(int32_t), ctx->stream));
-        CKC(ctx, cudaStreamSynchronize(ctx->stream));
-    }
     if (oerr) {
         CKC(ctx, cudaMemsetAsync(ctx->att_err + 1, 0, sizeof(int32_t), ctx->stream));
         CKC(ctx, cudaStreamSynchronize(ctx->stream));
         return ctx->fail(GSVCU_ERR_CUDA, "gsvcu_op_decode_attention: staged K/V never arrived (bounded wait gave up)");
+    }
+    if (perr) {   // (with both, this one waits for the next call)
+        CKC(ctx, cudaMemsetAsync(ctx->att_err + 3, 0, sizeof(int32_t), ctx->stream));
+        CKC(ctx, cudaStreamSynchronize(ctx->stream));
     }
     if (perr & PAGED_WAIT)
         return ctx->fail(GSVCU_ERR_CUDA, "gsvcu_op_chunk_attention: a bounded wait gave up");

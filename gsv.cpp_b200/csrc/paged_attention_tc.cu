@@ -253,7 +253,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
             blk = a.n_blocks;   // past the pool: zero fill
             if (jj < nt) {
                 const int key = key0(jj) + PAGE * (lane & 1);
-                if (key < c.len) {
+                if (c.sees(key)) {
                     const int page = i == 0 && !p.window ? first_page : tab[key / PAGE];
                     if (page >= 0 && page < p.kv.n_page) blk = ((page * p.kv.n_layer + p.kv.layer) * 2) * p.kv.n_head + h;
                     else bad = true;

@@ -28,8 +28,11 @@ __device__ __forceinline__ float ex2(float x) {
 struct ChunkRange {
     int row0, n, total, len;   // first packed row and rows of the chunk; kv_len as given, and cut to the table
     int r0, rows, p0, p1;      // the tile's packed rows, positions of the first and the last
-    int np, n1, t_lo, n_tiles;
+    int np, lo, hi, n1, t_lo, n_tiles;
     __device__ __forceinline__ int tile_of(int v) const { return v < n1 ? v : v - n1 + t_lo; }
+    // Whether some row of the tile sees a key of the page that starts at `key` (others are not looked up: with a window
+    // their place in the table may be stale).
+    __device__ __forceinline__ bool sees(int key) const { return key < np || (key < hi && key + PAGE > lo); }
 };
 
 // False: the tile has no rows. What is out of bounds is cut off, and reported when `report`.
@@ -51,15 +54,16 @@ __device__ __forceinline__ bool chunk_range(const ChunkAttnParams& p, int s, int
     c.p0 = c.total - c.n + c.r0 / group;
     c.p1 = c.total - c.n + (c.r0 + c.rows - 1) / group;
     c.np = max(0, min(np, c.len));
-    int hi = max(0, min(c.len, c.p1 + 1)), lo = p.window ? max(0, c.p0 - p.window + 1) : 0;
-    if (hi <= lo) lo = hi = 0;
+    c.hi = max(0, min(c.len, c.p1 + 1));
+    c.lo = p.window ? max(0, c.p0 - p.window + 1) : 0;
+    if (c.hi <= c.lo) c.lo = c.hi = 0;
     int t_hi;
-    if (c.np >= lo) {
+    if (c.np >= c.lo) {
         c.t_lo = c.n1 = 0;
-        t_hi = (max(c.np, hi) + key_tile - 1) / key_tile;
+        t_hi = (max(c.np, c.hi) + key_tile - 1) / key_tile;
     } else {
-        c.t_lo = lo / key_tile;
-        t_hi = (hi + key_tile - 1) / key_tile;
+        c.t_lo = c.lo / key_tile;
+        t_hi = (c.hi + key_tile - 1) / key_tile;
         c.n1 = min((c.np + key_tile - 1) / key_tile, c.t_lo);
     }
     c.n_tiles = c.n1 + t_hi - c.t_lo;

@@ -218,22 +218,28 @@ def _is_int32(dtype):
     return False
 
 
-def _ints(t, shape, what):
-    """Device address of a contiguous int32 tensor of this shape."""
+def _ints(t, shape, what, device):
+    """Address of a contiguous int32 tensor of this shape on CUDA device `device`."""
+    if t.get_device() != device:
+        raise ValueError(f"{what}: expected on CUDA device {device}, got {t.device}")
     if t.shape != shape or not t.is_contiguous() or not (t.dtype in _INT32 or _is_int32(t.dtype)):
         raise ValueError(f"{what}: contiguous int32 {list(shape)} expected, got {t.dtype} {list(t.shape)}")
     return t.data_ptr()
 
 
-def _floats(t, shape, what):
-    """Device address of a contiguous float32 tensor of this shape."""
+def _floats(t, shape, what, device):
+    """Address of a contiguous float32 tensor of this shape on CUDA device `device`."""
+    if t.get_device() != device:
+        raise ValueError(f"{what}: expected on CUDA device {device}, got {t.device}")
     if t.shape != shape or not t.is_contiguous() or _kv_type(t.dtype, what) != KV_F32:
         raise ValueError(f"{what}: contiguous float32 {list(shape)} expected, got {t.dtype} {list(t.shape)}")
     return t.data_ptr()
 
 
-def _row_stride(t, shape, what):
-    """Stride between the rows of a device tensor of this [rows][heads][head_dim] shape, heads side by side."""
+def _row_stride(t, shape, what, device):
+    """Stride between the rows of a [rows][heads][head_dim] tensor on CUDA device `device`, heads side by side."""
+    if t.get_device() != device:
+        raise ValueError(f"{what}: expected on CUDA device {device}, got {t.device}")
     if t.shape != shape:
         raise ValueError(f"{what}: {list(shape)} expected, got {list(t.shape)}")
     row, head, one = t.stride()
@@ -253,7 +259,7 @@ class PagedKV:
     def __init__(self, pool):
         if pool.dim() != 6 or pool.shape[2] != 2 or pool.shape[4] != 64 or not pool.is_contiguous():
             raise ValueError(f"pool: contiguous [page][layer][2][kv head][64][head dim] expected, got {list(pool.shape)}")
-        self.pool, self.dtype = pool, pool.dtype
+        self.pool, self.dtype, self.device = pool, pool.dtype, pool.get_device()
         self.n_kv_head, self.head_dim = pool.shape[3], pool.shape[5]
         self.desc = PagedKVDesc(pool.data_ptr(), _kv_type(pool.dtype, "pool"), pool.shape[0], pool.shape[1],
                                 pool.shape[3], pool.shape[5])
@@ -270,10 +276,11 @@ class ChunkBatch:
         if block_table.dim() != 2:
             raise ValueError("block_table: [n_seq][max_pages] expected")
         self.keep = (row_start, kv_len, block_table)
-        self.n_seq, self.n_rows = n_seq, n_rows
-        self.desc = ChunkBatchDesc(_ints(row_start, (n_seq + 1,), "row_start"), _ints(kv_len, (n_seq,), "kv_len"),
-                                   _ints(block_table, (n_seq, block_table.shape[1]), "block_table"), n_seq,
-                                   block_table.shape[1], n_rows, max_chunk, max_kv)
+        self.n_seq, self.n_rows, self.device = n_seq, n_rows, row_start.get_device()
+        self.desc = ChunkBatchDesc(
+            _ints(row_start, (n_seq + 1,), "row_start", self.device), _ints(kv_len, (n_seq,), "kv_len", self.device),
+            _ints(block_table, (n_seq, block_table.shape[1]), "block_table", self.device), n_seq, block_table.shape[1],
+            n_rows, max_chunk, max_kv)
         self.ref = C.byref(self.desc)
 
 
@@ -317,6 +324,7 @@ class Context:
             raise GsvcuError(rc, f"cannot open CUDA device {device} (needs an sm_100 GPU)")
         self.h = h
         self.hp = None
+        self.device = device
 
     def close(self):
         if getattr(self, "h", None):
@@ -493,16 +501,18 @@ class Context:
     def op_kv_append(self, cache: PagedKV, chunks: ChunkBatch, layer, q, k, v, q_out, cos=None, sin=None, pos=None,
                      pairs=False):
         """Append k, v rows [n_rows][kv heads][head dim] to the paged cache and rotate q into q_out (both may be
-        None); cos / sin: f32 [positions][rotated / 2], pos: int32 [n_rows] (None: the cache positions).
-        gsvcu_op_kv_append."""
-        n, D, H = chunks.n_rows, cache.head_dim, cache.n_kv_head
+        None); cos / sin: f32 [positions][rotated / 2], pos: int32 [n_rows] (None: the cache positions). Runs on the
+        context's stream (stream_handle()). gsvcu_op_kv_append."""
+        n, D, H, dev = chunks.n_rows, cache.head_dim, cache.n_kv_head, self.device
+        if cache.device != dev or chunks.device != dev:
+            raise ValueError(f"cache and batch must be on CUDA device {dev}")
         ty, shape = k.dtype, (n, H, D)
-        ks, vs = _row_stride(k, shape, "k"), _row_stride(v, shape, "v")
+        ks, vs = _row_stride(k, shape, "k", dev), _row_stride(v, shape, "v", dev)
         nq = qp = qs = op = os_ = 0
         if q is not None:
             nq, qp, op = q.shape[1], q.data_ptr(), q_out.data_ptr()
             shape = (n, nq, D)
-            qs, os_ = _row_stride(q, shape, "q"), _row_stride(q_out, shape, "q_out")
+            qs, os_ = _row_stride(q, shape, "q", dev), _row_stride(q_out, shape, "q_out", dev)
             if q_out.dtype != cache.dtype:
                 raise ValueError("q_out must have the cache's type")
         if v.dtype != ty or (q is not None and q.dtype != ty):
@@ -511,25 +521,27 @@ class Context:
         if cos is not None:
             shape = cos.shape
             n_pos, rot = shape[0], 2 * shape[1]
-            cp, sp = _floats(cos, shape, "cos"), _floats(sin, shape, "sin")
+            cp, sp = _floats(cos, shape, "cos", dev), _floats(sin, shape, "sin", dev)
         self._check(self.lib.gsvcu_op_kv_append(
             self.h, cache.ref, chunks.ref, layer, _kv_type(ty, "k"), nq, qp, qs, k.data_ptr(), ks, v.data_ptr(), vs, cp, sp,
-            n_pos, rot, 1 if pairs else 0, None if pos is None else _ints(pos, (n,), "pos"), op, os_))
+            n_pos, rot, 1 if pairs else 0, None if pos is None else _ints(pos, (n,), "pos", dev), op, os_))
 
     def op_chunk_attention(self, cache: PagedKV, chunks: ChunkBatch, layer, q, out, scale=None, prefix=None, window=0,
                            lse=None):
         """Attention of the batch's rows q [n_rows][heads][head dim] over the paged cache into out; scale None: 1 /
         sqrt(head dim); prefix: int32 [n_seq] keys that every row sees; window: keys a row looks back on (0: all);
-        lse: f32 [n_rows][heads]. gsvcu_op_chunk_attention."""
-        n, D, nq = chunks.n_rows, cache.head_dim, q.shape[1]
+        lse: f32 [n_rows][heads]. Runs on the context's stream (stream_handle()). gsvcu_op_chunk_attention."""
+        n, D, nq, dev = chunks.n_rows, cache.head_dim, q.shape[1], self.device
+        if cache.device != dev or chunks.device != dev:
+            raise ValueError(f"cache and batch must be on CUDA device {dev}")
         shape = (n, nq, D)
-        qs, os_ = _row_stride(q, shape, "q"), _row_stride(out, shape, "out")
+        qs, os_ = _row_stride(q, shape, "q", dev), _row_stride(out, shape, "out", dev)
         if q.dtype != cache.dtype or out.dtype != cache.dtype:
             raise ValueError("q and out must have the cache's type")
         self._check(self.lib.gsvcu_op_chunk_attention(
             self.h, cache.ref, chunks.ref, layer, nq, q.data_ptr(), qs, D ** -0.5 if scale is None else scale, window,
-            None if prefix is None else _ints(prefix, (chunks.n_seq,), "prefix"), out.data_ptr(), os_,
-            None if lse is None else _floats(lse, (n, nq), "lse")))
+            None if prefix is None else _ints(prefix, (chunks.n_seq,), "prefix", dev), out.data_ptr(), os_,
+            None if lse is None else _floats(lse, (n, nq), "lse", dev)))
 
     def op_sample(self, logits, V, eos, steps, rng_states, prev=None, top_k=15, top_p=1.0, temperature=1.0, rep=1.35):
         """logits: torch CUDA [B][V]; prev: list of int arrays (repetition windows). Returns (tokens, new states)."""

@@ -279,7 +279,8 @@ typedef struct {
 
 /* The batch (device arrays): sequence s owns the packed rows row_start[s] .. row_start[s + 1] - 1
  * (row_start [n_seq + 1], ascending), holds kv_len[s] keys with these rows and keeps key c in page
- * block_table[s][c / 64], slot c % 64 (block_table [n_seq][max_pages], max_pages <= 2^24; entries past its keys are not used).
+ * block_table[s][c / 64], slot c % 64 (block_table [n_seq][max_pages], max_pages <= 2^24; entries past its keys, and of pages that no row of the chunk sees,
+ * are not used).
  * Row i of n is the token at cache position kv_len[s] - n + i. Host sizes: n_rows packed rows, max_chunk at
  * least the longest chunk, max_kv at least the longest kv_len (0: max_pages * 64); the closer these are, the
  * better the work is cut up. A page outside the pool, or lengths outside these sizes, touch no memory
@@ -309,8 +310,9 @@ int gsvcu_op_kv_append(gsvcu_ctx* ctx, const gsvcu_paged_kv* kv, const gsvcu_chu
  * p - window): causal with a prefix that all rows see (prefix_dev null: none; the whole length: no mask) and a
  * sliding window. q and out rows have the cache's type (strides in elements, out not overlapping q);
  * lse_dev (may be null) [n_rows][n_q_head] gets the natural logarithm of each row's sum of exp(scale q.k).
- * A row that sees no key gives 0 and -infinity. Scores, softmax and sums are F32. Keys from kv_len on are
- * never read; keys below it must be finite where any row of the chunk may see them. */
+ * A row that sees no key gives 0 and -infinity. Scores, softmax and sums are F32. What the pages hold from kv_len
+ * on does not matter, nor do pages that no row sees; in the other pages every key and value has to be finite (a
+ * value that is not reaches rows that do not see it, as 0 times infinity). */
 int gsvcu_op_chunk_attention(gsvcu_ctx* ctx, const gsvcu_paged_kv* kv, const gsvcu_chunk_batch* batch, int32_t layer,
                              int32_t n_q_head, const void* q_dev, int64_t q_stride, float scale, int32_t window,
                              const int32_t* prefix_dev, void* out_dev, int64_t out_stride, float* lse_dev);

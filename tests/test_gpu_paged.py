@@ -268,6 +268,35 @@ def test_masked_values_may_be_anything(ctx):
         assert torch.equal(a, b) and torch.equal(a, d)
 
 
+@pytest.mark.parametrize("ty,dim,q", [("f16", 32, 1), ("bf16", 128, 5), ("f32", 64, 40), ("f16", 64, 150), ("bf16", 128, 300)])
+@pytest.mark.parametrize("prefix", [None, 70])
+def test_pages_behind_the_window_may_be_gone(ctx, ty, dim, q, prefix):
+    """A server with a sliding window gives back pages that no row sees any more: their table entries are stale and
+    what they hold is another sequence's, or NaN. Neither is touched nor reported."""
+    c = Case(ty, [q, 1], [2000, 900], 8, 2, dim)
+    window = 130
+    for s, (n, total) in enumerate(zip(c.q_len, c.kv_len)):
+        first = total - n - window + 1
+        for j in range(-(-total // PAGE)):
+            seen = (j + 1) * PAGE > first or (prefix and j * PAGE < prefix)
+            if not seen:
+                c.pool[int(c.table[s, j])] = float("nan")
+    x = c.rand(c.rows, c.heads, c.dim)
+    full = c.table.clone()
+    for s, (n, total) in enumerate(zip(c.q_len, c.kv_len)):
+        for j in range(-(-total // PAGE)):
+            if (j + 1) * PAGE <= total - n - window + 1 and not (prefix and j * PAGE < prefix):
+                c.table[s, j] = -7
+    out = torch.empty_like(x)
+    pf = None if prefix is None else torch.tensor([prefix] * 2, dtype=torch.int32, device="cuda")
+    cache, chunks = c.objects()
+    order(ctx).op_chunk_attention(cache, chunks, c.layer, x, out, prefix=pf, window=window)
+    ctx.sync()
+    c.table.copy_(full)
+    c.pool.nan_to_num_(0.0)
+    check_attention(c, x, out, None, dim ** -0.5, window, None if prefix is None else [prefix] * 2)
+
+
 def test_nothing_to_do(ctx):
     """No rows, or no sequences: nothing is touched, nothing is launched."""
     import gsvcu
@@ -484,6 +513,11 @@ def test_refusals(ctx):
     cos = torch.zeros(80, 40, device="cuda")
     with pytest.raises(gsvcu.GsvcuError):   # rotates more than a head holds
         ctx.op_kv_append(cache, chunks, 1, q, kv, kv, out, cos=cos, sin=cos)
+    for bad in (dict(q=q.cpu()), dict(out=out.cpu()), dict(cache=gsvcu.PagedKV(c.pool.cpu()))):   # host memory
+        with pytest.raises(ValueError):
+            ctx.op_chunk_attention(bad.get("cache", cache), chunks, 1, bad.get("q", q), bad.get("out", out))
+    with pytest.raises(ValueError):
+        gsvcu.ChunkBatch(c.row_start, c.kv.cpu(), c.table, 2, 2)
     odd = torch.empty(3, 1, 2, 1, PAGE, 48, dtype=torch.float16, device="cuda")
     one = torch.empty(2, 1, 48, dtype=torch.float16, device="cuda")
     with pytest.raises(gsvcu.GsvcuError) as e:
