@@ -431,6 +431,7 @@ struct gsvcu_ctx {
     size_t op_split_n = 0;
     int32_t* op_arrived = nullptr;    // its arrival counters, zero between launches
     size_t op_arrived_n = 0;
+    uint64_t op_chunk_ready = 0;      // its kernels whose shared-memory limit is raised
     // set when a bounded wait in a kernel gave up: [0] decode attention in the decode steps (read and
     // cleared with the slot state), [1] gsvcu_op_decode_attention (read and cleared by gsvcu_sync),
     // [2] the tcgen05 prefill GEMM (read and cleared at the end of each prefill pass),
@@ -1371,8 +1372,7 @@ int gsvcu_create(int device, gsvcu_ctx** out) {
     bool dense_usable = false;
     if (gemm_q8_init_device() != cudaSuccess || gemm_tc_init_device() != cudaSuccess ||
         gemm_fx_init_device() != cudaSuccess || attention_init_device() != cudaSuccess ||
-        logits_init_device() != cudaSuccess || chunk_attention_init_device() != cudaSuccess ||
-        dense_init_device(&dense_usable) != cudaSuccess) {
+        logits_init_device() != cudaSuccess || dense_init_device(&dense_usable) != cudaSuccess) {
         cudaGetLastError();
         return GSVCU_ERR_CUDA;
     }
@@ -1947,8 +1947,11 @@ int gsvcu_op_chunk_attention(gsvcu_ctx* ctx, const gsvcu_paged_kv* kv, const gsv
     }
     p.part = ctx->op_split;
     p.arrived = ctx->op_arrived;
-    const int kernels = launch_chunk_attention(p, plan, ctx->stream);
-    if (kernels == 0) return ctx->fail(GSVCU_ERR_CUDA, "gsvcu_op_chunk_attention: tensor map encoding failed");
+    const int kernels = launch_chunk_attention(p, plan, &ctx->op_chunk_ready, ctx->stream);
+    if (kernels == 0) {
+        cudaGetLastError();
+        return ctx->fail(GSVCU_ERR_CUDA, "gsvcu_op_chunk_attention: no tensor map or shared memory");
+    }
     CKC(ctx, cudaGetLastError());
     ctx->launches += kernels;
     return GSVCU_OK;

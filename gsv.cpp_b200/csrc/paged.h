@@ -70,10 +70,17 @@ struct ChunkAttnPlan {
     size_t part_floats = 0, arrivals = 0;
 };
 ChunkAttnPlan chunk_attention_plan(const ChunkAttnParams& p);
-// Kernels launched; 0: none (no tensor map).
-int launch_chunk_attention(const ChunkAttnParams& p, const ChunkAttnPlan& plan, cudaStream_t s);
-bool launch_chunk_attention_tc(const ChunkAttnParams& p, const ChunkAttnPlan& plan, cudaStream_t s);
-cudaError_t chunk_attention_init_device();   // dynamic shared-memory limits on the current device
-cudaError_t chunk_attention_tc_init_device();
+// Kernels launched; 0: none (no tensor map, or no room for the shared memory). `ready`: the caller's record of the
+// kernels whose shared-memory limit is raised on its device (zero at first; raising all 42 with the context would add
+// 16 ms to it).
+int launch_chunk_attention(const ChunkAttnParams& p, const ChunkAttnPlan& plan, uint64_t* ready, cudaStream_t s);
+bool launch_chunk_attention_tc(const ChunkAttnParams& p, const ChunkAttnPlan& plan, uint64_t* ready, cudaStream_t s);
+template <typename K>
+inline bool raise_smem(K kernel, size_t bytes, uint64_t* ready, int bit) {
+    if (*ready >> bit & 1u) return true;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) return false;
+    *ready |= (uint64_t)1 << bit;
+    return true;
+}
 
 }  // namespace gsvcu

@@ -536,19 +536,6 @@ void pick(int dtype, int dim, int row_tile, F f) {
 
 }  // namespace
 
-cudaError_t chunk_attention_init_device() {
-    cudaError_t e = cudaSuccess;
-    for (int ty : {GSVCU_KV_F16, GSVCU_KV_F32, GSVCU_KV_BF16})
-        for (int dim : {32, 64, 128})
-            for (int rows : {8, 16, 24, 32})
-                pick(ty, dim, rows, [&](auto k, size_t smem) {
-                    const cudaError_t r = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-                    if (e == cudaSuccess) e = r;
-                });
-    const cudaError_t r = chunk_attention_tc_init_device();
-    return e == cudaSuccess ? r : e;
-}
-
 ChunkAttnPlan chunk_attention_plan(const ChunkAttnParams& p) {
     const int D = p.kv.head_dim, size = p.kv.kv_dtype == GSVCU_KV_F32 ? 4 : 2;
     const int kt = key_tile(D, size);
@@ -646,11 +633,11 @@ static void launch_join(const ChunkAttnParams& p, const ChunkAttnPlan& c, bool v
     else launch_join_rows<T, 128>(p, c, vec, s);
 }
 
-int launch_chunk_attention(const ChunkAttnParams& p, const ChunkAttnPlan& plan, cudaStream_t s) {
+int launch_chunk_attention(const ChunkAttnParams& p, const ChunkAttnPlan& plan, uint64_t* ready, cudaStream_t s) {
     const size_t size = p.kv.kv_dtype == GSVCU_KV_F32 ? 4 : 2;
     const bool vec_out = ((uintptr_t)p.out & 15) == 0 && (p.out_stride * (int64_t)size) % 16 == 0;
     if (plan.tensor) {
-        if (!launch_chunk_attention_tc(p, plan, s)) return 0;
+        if (!launch_chunk_attention_tc(p, plan, ready, s)) return 0;
     } else {
         SplitArgs a;
         a.p = p;
@@ -663,9 +650,13 @@ int launch_chunk_attention(const ChunkAttnParams& p, const ChunkAttnPlan& plan, 
         a.vec_out = vec_out;
         a.join_apart = plan.join_apart;
         const int64_t ctas = (int64_t)p.batch.n_seq * plan.tiles * p.kv.n_head * plan.n_split;
+        const int bit = (p.kv.kv_dtype * 3 + p.kv.head_dim / 64) * 4 + plan.row_tile / 8 - 1;   // 0 .. 35
+        bool ok = false;
         pick(p.kv.kv_dtype, p.kv.head_dim, plan.row_tile, [&](auto k, size_t smem) {
-            launch_pdl(k, dim3((unsigned)ctas), dim3(NW * 32), smem, s, a);
+            ok = raise_smem(k, smem, ready, bit);
+            if (ok) launch_pdl(k, dim3((unsigned)ctas), dim3(NW * 32), smem, s, a);
         });
+        if (!ok) return 0;
     }
     if (!plan.join_apart) return 1;
     if (p.kv.kv_dtype == GSVCU_KV_F32) launch_join<float>(p, plan, vec_out, s);

@@ -633,18 +633,7 @@ void pick_tc(int dtype, int dim, F f) {
 
 }  // namespace
 
-cudaError_t chunk_attention_tc_init_device() {
-    cudaError_t e = cudaSuccess;
-    for (int ty : {GSVCU_KV_F16, GSVCU_KV_BF16})
-        for (int dim : {32, 64, 128})
-            pick_tc(ty, dim, [&](auto k, size_t smem) {
-                const cudaError_t r = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-                if (e == cudaSuccess) e = r;
-            });
-    return e;
-}
-
-bool launch_chunk_attention_tc(const ChunkAttnParams& p, const ChunkAttnPlan& plan, cudaStream_t s) {
+bool launch_chunk_attention_tc(const ChunkAttnParams& p, const ChunkAttnPlan& plan, uint64_t* ready, cudaStream_t s) {
     TcArgs a;
     a.p = p;
     a.group = p.n_q_head / p.kv.n_head;
@@ -669,10 +658,13 @@ bool launch_chunk_attention_tc(const ChunkAttnParams& p, const ChunkAttnPlan& pl
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
         return false;
     const int64_t ctas = (int64_t)p.batch.n_seq * plan.tiles * p.kv.n_head * plan.n_split;
+    const int bit = 36 + (p.kv.kv_dtype == GSVCU_KV_F16 ? 0 : 3) + D / 64;   // 36 .. 41
+    bool ok = false;
     pick_tc(p.kv.kv_dtype, D, [&](auto k, size_t smem) {
-        launch_pdl(k, dim3((unsigned)ctas), dim3(THREADS), smem, s, a);
+        ok = raise_smem(k, smem, ready, bit);
+        if (ok) launch_pdl(k, dim3((unsigned)ctas), dim3(THREADS), smem, s, a);
     });
-    return true;
+    return ok;
 }
 
 }  // namespace gsvcu
