@@ -581,14 +581,14 @@ ChunkAttnPlan chunk_attention_plan(const ChunkAttnParams& p) {
     const int max_tiles = (p.batch.max_kv + kt - 1) / kt;
     // Splits, measured on 148 SMs. Few units: one wave of CTAs (one sequence of 131072 keys: 88 us, 100 with two
     // waves). Several sequences: up to four waves, so that lengths even out (32 sequences of 1000 to 9000 keys: 134 us
-    // with two splits, 119 with four), while a split still streams 1 MB (64 sequences of 2100 keys at head dim 32: 37 us
-    // whole, 48 in two). A split keeps 4 tiles for each warp.
+    // with two splits, 117 with four), while a split still streams 512 KB (64 sequences of 2100 keys at head dim 32: 36 us
+    // whole, 40 in two). A split keeps 4 tiles for each warp.
     size_t smem = 0;
     pick(p.kv.kv_dtype, D, c.row_tile, [&](auto, size_t bytes) { smem = bytes; });
     const int64_t slots = 148 * (int64_t)(232448 / (smem + 1024));
     int64_t n = (slots + units / 2) / units;
     if (p.batch.n_seq > 1) {
-        const int64_t even = (4 * slots + units - 1) / units, whole = ((int64_t)p.batch.max_kv * 2 * D * size) >> 20;
+        const int64_t even = (4 * slots + units - 1) / units, whole = ((int64_t)p.batch.max_kv * 2 * D * size) >> 19;
         if (n < (even < whole ? even : whole)) n = even < whole ? even : whole;
     }
     const int least = 4 * NW;

@@ -566,7 +566,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
             const int64_t unit = ((int64_t)s * a.tiles + tile) * p.kv.n_head + h;
             float* part = p.part + unit * a.n_split * (a.row_tile * (D + 2));
             const float il = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-            if (ok) {
+            if (ok && n_act == 1) {
 #pragma unroll 1
                 for (int d = 0; d < D; d += 32) {
                     uint32_t o[32];
@@ -579,35 +579,53 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
                         for (int i = 0; i < 32; i++) o[i] = 0;
                     }
                     if (!mine) continue;
-                    if (n_act == 1) {
 #pragma unroll
-                        for (int i = 0; i < 32; i += 8) {
-                            float y[8];
+                    for (int i = 0; i < 32; i += 8) {
+                        float y[8];
 #pragma unroll
-                            for (int k = 0; k < 8; k++) y[k] = __uint_as_float(o[i + k]) * il;
-                            T* dst = (T*)p.out + row * p.out_stride + (int64_t)head * D + d + i;
-                            const uint4 u = make_uint4(pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]), pack2<T>(y[4], y[5]), pack2<T>(y[6], y[7]));
-                            if (a.vec_out) {
-                                *(uint4*)dst = u;
-                            } else {
-                                const T* e = (const T*)&u;
+                        for (int k = 0; k < 8; k++) y[k] = __uint_as_float(o[i + k]) * il;
+                        T* dst = (T*)p.out + row * p.out_stride + (int64_t)head * D + d + i;
+                        const uint4 u = make_uint4(pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]), pack2<T>(y[4], y[5]), pack2<T>(y[6], y[7]));
+                        if (a.vec_out) {
+                            *(uint4*)dst = u;
+                        } else {
+                            const T* e = (const T*)&u;
 #pragma unroll
-                                for (int k = 0; k < 8; k++) dst[k] = e[k];
-                            }
+                            for (int k = 0; k < 8; k++) dst[k] = e[k];
                         }
-                    } else {
-                        float* dst = part + ((int64_t)sp * a.row_tile + r) * D + d;
-#pragma unroll
-                        for (int i = 0; i < 32; i += 4)
-                            *(uint4*)(dst + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
                     }
                 }
-                if (mine) {
-                    if (n_act > 1)
-                        *(float2*)(part + (int64_t)a.n_split * a.row_tile * D + 2 * ((int64_t)sp * a.row_tile + r)) = make_float2(mref, l);
-                    else if (p.lse)
-                        p.lse[row * p.n_q_head + head] = mref == NEG_INF ? NEG_INF : (mref + log2f(l)) * LN2;
+                if (mine && p.lse)
+                    p.lse[row * p.n_q_head + head] = mref == NEG_INF ? NEG_INF : (mref + log2f(l)) * LN2;
+            } else if (ok) {
+                // Split results (f32, nt > 0) go through shared memory, where this row tile's queries are no longer needed, in
+                // two halves of the columns, so that a warp's stores cover whole rows (512 tokens over 8192 keys: 47.9 -> 45.0
+                // us; 16-bit outputs, half as wide, are faster straight from the registers): 16-byte pieces, swizzled by row.
+                uint8_t* stage = sm + (size_t)(128 * t + 32 * q) * D * 2;
+                auto place = [&](int fr, int piece) {
+                    return (uint4*)(stage + fr * D * 2 + ((piece ^ (D >= 64 ? fr & 7 : (fr >> 1) & 3)) << 4));
+                };
+#pragma unroll 1
+                for (int d0 = 0; d0 < D; d0 += D / 2) {
+#pragma unroll 1
+                    for (int d = 0; d < D / 2; d += 16) {
+                        float o[16];
+                        tmem_ld16(to + (uint32_t)(d0 + d), o);
+                        tmem_wait_ld();
+                        tmem_bind(o);
+#pragma unroll
+                        for (int k = 0; k < 16; k += 4) *(float4*)place(lane, (d + k) / 4) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+                    }
+                    __syncwarp();
+#pragma unroll 4
+                    for (int m = 0; m < D / 8; m++) {
+                        const int fr = (32 * m + lane) / (D / 8), pc = (32 * m + lane) % (D / 8), rr = 128 * t + 32 * q + fr;
+                        if (rr < c.rows) *(uint4*)(part + ((int64_t)sp * a.row_tile + rr) * D + d0 + pc * 4) = *place(fr, pc);
+                    }
+                    __syncwarp();
                 }
+                if (mine)
+                    *(float2*)(part + (int64_t)a.n_split * a.row_tile * D + 2 * ((int64_t)sp * a.row_tile + r)) = make_float2(mref, l);
             } else if (lane == 0) {
                 atomicOr(p.err, PAGED_WAIT);
                 *abort_flag = 1;
