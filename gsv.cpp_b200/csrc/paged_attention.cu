@@ -9,7 +9,8 @@
 // k_chunk_attn: one CTA per (sequence, row tile, kv head, key split). Its four warps take the split's key
 // tiles in turn, each with its own cp.async ring, running maximum, sum and output (in registers), so no
 // barrier stands inside the loop; they are joined at the end in warp order. With several splits the CTA that
-// arrives last joins the splits' results in split order (a fixed order: results do not depend on timing).
+// arrives last joins the splits' results of 8 rows, k_chunk_join those of more, in an order that the sizes alone decide
+// (results do not depend on timing).
 // Everything is transposed: S^T = K Q^T with 16 keys and 8 query rows per product, O^T = V^T P^T, because few
 // rows are the rule here (one decoding token of one head is one row) and 8 is the smaller side of mma.sync.
 // F16 / BF16 products run on mma.m16n8k16 with the weights split into two 16-bit parts (w = hi + lo), so
@@ -136,7 +137,7 @@ struct SplitArgs {
     ChunkAttnParams p;
     int group, tiles, n_split, split_tiles;
     float c;          // scale * log2(e)
-    bool vec_q, vec_out, join_apart;
+    bool vec_q, vec_out;
 };
 
 template <typename T, int D, int NT>
@@ -207,7 +208,8 @@ __global__ void __launch_bounds__(NW * 32) k_chunk_attn(SplitArgs a) {
         uint4 u = make_uint4(0, 0, 0, 0);
         if (r < rows) {
             const int tok = (r0 + r) / a.group, j = (r0 + r) % a.group;
-            const T* src = (const T*)p.q + (int64_t)(row0 + tok) * p.q_stride + (int64_t)(h * a.group + j) * D + pc * (16 / (int)sizeof(T));
+            const T* src = (const T*)p.q + (int64_t)(row0 + tok) * p.q_stride + (int64_t)(h * a.group + j) * D +
+                           pc * (16 / (int)sizeof(T));
             if (a.vec_q) {
                 u = *(const uint4*)src;
             } else {
@@ -507,10 +509,11 @@ __global__ void __launch_bounds__(NW * 32) k_chunk_attn(SplitArgs a) {
             if (d == 0) *(float2*)(part_ml + 2 * ((int64_t)sp * ROWS + r)) = make_float2(top, sum);
         }
     }
-    if (n_act == 1 || a.join_apart) return;
+    if (n_act == 1) return;
 
-    join_splits<T, D, ROWS, NW * 32>(p, c, s, tile, h, a.group, a.tiles, a.n_split, n_act, a.vec_out, tid,
-                                     (int*)(sm + C::OFF_ML + (size_t)NW * ROWS * 8), (float*)sm);
+    if constexpr (ROWS == 8)   // (more rows are joined by k_chunk_join)
+        join_splits<T, D, ROWS, NW * 32>(p, c, s, tile, h, a.group, a.tiles, a.n_split, n_act, a.vec_out, tid,
+                                         (int*)(sm + C::OFF_ML + (size_t)NW * ROWS * 8), (float*)sm);
 }
 
 // Calls f with the kernel's compile-time variant for (type, head dim, row tile).
@@ -624,8 +627,7 @@ static void launch_join_rows(const ChunkAttnParams& p, const ChunkAttnPlan& c, b
     auto go = [&](auto k) {
         launch_pdl(k, dim3((unsigned)ctas), dim3(256), 0, s, p, group, c.tiles, c.n_split, c.split_tiles, c.key_tile, vec);
     };
-    if (c.row_tile == 8) go(k_chunk_join<T, D, 8>);
-    else if (c.row_tile == 16) go(k_chunk_join<T, D, 16>);
+    if (c.row_tile == 16) go(k_chunk_join<T, D, 16>);
     else if (c.row_tile == 24) go(k_chunk_join<T, D, 24>);
     else if (c.row_tile == 32) go(k_chunk_join<T, D, 32>);
     else if constexpr (sizeof(T) == 2) {
@@ -655,7 +657,6 @@ int launch_chunk_attention(const ChunkAttnParams& p, const ChunkAttnPlan& plan, 
         a.c = p.scale * LOG2E;
         a.vec_q = ((uintptr_t)p.q & 15) == 0 && (p.q_stride * (int64_t)size) % 16 == 0;
         a.vec_out = vec_out;
-        a.join_apart = plan.join_apart;
         const int64_t ctas = (int64_t)p.batch.n_seq * plan.tiles * p.kv.n_head * plan.n_split;
         const int bit = (p.kv.kv_dtype * 3 + p.kv.head_dim / 64) * 4 + plan.row_tile / 8 - 1;   // 0 .. 35
         bool ok = false;

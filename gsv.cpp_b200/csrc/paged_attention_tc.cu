@@ -112,10 +112,12 @@ __device__ __forceinline__ bool wait_warp(uint32_t b, uint32_t parity, volatile 
     }
     return false;
 }
-#define R8(x, i) "+r"(x[i]), "+r"(x[i + 1]), "+r"(x[i + 2]), "+r"(x[i + 3]), "+r"(x[i + 4]), "+r"(x[i + 5]), "+r"(x[i + 6]), "+r"(x[i + 7])
+#define REG4(c, x, i) c(x[i]), c(x[i + 1]), c(x[i + 2]), c(x[i + 3])
+#define REG8(c, x, i) REG4(c, x, i), REG4(c, x, i + 4)
+#define R8(x, i) REG8("+r", x, i)
 #define R32(x) R8(x, 0), R8(x, 8), R8(x, 16), R8(x, 24)
-#define W8(x, i) "=r"(x[i]), "=r"(x[i + 1]), "=r"(x[i + 2]), "=r"(x[i + 3]), "=r"(x[i + 4]), "=r"(x[i + 5]), "=r"(x[i + 6]), "=r"(x[i + 7])
-#define V8(x, i) "r"(x[i]), "r"(x[i + 1]), "r"(x[i + 2]), "r"(x[i + 3]), "r"(x[i + 4]), "r"(x[i + 5]), "r"(x[i + 6]), "r"(x[i + 7])
+#define W8(x, i) REG8("=r", x, i)
+#define V8(x, i) REG8("r", x, i)
 // 32 tensor-memory columns of the warp's lanes; the values count after tmem_wait_ld + bind32.
 __device__ __forceinline__ void tmem_ld32(uint32_t a, uint32_t (&r)[32]) {
     asm volatile(
@@ -241,6 +243,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
         bar_init(drain, 1);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // (this warp's first copies come before the CTA meets)
     }
     // Warp 0's work: pair i is V of tile i - 1, then K of tile i (what the MMA warp needs together).
     int blk = 0;
@@ -260,7 +263,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
                 }
             }
         }
-        const uint32_t k0b = __shfl_sync(0xffffffffu, blk, (i & 15) * 2), k1b = __shfl_sync(0xffffffffu, blk, (i & 15) * 2 + 1);
+        const uint32_t k0b = __shfl_sync(0xffffffffu, blk, (i & 15) * 2);
+        const uint32_t k1b = __shfl_sync(0xffffffffu, blk, (i & 15) * 2 + 1);
         bool ok = true;
         if (lane == 0) {
             ok = bar_wait_short(empty(e), ((uint32_t)(i / L::NP) & 1u) ^ 1u, abort_flag);
@@ -307,7 +311,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
             u[m] = make_uint4(0, 0, 0, 0);
             if (r < c.rows) {
                 const int up = (int)(((float)(rem0 + r) + 0.5f) * inv), j = rem0 + r - up * a.group;
-                const T* src = (const T*)p.q + (int64_t)(c.row0 + tok0 + up) * p.q_stride + (int64_t)(h * a.group + j) * D + pc * 8;
+                const T* src = (const T*)p.q + (int64_t)(c.row0 + tok0 + up) * p.q_stride +
+                               (int64_t)(h * a.group + j) * D + pc * 8;
                 if (a.vec_q) {
                     u[m] = *(const uint4*)src;
                 } else {
@@ -585,7 +590,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
 #pragma unroll
                         for (int k = 0; k < 8; k++) y[k] = __uint_as_float(o[i + k]) * il;
                         T* dst = (T*)p.out + row * p.out_stride + (int64_t)head * D + d + i;
-                        const uint4 u = make_uint4(pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]), pack2<T>(y[4], y[5]), pack2<T>(y[6], y[7]));
+                        const uint4 u = make_uint4(pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]), pack2<T>(y[4], y[5]),
+                                                   pack2<T>(y[6], y[7]));
                         if (a.vec_out) {
                             *(uint4*)dst = u;
                         } else {
@@ -614,7 +620,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
                         tmem_wait_ld();
                         tmem_bind(o);
 #pragma unroll
-                        for (int k = 0; k < 16; k += 4) *(float4*)place(lane, (d + k) / 4) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+                        for (int k = 0; k < 16; k += 4)
+                            *(float4*)place(lane, (d + k) / 4) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
                     }
                     __syncwarp();
 #pragma unroll 4
@@ -625,7 +632,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
                     __syncwarp();
                 }
                 if (mine)
-                    *(float2*)(part + (int64_t)a.n_split * a.row_tile * D + 2 * ((int64_t)sp * a.row_tile + r)) = make_float2(mref, l);
+                    *(float2*)(part + (int64_t)a.n_split * a.row_tile * D + 2 * ((int64_t)sp * a.row_tile + r)) =
+                        make_float2(mref, l);
             } else if (lane == 0) {
                 atomicOr(p.err, PAGED_WAIT);
                 *abort_flag = 1;
