@@ -52,20 +52,22 @@ __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
     }
 }
 
-// Where a row goes: sequence found by the whole warp (lanes compare 32 starts at a time), page looked up.
+// Where a row goes: sequence found by the whole warp, page looked up.
 struct Place {
     int64_t slot;   // element offset of the row's (layer, K, head 0) within the pool, -1: not stored
     int pos;        // rotation position, clamped to the table
 };
 template <int D>
 __device__ __forceinline__ Place place_of(const KvAppendParams& p, int row, int lane, bool report) {
-    int s = 0;
-    for (int i = 0; i < p.batch.n_seq; i += 32) {
-        const bool past = i + lane < p.batch.n_seq && p.batch.row_start[i + lane + 1] <= row;
-        const unsigned m = __ballot_sync(0xffffffffu, past);
-        s += __popc(m);
-        if (m != 0xffffffffu) break;
+    // sequences that end at or before the row: 32 blocks at a time, then the 32 of one block (1200 sequences: 2 loads)
+    int s = 0, n = p.batch.n_seq;
+    while (n > 32) {
+        const int step = (n + 31) / 32, last = (lane + 1) * step - 1;
+        const int m = __popc(__ballot_sync(0xffffffffu, last < n && p.batch.row_start[s + last + 1] <= row));
+        s += m * step;
+        n = min(step, n - m * step);
     }
+    s += __popc(__ballot_sync(0xffffffffu, lane < n && p.batch.row_start[s + lane + 1] <= row));
     Place w{-1, 0};
     if (s >= p.batch.n_seq) {   // rows beyond the last sequence
         if (report) atomicOr(p.err, PAGED_BAD_LENGTH);
