@@ -1865,33 +1865,30 @@ static int paged_views(gsvcu_ctx* ctx, const gsvcu_paged_kv* kv, const gsvcu_chu
 
 static bool aligned_to(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
 
-int gsvcu_op_kv_append(gsvcu_ctx* ctx, const gsvcu_paged_kv* kv, const gsvcu_chunk_batch* batch, int32_t layer,
-                       int32_t row_dtype, int32_t n_q_head, const void* q_dev, int64_t q_stride, const void* k_dev,
-                       int64_t k_stride, const void* v_dev, int64_t v_stride, const float* cos_dev,
-                       const float* sin_dev, int32_t n_pos, int32_t rot_dim, int32_t rot_pairs, const int32_t* pos_dev,
-                       void* q_out_dev, int64_t q_out_stride) {
-    if (!ctx) return GSVCU_ERR_ARG;
+int gsvcu_op_kv_append(gsvcu_ctx* ctx, const gsvcu_kv_append* a) {
+    if (!ctx || !a) return GSVCU_ERR_ARG;
     KvAppendParams p;
-    TRY(paged_views(ctx, kv, batch, layer, n_q_head, p.kv, p.batch));
-    if (row_dtype != GSVCU_KV_F32 && row_dtype != kv->kv_dtype)
+    TRY(paged_views(ctx, a->kv, a->batch, a->layer, a->n_q_head, p.kv, p.batch));
+    const int n_q = a->n_q_head, kvd = a->kv->kv_dtype;
+    if (a->row_dtype != GSVCU_KV_F32 && a->row_dtype != kvd)
         return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_kv_append: rows must be F32 or the cache's type");
-    if (batch->n_rows > 0 && (!k_dev || !v_dev || (n_q_head > 0 && (!q_dev || !q_out_dev))))
+    if (a->batch->n_rows > 0 && (!a->k_dev || !a->v_dev || (n_q > 0 && (!a->q_dev || !a->q_out_dev))))
         return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_kv_append: null rows");
-    const int64_t D = kv->head_dim;
-    if (k_stride < kv->n_kv_head * D || v_stride < kv->n_kv_head * D ||
-        (n_q_head > 0 && (q_stride < n_q_head * D || q_out_stride < n_q_head * D)))
+    const int64_t D = a->kv->head_dim, kv_width = a->kv->n_kv_head * D;
+    if (a->k_stride < kv_width || a->v_stride < kv_width || (n_q > 0 && (a->q_stride < n_q * D || a->q_out_stride < n_q * D)))
         return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_kv_append: row stride shorter than its heads");
-    const size_t rs = row_dtype == GSVCU_KV_F32 ? 4 : 2, ks = kv->kv_dtype == GSVCU_KV_F32 ? 4 : 2;
-    if (!aligned_to(q_dev, rs) || !aligned_to(k_dev, rs) || !aligned_to(v_dev, rs) || !aligned_to(q_out_dev, ks))
+    const size_t rs = a->row_dtype == GSVCU_KV_F32 ? 4 : 2, ks = kvd == GSVCU_KV_F32 ? 4 : 2;
+    if (!aligned_to(a->q_dev, rs) || !aligned_to(a->k_dev, rs) || !aligned_to(a->v_dev, rs) || !aligned_to(a->q_out_dev, ks))
         return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_kv_append: rows not aligned to their element");
-    if (rot_dim < 0 || rot_dim > D || rot_dim % 2 || (rot_dim > 0 && (!cos_dev || !sin_dev || n_pos <= 0)) ||
-        rot_pairs < 0 || rot_pairs > 1)
+    if (a->rot_dim < 0 || a->rot_dim > D || a->rot_dim % 2 || a->rot_pairs < 0 || a->rot_pairs > 1 ||
+        (a->rot_dim > 0 && (!a->cos_dev || !a->sin_dev || a->n_pos <= 0)))
         return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_kv_append: rot_dim must be even, at most head_dim, with its cos / sin table");
-    p.row_dtype = row_dtype; p.n_q_head = n_q_head; p.q = q_dev; p.q_stride = q_stride; p.k = k_dev;
-    p.k_stride = k_stride; p.v = v_dev; p.v_stride = v_stride; p.cos = cos_dev; p.sin = sin_dev; p.n_pos = n_pos;
-    p.rot = rot_dim; p.pairs = rot_pairs; p.pos = pos_dev; p.q_out = q_out_dev; p.q_out_stride = q_out_stride;
+    p.row_dtype = a->row_dtype; p.n_q_head = n_q; p.q = a->q_dev; p.q_stride = a->q_stride; p.k = a->k_dev;
+    p.k_stride = a->k_stride; p.v = a->v_dev; p.v_stride = a->v_stride; p.cos = a->cos_dev; p.sin = a->sin_dev;
+    p.n_pos = a->n_pos; p.rot = a->rot_dim; p.pairs = a->rot_pairs; p.pos = a->pos_dev; p.q_out = a->q_out_dev;
+    p.q_out_stride = a->q_out_stride;
     p.err = ctx->att_err + 3;
-    if (batch->n_rows == 0 || batch->n_seq == 0) return GSVCU_OK;
+    if (a->batch->n_rows == 0 || a->batch->n_seq == 0) return GSVCU_OK;
     DeviceGuard g(ctx->device);
     launch_kv_append(p, ctx->stream);
     CKC(ctx, cudaGetLastError());
@@ -1899,27 +1896,28 @@ int gsvcu_op_kv_append(gsvcu_ctx* ctx, const gsvcu_paged_kv* kv, const gsvcu_chu
     return GSVCU_OK;
 }
 
-int gsvcu_op_chunk_attention(gsvcu_ctx* ctx, const gsvcu_paged_kv* kv, const gsvcu_chunk_batch* batch, int32_t layer,
-                             int32_t n_q_head, const void* q_dev, int64_t q_stride, float scale, int32_t window,
-                             const int32_t* prefix_dev, void* out_dev, int64_t out_stride, float* lse_dev) {
-    if (!ctx) return GSVCU_ERR_ARG;
+int gsvcu_op_chunk_attention(gsvcu_ctx* ctx, const gsvcu_chunk_attention* a) {
+    if (!ctx || !a) return GSVCU_ERR_ARG;
     ChunkAttnParams p;
-    TRY(paged_views(ctx, kv, batch, layer, n_q_head, p.kv, p.batch));
-    if (n_q_head <= 0 || (batch->n_rows > 0 && (!q_dev || !out_dev)))
+    TRY(paged_views(ctx, a->kv, a->batch, a->layer, a->n_q_head, p.kv, p.batch));
+    const gsvcu_paged_kv* kv = a->kv;
+    const gsvcu_chunk_batch* batch = a->batch;
+    if (a->n_q_head <= 0 || (batch->n_rows > 0 && (!a->q_dev || !a->out_dev)))
         return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_chunk_attention: null rows");
     const int64_t D = kv->head_dim;
-    if (q_stride < n_q_head * D || out_stride < n_q_head * D)
+    if (a->q_stride < a->n_q_head * D || a->out_stride < a->n_q_head * D)
         return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_chunk_attention: row stride shorter than its heads");
     const size_t ks = kv->kv_dtype == GSVCU_KV_F32 ? 4 : 2;
-    if (!aligned_to(q_dev, ks) || !aligned_to(out_dev, ks) || !aligned_to(lse_dev, 4))
+    if (!aligned_to(a->q_dev, ks) || !aligned_to(a->out_dev, ks) || !aligned_to(a->lse_dev, 4))
         return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_chunk_attention: rows not aligned to their element");
-    if (window < 0 || !std::isfinite(scale))
+    if (a->window < 0 || !std::isfinite(a->scale))
         return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_chunk_attention: window must be >= 0 and scale finite");
-    if ((int64_t)batch->n_rows * n_q_head > (1 << 30))
+    if ((int64_t)batch->n_rows * a->n_q_head > (1 << 30))
         return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_chunk_attention: more than 2^30 (row, head) pairs");
-    p.n_q_head = n_q_head; p.q = q_dev; p.q_stride = q_stride; p.scale = scale;
-    p.window = window < (1 << 30) ? window : 0;   // (wider than any cache)
-    p.prefix = prefix_dev; p.out = out_dev; p.out_stride = out_stride; p.lse = lse_dev; p.err = ctx->att_err + 3;
+    p.n_q_head = a->n_q_head; p.q = a->q_dev; p.q_stride = a->q_stride; p.scale = a->scale;
+    p.window = a->window < (1 << 30) ? a->window : 0;   // (wider than any cache)
+    p.prefix = a->prefix_dev; p.out = a->out_dev; p.out_stride = a->out_stride; p.lse = a->lse_dev;
+    p.err = ctx->att_err + 3;
     if (batch->n_rows == 0 || batch->n_seq == 0) return GSVCU_OK;
     const ChunkAttnPlan plan = chunk_attention_plan(p);
     if ((int64_t)batch->n_seq * plan.tiles * kv->n_kv_head * plan.n_split > INT32_MAX)

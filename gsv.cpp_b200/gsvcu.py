@@ -9,6 +9,7 @@ from __future__ import annotations
 import ctypes as C
 import os
 import re
+import struct
 
 import numpy as np
 
@@ -58,6 +59,24 @@ class ChunkBatchDesc(C.Structure):
                [(n, C.c_int32) for n in ("n_seq", "max_pages", "n_rows", "max_chunk", "max_kv")]
 
 
+class KvAppendArgs(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("kv", "batch", "q", "k", "v", "q_out")] + \
+               [(n, C.c_int64) for n in ("q_stride", "k_stride", "v_stride", "q_out_stride")] + \
+               [(n, C.c_void_p) for n in ("cos", "sin", "pos")] + \
+               [(n, C.c_int32) for n in ("layer", "row_dtype", "n_q_head", "n_pos", "rot_dim", "rot_pairs")]
+
+
+class ChunkAttentionArgs(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("kv", "batch", "q", "out", "lse", "prefix")] + \
+               [(n, C.c_int64) for n in ("q_stride", "out_stride")] + \
+               [(n, C.c_int32) for n in ("layer", "n_q_head", "window")] + [("scale", C.c_float)]
+
+
+# the two structs packed in one step (a step's layers call these often, and per-field conversion costs as much as the launch)
+_PACK_APPEND, _PACK_ATTENTION = struct.Struct("@6P4q3P6i"), struct.Struct("@6P2q3if")
+assert _PACK_APPEND.size == C.sizeof(KvAppendArgs) and _PACK_ATTENTION.size == C.sizeof(ChunkAttentionArgs)
+
+
 PROGRESS_FN = C.CFUNCTYPE(None, C.c_void_p, C.c_int32)
 
 _P, _I, _I64, _U64 = C.c_void_p, C.c_int32, C.c_int64, C.c_uint64
@@ -100,10 +119,8 @@ SIGNATURES = {
     "gsvcu_set_wait_fault": ([_P, _I], C.c_int),
     "gsvcu_set_prefill_gemm": ([_P, _I], C.c_int),
     "gsvcu_op_q8_gemm_tc": ([_P, _P, _P, _I, _P, _P, _I, _I, _P, _P, _I, _P, _P, _P], C.c_int),
-    "gsvcu_op_kv_append": ([_P, C.POINTER(PagedKVDesc), C.POINTER(ChunkBatchDesc), _I, _I, _I, _P, _I64, _P, _I64, _P,
-                            _I64, _P, _P, _I, _I, _I, _P, _P, _I64], C.c_int),
-    "gsvcu_op_chunk_attention": ([_P, C.POINTER(PagedKVDesc), C.POINTER(ChunkBatchDesc), _I, _I, _P, _I64, C.c_float, _I,
-                                  _P, _P, _I64, _P], C.c_int),
+    "gsvcu_op_kv_append": ([_P, C.POINTER(KvAppendArgs)], C.c_int),
+    "gsvcu_op_chunk_attention": ([_P, C.POINTER(ChunkAttentionArgs)], C.c_int),
     "gsvcu_op_pack_q8_0_f16": ([_P, _P, _I, _I, _P], C.c_int),
 }
 
@@ -238,19 +255,20 @@ def _floats(t, shape, what, device):
 
 def _row_stride(t, shape, what, device):
     """Stride between the rows of a [rows][heads][head_dim] tensor on CUDA device `device`, heads side by side."""
-    if t.get_device() != device:
-        raise ValueError(f"{what}: expected on CUDA device {device}, got {t.device}")
     if t.shape != shape:
         raise ValueError(f"{what}: {list(shape)} expected, got {list(t.shape)}")
+    if t.get_device() != device:
+        raise ValueError(f"{what}: expected on CUDA device {device}, got {t.device}")
     row, head, one = t.stride()
     n_rows, heads, head_dim = shape
+    width = heads * head_dim
+    if row >= width and head == head_dim and one == 1:
+        return row
     if one != 1 or (head != head_dim and heads > 1):
         raise ValueError(f"{what}: each row's heads must be contiguous")
-    if n_rows <= 1:
-        return heads * head_dim
-    if row < heads * head_dim:
+    if n_rows > 1 and row < width:
         raise ValueError(f"{what}: rows overlap")
-    return row
+    return max(row, width)
 
 
 class PagedKV:
@@ -263,7 +281,7 @@ class PagedKV:
         self.n_kv_head, self.head_dim = pool.shape[3], pool.shape[5]
         self.desc = PagedKVDesc(pool.data_ptr(), _kv_type(pool.dtype, "pool"), pool.shape[0], pool.shape[1],
                                 pool.shape[3], pool.shape[5])
-        self.ref = C.byref(self.desc)
+        self.addr = C.addressof(self.desc)
 
 
 class ChunkBatch:
@@ -281,7 +299,7 @@ class ChunkBatch:
             _ints(row_start, (n_seq + 1,), "row_start", self.device), _ints(kv_len, (n_seq,), "kv_len", self.device),
             _ints(block_table, (n_seq, block_table.shape[1]), "block_table", self.device), n_seq, block_table.shape[1],
             n_rows, max_chunk, max_kv)
-        self.ref = C.byref(self.desc)
+        self.addr = C.addressof(self.desc)
 
 
 class _Reqs:
@@ -325,6 +343,8 @@ class Context:
         self.h = h
         self.hp = None
         self.device = device
+        self._append, self._attention = KvAppendArgs(), ChunkAttentionArgs()
+        self._append_ref, self._attention_ref = C.byref(self._append), C.byref(self._attention)
 
     def close(self):
         if getattr(self, "h", None):
@@ -522,9 +542,10 @@ class Context:
             shape = cos.shape
             n_pos, rot = shape[0], 2 * shape[1]
             cp, sp = _floats(cos, shape, "cos", dev), _floats(sin, shape, "sin", dev)
-        self._check(self.lib.gsvcu_op_kv_append(
-            self.h, cache.ref, chunks.ref, layer, _kv_type(ty, "k"), nq, qp, qs, k.data_ptr(), ks, v.data_ptr(), vs, cp, sp,
-            n_pos, rot, 1 if pairs else 0, None if pos is None else _ints(pos, (n,), "pos", dev), op, os_))
+        _PACK_APPEND.pack_into(self._append, 0, cache.addr, chunks.addr, qp, k.data_ptr(), v.data_ptr(), op, qs, ks, vs, os_, cp,
+                               sp, 0 if pos is None else _ints(pos, (n,), "pos", dev), layer, _kv_type(ty, "k"), nq, n_pos,
+                               rot, 1 if pairs else 0)
+        self._check(self.lib.gsvcu_op_kv_append(self.h, self._append_ref))
 
     def op_chunk_attention(self, cache: PagedKV, chunks: ChunkBatch, layer, q, out, scale=None, prefix=None, window=0,
                            lse=None):
@@ -538,10 +559,12 @@ class Context:
         qs, os_ = _row_stride(q, shape, "q", dev), _row_stride(out, shape, "out", dev)
         if q.dtype != cache.dtype or out.dtype != cache.dtype:
             raise ValueError("q and out must have the cache's type")
-        self._check(self.lib.gsvcu_op_chunk_attention(
-            self.h, cache.ref, chunks.ref, layer, nq, q.data_ptr(), qs, D ** -0.5 if scale is None else scale, window,
-            None if prefix is None else _ints(prefix, (chunks.n_seq,), "prefix", dev), out.data_ptr(), os_,
-            None if lse is None else _floats(lse, (n, nq), "lse", dev)))
+        _PACK_ATTENTION.pack_into(
+            self._attention, 0, cache.addr, chunks.addr, q.data_ptr(), out.data_ptr(),
+            0 if lse is None else _floats(lse, (n, nq), "lse", dev),
+            0 if prefix is None else _ints(prefix, (chunks.n_seq,), "prefix", dev), qs, os_, layer, nq, window,
+            D ** -0.5 if scale is None else scale)
+        self._check(self.lib.gsvcu_op_chunk_attention(self.h, self._attention_ref))
 
     def op_sample(self, logits, V, eos, steps, rng_states, prev=None, top_k=15, top_p=1.0, temperature=1.0, rep=1.35):
         """logits: torch CUDA [B][V]; prev: list of int arrays (repetition windows). Returns (tokens, new states)."""

@@ -279,8 +279,8 @@ typedef struct {
 
 /* The batch (device arrays): sequence s owns the packed rows row_start[s] .. row_start[s + 1] - 1
  * (row_start [n_seq + 1], ascending), holds kv_len[s] keys with these rows and keeps key c in page
- * block_table[s][c / 64], slot c % 64 (block_table [n_seq][max_pages], max_pages <= 2^24; entries past its keys, and of pages that no row of the chunk sees,
- * are not used).
+ * block_table[s][c / 64], slot c % 64 (block_table [n_seq][max_pages], max_pages <= 2^24; entries past its keys, and of
+ * pages that no row of the chunk sees, are not used).
  * Row i of n is the token at cache position kv_len[s] - n + i. Host sizes: n_rows packed rows, max_chunk at
  * least the longest chunk, max_kv at least the longest kv_len (0: max_pages * 64); the closer these are, the
  * better the work is cut up. A page outside the pool, or lengths outside these sizes, touch no memory
@@ -299,11 +299,17 @@ typedef struct {
  * q_out_dev has the cache's type and may be q_dev itself (same type and stride). Rows whose cache position is
  * negative (a chunk longer than its kv_len) are not stored. A position outside the table is reported by the
  * next gsvcu_sync (GSVCU_ERR_ARG). */
-int gsvcu_op_kv_append(gsvcu_ctx* ctx, const gsvcu_paged_kv* kv, const gsvcu_chunk_batch* batch, int32_t layer,
-                       int32_t row_dtype, int32_t n_q_head, const void* q_dev, int64_t q_stride, const void* k_dev,
-                       int64_t k_stride, const void* v_dev, int64_t v_stride, const float* cos_dev,
-                       const float* sin_dev, int32_t n_pos, int32_t rot_dim, int32_t rot_pairs, const int32_t* pos_dev,
-                       void* q_out_dev, int64_t q_out_stride);
+typedef struct {
+    const gsvcu_paged_kv* kv;
+    const gsvcu_chunk_batch* batch;
+    const void *q_dev, *k_dev, *v_dev;
+    void* q_out_dev;
+    int64_t q_stride, k_stride, v_stride, q_out_stride;
+    const float *cos_dev, *sin_dev;
+    const int32_t* pos_dev;
+    int32_t layer, row_dtype, n_q_head, n_pos, rot_dim, rot_pairs;
+} gsvcu_kv_append;
+int gsvcu_op_kv_append(gsvcu_ctx* ctx, const gsvcu_kv_append* a);
 
 /* Attention of the batch's rows over the cache at `layer`. Query head h reads kv head h / (n_q_head /
  * n_kv_head). The row at position p sees key j < kv_len when j < prefix[s], or j <= p and (window 0 or j >
@@ -313,9 +319,18 @@ int gsvcu_op_kv_append(gsvcu_ctx* ctx, const gsvcu_paged_kv* kv, const gsvcu_chu
  * A row that sees no key gives 0 and -infinity. Scores, softmax and sums are F32. What the pages hold from kv_len
  * on does not matter, nor do pages that no row sees; in the other pages every key and value has to be finite (a
  * value that is not reaches rows that do not see it, as 0 times infinity). */
-int gsvcu_op_chunk_attention(gsvcu_ctx* ctx, const gsvcu_paged_kv* kv, const gsvcu_chunk_batch* batch, int32_t layer,
-                             int32_t n_q_head, const void* q_dev, int64_t q_stride, float scale, int32_t window,
-                             const int32_t* prefix_dev, void* out_dev, int64_t out_stride, float* lse_dev);
+typedef struct {
+    const gsvcu_paged_kv* kv;
+    const gsvcu_chunk_batch* batch;
+    const void* q_dev;
+    void* out_dev;
+    float* lse_dev;
+    const int32_t* prefix_dev;
+    int64_t q_stride, out_stride;
+    int32_t layer, n_q_head, window;
+    float scale;
+} gsvcu_chunk_attention;
+int gsvcu_op_chunk_attention(gsvcu_ctx* ctx, const gsvcu_chunk_attention* a);
 
 /* One sampling step per row (gsv_logits_to_probs + gsv_sample, reference src/gsv_sampler.cpp:8-89,
  * with the step < 11 EOS mask of src/gsv_ar.cpp:768): logits_dev [B][V] f32; prev_host [B][prev_stride]

@@ -179,10 +179,8 @@ def test_bench_weight_bytes_per_format(tmp_path):
 def test_paged_operators_null_arguments_are_rejected():
     """The paged-cache operators refuse a null context before any device work."""
     lib = gsvcu.load_library()
-    kv, batch = gsvcu.PagedKVDesc(), gsvcu.ChunkBatchDesc()
-    assert lib.gsvcu_op_kv_append(None, C.byref(kv), C.byref(batch), 0, 0, 0, None, 0, None, 0, None, 0, None, None, 0,
-                                  0, 0, None, None, 0) == -1
-    assert lib.gsvcu_op_chunk_attention(None, C.byref(kv), C.byref(batch), 0, 1, None, 0, 1.0, 0, None, None, 0, None) == -1
+    assert lib.gsvcu_op_kv_append(None, C.byref(gsvcu.KvAppendArgs())) == -1
+    assert lib.gsvcu_op_chunk_attention(None, C.byref(gsvcu.ChunkAttentionArgs())) == -1
 
 
 def test_paged_cache_and_batch_objects_check_their_tensors():

@@ -484,7 +484,12 @@ def test_work_queued_on_the_contexts_stream(ctx):
 
 
 def test_refusals(ctx):
+    import ctypes
     import gsvcu
+    assert ctx.lib.gsvcu_op_kv_append(ctx.h, None) == -1 and ctx.lib.gsvcu_op_chunk_attention(ctx.h, None) == -1
+    empty = gsvcu.KvAppendArgs(), gsvcu.ChunkAttentionArgs()   # null cache and batch
+    assert ctx.lib.gsvcu_op_kv_append(ctx.h, ctypes.byref(empty[0])) == -1
+    assert ctx.lib.gsvcu_op_chunk_attention(ctx.h, ctypes.byref(empty[1])) == -1
     c = Case("f16", [2], [70], 4, 2, 64)
     cache, chunks = c.objects()
     q, kv = c.rand(2, 4, 64), c.rand(2, 2, 64)
