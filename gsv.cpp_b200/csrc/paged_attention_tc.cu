@@ -50,7 +50,8 @@ struct Smem {
     static constexpr uint32_t TM_O = 2 * KT;
     static constexpr size_t OFF_RING = (size_t)ROWS * D * 2;      // after Q
     static constexpr size_t OFF_BAR = OFF_RING + (size_t)NP * 2 * ENTRY;
-    // full, empty [NP], S full [2], P full [2][2 halves], PV done [2], V landed, V cleared, drain
+    // full, empty [NP], S full [2], P full [2][2 halves], PV done [2] (one per row tile; with one row tile, for its key
+    // tiles in turn), V landed, V cleared, drain
     static constexpr int NBAR = 2 * NP + 11;
     static constexpr size_t SMEM = OFF_BAR + NBAR * 8 + 16 + 1024;
 };
@@ -433,7 +434,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
                         if (j + 1 < nt) scores(0, e, e);
                         ok = values(0, u, e, (uint32_t)j, turn);
                         if (!ok) break;
-                        commit(pvdone(0));
+                        commit(pvdone(u));
                         commit(empty(e));
                     }
                 }
@@ -479,6 +480,13 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
                 const int n = halves * j + t, b = n & 1;   // the scores' number, their buffer
                 const uint32_t ts = tl + (uint32_t)b * KT;
                 if (!bar_wait_short_warp(sfull(b), (uint32_t)n >> 1 & 1u, abort_flag)) { ok = false; break; }
+                // With one row tile a warp may be a whole tile ahead of the others, whose weights the product before still
+                // needs. Key tile j's product completes phase j / 2 of barrier j & 1; every warp takes each phase in turn (this
+                // one long done, so that the wait for the next is never satisfied by the phase before it).
+                if (halves == 1 && j > 1 && !bar_wait_short_warp(pvdone(j & 1), (uint32_t)(j - 2) >> 1 & 1u, abort_flag)) {
+                    ok = false;
+                    break;
+                }
                 tc_fence_after();
                 uint32_t x[4][32];
 #pragma unroll
@@ -516,7 +524,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
                     if (j > 0) {
                         // O must be at rest. With two row tiles it is: these scores were issued after the product before
                         if (halves == 1) {
-                            if (!bar_wait_short_warp(pvdone(t), (uint32_t)(j - 1) & 1u, abort_flag)) { ok = false; break; }
+                            if (!bar_wait_short_warp(pvdone((j - 1) & 1), (uint32_t)(j - 1) >> 1 & 1u, abort_flag)) { ok = false; break; }
                             tc_fence_after();
                         }
                         const float f = up == NEG_INF ? 1.0f : ex2(mref - up);
@@ -563,7 +571,10 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
                 else weights(std::true_type{});
                 l += f2lo(sum) + f2hi(sum);
             }
-            if (ok && nt > 0) ok = bar_wait_short_warp(pvdone(t), halves == 2 ? 0u : (uint32_t)(nt - 1) & 1u, abort_flag);
+            if (ok && nt > 0) {   // (two row tiles: one phase, after the last product)
+                const int last = halves == 2 ? t : (nt - 1) & 1;
+                ok = bar_wait_short_warp(pvdone(last), halves == 2 ? 0u : (uint32_t)(nt - 1) >> 1 & 1u, abort_flag);
+            }
             tc_fence_after();
             const bool mine = r < c.rows;
             const int tok = (c.r0 + r) / a.group, head = h * a.group + (c.r0 + r) % a.group;
