@@ -431,6 +431,7 @@ struct gsvcu_ctx {
     size_t op_split_n = 0;
     int32_t* op_arrived = nullptr;    // its arrival counters, zero between launches
     size_t op_arrived_n = 0;
+    std::vector<void*> op_outgrown;   // what these two outgrew, kept for captured graphs until the context ends
     uint64_t op_chunk_ready = 0;      // its kernels whose shared-memory limit is raised
     // set when a bounded wait in a kernel gave up: [0] decode attention in the decode steps (read and
     // cleared with the slot state), [1] gsvcu_op_decode_attention (read and cleared by gsvcu_sync),
@@ -507,6 +508,7 @@ gsvcu_ctx::~gsvcu_ctx() {
     if (op_a16) cudaFree(op_a16);
     if (op_split) cudaFree(op_split);
     if (op_arrived) cudaFree(op_arrived);
+    for (void* p : op_outgrown) cudaFree(p);
     if (att_err) cudaFree(att_err);
     for (cudaStream_t gs : gstream)
         if (gs) cudaStreamDestroy(gs);
@@ -1933,7 +1935,7 @@ int gsvcu_op_chunk_attention(gsvcu_ctx* ctx, const gsvcu_chunk_attention* a) {
             cudaGetLastError();
             return ctx->fail(GSVCU_ERR_OOM, "gsvcu_op_chunk_attention: no memory for the split results");
         }
-        if (*at) ctx->wallocs.push_back(*at);
+        if (*at) ctx->op_outgrown.push_back(*at);
         *at = fresh;
         *have = n;
         return GSVCU_OK;

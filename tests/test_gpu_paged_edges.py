@@ -6,7 +6,7 @@ pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip("torch")
 
-from test_gpu_paged import PAGE, Case, attend, ctx  # noqa: E402,F401
+from test_gpu_paged import PAGE, Case, attend, check_attention, ctx  # noqa: E402,F401
 
 
 def set_keys(c, s, dim, values):
@@ -38,3 +38,40 @@ def test_warps_of_a_row_tile_at_their_own_pace(ctx, ty, dim, rows):  # noqa: F81
     for _ in range(5):
         _, b, lb = attend(ctx, c, q=x)
         assert torch.equal(a, b) and torch.equal(la, lb)
+
+
+def decode_case(ty="f16", n=2, kv=3000, heads=4, kv_heads=2, dim=64, q=1, seed=0):
+    return Case(ty, [q] * n, [kv] * n, heads, kv_heads, dim, seed=seed)
+
+
+@pytest.mark.parametrize("q", [1, 5, 60])
+def test_captured_graphs_keep_their_scratch(tmp_path, q):
+    """A split call (joined by its last CTA, by a kernel of its own, on tcgen05) captured in a graph, then a larger call
+    that outgrows the scratch, then a model file that does not load: replays still give the result, on new contents."""
+    import gsvcu
+    own = gsvcu.Context(0)
+    small, large = decode_case(q=q), decode_case(n=6, kv=20000, heads=16, kv_heads=4, dim=128, q=q)
+    x = small.rand(small.rows, small.heads, small.dim)
+    out = torch.empty_like(x)
+    cache, chunks = small.objects()
+    attend(own, small, q=x)
+    stream = torch.cuda.ExternalStream(own.stream_handle())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        own.op_chunk_attention(cache, chunks, small.layer, x, out)
+    attend(own, large)
+    bad = tmp_path / "none.gguf"
+    bad.write_bytes(b"GGUF")
+    with pytest.raises(gsvcu.GsvcuError):
+        own.load(str(bad))
+    keep = [torch.full((1 << 20,), float("nan"), device="cuda") for _ in range(64)]   # (freed memory would be reused)
+    for _ in range(3):
+        x.normal_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            graph.replay()
+        own.sync()
+        check_attention(small, x, out, None, small.dim ** -0.5)
+        attend(own, large)
+    del graph, keep
+    own.close()
