@@ -1926,25 +1926,34 @@ int gsvcu_op_chunk_attention(gsvcu_ctx* ctx, const gsvcu_chunk_attention* a) {
         return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_chunk_attention: batch too large for one launch");
     DeviceGuard g(ctx->device);
     // Scratch at least doubles when it grows, and what it replaces stays until the context ends: captured graphs
-    // may hold its address.
-    auto grow = [&](void** at, size_t* have, size_t need) -> int {
+    // may hold its address. It does not grow in a capture: the zeros of the counters would only be recorded, and calls
+    // outside the graph would find none.
+    auto grow = [&](void** at, size_t* have, size_t need, bool zero) -> int {
         if (need <= *have) return GSVCU_OK;
+        cudaStreamCaptureStatus capture;
+        CKC(ctx, cudaStreamIsCapturing(ctx->stream, &capture));
+        if (capture != cudaStreamCaptureStatusNone)
+            return ctx->fail(GSVCU_ERR_STATE, "gsvcu_op_chunk_attention: run these sizes once before they are captured");
         const size_t n = std::max(need, 2 * *have);
         void* fresh = nullptr;
         if (cudaMalloc(&fresh, n * 4) != cudaSuccess) {
             cudaGetLastError();
             return ctx->fail(GSVCU_ERR_OOM, "gsvcu_op_chunk_attention: no memory for the split results");
         }
+        if (zero) {
+            const cudaError_t e = cudaMemsetAsync(fresh, 0, n * 4, ctx->stream);
+            if (e != cudaSuccess) {
+                cudaFree(fresh);
+                return ctx->fail(GSVCU_ERR_CUDA, cudaGetErrorString(e));
+            }
+        }
         if (*at) ctx->op_outgrown.push_back(*at);
         *at = fresh;
         *have = n;
         return GSVCU_OK;
     };
-    TRY(grow((void**)&ctx->op_split, &ctx->op_split_n, plan.part_floats));
-    if (plan.arrivals > ctx->op_arrived_n) {
-        TRY(grow((void**)&ctx->op_arrived, &ctx->op_arrived_n, plan.arrivals));
-        CKC(ctx, cudaMemsetAsync(ctx->op_arrived, 0, ctx->op_arrived_n * sizeof(int32_t), ctx->stream));
-    }
+    TRY(grow((void**)&ctx->op_split, &ctx->op_split_n, plan.part_floats, false));
+    TRY(grow((void**)&ctx->op_arrived, &ctx->op_arrived_n, plan.arrivals, true));
     p.part = ctx->op_split;
     p.arrived = ctx->op_arrived;
     const int kernels = launch_chunk_attention(p, plan, &ctx->op_chunk_ready, ctx->stream);

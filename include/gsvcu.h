@@ -268,7 +268,9 @@ int gsvcu_op_prefill_attention(gsvcu_ctx* ctx, const float* qkv_dev, int32_t n_s
 /* ---- Paged-cache operators (no counterpart in the reference): appending rows to a paged KV cache and
  * attention of a chunk of new tokens over it, for decoders of any head layout: prompts in chunks, a few
  * drafted tokens at once, single tokens. Both run on the context's stream, read the batch from device
- * memory and allocate nothing after a first call of the same sizes, so they can be captured in a graph. */
+ * memory and allocate nothing after a first call of the same sizes, so they can be captured in a graph (to be
+ * replayed on that stream too: the scratch is the context's). A capture that would have to allocate is refused
+ * (GSVCU_ERR_STATE). */
 
 /* The cache: pages [page][n_layer][K, V][n_kv_head][64 tokens][head_dim] of kv_dtype elements in pool_dev
  * (16-byte aligned); head_dim 32, 64 or 128. */

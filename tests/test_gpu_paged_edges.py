@@ -75,3 +75,36 @@ def test_captured_graphs_keep_their_scratch(tmp_path, q):
         attend(own, large)
     del graph, keep
     own.close()
+
+
+@pytest.mark.parametrize("mode", ["relaxed", "thread_local", "global"])
+def test_scratch_does_not_grow_in_a_capture(mode):
+    """A first split call inside a capture is refused and leaves nothing behind: the capture ends as usual, the same call
+    outside it is right, and then it can be captured."""
+    import gsvcu
+    own = gsvcu.Context(0)
+    c = decode_case()
+    x = c.rand(c.rows, c.heads, c.dim)
+    out = torch.empty_like(x)
+    cache, chunks = c.objects()
+    torch.cuda.synchronize()
+    stream = torch.cuda.ExternalStream(own.stream_handle())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream, capture_error_mode=mode):
+        out.zero_()
+        with pytest.raises(gsvcu.GsvcuError) as e:
+            own.op_chunk_attention(cache, chunks, c.layer, x, out)
+    assert e.value.code == -6 and "once before" in str(e.value)
+    attend(own, c, q=x)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream, capture_error_mode=mode):
+        own.op_chunk_attention(cache, chunks, c.layer, x, out)
+    for _ in range(2):
+        out.fill_(float("nan"))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            graph.replay()
+        own.sync()
+        check_attention(c, x, out, None, c.dim ** -0.5)
+    del graph
+    own.close()
