@@ -74,22 +74,20 @@ __device__ __forceinline__ Place place_of(const KvAppendParams& p, int row, int 
         return w;
     }
     const int first = p.batch.row_start[s], end = p.batch.row_start[s + 1];
-    const int c = p.batch.kv_len[s] - (end - row);   // cache position (negative: before the cache's start)
+    const int64_t c = (int64_t)p.batch.kv_len[s] - end + row;   // cache position (negative: before the cache's start)
     if (row >= first && c >= 0 && c < p.batch.max_pages * PAGE) {
-        const int page = p.batch.table[(int64_t)s * p.batch.max_pages + c / PAGE];
+        const int page = p.batch.table[(int64_t)s * p.batch.max_pages + (int)c / PAGE];
         if (page >= 0 && page < p.kv.n_page)
-            w.slot = (((int64_t)page * p.kv.n_layer + p.kv.layer) * 2 * p.kv.n_head * PAGE + c % PAGE) * D;
+            w.slot = (((int64_t)page * p.kv.n_layer + p.kv.layer) * 2 * p.kv.n_head * PAGE + (int)c % PAGE) * D;
         else if (report)
             atomicOr(p.err, PAGED_BAD_PAGE);
     } else if (report && (row < first || c >= 0)) {
         atomicOr(p.err, PAGED_BAD_LENGTH);
     }
     if (p.rot) {
-        w.pos = p.pos ? p.pos[row] : c;
-        if (w.pos < 0 || w.pos >= p.n_pos) {
-            if (report && (p.pos || c >= 0)) atomicOr(p.err, PAGED_BAD_POSITION);
-            w.pos = w.pos < 0 ? 0 : p.n_pos - 1;
-        }
+        const int64_t pos = p.pos ? p.pos[row] : c;
+        if (report && (pos < 0 || pos >= p.n_pos) && (p.pos || c >= 0)) atomicOr(p.err, PAGED_BAD_POSITION);
+        w.pos = pos < 0 ? 0 : pos < p.n_pos ? (int)pos : p.n_pos - 1;
     }
     return w;
 }

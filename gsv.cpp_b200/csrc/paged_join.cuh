@@ -39,15 +39,16 @@ struct ChunkRange {
 __device__ __forceinline__ bool chunk_range(const ChunkAttnParams& p, int s, int tile, int group, int tile_rows, int key_tile,
                                             bool report, ChunkRange& c) {
     c.row0 = p.batch.row_start[s];
-    c.n = p.batch.row_start[s + 1] - c.row0;
+    const int64_t n = (int64_t)p.batch.row_start[s + 1] - c.row0;
     c.total = p.batch.kv_len[s];   // positions count from the true length
     const int np = p.prefix ? p.prefix[s] : 0;
-    if (report && (c.row0 < 0 || c.n < 0 || c.row0 > p.batch.n_rows - c.n || c.total < 0 || c.total > p.batch.max_kv ||
-                   c.n > p.batch.max_chunk))
+    if (report && (c.row0 < 0 || n < 0 || c.row0 + n > p.batch.n_rows || c.total < 0 || c.total > p.batch.max_kv ||
+                   n > p.batch.max_chunk))
         atomicOr(p.err, PAGED_BAD_LENGTH);
-    c.len = max(0, min(c.total, p.batch.max_kv));
-    if (c.row0 < 0 || c.row0 > p.batch.n_rows) return false;
-    c.n = min(c.n, p.batch.n_rows - c.row0);
+    c.total = max(c.total, 0);
+    c.len = min(c.total, p.batch.max_kv);
+    if (c.row0 < 0 || c.row0 >= p.batch.n_rows || n <= 0) return false;
+    c.n = (int)min(n, (int64_t)(p.batch.n_rows - c.row0));   // (the sizes are at most 2^30 rows times query heads)
     c.r0 = tile * tile_rows;
     c.rows = min(tile_rows, c.n * group - c.r0);
     if (c.rows <= 0) return false;

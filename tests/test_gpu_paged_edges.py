@@ -108,3 +108,35 @@ def test_scratch_does_not_grow_in_a_capture(mode):
         check_attention(c, x, out, None, c.dim ** -0.5)
     del graph
     own.close()
+
+
+@pytest.mark.parametrize("ty", ["f16", "f32"])
+@pytest.mark.parametrize("group", [1, 3, 5, 7])
+@pytest.mark.parametrize("bounds", [(0, -723922764), (7, -1292124672), (8, -1199745), (0, -1599320890), (3, -2 ** 31),
+                                    (-5, 3), (8, 2 ** 31 - 1), (2 ** 31 - 1, -2 ** 31), (9, 9)])
+def test_row_bounds_far_outside_the_batch(ctx, ty, group, bounds):  # noqa: F811
+    """row_start with values whose differences and products pass 32 bits: the call reports them and writes nothing outside
+    its rows and pages."""
+    import gsvcu
+    c = Case(ty, [8], [70], 2 * group, 2, 64)
+    c.row_start.copy_(torch.tensor(bounds, dtype=torch.int32))
+    x, kv = c.rand(8, 2 * group, 64), c.rand(8, 2, 64)
+    guard = torch.full((72, 2 * group, 64), 7.0, dtype=c.dtype, device="cuda")
+    out = guard[32:40]
+    cache, chunks = c.objects()
+    for lens in (70, 0, -2 ** 31, 2 ** 31 - 1):
+        c.kv.fill_(lens)
+        torch.cuda.synchronize()
+        ctx.op_chunk_attention(cache, chunks, 1, x, out)
+        with pytest.raises(gsvcu.GsvcuError) as e:
+            ctx.sync()
+        assert e.value.code == -1 and "row_start" in str(e.value)
+        before = c.pool.clone()
+        torch.cuda.synchronize()
+        ctx.op_kv_append(cache, chunks, 1, x, kv, kv, out)
+        with pytest.raises(gsvcu.GsvcuError) as e:
+            ctx.sync()
+        assert e.value.code == -1
+        assert (guard[:32] == 7.0).all() and (guard[40:] == 7.0).all()
+        assert torch.equal(torch.nan_to_num(before[:, 0]), torch.nan_to_num(c.pool[:, 0]))   # (the other layer)
+    ctx.sync()
