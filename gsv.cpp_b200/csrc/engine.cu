@@ -1855,12 +1855,12 @@ static int paged_views(gsvcu_ctx* ctx, const gsvcu_paged_kv* kv, const gsvcu_chu
     if (!b->row_start_dev || !b->kv_len_dev || !b->block_table_dev)
         return ctx->fail(GSVCU_ERR_ARG, "chunk batch: null row_start, kv_len or block_table");
     if (b->n_seq < 0 || b->max_pages <= 0 || b->max_pages > (1 << 24) || b->n_rows < 0 || b->max_chunk < 0 ||
-        b->max_chunk > b->n_rows || (b->n_rows > 0 && b->max_chunk == 0) || b->max_kv < 0)
+        (b->n_rows > 0 && b->max_chunk == 0) || b->max_kv < 0)
         return ctx->fail(GSVCU_ERR_ARG, "chunk batch: sizes out of range");
     pv.pool = kv->pool_dev; pv.kv_dtype = kv->kv_dtype; pv.n_page = kv->n_page; pv.n_layer = kv->n_layer;
     pv.layer = layer; pv.n_head = kv->n_kv_head; pv.head_dim = kv->head_dim;
     cv.row_start = b->row_start_dev; cv.kv_len = b->kv_len_dev; cv.table = b->block_table_dev;
-    cv.n_seq = b->n_seq; cv.max_pages = b->max_pages; cv.n_rows = b->n_rows; cv.max_chunk = b->max_chunk;
+    cv.n_seq = b->n_seq; cv.max_pages = b->max_pages; cv.n_rows = b->n_rows; cv.max_chunk = std::min(b->max_chunk, b->n_rows);
     cv.max_kv = b->max_kv > 0 ? std::min(b->max_kv, b->max_pages * PAGE) : b->max_pages * PAGE;
     return GSVCU_OK;
 }

@@ -74,7 +74,9 @@ __device__ __forceinline__ Place place_of(const KvAppendParams& p, int row, int 
         return w;
     }
     const int first = p.batch.row_start[s], end = p.batch.row_start[s + 1];
-    const int64_t c = (int64_t)p.batch.kv_len[s] - end + row;   // cache position (negative: before the cache's start)
+    const int len = p.batch.kv_len[s];
+    const int64_t c = (int64_t)len - end + row;   // cache position (negative: before the cache's start)
+    if (report && (len < 0 || len > p.batch.max_kv || (int64_t)end - first > p.batch.max_chunk)) atomicOr(p.err, PAGED_BAD_LENGTH);
     if (row >= first && c >= 0 && c < p.batch.max_pages * PAGE) {
         const int page = p.batch.table[(int64_t)s * p.batch.max_pages + (int)c / PAGE];
         if (page >= 0 && page < p.kv.n_page)

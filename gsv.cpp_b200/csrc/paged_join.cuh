@@ -43,7 +43,8 @@ __device__ __forceinline__ bool chunk_range(const ChunkAttnParams& p, int s, int
     c.total = p.batch.kv_len[s];   // positions count from the true length
     const int np = p.prefix ? p.prefix[s] : 0;
     if (report && (c.row0 < 0 || n < 0 || c.row0 + n > p.batch.n_rows || c.total < 0 || c.total > p.batch.max_kv ||
-                   n > p.batch.max_chunk))
+                   n > p.batch.max_chunk || (s == 0 && c.row0 != 0) ||
+                   (s == p.batch.n_seq - 1 && c.row0 + n != p.batch.n_rows)))   // (rows that no sequence owns)
         atomicOr(p.err, PAGED_BAD_LENGTH);
     c.total = max(c.total, 0);
     c.len = min(c.total, p.batch.max_kv);

@@ -283,10 +283,12 @@ typedef struct {
  * (row_start [n_seq + 1], ascending), holds kv_len[s] keys with these rows and keeps key c in page
  * block_table[s][c / 64], slot c % 64 (block_table [n_seq][max_pages], max_pages <= 2^24; entries past its keys, and of
  * pages that no row of the chunk sees, are not used).
- * Row i of n is the token at cache position kv_len[s] - n + i. Host sizes: n_rows packed rows, max_chunk at
- * least the longest chunk, max_kv at least the longest kv_len (0: max_pages * 64); the closer these are, the
- * better the work is cut up. A page outside the pool, or lengths outside these sizes, touch no memory
- * outside the arrays; the rows they concern are undefined, and the next gsvcu_sync returns GSVCU_ERR_ARG. */
+ * Row i of n is the token at cache position kv_len[s] - n + i. Host sizes: n_rows packed rows (row_start[0] = 0,
+ * row_start[n_seq] = n_rows), max_chunk at least the longest chunk, max_kv at least the longest kv_len (0: max_pages *
+ * 64); the closer these are, the better the work is cut up. A page outside the pool, a row that no sequence owns, or
+ * lengths outside these sizes (kv_len below 0 or above max_kv or the table, a chunk above max_chunk) touch no memory
+ * outside the arrays; the rows they concern are undefined, and after either operator the next gsvcu_sync returns
+ * GSVCU_ERR_ARG. Without rows or without sequences nothing is done. */
 typedef struct {
     const int32_t *row_start_dev, *kv_len_dev, *block_table_dev;
     int32_t n_seq, max_pages, n_rows, max_chunk, max_kv;

@@ -113,7 +113,7 @@ def test_scratch_does_not_grow_in_a_capture(mode):
 @pytest.mark.parametrize("ty", ["f16", "f32"])
 @pytest.mark.parametrize("group", [1, 3, 5, 7])
 @pytest.mark.parametrize("bounds", [(0, -723922764), (7, -1292124672), (8, -1199745), (0, -1599320890), (3, -2 ** 31),
-                                    (-5, 3), (8, 2 ** 31 - 1), (2 ** 31 - 1, -2 ** 31), (9, 9)])
+                                    (-5, 3), (-2 ** 31, 2 ** 31 - 1), (8, 2 ** 31 - 1), (2 ** 31 - 1, -2 ** 31), (9, 9)])
 def test_row_bounds_far_outside_the_batch(ctx, ty, group, bounds):  # noqa: F811
     """row_start with values whose differences and products pass 32 bits: the call reports them and writes nothing outside
     its rows and pages."""
@@ -140,3 +140,45 @@ def test_row_bounds_far_outside_the_batch(ctx, ty, group, bounds):  # noqa: F811
         assert (guard[:32] == 7.0).all() and (guard[40:] == 7.0).all()
         assert torch.equal(torch.nan_to_num(before[:, 0]), torch.nan_to_num(c.pool[:, 0]))   # (the other layer)
     ctx.sync()
+
+
+@pytest.mark.parametrize("ty", ["f16", "f32"])
+@pytest.mark.parametrize("q", [2, 70])
+def test_both_operators_report_the_same_bounds(ctx, ty, q):  # noqa: F811
+    """Lengths inside the table but outside the given sizes, and rows that no sequence owns, are reported after either
+    operator; a bound on the chunks that is wider than the batch is none of these."""
+    import gsvcu
+    c = Case(ty, [q, q], [q + 100, q + 30], 4, 2, 64, max_pages=8)
+    x, kv = c.rand(2 * q, 4, 64), c.rand(2 * q, 2, 64)
+    out = torch.empty_like(x)
+
+    def reported(chunks):
+        cache = gsvcu.PagedKV(c.pool)
+        found = []
+        for call in (lambda: ctx.op_kv_append(cache, chunks, 1, x, kv, kv, out),
+                     lambda: ctx.op_chunk_attention(cache, chunks, 1, x, out)):
+            torch.cuda.synchronize()
+            call()
+            try:
+                ctx.sync()
+                found.append(None)
+            except gsvcu.GsvcuError as e:
+                assert e.code == -1
+                found.append("kv_len" in str(e))
+        return found
+
+    def batch(max_chunk=q, max_kv=q + 100):
+        return gsvcu.ChunkBatch(c.row_start, c.kv, c.table, 2 * q, max_chunk, max_kv)
+
+    assert reported(batch()) == [None, None]
+    assert reported(batch(max_chunk=2 * q + 999)) == [None, None]
+    assert reported(batch(max_kv=q + 99)) == [True, True]
+    assert reported(batch(max_chunk=q - 1)) == [True, True]
+    for bounds in ((0, q, 2 * q - 1), (1, q, 2 * q)):
+        c.row_start.copy_(torch.tensor(bounds, dtype=torch.int32))
+        assert reported(batch()) == [True, True], bounds
+    c.row_start.copy_(torch.tensor([0, q, 2 * q], dtype=torch.int32))
+    c.kv[1] = -1
+    assert reported(batch()) == [True, True]
+    c.kv[1] = q + 30
+    attend(ctx, c, max_chunk=100000)
