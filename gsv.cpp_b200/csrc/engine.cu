@@ -1912,8 +1912,8 @@ int gsvcu_op_chunk_attention(gsvcu_ctx* ctx, const gsvcu_chunk_attention* a) {
     const size_t ks = kv->kv_dtype == GSVCU_KV_F32 ? 4 : 2;
     if (!aligned_to(a->q_dev, ks) || !aligned_to(a->out_dev, ks) || !aligned_to(a->lse_dev, 4))
         return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_chunk_attention: rows not aligned to their element");
-    if (a->window < 0 || !std::isfinite(a->scale))
-        return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_chunk_attention: window must be >= 0 and scale finite");
+    if (a->window < 0 || !(std::fabs(a->scale) <= 1e38f))   // (times log2(e) it has to be finite too)
+        return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_chunk_attention: window must be >= 0 and scale finite, at most 1e38");
     if ((int64_t)batch->n_rows * a->n_q_head > (1 << 30))
         return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_chunk_attention: more than 2^30 (row, head) pairs");
     p.n_q_head = a->n_q_head; p.q = a->q_dev; p.q_stride = a->q_stride; p.scale = a->scale;

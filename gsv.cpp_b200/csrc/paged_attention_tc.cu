@@ -145,9 +145,15 @@ __device__ __forceinline__ void tmem_st16u(uint32_t a, const uint32_t (&r)[16]) 
 
 // The lowest n bits (n cut to 0 .. 32).
 __device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : 0xffffffffu >> (32 - min(n, 32)); }
+// Maxima that keep a NaN.
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float y;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+__device__ __forceinline__ float max2(float a, float b) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
     return y;
 }
 template <typename T> __device__ __forceinline__ uint32_t pack2(float x, float y);
@@ -166,6 +172,7 @@ constexpr int EVERY = 4;
 // 2^x of two values on the FMA pipe: x = n + f with n the nearest integer (by the 1.5 * 2^23 addend) and
 // |f| <= 1/2, 2^f by its relative minimax polynomial (least squares with Lawson's weights: degree 3 for BF16,
 // relative error 7.5e-5; degree 4 for F16, 2.6e-6), n added to the exponent. Below 2^-126: 2^-126.
+// x must not be NaN (rows that hold one have a NaN reference, and the sums and products of their other pairs are NaN).
 template <typename T>
 __device__ __forceinline__ uint64_t ex2_pair(uint64_t x) {
     x = f2pack(fmaxf(f2lo(x), -126.0f), fmaxf(f2hi(x), -126.0f));
@@ -515,12 +522,15 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
                     mx[k] = __uint_as_float(x[k][0]);
 #pragma unroll
                     for (int i = 1; i < 31; i += 2) mx[k] = max3(mx[k], __uint_as_float(x[k][i]), __uint_as_float(x[k][i + 1]));
-                    mx[k] = fmaxf(mx[k], __uint_as_float(x[k][31]));
+                    mx[k] = max2(mx[k], __uint_as_float(x[k][31]));
                 }
-                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.c;
-                // raise the reference maximum of the warp's rows when one of them needs it
-                if (__any_sync(0xffffffffu, top > mref + TAU)) {
-                    const float up = fmaxf(mref, top);
+                const float top = max2(max2(mx[0], mx[1]), max2(mx[2], mx[3])) * a.c;
+                // Raise the reference maximum of the warp's rows when one of them needs it. A score that is NaN or has
+                // overflowed makes the row's reference NaN, and with it all that the row gives: the polynomial would take the
+                // exponent of such a score for a small one.
+                if (__any_sync(0xffffffffu, !(top <= mref + TAU))) {
+                    float up = max2(mref, top);
+                    if (up == -NEG_INF) up = __int_as_float(0x7fffffff);
                     if (j > 0) {
                         // O must be at rest. With two row tiles it is: these scores were issued after the product before
                         if (halves == 1) {
@@ -613,7 +623,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
                     }
                 }
                 if (mine && p.lse)
-                    p.lse[row * p.n_q_head + head] = mref == NEG_INF ? NEG_INF : (mref + log2f(l)) * LN2;
+                    p.lse[row * p.n_q_head + head] = (mref + log2f(l)) * LN2;   // (nothing seen: both -infinity)
             } else if (ok) {
                 // Split results (f32, nt > 0) go through shared memory, where this row tile's queries are no longer needed, in
                 // two halves of the columns, so that a warp's stores cover whole rows (512 tokens over 8192 keys: 47.9 -> 45.0

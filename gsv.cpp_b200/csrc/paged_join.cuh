@@ -93,13 +93,13 @@ template <typename T, int D>
 __device__ __forceinline__ void finish(const ChunkAttnParams& p, const ChunkRange& c, bool vec, int group, int h, int r, int d,
                                        float top, float sum, float (&x)[4]) {
     const int tok = (c.r0 + r) / group, head = h * group + (c.r0 + r) % group;
-    if (top != NEG_INF) {
+    if (sum != 0.0f) {   // (a row that sees nothing stays 0; one whose scores are all NaN has no maximum either, but a NaN sum)
 #pragma unroll
         for (int k = 0; k < 4; k++) x[k] = x[k] / sum;
     }
     store_out<T, D>(p, vec, c.row0 + tok, head, d, x);
     if (p.lse && d == 0)
-        p.lse[(int64_t)(c.row0 + tok) * p.n_q_head + head] = top == NEG_INF ? NEG_INF : (top + log2f(sum)) * LN2;
+        p.lse[(int64_t)(c.row0 + tok) * p.n_q_head + head] = (top + log2f(sum)) * LN2;   // (nothing seen: both -infinity)
 }
 
 // Splits g, g + per, ... of n_act added up for four outputs of row r; 8 loads in flight whatever the count.

@@ -322,7 +322,8 @@ int gsvcu_op_kv_append(gsvcu_ctx* ctx, const gsvcu_kv_append* a);
  * lse_dev (may be null) [n_rows][n_q_head] gets the natural logarithm of each row's sum of exp(scale q.k).
  * A row that sees no key gives 0 and -infinity. Scores, softmax and sums are F32. What the pages hold from kv_len
  * on does not matter, nor do pages that no row sees; in the other pages every key and value has to be finite (a
- * value that is not reaches rows that do not see it, as 0 times infinity). */
+ * value that is not reaches rows that do not see it, as 0 times infinity). A row with a score that is NaN or overflows to
+ * infinity is NaN, a score of minus infinity has weight 0 (F32 caches: NaN too); |scale| at most 1e38. */
 typedef struct {
     const gsvcu_paged_kv* kv;
     const gsvcu_chunk_batch* batch;

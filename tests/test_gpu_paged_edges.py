@@ -182,3 +182,73 @@ def test_both_operators_report_the_same_bounds(ctx, ty, q):  # noqa: F811
     assert reported(batch()) == [True, True]
     c.kv[1] = q + 30
     attend(ctx, c, max_chunk=100000)
+
+
+@pytest.mark.parametrize("ty,dim,q", [("bf16", 128, 1), ("bf16", 64, 60), ("bf16", 128, 200), ("bf16", 32, 300), ("f32", 64, 1),
+                                      ("f32", 64, 40)])
+@pytest.mark.parametrize("at", [5, 6, 7, 63, 70, 134, 391])
+@pytest.mark.parametrize("kv", [400, 5000])
+def test_scores_that_overflow_make_their_rows_nan(ctx, ty, dim, q, at, kv):  # noqa: F811
+    """Finite queries and keys whose product is infinite: as exp(inf - inf) the row and its log-sum-exp are NaN, whichever
+    key it is; a product of minus infinity has weight 0 (F32: NaN, its two parts overflow apart); other rows are not
+    touched."""
+    c = Case(ty, [q], [kv + q], 2, 1, dim)
+    x = c.rand(q, 2, dim)
+    x[:, :, :3] = 0.0
+    zero = torch.zeros(kv + q, device="cuda")
+    for d in range(3):
+        set_keys(c, 0, d, zero)
+    _, base, base_lse = attend(ctx, c, q=x)
+    big = zero.clone()
+    big[at] = 1e30
+    set_keys(c, 0, 0, big)
+    set_keys(c, 0, 1, -big)
+    rows = torch.arange(q, device="cuda") % 40 == 0
+    cache, chunks = c.objects()
+    out, lse = torch.empty_like(x), torch.empty(q, 2, device="cuda")
+    for d in (0, 1):
+        y = x.clone()
+        y[rows, 0, d] = 1e30
+        torch.cuda.synchronize()
+        ctx.op_chunk_attention(cache, chunks, c.layer, y, out, lse=lse)
+        ctx.sync()
+        if d == 0 or ty == "f32":
+            assert out[rows, 0].isnan().all() and lse[rows, 0].isnan().all(), d
+        else:
+            assert torch.isfinite(out).all() and torch.isfinite(lse).all()
+            # one key of weight about exp(|q| |k| / sqrt(dim)) / kv less
+            assert ((lse[rows, 0] - base_lse[rows, 0]).abs() < 0.2).all()
+        rest = torch.ones_like(lse, dtype=torch.bool)
+        rest[rows, 0] = False
+        assert torch.allclose(out[rest].float(), base[rest].float(), rtol=2.0 ** -6, atol=2.0 ** -6), d
+        assert torch.allclose(lse[rest], base_lse[rest], rtol=1e-5, atol=1e-4), d
+
+
+@pytest.mark.parametrize("ty,dim,q", [("f16", 32, 1), ("bf16", 128, 5), ("f32", 64, 40), ("f16", 64, 60), ("bf16", 128, 300)])
+@pytest.mark.parametrize("kv", [70, 5000])
+def test_a_query_of_nan_makes_its_row_nan(ctx, ty, dim, q, kv):  # noqa: F811
+    c = Case(ty, [q], [kv + q], 2, 1, dim)
+    x, base, base_lse = attend(ctx, c)
+    y = x.clone()
+    y[q // 2, 1, 3] = float("nan")
+    cache, chunks = c.objects()
+    out, lse = torch.empty_like(x), torch.empty(q, 2, device="cuda")
+    torch.cuda.synchronize()
+    ctx.op_chunk_attention(cache, chunks, c.layer, y, out, lse=lse)
+    ctx.sync()
+    assert out[q // 2, 1].isnan().all() and lse[q // 2, 1].isnan()
+    rest = torch.ones_like(lse, dtype=torch.bool)
+    rest[q // 2, 1] = False
+    assert torch.allclose(out[rest].float(), base[rest].float(), rtol=2.0 ** -6, atol=2.0 ** -6)
+    assert torch.allclose(lse[rest], base_lse[rest], rtol=1e-5, atol=1e-4)
+
+
+def test_scales_past_the_range_are_refused(ctx):  # noqa: F811
+    import gsvcu
+    c = Case("f16", [1], [5], 1, 1, 32)
+    x = c.rand(1, 1, 32)
+    cache, chunks = c.objects()
+    for scale in (3e38, -3e38, float("inf"), float("nan")):
+        with pytest.raises(gsvcu.GsvcuError) as e:
+            ctx.op_chunk_attention(cache, chunks, 1, x, x.clone(), scale=scale)
+        assert e.value.code == -1 and "scale" in str(e.value)
