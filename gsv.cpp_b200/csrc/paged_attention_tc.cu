@@ -170,27 +170,20 @@ template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float x, fl
 // and SM) would need 2048 cycles for two row tiles of 128 keys, as many as their products at head dim 128.
 constexpr int EVERY = 4;
 // 2^x of two values on the FMA pipe: x = n + f with n the nearest integer (by the 1.5 * 2^23 addend) and
-// |f| <= 1/2, 2^f by its relative minimax polynomial (least squares with Lawson's weights: degree 3 for BF16,
-// relative error 7.5e-5; degree 4 for F16, 2.6e-6), n added to the exponent. Below 2^-126: 2^-126.
+// |f| <= 1/2, 2^f by its relative minimax polynomial of degree 4 (least squares with Lawson's weights; relative error
+// 2.7e-6, which the sums and the log-sum-exp take too: degree 5, 2.1e-7, made F16 chunks 1 to 3 % slower), n added to
+// the exponent. Below 2^-126: 2^-126.
 // x must not be NaN (rows that hold one have a NaN reference, and the sums and products of their other pairs are NaN).
-template <typename T>
 __device__ __forceinline__ uint64_t ex2_pair(uint64_t x) {
     x = f2pack(fmaxf(f2lo(x), -126.0f), fmaxf(f2hi(x), -126.0f));
     const uint64_t big = f2pack(12582912.0f, 12582912.0f), nbig = f2pack(-12582912.0f, -12582912.0f);
     const uint64_t n = fadd2(x, big);
     const uint64_t f = ffma2(fadd2(n, nbig), f2pack(-1.0f, -1.0f), x);
     auto k = [](float v) { return f2pack(v, v); };
-    uint64_t y;
-    if constexpr (__is_same(T, __half)) {
-        y = ffma2(f, k(0x1.3997d6p-7f), k(0x1.ca1440p-5f));
-        y = ffma2(f, y, k(0x1.ec06dap-3f));
-        y = ffma2(f, y, k(0x1.62e0dcp-1f));
-        y = ffma2(f, y, k(0x1.ffffe8p-1f));
-    } else {
-        y = ffma2(f, k(0x1.c3f760p-5f), k(0x1.f0de1ap-3f));
-        y = ffma2(f, y, k(0x1.62f31ap-1f));
-        y = ffma2(f, y, k(0x1.fff692p-1f));
-    }
+    uint64_t y = ffma2(f, k(0x1.3997d6p-7f), k(0x1.ca1440p-5f));
+    y = ffma2(f, y, k(0x1.ec06dap-3f));
+    y = ffma2(f, y, k(0x1.62e0dcp-1f));
+    y = ffma2(f, y, k(0x1.ffffe8p-1f));
     return f2pack(__int_as_float(__float_as_int(f2lo(y)) + (__float_as_int(f2lo(n)) << 23)),
                   __int_as_float(__float_as_int(f2hi(y)) + (__float_as_int(f2hi(n)) << 23)));
 }
@@ -563,7 +556,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
 #pragma unroll
                         for (int i = 0; i < 16; i++) {
                             uint64_t e = ffma2(f2pack(__uint_as_float(x[k][2 * i]), __uint_as_float(x[k][2 * i + 1])), c2, ref2);
-                            if (!decltype(tested)::value && i % EVERY == EVERY - 1) e = ex2_pair<T>(e);
+                            if (!decltype(tested)::value && i % EVERY == EVERY - 1) e = ex2_pair(e);
                             else e = f2pack(ex2(f2lo(e)), ex2(f2hi(e)));
                             sum = fadd2(sum, e);
                             w[i] = pack2<T>(f2lo(e), f2hi(e));

@@ -252,3 +252,19 @@ def test_scales_past_the_range_are_refused(ctx):  # noqa: F811
         with pytest.raises(gsvcu.GsvcuError) as e:
             ctx.op_chunk_attention(cache, chunks, 1, x, x.clone(), scale=scale)
         assert e.value.code == -1 and "scale" in str(e.value)
+
+
+@pytest.mark.parametrize("ty", ["f16", "bf16"])
+@pytest.mark.parametrize("at", [4, 5, 6, 7, 77, 78, 79])
+def test_one_key_that_outweighs_the_rest(ctx, ty, at):  # noqa: F811
+    """One key holds all but a ten-thousandth of the weight, at any place among the columns: its exponential alone decides
+    the sum, so that the log-sum-exp shows the exponential's error."""
+    c = Case(ty, [200], [500], 2, 2, 32)
+    q = torch.zeros(200, 2, 32, dtype=c.dtype, device="cuda")
+    q[:, :, 0] = 5.0
+    for d in range(32):
+        set_keys(c, 0, d, torch.zeros(500, device="cuda"))
+    key = torch.zeros(500, device="cuda")
+    key[at] = 17.0
+    set_keys(c, 0, 0, key)
+    attend(ctx, c, q=q)
