@@ -14,7 +14,8 @@
 // Everything is transposed: S^T = K Q^T with 16 keys and 8 query rows per product, O^T = V^T P^T, because few
 // rows are the rule here (one decoding token of one head is one row) and 8 is the smaller side of mma.sync.
 // F16 / BF16 products run on mma.m16n8k16 with the weights split into two 16-bit parts (w = hi + lo), so
-// rounding them costs nothing against the output's own rounding; F32 ones on mma.m16n8k8.tf32 with both
+// rounding them costs nothing against the output's own rounding (F16 weights are kept 2^14 up, where hi and lo have 22 bits
+// down to 2^-17 of the running maximum's and the last one at 2^-38); F32 ones on mma.m16n8k8.tf32 with both
 // operands in two parts (three products), which leaves an error near 2^-22. Sums, maxima and outputs are f32.
 // Keys past kv_len are never read (zero-filled), keys that a row must not see get weight 0.
 // Decode is bound by HBM: every key is read once, 12 to 16 KB in flight per warp (64 sequences of 600 to 2100 keys, 16
@@ -30,6 +31,7 @@ namespace gsvcu {
 namespace {
 
 constexpr int NW = 4;   // warps per CTA
+template <typename T> constexpr float BIAS = __is_same(T, __half) ? 14.0f : 0.0f;   // weights are 2^BIAS exp(s - maximum)
 // Keys of one warp's tile: 8 KB of K and V, 16 KB for wide F32 rows (a product takes 16 keys at least), 4 KB for
 // F16 / BF16 heads of 32, where the CTAs are short and four of them fit an SM (64 slots: 36.9 us against 38.4).
 __host__ __device__ constexpr int key_tile(int dim, int size) {
@@ -381,7 +383,7 @@ __global__ void __launch_bounds__(NW * 32) k_chunk_attn(SplitArgs a) {
                     }
                     m[b][e] = top;
                 }
-                const float ref = m[b][e] == NEG_INF ? 0.0f : m[b][e];
+                const float ref = m[b][e] == NEG_INF ? 0.0f : m[b][e] - BIAS<T>;
 #pragma unroll
                 for (int j = 0; j < KT / 16; j++)
 #pragma unroll
@@ -474,7 +476,7 @@ __global__ void __launch_bounds__(NW * 32) k_chunk_attn(SplitArgs a) {
             x += __shfl_xor_sync(0xffffffffu, x, 16);
             const int r = warp * ROWS + b * 8 + col + e;
             if (lane < 4) {
-                ml[2 * r] = m[b][e];
+                ml[2 * r] = m[b][e] - BIAS<T>;   // (what the weights refer to)
                 ml[2 * r + 1] = x;
             }
 #pragma unroll

@@ -12,8 +12,10 @@
 // The MMAs of one row tile run under the other's softmax: S0 S1 | PV0 S0' PV1 S1' | ... Each thread takes its
 // 128 scores into registers, writes the weights P over them in tensor memory as 16-bit pairs, and keeps the
 // row's sum. A row's reference maximum is raised only when a tile exceeds it by more than 2^TAU, then O in
-// tensor memory is scaled once its last PV is done; so P <= 2^TAU, far inside F16. Weights are rounded to the
-// cache's type for the product: with the output's own rounding that is sqrt(2) of it, and the sums stay f32.
+// tensor memory is scaled once its last PV is done. Weights are rounded to the cache's type for the product: with
+// the output's own rounding that is sqrt(2) of it, and the sums stay f32. F16 weights are kept 2^BIAS up (P <= 2^(TAU +
+// BIAS) = 2^15), so that their 11 bits reach down to 2^-25 of the maximum and the last one to 2^-35 (a long light tail
+// beside one heavy key); the factor is in the reference, so sums, splits and the log-sum-exp need nothing for it.
 // Tensor memory: S0 | S1 (128 columns each; P over their first 64) | O0 | O1. With one row tile its key tiles take
 // the two score buffers in turn, and the next scores are computed beside the softmax.
 // Products of two row tiles and 128 keys take 2048 cycles at head dim 128, a softmax warp ~1850 per tile; what bounds the
@@ -37,7 +39,10 @@ using namespace tc;
 constexpr int KT = 128;                 // keys per tile
 constexpr int ROWS = 256;               // packed rows per CTA, two row tiles (one of 128 when the call has few CTAs)
 constexpr int THREADS = 384;
-constexpr float TAU = 8.0f;             // log2 headroom of P above the row's reference maximum
+// Log2 headroom of P above the row's reference maximum, and how far up the weights are kept. F16: TAU 5, 4 or 3 cost
+// about 1 % over TAU 8 on scores of deviation 1, TAU 1 2 to 7 %.
+template <typename T> constexpr float TAU = __is_same(T, __half) ? 4.0f : 8.0f;
+template <typename T> constexpr float BIAS = __is_same(T, __half) ? 11.0f : 0.0f;
 
 template <int D>
 struct Smem {
@@ -474,7 +479,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
             const uint32_t tl = tmem + ((uint32_t)(32 * q) << 16), to = tl + L::TM_O + (uint32_t)t * 128;
             const int pos = c.total - c.n + (c.r0 + min(r, c.rows - 1)) / a.group;
             const int see_hi = min(c.len, pos + 1), see_lo = p.window ? pos - p.window + 1 : 0;
-            float mref = NEG_INF, l = 0.0f;
+            float mref = NEG_INF, l = 0.0f;   // reference (a maximum less BIAS), sum of the weights
             bool ok = true;
             for (int j = 0; j < nt && ok; j++) {
                 const int n = halves * j + t, b = n & 1;   // the scores' number, their buffer
@@ -521,8 +526,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
                 // Raise the reference maximum of the warp's rows when one of them needs it. A score that is NaN or has
                 // overflowed makes the row's reference NaN, and with it all that the row gives: the polynomial would take the
                 // exponent of such a score for a small one.
-                if (__any_sync(0xffffffffu, !(top <= mref + TAU))) {
-                    float up = max2(mref, top);
+                if (__any_sync(0xffffffffu, !(top <= mref + (TAU<T> + BIAS<T>)))) {
+                    float up = max2(mref, top - BIAS<T>);
                     if (up == -NEG_INF) up = __int_as_float(0x7fffffff);
                     if (j > 0) {
                         // O must be at rest. With two row tiles it is: these scores were issued after the product before

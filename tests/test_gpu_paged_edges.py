@@ -268,3 +268,21 @@ def test_one_key_that_outweighs_the_rest(ctx, ty, at):  # noqa: F811
     key[at] = 17.0
     set_keys(c, 0, 0, key)
     attend(ctx, c, q=q)
+
+
+@pytest.mark.parametrize("ty,q", [("f16", 1), ("f16", 4), ("f16", 24), ("f16", 40), ("f16", 150), ("bf16", 1), ("bf16", 40)])
+@pytest.mark.parametrize("below,spread", [(25.1, 0.0), (24.0, 0.3), (22.0, 0.0)])
+def test_a_sink_beside_a_long_light_tail(ctx, ty, q, below, spread):  # noqa: F811
+    """One key of value 0 holds nearly all the weight, 16383 others 2^-22 to 2^-25 of its weight each: the output is the
+    tail's. F16 holds weights down to 2^-24 with few bits and none below 2^-25."""
+    n_seq, kv = 10, 16384
+    c = Case(ty, [q] * n_seq, [kv] * n_seq, 8, 8, 64)
+    x = torch.zeros(c.rows, 8, 64, dtype=c.dtype, device="cuda")
+    x[:, :, 0] = 8.0
+    c.pool[:, :, 1] = c.pool[:, :, 1].abs() + 0.5
+    for s in range(n_seq):
+        key = torch.randn(kv, generator=c.gen, device="cuda") * spread
+        key[0] = below * 0.6931
+        set_keys(c, s, 0, key)
+        c.pool[int(c.table[s, 0]), c.layer, 1, :, 0] = 0.0
+    attend(ctx, c, q=x)
