@@ -526,6 +526,10 @@ class Context:
         n, D, H, dev = chunks.n_rows, cache.head_dim, cache.n_kv_head, self.device
         if cache.device != dev or chunks.device != dev:
             raise ValueError(f"cache and batch must be on CUDA device {dev}")
+        if (q is None) != (q_out is None):
+            raise ValueError("q and q_out belong together")
+        if (cos is None) != (sin is None) or (cos is not None and cos.dim() != 2):
+            raise ValueError("cos and sin: [positions][rotated / 2] expected, both or none")
         ty, shape = k.dtype, (n, H, D)
         ks, vs = _row_stride(k, shape, "k", dev), _row_stride(v, shape, "v", dev)
         nq = qp = qs = op = os_ = 0

@@ -286,3 +286,20 @@ def test_a_sink_beside_a_long_light_tail(ctx, ty, q, below, spread):  # noqa: F8
         set_keys(c, s, 0, key)
         c.pool[int(c.table[s, 0]), c.layer, 1, :, 0] = 0.0
     attend(ctx, c, q=x)
+
+
+def test_append_refuses_half_given_arguments(ctx):  # noqa: F811
+    """A table of angles with broadcast dimensions (its rows would be taken for other positions' angles), one table without
+    the other, queries without their output."""
+    c = Case("f16", [2], [70], 4, 2, 64)
+    cache, chunks = c.objects()
+    q, kv = c.rand(2, 4, 64), c.rand(2, 2, 64)
+    out, angle = torch.empty_like(q), torch.zeros(80, 32, device="cuda")
+    for bad in (dict(cos=angle[:, None], sin=angle[:, None]), dict(cos=angle[:, :, None], sin=angle[:, :, None]), dict(cos=angle),
+                dict(sin=angle), dict(cos=angle[0], sin=angle[0]), dict(q_out=None), dict(q=None)):
+        args = dict(q=q, k=kv, v=kv, q_out=out)
+        args.update(bad)
+        with pytest.raises(ValueError):
+            ctx.op_kv_append(cache, chunks, 1, **args)
+    ctx.op_kv_append(cache, chunks, 1, q, kv, kv, out, cos=angle, sin=angle)
+    ctx.sync()
