@@ -6,7 +6,7 @@ pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip("torch")
 
-from test_gpu_paged import PAGE, Case, attend, check_attention, ctx  # noqa: E402,F401
+from test_gpu_paged import PAGE, Case, attend, check_append, check_attention, ctx  # noqa: E402,F401
 
 
 def set_keys(c, s, dim, values):
@@ -303,3 +303,17 @@ def test_append_refuses_half_given_arguments(ctx):  # noqa: F811
             ctx.op_kv_append(cache, chunks, 1, **args)
     ctx.op_kv_append(cache, chunks, 1, q, kv, kv, out, cos=angle, sin=angle)
     ctx.sync()
+
+
+@pytest.mark.parametrize("rows", [1500, 3000, 6000])
+@pytest.mark.parametrize("ty,row_ty,dim,rot,pairs", [("bf16", "bf16", 128, 128, False), ("f16", "f32", 32, 32, True),
+                                                     ("f32", "f32", 64, 32, False), ("f16", "f16", 32, 16, False)])
+def test_append_of_many_rows(ctx, ty, row_ty, dim, rot, pairs, rows):  # noqa: F811
+    """Prompt chunks of so many rows that a row takes 128, 64 or 32 threads, beside short ones."""
+    check_append(ctx, ty, row_ty, 6, 2, dim, rot, pairs, q_len=(rows - 141, 1, 0, 140), kv_len=(rows - 141, 77, 5, 200))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_f32_row_tiles_of_24_are_joined(ctx, dim):  # noqa: F811
+    """F32 chunks whose plan takes 24-row tiles and splits the keys."""
+    attend(ctx, Case("f32", [240, 240, 131, 240, 5], [4000, 3999, 4000, 700, 3000], 5, 5, dim))
