@@ -1920,6 +1920,8 @@ int gsvcu_op_chunk_attention(gsvcu_ctx* ctx, const gsvcu_chunk_attention* a) {
     p.window = a->window < (1 << 30) ? a->window : 0;   // (wider than any cache)
     p.prefix = a->prefix_dev; p.out = a->out_dev; p.out_stride = a->out_stride; p.lse = a->lse_dev;
     p.err = ctx->att_err + 3;
+    p.fault_extra_tx = ctx->fault_extra_tx;
+    p.poll_limit = ctx->fault_poll_limit;
     if (batch->n_rows == 0 || batch->n_seq == 0) return GSVCU_OK;
     const ChunkAttnPlan plan = chunk_attention_plan(p);
     if ((int64_t)batch->n_seq * plan.tiles * kv->n_kv_head * plan.n_split > INT32_MAX)

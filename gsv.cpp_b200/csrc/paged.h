@@ -57,6 +57,9 @@ struct ChunkAttnParams {
     int32_t* err = nullptr;
     float* part = nullptr;       // scratch of chunk_attention_plan
     int32_t* arrived = nullptr;  // zero between launches
+    // failure-path tests (gsvcu_set_wait_fault): bytes that a pair's barrier expects beyond its copies, polls of its wait (0: the
+    // usual limit)
+    uint32_t fault_extra_tx = 0, poll_limit = 0;
 };
 // How one call is cut up, from the sizes alone; scratch it needs.
 struct ChunkAttnPlan {

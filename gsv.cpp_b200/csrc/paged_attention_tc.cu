@@ -111,8 +111,8 @@ __device__ __forceinline__ void commit(uint32_t bar) {
         : "memory");
 }
 // Bounded wait of a converged warp, with a warp-uniform result.
-__device__ __forceinline__ bool wait_warp(uint32_t b, uint32_t parity, volatile int* abort_flag) {
-    for (uint32_t it = 0; it < TC_SPIN_LIMIT; it++) {
+__device__ __forceinline__ bool wait_warp(uint32_t b, uint32_t parity, volatile int* abort_flag, uint32_t limit = TC_SPIN_LIMIT) {
+    for (uint32_t it = 0; it < limit; it++) {
         if (__any_sync(0xffffffffu, bar_try_short(b, parity))) return true;
         if (__any_sync(0xffffffffu, *abort_flag)) return false;
     }
@@ -276,7 +276,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
             ok = bar_wait_short(empty(e), ((uint32_t)(i / L::NP) & 1u) ^ 1u, abort_flag);
             if (ok) {
                 const bool has_v = i > 0, has_k = i < nt;
-                bar_expect_tx(full(e), ((int)has_v + (int)has_k) * L::ENTRY);
+                bar_expect_tx(full(e), ((int)has_v + (int)has_k) * L::ENTRY + (has_v ? p.fault_extra_tx : 0u));
                 const uint32_t dst = su32(sm + L::OFF_RING + (size_t)e * 2 * L::ENTRY);
                 auto load = [&](uint32_t to, uint32_t b0, uint32_t b1) {
 #pragma unroll
@@ -360,7 +360,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
                 }
                 // every copy has landed before the CTA may end
                 for (int k = i - 1; k >= 0 && k >= i - L::NP; k--)
-                    for (uint32_t it = 0; it < TC_POLL_LIMIT; it++)
+                    for (uint32_t it = 0; it < min(TC_POLL_LIMIT, p.poll_limit); it++)
                         if (bar_try(full(k % L::NP), (uint32_t)(k / L::NP) & 1u)) break;
             }
         } else if (warp == 1) {
@@ -404,7 +404,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
             }
             // V of tile j and K of tile j + 1 are pair j + 1; at the last tile V has to be cleared first
             auto wait_pair = [&](int j, int e, uint32_t parity) -> bool {
-                if (!wait_warp(full(e), parity, abort_flag)) return false;
+                if (!wait_warp(full(e), parity, abort_flag, p.poll_limit)) return false;
                 if (j + 1 < nt || !cut) return true;
                 if (lane == 0) bar_arrive(vhere);
                 return wait_warp(vclear, 0, abort_flag);
@@ -681,6 +681,7 @@ void pick_tc(int dtype, int dim, F f) {
 bool launch_chunk_attention_tc(const ChunkAttnParams& p, const ChunkAttnPlan& plan, uint64_t* ready, cudaStream_t s) {
     TcArgs a;
     a.p = p;
+    if (!a.p.poll_limit) a.p.poll_limit = TC_SPIN_LIMIT;
     a.group = p.n_q_head / p.kv.n_head;
     a.row_tile = plan.row_tile;
     a.tiles = plan.tiles;

@@ -463,7 +463,7 @@ class Context:
         self._check(self.lib.gsvcu_set_prefill_gemm(self.h, int(mode)))
 
     def set_wait_fault(self, on):
-        """Test-only: make this context's decode-attention page waits run out (gsvcu_set_wait_fault)."""
+        """Test-only: make this context's decode- and chunk-attention page waits run out (gsvcu_set_wait_fault)."""
         self._check(self.lib.gsvcu_set_wait_fault(self.h, 1 if on else 0))
 
     def stream_handle(self):

@@ -501,7 +501,9 @@ int gsvcu_sync(gsvcu_ctx* ctx);
  * its page mbarrier than it stages and gives up after 4096 polls, so its bounded wait runs out: the
  * next status read of generate / serve (or gsvcu_sync after an op call) returns GSVCU_ERR_CUDA with
  * "staged K/V never arrived", and the context stays usable. Nothing faults: the staged copies all
- * complete, only the expected count is never reached. on = 0 (default) restores normal operation. */
+ * complete, only the expected count is never reached. The same holds for the page waits of gsvcu_op_chunk_attention
+ * with many rows (from a block's second pair of copies on, "a bounded wait gave up"). on = 0 (default) restores normal
+ * operation. */
 int gsvcu_set_wait_fault(gsvcu_ctx* ctx, int32_t on);
 
 #ifdef __cplusplus

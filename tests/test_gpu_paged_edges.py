@@ -317,3 +317,27 @@ def test_append_of_many_rows(ctx, ty, row_ty, dim, rot, pairs, rows):  # noqa: F
 def test_f32_row_tiles_of_24_are_joined(ctx, dim):  # noqa: F811
     """F32 chunks whose plan takes 24-row tiles and splits the keys."""
     attend(ctx, Case("f32", [240, 240, 131, 240, 5], [4000, 3999, 4000, 700, 3000], 5, 5, dim))
+
+
+@pytest.mark.parametrize("ty,dim", [("f16", 64), ("bf16", 128)])
+@pytest.mark.parametrize("q,kv", [(60, 60), (60, 900), (300, 300), (300, 2000), (90, 9000)])
+def test_page_waits_that_run_out_are_reported(ctx, ty, dim, q, kv):  # noqa: F811
+    """Every pair of page copies from the second on expects 16 bytes more than it gets (the copies themselves complete) and
+    its wait has a short limit: the call ends with products under way, the next sync reports it once, and the same call
+    without the fault is right."""
+    import gsvcu
+    c = Case(ty, [q, 0, q], [kv, 5, kv], 4, 2, dim)
+    x = c.rand(c.rows, c.heads, dim)
+    out = torch.empty_like(x)
+    cache, chunks = c.objects()
+    torch.cuda.synchronize()
+    ctx.set_wait_fault(True)
+    try:
+        ctx.op_chunk_attention(cache, chunks, c.layer, x, out)
+        with pytest.raises(gsvcu.GsvcuError) as e:
+            ctx.sync()
+        assert e.value.code == -2 and "gave up" in str(e.value)
+    finally:
+        ctx.set_wait_fault(False)
+    ctx.sync()
+    attend(ctx, c, q=x)
