@@ -1835,6 +1835,8 @@ int gsvcu_op_prefill_attention(gsvcu_ctx* ctx, const float* qkv_dev, int32_t n_s
     return GSVCU_OK;
 }
 
+static bool aligned_to(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
+
 // The cache and batch descriptions of the paged-cache operators, checked on the host.
 static int paged_views(gsvcu_ctx* ctx, const gsvcu_paged_kv* kv, const gsvcu_chunk_batch* b, int32_t layer,
                        int32_t n_q_head, PagedView& pv, ChunkView& cv) {
@@ -1854,6 +1856,8 @@ static int paged_views(gsvcu_ctx* ctx, const gsvcu_paged_kv* kv, const gsvcu_chu
         return ctx->fail(GSVCU_ERR_ARG, "paged cache: n_q_head must be a multiple of n_kv_head");
     if (!b->row_start_dev || !b->kv_len_dev || !b->block_table_dev)
         return ctx->fail(GSVCU_ERR_ARG, "chunk batch: null row_start, kv_len or block_table");
+    if (!aligned_to(b->row_start_dev, 4) || !aligned_to(b->kv_len_dev, 4) || !aligned_to(b->block_table_dev, 4))
+        return ctx->fail(GSVCU_ERR_ARG, "chunk batch: arrays not aligned to their element");
     if (b->n_seq < 0 || b->max_pages <= 0 || b->max_pages > (1 << 24) || b->n_rows < 0 || b->max_chunk < 0 ||
         (b->n_rows > 0 && b->max_chunk == 0) || b->max_kv < 0)
         return ctx->fail(GSVCU_ERR_ARG, "chunk batch: sizes out of range");
@@ -1864,8 +1868,6 @@ static int paged_views(gsvcu_ctx* ctx, const gsvcu_paged_kv* kv, const gsvcu_chu
     cv.max_kv = b->max_kv > 0 ? std::min(b->max_kv, b->max_pages * PAGE) : b->max_pages * PAGE;
     return GSVCU_OK;
 }
-
-static bool aligned_to(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
 
 int gsvcu_op_kv_append(gsvcu_ctx* ctx, const gsvcu_kv_append* a) {
     if (!ctx || !a) return GSVCU_ERR_ARG;
@@ -1880,8 +1882,9 @@ int gsvcu_op_kv_append(gsvcu_ctx* ctx, const gsvcu_kv_append* a) {
     if (a->k_stride < kv_width || a->v_stride < kv_width || (n_q > 0 && (a->q_stride < n_q * D || a->q_out_stride < n_q * D)))
         return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_kv_append: row stride shorter than its heads");
     const size_t rs = a->row_dtype == GSVCU_KV_F32 ? 4 : 2, ks = kvd == GSVCU_KV_F32 ? 4 : 2;
-    if (!aligned_to(a->q_dev, rs) || !aligned_to(a->k_dev, rs) || !aligned_to(a->v_dev, rs) || !aligned_to(a->q_out_dev, ks))
-        return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_kv_append: rows not aligned to their element");
+    if (!aligned_to(a->q_dev, rs) || !aligned_to(a->k_dev, rs) || !aligned_to(a->v_dev, rs) || !aligned_to(a->q_out_dev, ks) ||
+        !aligned_to(a->cos_dev, 4) || !aligned_to(a->sin_dev, 4) || !aligned_to(a->pos_dev, 4))
+        return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_kv_append: rows, tables or positions not aligned to their element");
     if (a->rot_dim < 0 || a->rot_dim > D || a->rot_dim % 2 || a->rot_pairs < 0 || a->rot_pairs > 1 ||
         (a->rot_dim > 0 && (!a->cos_dev || !a->sin_dev || a->n_pos <= 0)))
         return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_kv_append: rot_dim must be even, at most head_dim, with its cos / sin table");
@@ -1910,8 +1913,8 @@ int gsvcu_op_chunk_attention(gsvcu_ctx* ctx, const gsvcu_chunk_attention* a) {
     if (a->q_stride < a->n_q_head * D || a->out_stride < a->n_q_head * D)
         return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_chunk_attention: row stride shorter than its heads");
     const size_t ks = kv->kv_dtype == GSVCU_KV_F32 ? 4 : 2;
-    if (!aligned_to(a->q_dev, ks) || !aligned_to(a->out_dev, ks) || !aligned_to(a->lse_dev, 4))
-        return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_chunk_attention: rows not aligned to their element");
+    if (!aligned_to(a->q_dev, ks) || !aligned_to(a->out_dev, ks) || !aligned_to(a->lse_dev, 4) || !aligned_to(a->prefix_dev, 4))
+        return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_chunk_attention: rows or prefix lengths not aligned to their element");
     if (a->window < 0 || !(std::fabs(a->scale) <= 1e38f))   // (times log2(e) it has to be finite too)
         return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_chunk_attention: window must be >= 0 and scale finite, at most 1e38");
     if ((int64_t)batch->n_rows * a->n_q_head > (1 << 30))

@@ -341,3 +341,37 @@ def test_page_waits_that_run_out_are_reported(ctx, ty, dim, q, kv):  # noqa: F81
         ctx.set_wait_fault(False)
     ctx.sync()
     attend(ctx, c, q=x)
+
+
+def test_addresses_off_their_elements_are_refused(ctx):  # noqa: F811
+    """Through the C structs: every array at an address that is not a multiple of its element is refused before a launch."""
+    import ctypes
+    import gsvcu
+    c = Case("f16", [2], [70], 4, 2, 64)
+    q, kv = c.rand(2, 4, 64), c.rand(2, 2, 64)
+    f32, ints = torch.zeros(80 * 32, device="cuda"), torch.zeros(8, dtype=torch.int32, device="cuda")
+    cache, chunks = c.objects()
+    before, launches = c.pool.clone(), ctx.kernel_launches()
+    append = dict(q=q.data_ptr(), k=kv.data_ptr(), v=kv.data_ptr(), q_out=q.data_ptr(), cos=f32.data_ptr(), sin=f32.data_ptr(),
+                  pos=ints.data_ptr(), q_stride=256, k_stride=128, v_stride=128, q_out_stride=256, layer=1, row_dtype=0,
+                  n_q_head=4, n_pos=80, rot_dim=64)
+    attention = dict(q=q.data_ptr(), out=q.data_ptr(), lse=f32.data_ptr(), prefix=ints.data_ptr(), q_stride=256, out_stride=256,
+                     layer=1, n_q_head=4, scale=1.0)
+    torch.cuda.synchronize()
+
+    def call(fn, struct, args, batch=chunks.desc):
+        a = struct(kv=ctypes.addressof(cache.desc), batch=ctypes.addressof(batch), **args)
+        return getattr(ctx.lib, fn)(ctx.h, ctypes.byref(a))
+
+    for fn, struct, args, names in (("gsvcu_op_kv_append", gsvcu.KvAppendArgs, append, ("q", "k", "v", "q_out", "cos", "sin", "pos")),
+                                    ("gsvcu_op_chunk_attention", gsvcu.ChunkAttentionArgs, attention, ("q", "out", "lse", "prefix"))):
+        for name in names:
+            for off in (1, 2, 3) if name in ("cos", "sin", "pos", "lse", "prefix") else (1,):
+                assert call(fn, struct, dict(args, **{name: args[name] + off})) == -1, (fn, name, off)
+        for name in ("row_start", "kv_len", "block_table"):
+            batch = gsvcu.ChunkBatchDesc.from_buffer_copy(chunks.desc)
+            setattr(batch, name, getattr(batch, name) + 2)
+            assert call(fn, struct, args, batch) == -1, (fn, name)
+    ctx.sync()
+    assert ctx.kernel_launches() == launches
+    assert torch.equal(torch.nan_to_num(before), torch.nan_to_num(c.pool))
