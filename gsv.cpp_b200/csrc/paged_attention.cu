@@ -18,9 +18,11 @@
 // down to 2^-17 of the running maximum's and the last one at 2^-38); F32 ones on mma.m16n8k8.tf32 with both
 // operands in two parts (three products), which leaves an error near 2^-22. Sums, maxima and outputs are f32.
 // Keys past kv_len are never read (zero-filled), keys that a row must not see get weight 0.
-// Decode is bound by HBM: every key is read once, 12 to 16 KB in flight per warp (64 sequences of 600 to 2100 keys, 16
-// heads of 32: 35 us, 5.1 TB/s; one of 131072 keys, 32/8 heads of 128: 88 us, 6.1 TB/s). F32 chunks are bound by the
-// tensor pipe and the splitting of operands (4 chunks of up to 333 rows, 16 heads of 32: 67 us).
+// Decode is bound by HBM: every key is read once, 8 KB (16-bit heads of 32) or 16 KB in flight per warp (64 sequences of
+// 600 to 2100 keys, 16 heads of 32: 34.5 us, 5.2 TB/s; one of 131072 keys, 32/8 heads of 128: 88 us, 6.1 TB/s). F32 chunks
+// are bound by the tensor pipe and the splitting of operands (4 chunks of up to 333 rows, 16 heads of 32: 67 us). F32 single
+// tokens: the 64 sequences 80 us, 4.5 TB/s; one of 131072 keys, 32/8 heads of 128, 465 us, 2.3 TB/s, because its 152 CTAs
+// are four more than the one per SM that 130 KB of shared memory allow.
 #include <cuda_bf16.h>
 
 #include "kernels.h"
@@ -591,8 +593,8 @@ ChunkAttnPlan chunk_attention_plan(const ChunkAttnParams& p) {
     c.tiles = (int)((packed + c.row_tile - 1) / c.row_tile);
     const int64_t units = (int64_t)p.batch.n_seq * c.tiles * p.kv.n_head;
     const int max_tiles = (p.batch.max_kv + kt - 1) / kt;
-    // Splits, measured on 148 SMs. Few units: one wave of CTAs (one sequence of 131072 keys: 88 us, 100 with two
-    // waves). Several sequences: up to four waves, so that lengths even out (32 sequences of 1000 to 9000 keys: 134 us
+    // Splits, measured on 148 SMs. Few units: about one wave of CTAs (one sequence of 131072 keys: 88 us, 100 with two
+    // waves; the nearest count of splits, which can be a few CTAs more than fit at once). Several sequences: up to four waves, so that lengths even out (32 sequences of 1000 to 9000 keys: 134 us
     // with two splits, 117 with four), while a split still streams 512 KB (64 sequences of 2100 keys at head dim 32: 36 us
     // whole, 40 in two). A split keeps 4 tiles for each warp.
     size_t smem = 0;

@@ -20,7 +20,7 @@
 // the two score buffers in turn, and the next scores are computed beside the softmax.
 // Products of two row tiles and 128 keys take 2048 cycles at head dim 128, a softmax warp ~1850 per tile; what bounds the
 // kernel is the chain weights -> last product -> next scores -> wake, ~2950 cycles (4096 rows over 16384 keys, 32/8 heads of
-// 128: 790 to 900 us with the power cap, 1.1 to 1.2 PFLOP/s), at head dims 32 and 64 the softmax warps' instructions.
+// 128: 810 to 945 us with the power cap, 1.0 to 1.2 PFLOP/s), at head dims 32 and 64 the softmax warps' instructions.
 // V rows past kv_len in the last tile are zeroed in shared memory before its product, absent pages are
 // zero-filled by TMA (a block index past the pool), masked keys get weight 0.
 #include <cuda_bf16.h>
@@ -532,7 +532,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
                     if (j > 0) {
                         // O must be at rest. With two row tiles it is: these scores were issued after the product before
                         if (halves == 1) {
-                            if (!bar_wait_short_warp(pvdone((j - 1) & 1), (uint32_t)(j - 1) >> 1 & 1u, abort_flag)) { ok = false; break; }
+                            ok = bar_wait_short_warp(pvdone((j - 1) & 1), (uint32_t)(j - 1) >> 1 & 1u, abort_flag);
+                            if (!ok) break;
                             tc_fence_after();
                         }
                         const float f = up == NEG_INF ? 1.0f : ex2(mref - up);

@@ -522,7 +522,8 @@ class Context:
                      pairs=False):
         """Append k, v rows [n_rows][kv heads][head dim] to the paged cache and rotate q into q_out (both may be
         None); cos / sin: f32 [positions][rotated / 2], pos: int32 [n_rows] (None: the cache positions). Runs on the
-        context's stream (stream_handle()). gsvcu_op_kv_append."""
+        context's stream (stream_handle()), which torch's own streams are not ordered with: make, use and free the tensors
+        under torch.cuda.ExternalStream(stream_handle()), or synchronise. gsvcu_op_kv_append."""
         n, D, H, dev = chunks.n_rows, cache.head_dim, cache.n_kv_head, self.device
         if cache.device != dev or chunks.device != dev:
             raise ValueError(f"cache and batch must be on CUDA device {dev}")
@@ -555,7 +556,7 @@ class Context:
                            lse=None):
         """Attention of the batch's rows q [n_rows][heads][head dim] over the paged cache into out; scale None: 1 /
         sqrt(head dim); prefix: int32 [n_seq] keys that every row sees; window: keys a row looks back on (0: all);
-        lse: f32 [n_rows][heads]. Runs on the context's stream (stream_handle()). gsvcu_op_chunk_attention."""
+        lse: f32 [n_rows][heads]. Streams as in op_kv_append. gsvcu_op_chunk_attention."""
         n, D, nq, dev = chunks.n_rows, cache.head_dim, q.shape[1], self.device
         if cache.device != dev or chunks.device != dev:
             raise ValueError(f"cache and batch must be on CUDA device {dev}")

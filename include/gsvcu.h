@@ -320,10 +320,12 @@ int gsvcu_op_kv_append(gsvcu_ctx* ctx, const gsvcu_kv_append* a);
  * p - window): causal with a prefix that all rows see (prefix_dev null: none; the whole length: no mask) and a
  * sliding window. q and out rows have the cache's type (strides in elements, out not overlapping q);
  * lse_dev (may be null) [n_rows][n_q_head] gets the natural logarithm of each row's sum of exp(scale q.k).
- * A row that sees no key gives 0 and -infinity. Scores, softmax and sums are F32. What the pages hold from kv_len
- * on does not matter, nor do pages that no row sees; in the other pages every key and value has to be finite (a
- * value that is not reaches rows that do not see it, as 0 times infinity). A row with a score that is NaN or overflows to
- * infinity is NaN, a score of minus infinity has weight 0 (F32 caches: NaN too); |scale| at most 1e38. */
+ * A row that sees no key gives 0 and -infinity. Scores, softmax and sums are F32, exponentials within 2.7e-6; with more
+ * than 32 rows times query heads of a kv head the weights are rounded to the cache's type for the product with the values
+ * (F16: 11 bits down to 2^-25 of the row's largest, none below 2^-36). What the pages hold from kv_len on does not
+ * matter, nor do pages that no row sees; in the other pages every key and value has to be finite (a value that is not
+ * reaches rows that do not see it, as 0 times infinity) and in F32 below 2^128 - 2^115. A row with a score that is NaN
+ * or overflows to infinity is NaN, a score of minus infinity has weight 0 (F32 caches: NaN too); |scale| at most 1e38. */
 typedef struct {
     const gsvcu_paged_kv* kv;
     const gsvcu_chunk_batch* batch;
