@@ -432,7 +432,7 @@ struct gsvcu_ctx {
     int32_t* op_arrived = nullptr;    // its arrival counters, zero between launches
     size_t op_arrived_n = 0;
     std::vector<void*> op_outgrown;   // what these two outgrew, kept for captured graphs until the context ends
-    uint64_t op_chunk_ready = 0;      // its kernels whose shared-memory limit is raised
+    uint64_t op_chunk_ready[2] = {0, 0};   // its kernels whose shared-memory limit is raised
     // set when a bounded wait in a kernel gave up: [0] decode attention in the decode steps (read and
     // cleared with the slot state), [1] gsvcu_op_decode_attention (read and cleared by gsvcu_sync),
     // [2] the tcgen05 prefill GEMM (read and cleared at the end of each prefill pass),
@@ -1841,8 +1841,8 @@ static bool aligned_to(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)
 static int paged_views(gsvcu_ctx* ctx, const gsvcu_paged_kv* kv, const gsvcu_chunk_batch* b, int32_t layer,
                        int32_t n_q_head, PagedView& pv, ChunkView& cv) {
     if (!kv || !b) return ctx->fail(GSVCU_ERR_ARG, "paged cache: null cache or batch");
-    if (kv->kv_dtype != GSVCU_KV_F16 && kv->kv_dtype != GSVCU_KV_F32 && kv->kv_dtype != GSVCU_KV_BF16)
-        return ctx->fail(GSVCU_ERR_ARG, "paged cache: kv_dtype must be F16, F32 or BF16");
+    if (kv->kv_dtype != GSVCU_KV_F16 && kv->kv_dtype != GSVCU_KV_F32 && kv->kv_dtype != GSVCU_KV_BF16 && !is_q4(kv->kv_dtype))
+        return ctx->fail(GSVCU_ERR_ARG, "paged cache: kv_dtype must be F16, F32, BF16 or 4 bits with F16 or BF16 rows");
     if (!kv->pool_dev || ((uintptr_t)kv->pool_dev & 15))
         return ctx->fail(GSVCU_ERR_ARG, "paged cache: pool_dev must be 16-byte aligned device memory");
     if (kv->n_page <= 0 || kv->n_layer <= 0 || kv->n_kv_head <= 0)
@@ -1869,25 +1869,32 @@ static int paged_views(gsvcu_ctx* ctx, const gsvcu_paged_kv* kv, const gsvcu_chu
     return GSVCU_OK;
 }
 
-int gsvcu_op_kv_append(gsvcu_ctx* ctx, const gsvcu_kv_append* a) {
+int gsvcu_op_kv_append_norm(gsvcu_ctx* ctx, const gsvcu_kv_append* a, const gsvcu_head_norm* norm) {
     if (!ctx || !a) return GSVCU_ERR_ARG;
     KvAppendParams p;
     TRY(paged_views(ctx, a->kv, a->batch, a->layer, a->n_q_head, p.kv, p.batch));
-    const int n_q = a->n_q_head, kvd = a->kv->kv_dtype;
+    const int n_q = a->n_q_head, kvd = row_type(a->kv->kv_dtype);
     if (a->row_dtype != GSVCU_KV_F32 && a->row_dtype != kvd)
-        return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_kv_append: rows must be F32 or the cache's type");
+        return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_kv_append: rows must be F32 or the cache's row type");
     if (a->batch->n_rows > 0 && (!a->k_dev || !a->v_dev || (n_q > 0 && (!a->q_dev || !a->q_out_dev))))
         return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_kv_append: null rows");
     const int64_t D = a->kv->head_dim, kv_width = a->kv->n_kv_head * D;
     if (a->k_stride < kv_width || a->v_stride < kv_width || (n_q > 0 && (a->q_stride < n_q * D || a->q_out_stride < n_q * D)))
         return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_kv_append: row stride shorter than its heads");
-    const size_t rs = a->row_dtype == GSVCU_KV_F32 ? 4 : 2, ks = kvd == GSVCU_KV_F32 ? 4 : 2;
+    const size_t rs = type_size(a->row_dtype), ks = type_size(kvd);
     if (!aligned_to(a->q_dev, rs) || !aligned_to(a->k_dev, rs) || !aligned_to(a->v_dev, rs) || !aligned_to(a->q_out_dev, ks) ||
         !aligned_to(a->cos_dev, 4) || !aligned_to(a->sin_dev, 4) || !aligned_to(a->pos_dev, 4))
         return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_kv_append: rows, tables or positions not aligned to their element");
     if (a->rot_dim < 0 || a->rot_dim > D || a->rot_dim % 2 || a->rot_pairs < 0 || a->rot_pairs > 1 ||
         (a->rot_dim > 0 && (!a->cos_dev || !a->sin_dev || a->n_pos <= 0)))
         return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_kv_append: rot_dim must be even, at most head_dim, with its cos / sin table");
+    if (norm) {
+        if (!aligned_to(norm->q_weight_dev, 4) || !aligned_to(norm->k_weight_dev, 4))
+            return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_kv_append_norm: weights not aligned to their element");
+        if (!(norm->eps >= 0.0f) || std::isinf(norm->eps))
+            return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_kv_append_norm: eps must be finite and not negative");
+        p.q_norm = norm->q_weight_dev; p.k_norm = norm->k_weight_dev; p.eps = norm->eps;
+    }
     p.row_dtype = a->row_dtype; p.n_q_head = n_q; p.q = a->q_dev; p.q_stride = a->q_stride; p.k = a->k_dev;
     p.k_stride = a->k_stride; p.v = a->v_dev; p.v_stride = a->v_stride; p.cos = a->cos_dev; p.sin = a->sin_dev;
     p.n_pos = a->n_pos; p.rot = a->rot_dim; p.pairs = a->rot_pairs; p.pos = a->pos_dev; p.q_out = a->q_out_dev;
@@ -1895,7 +1902,33 @@ int gsvcu_op_kv_append(gsvcu_ctx* ctx, const gsvcu_kv_append* a) {
     p.err = ctx->att_err + 3;
     if (a->batch->n_rows == 0 || a->batch->n_seq == 0) return GSVCU_OK;
     DeviceGuard g(ctx->device);
-    launch_kv_append(p, ctx->stream);
+    if (p.q_norm || p.k_norm || is_q4(p.kv.kv_dtype)) launch_kv_append_norm(p, ctx->stream);
+    else launch_kv_append(p, ctx->stream);
+    CKC(ctx, cudaGetLastError());
+    ctx->launches++;
+    return GSVCU_OK;
+}
+
+int gsvcu_op_kv_append(gsvcu_ctx* ctx, const gsvcu_kv_append* a) { return gsvcu_op_kv_append_norm(ctx, a, nullptr); }
+
+int gsvcu_op_kv_read(gsvcu_ctx* ctx, const gsvcu_kv_read* a) {
+    if (!ctx || !a) return GSVCU_ERR_ARG;
+    KvReadParams p;
+    TRY(paged_views(ctx, a->kv, a->batch, a->layer, a->kv ? a->kv->n_kv_head : 0, p.kv, p.batch));
+    if (a->row_dtype != GSVCU_KV_F32 && a->row_dtype != row_type(a->kv->kv_dtype))
+        return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_kv_read: rows must be F32 or the cache's row type");
+    if (a->batch->n_rows > 0 && (!a->k_dev || !a->v_dev)) return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_kv_read: null rows");
+    const int64_t width = (int64_t)a->kv->n_kv_head * a->kv->head_dim;
+    if (a->k_stride < width || a->v_stride < width)
+        return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_kv_read: row stride shorter than its heads");
+    const size_t rs = type_size(a->row_dtype);
+    if (!aligned_to(a->k_dev, rs) || !aligned_to(a->v_dev, rs))
+        return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_kv_read: rows not aligned to their element");
+    p.row_dtype = a->row_dtype; p.k = a->k_dev; p.k_stride = a->k_stride; p.v = a->v_dev; p.v_stride = a->v_stride;
+    p.err = ctx->att_err + 3;
+    if (a->batch->n_rows == 0 || a->batch->n_seq == 0) return GSVCU_OK;
+    DeviceGuard g(ctx->device);
+    launch_kv_read(p, ctx->stream);
     CKC(ctx, cudaGetLastError());
     ctx->launches++;
     return GSVCU_OK;
@@ -1912,7 +1945,7 @@ int gsvcu_op_chunk_attention(gsvcu_ctx* ctx, const gsvcu_chunk_attention* a) {
     const int64_t D = kv->head_dim;
     if (a->q_stride < a->n_q_head * D || a->out_stride < a->n_q_head * D)
         return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_chunk_attention: row stride shorter than its heads");
-    const size_t ks = kv->kv_dtype == GSVCU_KV_F32 ? 4 : 2;
+    const size_t ks = type_size(kv->kv_dtype);
     if (!aligned_to(a->q_dev, ks) || !aligned_to(a->out_dev, ks) || !aligned_to(a->lse_dev, 4) || !aligned_to(a->prefix_dev, 4))
         return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_chunk_attention: rows or prefix lengths not aligned to their element");
     if (a->window < 0 || !(std::fabs(a->scale) <= 1e38f))   // (times log2(e) it has to be finite too)
@@ -1961,7 +1994,7 @@ int gsvcu_op_chunk_attention(gsvcu_ctx* ctx, const gsvcu_chunk_attention* a) {
     TRY(grow((void**)&ctx->op_arrived, &ctx->op_arrived_n, plan.arrivals, true));
     p.part = ctx->op_split;
     p.arrived = ctx->op_arrived;
-    const int kernels = launch_chunk_attention(p, plan, &ctx->op_chunk_ready, ctx->stream);
+    const int kernels = launch_chunk_attention(p, plan, ctx->op_chunk_ready, ctx->stream);
     if (kernels == 0) {
         cudaGetLastError();
         return ctx->fail(GSVCU_ERR_CUDA, "gsvcu_op_chunk_attention: no tensor map or shared memory");

@@ -1,6 +1,7 @@
 // paged.h -- host-side launchers of the paged-cache operators (internal to the library): appending keys
-// and values with the position rotation (paged_append.cu) and attention of a chunk of new tokens over the
-// paged cache (paged_attention.cu).
+// and values with the position rotation (paged_append.cu; with head norms or into 4 bits paged_append_norm.cu), reading
+// them back (paged_read.cu) and attention of a chunk of new tokens over the paged cache (paged_attention.cu; over 4 bits
+// paged_attention_q4.cu).
 #pragma once
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -11,6 +12,13 @@ namespace gsvcu {
 
 // Bits of the operators' device status word (reported by gsvcu_sync).
 enum { PAGED_BAD_PAGE = 1, PAGED_BAD_LENGTH = 2, PAGED_BAD_POSITION = 4, PAGED_WAIT = 8 };
+
+// 4-bit caches: a kv_dtype names the type of the rows beside it too.
+inline bool is_q4(int kv_dtype) { return kv_dtype == GSVCU_KV_Q4_F16 || kv_dtype == GSVCU_KV_Q4_BF16; }
+inline int row_type(int kv_dtype) {
+    return kv_dtype == GSVCU_KV_Q4_F16 ? GSVCU_KV_F16 : kv_dtype == GSVCU_KV_Q4_BF16 ? GSVCU_KV_BF16 : kv_dtype;
+}
+inline size_t type_size(int kv_dtype) { return kv_dtype == GSVCU_KV_F32 ? 4 : 2; }   // (of a row's element)
 
 // The cache: pages [page][n_layer][K, V][n_head][PAGE][head_dim] of kv_dtype, seen at one layer.
 struct PagedView {
@@ -39,8 +47,21 @@ struct KvAppendParams {
     void* q_out = nullptr;          // rotated q in kv_dtype
     int64_t q_out_stride = 0;
     int32_t* err = nullptr;
+    const float *q_norm = nullptr, *k_norm = nullptr;   // [head_dim] weights of the head norms, null: none
+    float eps = 0.0f;
 };
 void launch_kv_append(const KvAppendParams& p, cudaStream_t s);
+void launch_kv_append_norm(const KvAppendParams& p, cudaStream_t s);   // head norms and 4-bit caches
+
+struct KvReadParams {
+    PagedView kv;
+    ChunkView batch;
+    int row_dtype = GSVCU_KV_F32;
+    void *k = nullptr, *v = nullptr;
+    int64_t k_stride = 0, v_stride = 0;   // elements between rows
+    int32_t* err = nullptr;
+};
+void launch_kv_read(const KvReadParams& p, cudaStream_t s);
 
 struct ChunkAttnParams {
     PagedView kv;
@@ -73,10 +94,14 @@ struct ChunkAttnPlan {
     size_t part_floats = 0, arrivals = 0;
 };
 ChunkAttnPlan chunk_attention_plan(const ChunkAttnParams& p);
-// Kernels launched; 0: none (no tensor map, or no room for the shared memory). `ready`: the caller's record of the
-// kernels whose shared-memory limit is raised on its device (zero at first; raising all 42 with the context would add
-// 16 ms to it).
+// Kernels launched; 0: none (no tensor map, or no room for the shared memory). `ready`: the caller's record (two words) of
+// the kernels whose shared-memory limit is raised on its device (zero at first; raising the 42 of the first word with the
+// context would add 16 ms to it).
 int launch_chunk_attention(const ChunkAttnParams& p, const ChunkAttnPlan& plan, uint64_t* ready, cudaStream_t s);
+// 4-bit caches: their plan, and their kernel for few rows (false: no room for its shared memory). `ready`: as above, a
+// word of its own.
+ChunkAttnPlan chunk_attention_q4_plan(const ChunkAttnParams& p);
+bool launch_chunk_attention_q4(const ChunkAttnParams& p, const ChunkAttnPlan& plan, uint64_t* ready, cudaStream_t s);
 bool launch_chunk_attention_tc(const ChunkAttnParams& p, const ChunkAttnPlan& plan, uint64_t* ready, cudaStream_t s);
 template <typename K>
 inline bool raise_smem(K kernel, size_t bytes, uint64_t* ready, int bit) {

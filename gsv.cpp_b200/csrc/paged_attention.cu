@@ -544,6 +544,7 @@ void pick(int dtype, int dim, int row_tile, F f) {
 }  // namespace
 
 ChunkAttnPlan chunk_attention_plan(const ChunkAttnParams& p) {
+    if (is_q4(p.kv.kv_dtype)) return chunk_attention_q4_plan(p);
     const int D = p.kv.head_dim, size = p.kv.kv_dtype == GSVCU_KV_F32 ? 4 : 2;
     const int kt = key_tile(D, size);
     const int64_t packed = (int64_t)p.batch.max_chunk * (p.n_q_head / p.kv.n_head);
@@ -647,10 +648,13 @@ static void launch_join(const ChunkAttnParams& p, const ChunkAttnPlan& c, bool v
 }
 
 int launch_chunk_attention(const ChunkAttnParams& p, const ChunkAttnPlan& plan, uint64_t* ready, cudaStream_t s) {
-    const size_t size = p.kv.kv_dtype == GSVCU_KV_F32 ? 4 : 2;
+    const int ty = row_type(p.kv.kv_dtype);
+    const size_t size = type_size(ty);
     const bool vec_out = ((uintptr_t)p.out & 15) == 0 && (p.out_stride * (int64_t)size) % 16 == 0;
     if (plan.tensor) {
         if (!launch_chunk_attention_tc(p, plan, ready, s)) return 0;
+    } else if (is_q4(p.kv.kv_dtype)) {
+        if (!launch_chunk_attention_q4(p, plan, ready + 1, s)) return 0;
     } else {
         SplitArgs a;
         a.p = p;
@@ -671,8 +675,8 @@ int launch_chunk_attention(const ChunkAttnParams& p, const ChunkAttnPlan& plan, 
         if (!ok) return 0;
     }
     if (!plan.join_apart) return 1;
-    if (p.kv.kv_dtype == GSVCU_KV_F32) launch_join<float>(p, plan, vec_out, s);
-    else if (p.kv.kv_dtype == GSVCU_KV_F16) launch_join<__half>(p, plan, vec_out, s);
+    if (ty == GSVCU_KV_F32) launch_join<float>(p, plan, vec_out, s);
+    else if (ty == GSVCU_KV_F16) launch_join<__half>(p, plan, vec_out, s);
     else launch_join<__nv_bfloat16>(p, plan, vec_out, s);
     return 2;
 }

@@ -1,0 +1,52 @@
+// paged_q4.cuh -- the 4-bit paged cache: how a block is laid out and how a group of 32 elements is quantised.
+//
+// A block ((page, layer, K or V, head): 64 tokens) holds the codes of all tokens, D / 2 bytes each, then their scales, one
+// F16 per token and group of 32. Element e of a token has the value scale[e / 32] * (code[e] - 8). Eight elements 8 w ..
+// 8 w + 7 are one 32-bit word, element e at bits 4 (e % 8); word w stands at place (w % 4) * (D / 32) + w / 4 of its token:
+// lane t of four, which takes the words 4 G + t of every group G in a tensor-core fragment, then finds them side by side.
+//
+// The group's element of the largest magnitude, m (a negative one before a positive one), gets code 0: the scale is -m / 8,
+// kept within +- 2720, rounded to BF16 and then to F16. With its 8 significant bits scale * (code - 8) and 24 * scale are
+// exact in F16, so that the attention's products read the cache without a further rounding. The codes are
+// floor(x * (1 / scale) + 8.5) in f32, every operation rounded, kept within 0 .. 15. A group with a NaN or an infinity has the
+// scale NaN.
+#pragma once
+#include <cuda_bf16.h>
+
+#include "common.cuh"
+
+namespace gsvcu {
+namespace {
+
+template <int D>
+struct Q4Block {
+    static constexpr int ROW = D / 2, SCALES = D / 16;   // bytes of a token's codes and scales
+    static constexpr int OFF_SCALES = PAGE * ROW;
+    static constexpr int BYTES = PAGE * (ROW + SCALES);
+};
+// Byte of word w (elements 8 w ..) in its token's codes.
+template <int D>
+__device__ __forceinline__ int q4_place(int w) { return ((w & 3) * (D / 32) + (w >> 2)) * 4; }
+
+// Order of elements by magnitude, a negative one before a positive one of the same.
+__device__ __forceinline__ uint32_t q4_key(float x) {
+    const uint32_t u = __float_as_uint(x);
+    return (u << 1) | (u >> 31);
+}
+// Scale of a group whose largest key is `key`, and the factor of its codes.
+__device__ __forceinline__ __half q4_scale(uint32_t key, float& inv) {
+    const float m = __uint_as_float(key >> 1);
+    float t = fminf(m * 0.125f, 2720.0f);
+    if (!(key & 1u)) t = -t;
+    if ((key >> 1) >= 0x7f800000u) t = __uint_as_float(0x7fffffffu);
+    const __half d = __float2half_rn(__bfloat162float(__float2bfloat16_rn(t)));
+    const float f = __half2float(d);
+    inv = f != 0.0f ? __fdiv_rn(1.0f, f) : 0.0f;
+    return d;
+}
+__device__ __forceinline__ uint32_t q4_code(float x, float inv) {
+    return (uint32_t)(int)fminf(fmaxf(__fadd_rn(__fmul_rn(x, inv), 8.5f), 0.0f), 15.0f);   // (a NaN: 0)
+}
+
+}  // namespace
+}  // namespace gsvcu

@@ -19,7 +19,7 @@ HEADER = os.path.join(os.path.dirname(HERE), "include", "gsvcu.h")
 
 OK = 0
 ERR = {-1: "ARG", -2: "CUDA", -3: "OOM", -4: "IO", -5: "FORMAT", -6: "STATE", -7: "DEVICE"}
-KV_F16, KV_F32, KV_BF16 = 0, 1, 2
+KV_F16, KV_F32, KV_BF16, KV_Q4_F16, KV_Q4_BF16 = 0, 1, 2, 3, 4
 EPI_BIAS, EPI_RESID, EPI_RELU_Q8 = 0, 1, 2
 
 
@@ -66,15 +66,26 @@ class KvAppendArgs(C.Structure):
                [(n, C.c_int32) for n in ("layer", "row_dtype", "n_q_head", "n_pos", "rot_dim", "rot_pairs")]
 
 
+class HeadNorm(C.Structure):
+    _fields_ = [("q_weight", C.c_void_p), ("k_weight", C.c_void_p), ("eps", C.c_float)]
+
+
+class KvReadArgs(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("kv", "batch", "k", "v")] + [(n, C.c_int64) for n in ("k_stride", "v_stride")] + \
+               [(n, C.c_int32) for n in ("layer", "row_dtype")]
+
+
 class ChunkAttentionArgs(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in ("kv", "batch", "q", "out", "lse", "prefix")] + \
                [(n, C.c_int64) for n in ("q_stride", "out_stride")] + \
                [(n, C.c_int32) for n in ("layer", "n_q_head", "window")] + [("scale", C.c_float)]
 
 
-# the two structs packed in one step (a step's layers call these often, and per-field conversion costs as much as the launch)
+# the structs packed in one step (a step's layers call these often, and per-field conversion costs as much as the launch)
 _PACK_APPEND, _PACK_ATTENTION = struct.Struct("@6P4q3P6i"), struct.Struct("@6P2q3if")
+_PACK_NORM, _PACK_READ = struct.Struct("@2Pf4x"), struct.Struct("@4P2q2i")
 assert _PACK_APPEND.size == C.sizeof(KvAppendArgs) and _PACK_ATTENTION.size == C.sizeof(ChunkAttentionArgs)
+assert _PACK_NORM.size == C.sizeof(HeadNorm) and _PACK_READ.size == C.sizeof(KvReadArgs)
 
 
 PROGRESS_FN = C.CFUNCTYPE(None, C.c_void_p, C.c_int32)
@@ -120,6 +131,8 @@ SIGNATURES = {
     "gsvcu_set_prefill_gemm": ([_P, _I], C.c_int),
     "gsvcu_op_q8_gemm_tc": ([_P, _P, _P, _I, _P, _P, _I, _I, _P, _P, _I, _P, _P, _P], C.c_int),
     "gsvcu_op_kv_append": ([_P, C.POINTER(KvAppendArgs)], C.c_int),
+    "gsvcu_op_kv_append_norm": ([_P, C.POINTER(KvAppendArgs), C.POINTER(HeadNorm)], C.c_int),
+    "gsvcu_op_kv_read": ([_P, C.POINTER(KvReadArgs)], C.c_int),
     "gsvcu_op_chunk_attention": ([_P, C.POINTER(ChunkAttentionArgs)], C.c_int),
     "gsvcu_op_pack_q8_0_f16": ([_P, _P, _I, _I, _P], C.c_int),
 }
@@ -212,6 +225,7 @@ def _ptr(a):
 
 
 _KV_TYPES = {"torch.float16": KV_F16, "torch.float32": KV_F32, "torch.bfloat16": KV_BF16}
+_Q4_TYPES = {KV_F16: KV_Q4_F16, KV_BF16: KV_Q4_BF16}   # 4-bit caches by the type of their rows
 _KV_TYPE_OF = {}   # the same by dtype object, filled as they are met (this module does not import torch)
 
 
@@ -272,15 +286,30 @@ def _row_stride(t, shape, what, device):
 
 
 class PagedKV:
-    """A paged KV cache (gsvcu_paged_kv) over a device tensor [page][layer][2][kv head][64][head dim]."""
+    """A paged KV cache (gsvcu_paged_kv) over a device tensor [page][layer][2][kv head][64][head dim], or one held in 4
+    bits over a uint8 tensor [page][layer][2][kv head][64][9 / 16 head dim] with the type of its rows (queries, outputs,
+    rows read back), float16 or bfloat16. dtype: that of the rows beside the cache."""
 
-    def __init__(self, pool):
+    def __init__(self, pool, rows=None):
+        quantised = str(pool.dtype) == "torch.uint8"
+        last = "9 / 16 head dim" if quantised else "head dim"
         if pool.dim() != 6 or pool.shape[2] != 2 or pool.shape[4] != 64 or not pool.is_contiguous():
-            raise ValueError(f"pool: contiguous [page][layer][2][kv head][64][head dim] expected, got {list(pool.shape)}")
-        self.pool, self.dtype, self.device = pool, pool.dtype, pool.get_device()
+            raise ValueError(f"pool: contiguous [page][layer][2][kv head][64][{last}] expected, got {list(pool.shape)}")
+        self.pool, self.device = pool, pool.get_device()
         self.n_kv_head, self.head_dim = pool.shape[3], pool.shape[5]
-        self.desc = PagedKVDesc(pool.data_ptr(), _kv_type(pool.dtype, "pool"), pool.shape[0], pool.shape[1],
-                                pool.shape[3], pool.shape[5])
+        if quantised:
+            self.dtype = rows
+            kv_dtype = _Q4_TYPES.get(_KV_TYPES.get(str(rows)))
+            if kv_dtype is None:
+                raise ValueError(f"rows: float16 or bfloat16 expected beside a 4-bit pool, got {rows}")
+            if self.head_dim % 9:
+                raise ValueError(f"pool: [64][9 / 16 head dim] bytes per block expected, got {list(pool.shape)}")
+            self.head_dim = self.head_dim // 9 * 16
+        else:
+            self.dtype, kv_dtype = pool.dtype, _kv_type(pool.dtype, "pool")
+            if rows is not None and rows != pool.dtype:
+                raise ValueError(f"rows: the pool's type expected, got {rows}")
+        self.desc = PagedKVDesc(pool.data_ptr(), kv_dtype, pool.shape[0], pool.shape[1], pool.shape[3], self.head_dim)
         self.addr = C.addressof(self.desc)
 
 
@@ -343,8 +372,9 @@ class Context:
         self.h = h
         self.hp = None
         self.device = device
-        self._append, self._attention = KvAppendArgs(), ChunkAttentionArgs()
+        self._append, self._attention, self._norm, self._read = KvAppendArgs(), ChunkAttentionArgs(), HeadNorm(), KvReadArgs()
         self._append_ref, self._attention_ref = C.byref(self._append), C.byref(self._attention)
+        self._norm_ref, self._read_ref = C.byref(self._norm), C.byref(self._read)
 
     def close(self):
         if getattr(self, "h", None):
@@ -519,11 +549,12 @@ class Context:
                                                         _ptr(out_q), _ptr(out_d), _ptr(out_f32)))
 
     def op_kv_append(self, cache: PagedKV, chunks: ChunkBatch, layer, q, k, v, q_out, cos=None, sin=None, pos=None,
-                     pairs=False):
+                     pairs=False, q_norm=None, k_norm=None, eps=1e-6):
         """Append k, v rows [n_rows][kv heads][head dim] to the paged cache and rotate q into q_out (both may be
-        None); cos / sin: f32 [positions][rotated / 2], pos: int32 [n_rows] (None: the cache positions). Runs on the
+        None); cos / sin: f32 [positions][rotated / 2], pos: int32 [n_rows] (None: the cache positions); q_norm / k_norm:
+        f32 [head dim] weights of an RMS norm of every q / k head before the rotation (None: none). Runs on the
         context's stream (stream_handle()), which torch's own streams are not ordered with: make, use and free the tensors
-        under torch.cuda.ExternalStream(stream_handle()), or synchronise. gsvcu_op_kv_append."""
+        under torch.cuda.ExternalStream(stream_handle()), or synchronise. gsvcu_op_kv_append, gsvcu_op_kv_append_norm."""
         n, D, H, dev = chunks.n_rows, cache.head_dim, cache.n_kv_head, self.device
         if cache.device != dev or chunks.device != dev:
             raise ValueError(f"cache and batch must be on CUDA device {dev}")
@@ -550,11 +581,33 @@ class Context:
         _PACK_APPEND.pack_into(self._append, 0, cache.addr, chunks.addr, qp, k.data_ptr(), v.data_ptr(), op, qs, ks, vs, os_, cp,
                                sp, 0 if pos is None else _ints(pos, (n,), "pos", dev), layer, _kv_type(ty, "k"), nq, n_pos,
                                rot, 1 if pairs else 0)
-        self._check(self.lib.gsvcu_op_kv_append(self.h, self._append_ref))
+        if q_norm is None and k_norm is None:
+            self._check(self.lib.gsvcu_op_kv_append(self.h, self._append_ref))
+            return
+        shape = (D,)
+        _PACK_NORM.pack_into(self._norm, 0, 0 if q_norm is None else _floats(q_norm, shape, "q_norm", dev),
+                             0 if k_norm is None else _floats(k_norm, shape, "k_norm", dev), eps)
+        self._check(self.lib.gsvcu_op_kv_append_norm(self.h, self._append_ref, self._norm_ref))
+
+    def op_kv_read(self, cache: PagedKV, chunks: ChunkBatch, layer, k, v):
+        """Read the batch's tokens back from the paged cache into k, v rows [n_rows][kv heads][head dim] of float32 or the
+        cache's (row) type: a sequence's chunk is its last tokens, all of them when it is kv_len long. Streams as in
+        op_kv_append. gsvcu_op_kv_read."""
+        dev, ty = self.device, k.dtype
+        if cache.device != dev or chunks.device != dev:
+            raise ValueError(f"cache and batch must be on CUDA device {dev}")
+        if v.dtype != ty:
+            raise ValueError("k and v must have one type")
+        shape = (chunks.n_rows, cache.n_kv_head, cache.head_dim)
+        ks, vs = _row_stride(k, shape, "k", dev), _row_stride(v, shape, "v", dev)
+        _PACK_READ.pack_into(self._read, 0, cache.addr, chunks.addr, k.data_ptr(), v.data_ptr(), ks, vs, layer,
+                             _kv_type(ty, "k"))
+        self._check(self.lib.gsvcu_op_kv_read(self.h, self._read_ref))
 
     def op_chunk_attention(self, cache: PagedKV, chunks: ChunkBatch, layer, q, out, scale=None, prefix=None, window=0,
                            lse=None):
-        """Attention of the batch's rows q [n_rows][heads][head dim] over the paged cache into out; scale None: 1 /
+        """Attention of the batch's rows q [n_rows][heads][head dim] over the paged cache into out, both of the cache's
+        (row) type; scale None: 1 /
         sqrt(head dim); prefix: int32 [n_seq] keys that every row sees; window: keys a row looks back on (0: all);
         lse: f32 [n_rows][heads]. Streams as in op_kv_append. gsvcu_op_chunk_attention."""
         n, D, nq, dev = chunks.n_rows, cache.head_dim, q.shape[1], self.device

@@ -33,9 +33,9 @@ enum {
     GSVCU_ERR_DEVICE = -7    /* device is not an sm_100 GPU or does not exist */
 };
 
-/* Element types of a KV cache. BF16 is for the paged-cache operators (gsvcu_op_kv_append,
- * gsvcu_op_chunk_attention); the AR model's own cache is F16 or F32. */
-enum { GSVCU_KV_F16 = 0, GSVCU_KV_F32 = 1, GSVCU_KV_BF16 = 2 };
+/* Element types of a KV cache. BF16 and 4 bits (with the type of the rows beside the cache in the name) are for the
+ * paged-cache operators (gsvcu_op_kv_append and the ones after it); the AR model's own cache is F16 or F32. */
+enum { GSVCU_KV_F16 = 0, GSVCU_KV_F32 = 1, GSVCU_KV_BF16 = 2, GSVCU_KV_Q4_F16 = 3, GSVCU_KV_Q4_BF16 = 4 };
 
 typedef struct gsvcu_ctx gsvcu_ctx;
 
@@ -265,15 +265,24 @@ int gsvcu_op_prefill_attention(gsvcu_ctx* ctx, const float* qkv_dev, int32_t n_s
                                const int32_t* seq_len, const int32_t* text_len, int8_t* out_q_dev,
                                uint16_t* out_d_dev, float* out_f32_dev);
 
-/* ---- Paged-cache operators (no counterpart in the reference): appending rows to a paged KV cache and
- * attention of a chunk of new tokens over it, for decoders of any head layout: prompts in chunks, a few
- * drafted tokens at once, single tokens. Both run on the context's stream, read the batch from device
- * memory and allocate nothing after a first call of the same sizes, so they can be captured in a graph (to be
+/* ---- Paged-cache operators (no counterpart in the reference): appending rows to a paged KV cache (normalised for each
+ * head and rotated on the way), reading them back, and attention of a chunk of new tokens over it, for decoders of any
+ * head layout: prompts in chunks, a few drafted tokens at once, single tokens. They run on the context's stream, read the
+ * batch from device memory and allocate nothing after a first call of the same sizes, so they can be captured in a graph (to be
  * replayed on that stream too: the scratch is the context's). A capture that would have to allocate is refused
  * (GSVCU_ERR_STATE). */
 
 /* The cache: pages [page][n_layer][K, V][n_kv_head][64 tokens][head_dim] of kv_dtype elements in pool_dev
- * (16-byte aligned); head_dim 32, 64 or 128. */
+ * (16-byte aligned); head_dim 32, 64 or 128. Rows beside it (queries, outputs, rows read back) have its type.
+ *
+ * 4 bits (GSVCU_KV_Q4_F16, GSVCU_KV_Q4_BF16: the same bytes, with rows of F16 or BF16): a block ((page, layer, K or V,
+ * head), 64 tokens) takes 36 head_dim bytes: the codes of all tokens, head_dim / 2 bytes each, then their scales, head_dim
+ * / 32 F16 each. Element e of a token is scale[e / 32] * (code[e] - 8), as in Q4_0. Elements 8 w .. 8 w + 7 are one
+ * little-endian 32-bit word, element e at bits 4 (e % 8); word w stands at place (w % 4) * (head_dim / 32) + w / 4 of its
+ * token. Written by gsvcu_op_kv_append, m being the group's element of the largest magnitude (of both signs the negative
+ * one): scale = -m / 8, kept within +- 2720 (elements beyond +- 21,760 saturate), rounded to BF16 and then to F16; code =
+ * floor(x * (1 / scale) + 8.5) in F32, kept within 0 .. 15 (scale 0: 8). A group with a NaN or an infinity reads back as NaN.
+ * Scales of more than 8 significant bits (a cache written by other means) are read with their products rounded to F16. */
 typedef struct {
     void* pool_dev;
     int32_t kv_dtype, n_page, n_layer, n_kv_head, head_dim;
@@ -287,7 +296,7 @@ typedef struct {
  * row_start[n_seq] = n_rows), max_chunk at least the longest chunk, max_kv at least the longest kv_len (0: max_pages *
  * 64); the closer these are, the better the work is cut up. A page outside the pool, a row that no sequence owns, or
  * lengths outside these sizes (kv_len below 0 or above max_kv or the table, a chunk above max_chunk) touch no memory
- * outside the arrays; the rows they concern are undefined, and after either operator the next gsvcu_sync returns
+ * outside the arrays; the rows they concern are undefined, and after any of the operators the next gsvcu_sync returns
  * GSVCU_ERR_ARG. Without rows or without sequences nothing is done. */
 typedef struct {
     const int32_t *row_start_dev, *kv_len_dev, *block_table_dev;
@@ -299,8 +308,8 @@ typedef struct {
  * elements of every q and k head are rotated first: a' = a cos - b sin, b' = a sin + b cos with a, b =
  * elements i and i + rot_dim / 2 (rot_pairs 0) or 2 i and 2 i + 1 (rot_pairs 1) and cos / sin [n_pos][rot_dim
  * / 2] at the row's position: pos_dev[row], or its cache position when pos_dev is null. rot_dim 0: no
- * rotation. Rows are F32 or the cache's type (row_dtype); sums in F32, one rounding to the cache's type.
- * q_out_dev has the cache's type and may be q_dev itself (same type and stride). Rows whose cache position is
+ * rotation. Rows are F32 or the cache's (row) type (row_dtype); sums in F32, one rounding to the cache's type.
+ * q_out_dev has the cache's (row) type and may be q_dev itself (same type and stride). Rows whose cache position is
  * negative (a chunk longer than its kv_len) are not stored. A position outside the table is reported by the
  * next gsvcu_sync (GSVCU_ERR_ARG). */
 typedef struct {
@@ -315,10 +324,32 @@ typedef struct {
 } gsvcu_kv_append;
 int gsvcu_op_kv_append(gsvcu_ctx* ctx, const gsvcu_kv_append* a);
 
+/* The same with a norm for each head before the rotation: y = x / sqrt(mean(x^2) + eps) * weight over the head's
+ * elements, q heads with q_weight_dev, k heads with k_weight_dev ([head_dim] F32; null: those heads are not normalised),
+ * in F32 with the sum of the squares in 64 bits. eps finite, not negative. norm null: gsvcu_op_kv_append. */
+typedef struct {
+    const float *q_weight_dev, *k_weight_dev;
+    float eps;
+} gsvcu_head_norm;
+int gsvcu_op_kv_append_norm(gsvcu_ctx* ctx, const gsvcu_kv_append* a, const gsvcu_head_norm* norm);
+
+/* Read back: the keys and values that the cache holds at `layer` for the batch's tokens, as rows [n_rows][n_kv_head]
+ * [head_dim] (strides in elements between rows) of F32 or the cache's (row) type (row_dtype), exact but for the rounding
+ * of 4-bit values to BF16. Row i of a chunk of n is the token at cache position kv_len[s] - n + i: a chunk of kv_len[s]
+ * rows gives the whole sequence. Rows whose cache position is negative are left as they are. */
+typedef struct {
+    const gsvcu_paged_kv* kv;
+    const gsvcu_chunk_batch* batch;
+    void *k_dev, *v_dev;
+    int64_t k_stride, v_stride;
+    int32_t layer, row_dtype;
+} gsvcu_kv_read;
+int gsvcu_op_kv_read(gsvcu_ctx* ctx, const gsvcu_kv_read* a);
+
 /* Attention of the batch's rows over the cache at `layer`. Query head h reads kv head h / (n_q_head /
  * n_kv_head). The row at position p sees key j < kv_len when j < prefix[s], or j <= p and (window 0 or j >
  * p - window): causal with a prefix that all rows see (prefix_dev null: none; the whole length: no mask) and a
- * sliding window. q and out rows have the cache's type (strides in elements, out not overlapping q);
+ * sliding window. q and out rows have the cache's (row) type (strides in elements, out not overlapping q);
  * lse_dev (may be null) [n_rows][n_q_head] gets the natural logarithm of each row's sum of exp(scale q.k).
  * A row that sees no key gives 0 and -infinity. Scores, softmax and sums are F32, exponentials within 2.7e-6; with more
  * than 32 rows times query heads of a kv head the weights are rounded to the cache's type for the product with the values
@@ -495,7 +526,7 @@ void* gsvcu_stream(const gsvcu_ctx* ctx);
 
 /* Synchronise the context's stream. Also reports, once, what the kernels found since the last call: a bounded
  * wait of gsvcu_op_decode_attention or gsvcu_op_chunk_attention that gave up (GSVCU_ERR_CUDA), pages, lengths
- * or positions outside their arrays in gsvcu_op_kv_append / gsvcu_op_chunk_attention (GSVCU_ERR_ARG). */
+ * or positions outside their arrays in gsvcu_op_kv_append / gsvcu_op_kv_read / gsvcu_op_chunk_attention (GSVCU_ERR_ARG). */
 int gsvcu_sync(gsvcu_ctx* ctx);
 
 /* Failure-path testing (no counterpart in the reference, whose KV allocation failure exits the process,
