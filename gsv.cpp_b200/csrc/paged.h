@@ -94,6 +94,7 @@ struct ChunkAttnPlan {
     size_t part_floats = 0, arrivals = 0;
 };
 ChunkAttnPlan chunk_attention_plan(const ChunkAttnParams& p);
+ChunkAttnPlan chunk_attention_tc_plan(const ChunkAttnParams& p);   // (more than 32 packed rows of a 16-bit type, scale not 0)
 // Kernels launched; 0: none (no tensor map, or no room for the shared memory). `ready`: the caller's record (two words) of
 // the kernels whose shared-memory limit is raised on its device (zero at first; raising the 42 of the first word with the
 // context would add 16 ms to it).

@@ -543,46 +543,51 @@ void pick(int dtype, int dim, int row_tile, F f) {
 
 }  // namespace
 
+ChunkAttnPlan chunk_attention_tc_plan(const ChunkAttnParams& p) {
+    const int D = p.kv.head_dim;
+    const int64_t packed = (int64_t)p.batch.max_chunk * (p.n_q_head / p.kv.n_head);
+    ChunkAttnPlan c;
+    // Many rows of 16-bit types: the tcgen05 kernel (a zero scale would multiply masked -infinities by 0 there).
+    // Row tiles per CTA and key splits by the shortest estimate, in units of 100 cycles: a key tile of 128 takes 29 for
+    // two row tiles and 20 for one, splitting and joining 150, CTAs run in waves of one per SM. Measured: 4 chunks
+    // of up to 570 rows over 1200 keys, 4 heads of 64: 16.4 us with one row tile, 23.9 with two in two splits; 512
+    // tokens over 8192 keys (16/4 x 128): 54 us with one row tile in two splits, 48 with two in four.
+    c.tensor = true;
+    const int max_tiles = (p.batch.max_kv + 127) / 128;
+    int64_t best = INT64_MAX;
+    int n = 1;
+    for (int rows = 256; rows >= 128; rows /= 2) {
+        if (rows == 128 && packed <= 128) break;   // (one row tile already)
+        const int64_t tiles = (packed + rows - 1) / rows, units = p.batch.n_seq * tiles * p.kv.n_head;
+        const int64_t fit = 148 / units < max_tiles ? 148 / units : max_tiles;
+        for (int64_t m : {(int64_t)1, fit}) {
+            if (m < 1) continue;
+            const int64_t waves = (units * m + 147) / 148, per = (max_tiles + m - 1) / m;
+            const int64_t cost = waves * per * (rows == 256 && packed > 128 ? 29 : 20) + (m > 1 ? 150 : 0);
+            if (cost < best) {
+                best = cost;
+                n = (int)m;
+                c.row_tile = rows;
+                c.tiles = (int)tiles;
+            }
+        }
+    }
+    const int64_t units = (int64_t)p.batch.n_seq * c.tiles * p.kv.n_head;
+    c.split_tiles = (max_tiles + n - 1) / n;
+    c.n_split = (max_tiles + c.split_tiles - 1) / c.split_tiles;
+    c.key_tile = 128;
+    c.join_apart = c.n_split > 1;
+    if (c.n_split > 1) c.part_floats = (size_t)units * c.n_split * c.row_tile * (D + 2);
+    return c;
+}
+
 ChunkAttnPlan chunk_attention_plan(const ChunkAttnParams& p) {
     if (is_q4(p.kv.kv_dtype)) return chunk_attention_q4_plan(p);
     const int D = p.kv.head_dim, size = p.kv.kv_dtype == GSVCU_KV_F32 ? 4 : 2;
     const int kt = key_tile(D, size);
     const int64_t packed = (int64_t)p.batch.max_chunk * (p.n_q_head / p.kv.n_head);
+    if (size == 2 && packed > 32 && p.scale != 0.0f) return chunk_attention_tc_plan(p);
     ChunkAttnPlan c;
-    if (size == 2 && packed > 32 && p.scale != 0.0f) {
-        // Many rows of 16-bit types: the tcgen05 kernel (a zero scale would multiply masked -infinities by 0 there).
-        // Row tiles per CTA and key splits by the shortest estimate, in units of 100 cycles: a key tile of 128 takes 29 for
-        // two row tiles and 20 for one, splitting and joining 150, CTAs run in waves of one per SM. Measured: 4 chunks
-        // of up to 570 rows over 1200 keys, 4 heads of 64: 16.4 us with one row tile, 23.9 with two in two splits; 512
-        // tokens over 8192 keys (16/4 x 128): 54 us with one row tile in two splits, 48 with two in four.
-        c.tensor = true;
-        const int max_tiles = (p.batch.max_kv + 127) / 128;
-        int64_t best = INT64_MAX;
-        int n = 1;
-        for (int rows = 256; rows >= 128; rows /= 2) {
-            if (rows == 128 && packed <= 128) break;   // (one row tile already)
-            const int64_t tiles = (packed + rows - 1) / rows, units = p.batch.n_seq * tiles * p.kv.n_head;
-            const int64_t fit = 148 / units < max_tiles ? 148 / units : max_tiles;
-            for (int64_t m : {(int64_t)1, fit}) {
-                if (m < 1) continue;
-                const int64_t waves = (units * m + 147) / 148, per = (max_tiles + m - 1) / m;
-                const int64_t cost = waves * per * (rows == 256 && packed > 128 ? 29 : 20) + (m > 1 ? 150 : 0);
-                if (cost < best) {
-                    best = cost;
-                    n = (int)m;
-                    c.row_tile = rows;
-                    c.tiles = (int)tiles;
-                }
-            }
-        }
-        const int64_t units = (int64_t)p.batch.n_seq * c.tiles * p.kv.n_head;
-        c.split_tiles = (max_tiles + n - 1) / n;
-        c.n_split = (max_tiles + c.split_tiles - 1) / c.split_tiles;
-        c.key_tile = 128;
-        c.join_apart = c.n_split > 1;
-        if (c.n_split > 1) c.part_floats = (size_t)units * c.n_split * c.row_tile * (D + 2);
-        return c;
-    }
     c.row_tile = packed >= 32 ? 32 : (int)(packed + 7) / 8 * 8;
     if (size == 4 && D > 32 && packed > 32) {
         // F32 heads of 64 and 128: 32 rows leave no registers to overlap anything (2 chunks of 1500 rows over 3000 keys,
@@ -652,7 +657,7 @@ int launch_chunk_attention(const ChunkAttnParams& p, const ChunkAttnPlan& plan, 
     const size_t size = type_size(ty);
     const bool vec_out = ((uintptr_t)p.out & 15) == 0 && (p.out_stride * (int64_t)size) % 16 == 0;
     if (plan.tensor) {
-        if (!launch_chunk_attention_tc(p, plan, ready, s)) return 0;
+        if (!launch_chunk_attention_tc(p, plan, is_q4(p.kv.kv_dtype) ? ready + 1 : ready, s)) return 0;
     } else if (is_q4(p.kv.kv_dtype)) {
         if (!launch_chunk_attention_q4(p, plan, ready + 1, s)) return 0;
     } else {

@@ -48,15 +48,6 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t bits(__half2 h) { return *(const uint32_t*)&h; }
-__device__ __forceinline__ __half2 half2_of(uint32_t u) { return *(const __half2*)&u; }
-// (x & mask) | bits
-template <uint32_t MASK, uint32_t BITS>
-__device__ __forceinline__ uint32_t field(uint32_t x) {
-    uint32_t y;
-    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(y) : "r"(x), "n"(MASK), "n"(BITS));
-    return y;
-}
 // Codes 0 .. 7 of a word, less 8, as the pairs (0, 4), (1, 5), (2, 6), (3, 7): under the exponent of 1024 a code in bits 0
 // .. 3 is 1024 + code, one in bits 4 .. 7 is 1024 + 16 code.
 __device__ __forceinline__ void codes(uint32_t w, uint32_t (&x)[4]) {
@@ -66,13 +57,6 @@ __device__ __forceinline__ void codes(uint32_t w, uint32_t (&x)[4]) {
     x[1] = bits(__hfma2(half2_of(field<0x00f000f0u, 0x64006400u>(w)), up, high));
     x[2] = bits(__hadd2(half2_of(field<0x000f000fu, 0x64006400u>(v)), low));
     x[3] = bits(__hfma2(half2_of(field<0x00f000f0u, 0x64006400u>(v)), up, high));
-}
-// scale * (code - 8) of the four codes in each half of x: element i, of the low half's key and the high half's.
-__device__ __forceinline__ void values(uint32_t x, __half2 d, __half2 m24d, uint32_t (&v)[4]) {
-    v[0] = bits(__hfma2(half2_of(field<0x03c003c0u, 0x4c004c00u>(x << 6)), d, m24d));
-    v[1] = bits(__hfma2(half2_of(field<0x03c003c0u, 0x4c004c00u>(x << 2)), d, m24d));
-    v[2] = bits(__hfma2(half2_of(field<0x03c003c0u, 0x4c004c00u>(x >> 2)), d, m24d));
-    v[3] = bits(__hfma2(half2_of(field<0x03c003c0u, 0x4c004c00u>(x >> 6)), d, m24d));
 }
 // Two F16 values, x in the low half, and what their rounding left over.
 __device__ __forceinline__ uint32_t pack_split(float x, float y, uint32_t& rest) {
@@ -379,8 +363,8 @@ __global__ void __launch_bounds__(NW * 32) k_chunk_attn_q4(SplitArgs a) {
                         const __half2 dd = half2_of(__byte_perm(dx[0], dy[0], g ? 0x7632 : 0x5410));
                         const __half2 off = __hmul2(dd, __float2half2_rn(-24.0f));
                         uint32_t lo[4], hi[4];
-                        values(__byte_perm(x[g], y[g], 0x5410), dd, off, lo);
-                        values(__byte_perm(x[g], y[g], 0x7632), dd, off, hi);
+                        q4_values(__byte_perm(x[g], y[g], 0x5410), dd, off, lo);
+                        q4_values(__byte_perm(x[g], y[g], 0x7632), dd, off, hi);
 #pragma unroll
                         for (int k = 0; k < 4; k++) { v[e][g * 8 + k] = lo[k]; v[e][g * 8 + 4 + k] = hi[k]; }
                     }
@@ -392,8 +376,8 @@ __global__ void __launch_bounds__(NW * 32) k_chunk_attn_q4(SplitArgs a) {
                     const uint32_t dy = lds16(vs + (key + 1) * B::SCALES + (kr & 1) * 2);
                     const __half2 dd = half2_of(dx | dy << 16), off = __hmul2(dd, __float2half2_rn(-24.0f));
                     uint32_t lo[4], hi[4];
-                    values(__byte_perm(x[0], y[0], 0x5410), dd, off, lo);
-                    values(__byte_perm(x[0], y[0], 0x7632), dd, off, hi);
+                    q4_values(__byte_perm(x[0], y[0], 0x5410), dd, off, lo);
+                    q4_values(__byte_perm(x[0], y[0], 0x7632), dd, off, hi);
 #pragma unroll
                     for (int k = 0; k < 4; k++) { v[e][k] = lo[k]; v[e][4 + k] = hi[k]; }
                 } else {
@@ -401,7 +385,7 @@ __global__ void __launch_bounds__(NW * 32) k_chunk_attn_q4(SplitArgs a) {
                     uint32_t dx[1], lo[4];
                     lds<1>(vs + key * B::SCALES, dx);   // (key is even)
                     const __half2 dd = half2_of(dx[0]), off = __hmul2(dd, __float2half2_rn(-24.0f));
-                    values(x | y << 16, dd, off, lo);
+                    q4_values(x | y << 16, dd, off, lo);
 #pragma unroll
                     for (int k = 0; k < 4; k++) v[e][k] = lo[k];
                 }
@@ -502,6 +486,7 @@ void pick(int dtype, int dim, int row_tile, F f) {
 ChunkAttnPlan chunk_attention_q4_plan(const ChunkAttnParams& p) {
     const int D = p.kv.head_dim, kt = key_tile(D);
     const int64_t packed = (int64_t)p.batch.max_chunk * (p.n_q_head / p.kv.n_head);
+    if (packed > 32 && p.scale != 0.0f) return chunk_attention_tc_plan(p);
     ChunkAttnPlan c;
     c.row_tile = packed >= 32 ? 32 : (int)(packed + 7) / 8 * 8;
     c.tiles = (int)((packed + c.row_tile - 1) / c.row_tile);

@@ -29,6 +29,7 @@
 
 #include "paged.h"
 #include "paged_join.cuh"
+#include "paged_q4.cuh"
 #include "tc_common.cuh"
 
 namespace gsvcu {
@@ -38,13 +39,13 @@ using namespace tc;
 
 constexpr int KT = 128;                 // keys per tile
 constexpr int ROWS = 256;               // packed rows per CTA, two row tiles (one of 128 when the call has few CTAs)
-constexpr int THREADS = 384;
+constexpr int THREADS = 384, THREADS_Q4 = 512;   // 4-bit caches: 4 warps more, which unpack the key tiles
 // Log2 headroom of P above the row's reference maximum, and how far up the weights are kept. F16: TAU 5, 4 or 3 cost
 // about 1 % over TAU 8 on scores of deviation 1, TAU 1 2 to 7 %.
 template <typename T> constexpr float TAU = __is_same(T, __half) ? 4.0f : 8.0f;
 template <typename T> constexpr float BIAS = __is_same(T, __half) ? 11.0f : 0.0f;
 
-template <int D>
+template <int D, bool Q4>
 struct Smem {
     static constexpr int RB = D >= 64 ? 128 : 2 * D;              // bytes of a swizzled row
     static constexpr int ATOMS = D >= 64 ? D / 64 : 1;            // 64-dim column blocks of a tile
@@ -54,11 +55,15 @@ struct Smem {
     // first half of its scores, then O.
     static constexpr uint32_t TM_O = 2 * KT;
     static constexpr size_t OFF_RING = (size_t)ROWS * D * 2;      // after Q
-    static constexpr size_t OFF_BAR = OFF_RING + (size_t)NP * 2 * ENTRY;
+    // 4 bits: K and V tiles as they lie in the cache (two blocks of 64 keys), K0 V0 K1 V1 .. in turn
+    static constexpr int NS = Q4 ? (D == 128 ? 3 : 4) : 0;
+    static constexpr int PACKED = 2 * Q4Block<D>::BYTES;
+    static constexpr size_t OFF_STAGE = OFF_RING + (size_t)NP * 2 * ENTRY;
+    static constexpr size_t OFF_BAR = OFF_STAGE + (size_t)NS * PACKED;
     // full, empty [NP], S full [2], P full [2][2 halves], PV done [2] (one per row tile; with one row tile, for its key
-    // tiles in turn), V landed, V cleared, drain
-    static constexpr int NBAR = 2 * NP + 11;
-    static constexpr size_t SMEM = OFF_BAR + NBAR * 8 + 16 + 1024;
+    // tiles in turn), V landed, V cleared, drain; 4 bits: packed tile landed, unpacked [NS]
+    static constexpr int NBAR = 2 * NP + 11 + 2 * NS;
+    static constexpr size_t SMEM = OFF_BAR + NBAR * 8 + 16 + 4 * NS + 1024;
 };
 
 struct TcArgs {
@@ -193,10 +198,71 @@ __device__ __forceinline__ uint64_t ex2_pair(uint64_t x) {
                   __int_as_float(__float_as_int(f2hi(y)) + (__float_as_int(f2hi(n)) << 23)));
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_constant__ TcArgs a) {
-    using L = Smem<D>;
-    constexpr int TY = __is_same(T, __half) ? 0 : 1;
+// Output column of element k of 8: unpacked values lie as (0, 4), (1, 5), (2, 6), (3, 7).
+template <bool Q4>
+constexpr __device__ int column(int k) { return !Q4 ? k : k < 4 ? 2 * k : 2 * k - 7; }
+// Untiled copy of `bytes` (a multiple of 16, both addresses 16-byte aligned) completing on an mbarrier.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+                 "r"(bytes), "r"(bar)
+                 : "memory");
+}
+// Eight 16-bit elements of T as F16 pairs in the order of the unpacked codes: (0, 4), (1, 5), (2, 6), (3, 7).
+template <typename T>
+__device__ __forceinline__ uint4 as_codes_lie(uint4 u) {
+    const T* x = (const T*)&u;
+    auto two = [&](int k) { return pack2<__half>((float)x[k], (float)x[k + 4]); };
+    return make_uint4(two(0), two(1), two(2), two(3));
+}
+// The unpacking warp's part of a packed tile (two blocks of 64 tokens): 32 of its 128 keys from `first` on, into the
+// operand's swizzled rows. A lane takes the words 4 G + t of a key, so a word's 8 elements (in the order of q4_values) are
+// one 16-byte piece of the row. Tokens from `end` on, and of blocks that are not held, are zero.
+template <int D>
+__device__ __forceinline__ void unpack_tile(const uint8_t* packed, uint8_t* entry, int first, int lane, int end, int held) {
+    using B = Q4Block<D>;
+    constexpr int G = D / 32, RB = D >= 64 ? 128 : 2 * D;
+    const int t = lane & 3;
+    // key of the lane among 8: with 128-byte rows two neighbours are 4 apart, whose pieces fall into different banks
+    const int k8 = D >= 64 ? (lane >> 3) + (lane & 4) : lane >> 2;
+#pragma unroll 2
+    for (int u = 0; u < 4; u++) {
+        const int key = first + u * 8 + k8, token = key & (PAGE - 1);
+        const uint8_t* block = packed + (key / PAGE) * B::BYTES;
+        uint32_t w[G];
+        __half d[G];
+        if constexpr (G == 4) {
+            const uint4 x = *(const uint4*)(block + token * B::ROW + t * 16);
+            const uint2 y = *(const uint2*)(block + B::OFF_SCALES + token * B::SCALES);
+            w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
+            d[0] = __low2half(half2_of(y.x)); d[1] = __high2half(half2_of(y.x));
+            d[2] = __low2half(half2_of(y.y)); d[3] = __high2half(half2_of(y.y));
+        } else if constexpr (G == 2) {
+            const uint2 x = *(const uint2*)(block + token * B::ROW + t * 8);
+            const __half2 y = half2_of(*(const uint32_t*)(block + B::OFF_SCALES + token * B::SCALES));
+            w[0] = x.x; w[1] = x.y;
+            d[0] = __low2half(y); d[1] = __high2half(y);
+        } else {
+            w[0] = *(const uint32_t*)(block + token * B::ROW + t * 4);
+            d[0] = *(const __half*)(block + B::OFF_SCALES + token * B::SCALES);
+        }
+        const bool in = key < end && (held >> (key / PAGE) & 1);
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+            const __half2 dd = __half2half2(in ? d[g] : __float2half_rn(0.0f)), off = __hmul2(dd, __float2half2_rn(-24.0f));
+            uint32_t v[4];
+            q4_values(w[g], dd, off, v);
+            const int atom = g / 2, piece = D >= 64 ? (g & 1) * 4 + t : t, swz = D >= 64 ? key & 7 : (key >> 1) & 3;
+            *(uint4*)(entry + (size_t)atom * KT * RB + key * RB + ((piece ^ swz) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
+        }
+    }
+}
+
+template <typename T, int D, bool Q4>
+__global__ void __launch_bounds__(Q4 ? THREADS_Q4 : THREADS, 1) k_chunk_attn_tc(const __grid_constant__ TcArgs a) {
+    using L = Smem<D, Q4>;
+    using CT = typename std::conditional<Q4, __half, T>::type;   // what the products read
+    constexpr int NT = Q4 ? THREADS_Q4 : THREADS;
+    constexpr int TY = __is_same(CT, __half) ? 0 : 1;
     constexpr uint32_t ID_S = instr(TY, 0, KT), ID_O = instr(TY, 1, D);
     extern __shared__ uint8_t smem_raw[];
     uint8_t* sm = smem_raw + ((1024u - (su32(smem_raw) & 1023u)) & 1023u);
@@ -209,8 +275,11 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
     auto pfull = [&](int b, int half) { return bar0 + 8u * (2 * L::NP + 2 + 2 * b + half); };
     auto pvdone = [&](int t) { return bar0 + 8u * (2 * L::NP + 6 + t); };
     const uint32_t vhere = pvdone(2), vclear = vhere + 8, drain = vhere + 16;
+    auto landed = [&](int n) { return drain + 8u + 8u * n; };
+    auto unpacked = [&](int n) { return drain + 8u + 8u * (L::NS + n); };
     uint32_t* tmem_slot = (uint32_t*)(sm + L::OFF_BAR + L::NBAR * 8);
     volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
+    int* held_mask = (int*)(tmem_slot + 4);   // [NS] which blocks of a packed tile are there
 
     int id = blockIdx.x;
     const int sp = id % a.n_split;
@@ -218,7 +287,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
     const int h = id % p.kv.n_head;
     id /= p.kv.n_head;
     const int s = id % p.batch.n_seq, tile = a.tiles - 1 - id / p.batch.n_seq;   // the last rows see most keys: first
-    if (tid == 0) asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&a.map) : "memory");
+    if (!Q4 && tid == 0) asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&a.map) : "memory");
     griddep_wait();
     griddep_launch();
 
@@ -237,7 +306,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
     auto key0 = [&](int j) { return c.tile_of(v0 + j) * KT; };
 
     if (tid == 0) {
-        for (int e = 0; e < L::NP; e++) { bar_init(full(e), 1); bar_init(empty(e), 1); }
+        for (int e = 0; e < L::NP; e++) { bar_init(full(e), Q4 ? 4 : 1); bar_init(empty(e), 1); }
+        for (int n = 0; n < L::NS; n++) { bar_init(landed(n), 1); bar_init(unpacked(n), 4); }
         for (int b = 0; b < 2; b++) {
             bar_init(sfull(b), 1);
             bar_init(pfull(b, 0), 4);
@@ -294,10 +364,45 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
         v1b = k1b;
         return __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
     };
-    const int pairs = nt > 0 ? nt + 1 : 0, early = min(pairs, L::NP);   // the first ones find the ring empty
+    // 4 bits: copy n is K of tile n / 2 when even, V when odd, both blocks as they lie.
+    auto load_packed = [&](int n) -> bool {
+        const int j = n >> 1, st = n % max(L::NS, 1);
+        if ((n & 31) == 0) {   // the blocks of 16 tiles: lane = (tile, page)
+            const int jj = j + (lane >> 1);
+            blk = -1;
+            if (jj < nt) {
+                const int key = key0(jj) + PAGE * (lane & 1);
+                if (c.sees(key)) {
+                    const int page = n == 0 && !p.window ? first_page : tab[key / PAGE];
+                    if (page >= 0 && page < p.kv.n_page) blk = ((page * p.kv.n_layer + p.kv.layer) * 2) * p.kv.n_head + h;
+                    else bad = true;
+                }
+            }
+        }
+        const int b0 = __shfl_sync(0xffffffffu, blk, (j & 15) * 2), b1 = __shfl_sync(0xffffffffu, blk, (j & 15) * 2 + 1);
+        bool ok = true;
+        if (lane == 0) {
+            ok = bar_wait_short(unpacked(st), ((uint32_t)(n / max(L::NS, 1)) & 1u) ^ 1u, abort_flag);
+            if (ok) {
+                constexpr uint32_t BYTES = Q4Block<D>::BYTES;
+                held_mask[st] = (b0 >= 0 ? 1 : 0) | (b1 >= 0 ? 2 : 0);
+                bar_expect_tx(landed(st), ((b0 >= 0) + (b1 >= 0)) * BYTES + (n > 0 ? p.fault_extra_tx : 0u));
+                const uint32_t dst = su32(sm + L::OFF_STAGE + (size_t)st * L::PACKED);
+                const uint8_t* pool = (const uint8_t*)p.kv.pool + (n & 1) * (int64_t)p.kv.n_head * BYTES;
+                if (b0 >= 0) bulk_load(dst, pool + (int64_t)b0 * BYTES, BYTES, landed(st));
+                if (b1 >= 0) bulk_load(dst + BYTES, pool + (int64_t)b1 * BYTES, BYTES, landed(st));
+            }
+        }
+        return __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+    };
+    const int pairs = nt > 0 ? nt + 1 : 0;
+    const int loads = Q4 ? 2 * max(nt, 0) : pairs, early = min(loads, Q4 ? L::NS : L::NP);   // the first ones find the ring empty
     if (warp == 0) {
         __syncwarp();
-        for (int i = 0; i < early; i++) load_pair(i);
+        for (int i = 0; i < early; i++) {
+            if constexpr (Q4) load_packed(i);
+            else load_pair(i);
+        }
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(su32(tmem_slot)), "r"(512)
@@ -306,7 +411,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
     }
     // Q, swizzled as the MMA reads it ([tile][64-dim block][128 rows][RB bytes]), zero past the CTA's rows; four loads
     // in flight per thread (one at a time this was a third of a short call)
-    constexpr int STEP = THREADS - 32;
+    constexpr int STEP = NT - 32;
     const int tok0 = c.r0 / a.group, rem0 = c.r0 % a.group;
     const float inv = 1.0f / (float)a.group;   // (x + 1/2) / group is far enough from whole numbers for x < 2^20
     for (int i0 = tid - 32; warp > 0 && i0 < 128 * halves * (D / 8); i0 += 4 * STEP) {
@@ -332,6 +437,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
         for (int m = 0; m < 4; m++) {
             const int i = i0 + m * STEP, r = i / (D / 8), pc = i % (D / 8);
             if (r >= 128 * halves) break;
+            if constexpr (Q4) u[m] = as_codes_lie<T>(u[m]);
             if (a.negate) { u[m].x ^= 0x80008000u; u[m].y ^= 0x80008000u; u[m].z ^= 0x80008000u; u[m].w ^= 0x80008000u; }
             const int rt = r & 127, atom = D >= 64 ? pc / 8 : 0, ch = D >= 64 ? pc % 8 : pc;
             const int swz = L::RB == 128 ? rt & 7 : (rt >> 1) & 3;
@@ -344,13 +450,47 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
 
-    // Registers move from the TMA / MMA warps to the softmax: 128 x 104 + 256 x 200 = 384 x 168, the launch's own.
-    if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+    // Registers move from the TMA / MMA warps to the softmax: 128 x 104 + 256 x 200 = 384 x 168, the launch's own (4 bits:
+    // 256 x 56 + 256 x 200 = 512 x 128).
+    if (Q4 && warp >= 12) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        bool ok = true;
+        for (int i = 0; i < pairs && ok; i++) {
+            const int e = i % L::NP;
+            uint8_t* entry = sm + L::OFF_RING + (size_t)e * 2 * L::ENTRY;   // V, then K
+            ok = wait_warp(empty(e), ((uint32_t)(i / L::NP) & 1u) ^ 1u, abort_flag);
+            for (int which = i > 0 ? 0 : 1; which < (i < nt ? 2 : 1) && ok; which++) {
+                const int n = 2 * i - 1 + which, st = n % max(L::NS, 1);
+                ok = wait_warp(landed(st), (uint32_t)(n / max(L::NS, 1)) & 1u, abort_flag, p.poll_limit);
+                if (!ok) break;
+                const int j = n >> 1;
+                unpack_tile<D>(sm + L::OFF_STAGE + (size_t)st * L::PACKED, entry + which * L::ENTRY, (warp - 12) * 32, lane,
+                               which ? KT : c.len - key0(j), held_mask[st]);
+                __syncwarp();
+                if (lane == 0) bar_arrive(unpacked(st));
+            }
+            if (ok) {
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) bar_arrive(full(e));
+            }
+        }
+        if (!ok && lane == 0) {
+            atomicOr(p.err, PAGED_WAIT);
+            *abort_flag = 1;
+        }
+        tc_fence_before();
+        __syncthreads();
+    } else if (warp < 4) {
+        if constexpr (Q4) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        else asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
         if (warp == 0) {
             int i = early;
             bool ok = true;
-            for (; i < pairs && ok; i++) ok = load_pair(i);
+            for (; i < loads && ok; i++) {
+                if constexpr (Q4) ok = load_packed(i);
+                else ok = load_pair(i);
+            }
             if (bad) atomicOr(p.err, PAGED_BAD_PAGE);
             if (lane == 0) {
                 if (!ok) {
@@ -359,15 +499,16 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
                     i--;   // its copies were not issued
                 }
                 // every copy has landed before the CTA may end
-                for (int k = i - 1; k >= 0 && k >= i - L::NP; k--)
+                constexpr int N = Q4 ? L::NS : L::NP;
+                for (int k = i - 1; k >= 0 && k >= i - N; k--)
                     for (uint32_t it = 0; it < min(TC_POLL_LIMIT, p.poll_limit); it++)
-                        if (bar_try(full(k % L::NP), (uint32_t)(k / L::NP) & 1u)) break;
+                        if (bar_try(Q4 ? landed(k % N) : full(k % N), (uint32_t)(k / N) & 1u)) break;
             }
         } else if (warp == 1) {
             constexpr uint32_t HI = DESC_HI<L::RB>;
             const uint32_t tm = __reduce_or_sync(0xffffffffu, tmem);   // (into a uniform register)
             const uint32_t sq = su32(sm), ring = su32(sm + L::OFF_RING);
-            const bool cut = nt > 0 && key0(nt - 1) + KT > c.len;
+            const bool cut = !Q4 && nt > 0 && key0(nt - 1) + KT > c.len;
             // The loop is unrolled over the ring, so addresses and most phases are constants: this warp shares its
             // scheduler with two softmax warps, and every instruction between two products is idle tensor time.
             auto scores = [&](int t, int b, int e) {   // S buffer b = Q_t K^T with the K of pair e
@@ -454,7 +595,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
                     if (__any_sync(0xffffffffu, bar_try(drain, 0))) break;
             }
             __syncwarp();
-        } else if (warp == 2 && nt > 0 && key0(nt - 1) + KT > c.len) {
+        } else if (!Q4 && warp == 2 && nt > 0 && key0(nt - 1) + KT > c.len) {
             // V rows past the last key: whatever the page holds there becomes 0
             const int e = nt % L::NP, n16 = L::RB / 16;
             if (wait_warp(vhere, 0, abort_flag) && wait_warp(full(e), (uint32_t)(nt / L::NP) & 1u, abort_flag)) {
@@ -526,8 +667,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
                 // Raise the reference maximum of the warp's rows when one of them needs it. A score that is NaN or has
                 // overflowed makes the row's reference NaN, and with it all that the row gives: the polynomial would take the
                 // exponent of such a score for a small one.
-                if (__any_sync(0xffffffffu, !(top <= mref + (TAU<T> + BIAS<T>)))) {
-                    float up = max2(mref, top - BIAS<T>);
+                if (__any_sync(0xffffffffu, !(top <= mref + (TAU<CT> + BIAS<CT>)))) {
+                    float up = max2(mref, top - BIAS<CT>);
                     if (up == -NEG_INF) up = __int_as_float(0x7fffffff);
                     if (j > 0) {
                         // O must be at rest. With two row tiles it is: these scores were issued after the product before
@@ -565,7 +706,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
                             if (!decltype(tested)::value && i % EVERY == EVERY - 1) e = ex2_pair(e);
                             else e = f2pack(ex2(f2lo(e)), ex2(f2hi(e)));
                             sum = fadd2(sum, e);
-                            w[i] = pack2<T>(f2lo(e), f2hi(e));
+                            w[i] = pack2<CT>(f2lo(e), f2hi(e));
                         }
                         tmem_st16u(ts + 16u * k, w);
                         if (k & 1) {   // half of the tile's weights: their product may start
@@ -608,7 +749,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
                     for (int i = 0; i < 32; i += 8) {
                         float y[8];
 #pragma unroll
-                        for (int k = 0; k < 8; k++) y[k] = __uint_as_float(o[i + k]) * il;
+                        for (int k = 0; k < 8; k++) y[k] = __uint_as_float(o[i + column<Q4>(k)]) * il;
                         T* dst = (T*)p.out + row * p.out_stride + (int64_t)head * D + d + i;
                         const uint4 u = make_uint4(pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]), pack2<T>(y[4], y[5]),
                                                    pack2<T>(y[6], y[7]));
@@ -640,8 +781,12 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
                         tmem_wait_ld();
                         tmem_bind(o);
 #pragma unroll
-                        for (int k = 0; k < 16; k += 4)
-                            *(float4*)place(lane, (d + k) / 4) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+                        for (int k = 0; k < 16; k += 4) {
+                            const float* y = o + (k & 8);
+                            const int m = k & 4;
+                            *(float4*)place(lane, (d + k) / 4) = make_float4(y[column<Q4>(m)], y[column<Q4>(m + 1)],
+                                                                             y[column<Q4>(m + 2)], y[column<Q4>(m + 3)]);
+                        }
                     }
                     __syncwarp();
 #pragma unroll 4
@@ -664,17 +809,18 @@ __global__ void __launch_bounds__(THREADS, 1) k_chunk_attn_tc(const __grid_const
     }
 }
 
+template <typename T, bool Q4, typename F>
+void pick_tc_dim(int dim, F f) {
+    if (dim == 32) f(k_chunk_attn_tc<T, 32, Q4>, Smem<32, Q4>::SMEM);
+    else if (dim == 64) f(k_chunk_attn_tc<T, 64, Q4>, Smem<64, Q4>::SMEM);
+    else f(k_chunk_attn_tc<T, 128, Q4>, Smem<128, Q4>::SMEM);
+}
 template <typename F>
 void pick_tc(int dtype, int dim, F f) {
-    if (dtype == GSVCU_KV_F16) {
-        if (dim == 32) f(k_chunk_attn_tc<__half, 32>, Smem<32>::SMEM);
-        else if (dim == 64) f(k_chunk_attn_tc<__half, 64>, Smem<64>::SMEM);
-        else f(k_chunk_attn_tc<__half, 128>, Smem<128>::SMEM);
-    } else {
-        if (dim == 32) f(k_chunk_attn_tc<__nv_bfloat16, 32>, Smem<32>::SMEM);
-        else if (dim == 64) f(k_chunk_attn_tc<__nv_bfloat16, 64>, Smem<64>::SMEM);
-        else f(k_chunk_attn_tc<__nv_bfloat16, 128>, Smem<128>::SMEM);
-    }
+    if (dtype == GSVCU_KV_F16) pick_tc_dim<__half, false>(dim, f);
+    else if (dtype == GSVCU_KV_BF16) pick_tc_dim<__nv_bfloat16, false>(dim, f);
+    else if (dtype == GSVCU_KV_Q4_F16) pick_tc_dim<__half, true>(dim, f);
+    else pick_tc_dim<__nv_bfloat16, true>(dim, f);
 }
 
 }  // namespace
@@ -694,22 +840,24 @@ bool launch_chunk_attention_tc(const ChunkAttnParams& p, const ChunkAttnPlan& pl
     a.vec_q = ((uintptr_t)p.q & 15) == 0 && p.q_stride % 8 == 0;
     a.vec_out = ((uintptr_t)p.out & 15) == 0 && p.out_stride % 8 == 0;
     const int D = p.kv.head_dim;
-    const EncodeTiledFn encode = encode_fn();
-    if (!encode) return false;
+    const bool q4 = is_q4(p.kv.kv_dtype);
+    const EncodeTiledFn encode = q4 ? nullptr : encode_fn();
+    if (!q4 && !encode) return false;
     const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)PAGE, (cuuint64_t)a.n_blocks};
     const cuuint64_t strides[2] = {(cuuint64_t)D * 2, (cuuint64_t)PAGE * D * 2};
     const cuuint32_t box[3] = {(cuuint32_t)(D < 64 ? D : 64), (cuuint32_t)PAGE, 1}, step[3] = {1, 1, 1};
-    if (encode(&a.map, p.kv.kv_dtype == GSVCU_KV_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+    if (!q4 && encode(&a.map, p.kv.kv_dtype == GSVCU_KV_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
                p.kv.pool, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
                D >= 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
         return false;
     const int64_t ctas = (int64_t)p.batch.n_seq * plan.tiles * p.kv.n_head * plan.n_split;
-    const int bit = 36 + (p.kv.kv_dtype == GSVCU_KV_F16 ? 0 : 3) + D / 64;   // 36 .. 41
+    const bool f16 = row_type(p.kv.kv_dtype) == GSVCU_KV_F16;
+    const int bit = (q4 ? 24 : 36) + (f16 ? 0 : 3) + D / 64;   // 36 .. 41; 4 bits (their own word): 24 .. 29
     bool ok = false;
     pick_tc(p.kv.kv_dtype, D, [&](auto k, size_t smem) {
         ok = raise_smem(k, smem, ready, bit);
-        if (ok) launch_pdl(k, dim3((unsigned)ctas), dim3(THREADS), smem, s, a);
+        if (ok) launch_pdl(k, dim3((unsigned)ctas), dim3(q4 ? THREADS_Q4 : THREADS), smem, s, a);
     });
     return ok;
 }

@@ -48,5 +48,24 @@ __device__ __forceinline__ uint32_t q4_code(float x, float inv) {
     return (uint32_t)(int)fminf(fmaxf(__fadd_rn(__fmul_rn(x, inv), 8.5f), 0.0f), 15.0f);   // (a NaN: 0)
 }
 
+__device__ __forceinline__ uint32_t bits(__half2 h) { return *(const uint32_t*)&h; }
+__device__ __forceinline__ __half2 half2_of(uint32_t u) { return *(const __half2*)&u; }
+// (x & mask) | bits
+template <uint32_t MASK, uint32_t BITS>
+__device__ __forceinline__ uint32_t field(uint32_t x) {
+    uint32_t y;
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(y) : "r"(x), "n"(MASK), "n"(BITS));
+    return y;
+}
+// scale * (code - 8) of the four codes in each half of x: v[i] = code i of the low half with d's low half, and of the high
+// half (of a whole word: elements i and i + 4). A code moved to bits 6 .. 9 under the exponent of 16 is 16 + code, times d
+// less 24 d.
+__device__ __forceinline__ void q4_values(uint32_t x, __half2 d, __half2 m24d, uint32_t (&v)[4]) {
+    v[0] = bits(__hfma2(half2_of(field<0x03c003c0u, 0x4c004c00u>(x << 6)), d, m24d));
+    v[1] = bits(__hfma2(half2_of(field<0x03c003c0u, 0x4c004c00u>(x << 2)), d, m24d));
+    v[2] = bits(__hfma2(half2_of(field<0x03c003c0u, 0x4c004c00u>(x >> 2)), d, m24d));
+    v[3] = bits(__hfma2(half2_of(field<0x03c003c0u, 0x4c004c00u>(x >> 6)), d, m24d));
+}
+
 }  // namespace
 }  // namespace gsvcu

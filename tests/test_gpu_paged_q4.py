@@ -298,6 +298,54 @@ def test_large_and_tiny_groups(ctx, ty, dim, q):  # noqa: F811
     assert float(out.abs().max()) > 100.0
 
 
+@pytest.mark.parametrize("ty,dim", [("bf16", 128), ("f16", 64), ("bf16", 32)])
+@pytest.mark.parametrize("rows", [128, 101])
+def test_warps_of_a_row_tile_at_their_own_pace(ctx, ty, dim, rows):  # noqa: F811
+    """One tile of up to 128 rows over 12 key tiles in one pass: scores that climb from key tile to key tile for the rows of
+    one warp, of two, of every fifth row or of all, beside rows whose maximum stays."""
+    n_seq, kv = 10, 1500
+    c = Q4Case(ty, [rows] * n_seq, [kv] * n_seq, 8, 8, dim)
+    q = c.rand(c.rows, c.heads, dim)
+    q[:, :, 0] = 0.0
+    v = torch.randn(c.pool.shape[0], 2, 8, PAGE, dim, generator=c.gen, device="cuda")
+    warp = torch.arange(rows, device="cuda") // 32
+    climbs = [warp == 0, warp == 1, warp == 2, warp == 3, (warp == 0) | (warp == 3), warp % 2 == 0, warp >= 0, warp < 0,
+              (torch.arange(rows, device="cuda") % 5) == 0, warp == 2]
+    for s in range(n_seq):
+        step = torch.arange(24 * PAGE, device="cuda") // 128 // (1 if s != 9 else 2)
+        p = c.table[s, :24].long()
+        v[p, 0, :, :, 0] = step.float().view(24, 1, PAGE).expand(24, 8, PAGE)
+        q[s * rows:(s + 1) * rows, :, 0] = (climbs[s].float() * 10.0 * dim ** 0.5)[:, None].to(c.dtype)
+    c.set_values(v)
+    x, a, la = attend(ctx, c, q=q)
+    for _ in range(3):
+        _, b, lb = attend(ctx, c, q=x)
+        assert torch.equal(a, b) and torch.equal(la, lb)
+
+
+@pytest.mark.parametrize("ty,dim", [("f16", 64), ("bf16", 128), ("f16", 32)])
+@pytest.mark.parametrize("q,kv", [(60, 60), (60, 900), (300, 300), (300, 2000), (90, 9000)])
+def test_page_waits_that_run_out_are_reported(ctx, ty, dim, q, kv):  # noqa: F811
+    """Every copy from the second on is expected to bring 16 bytes more than it does (the copies themselves complete) and its
+    wait has a short limit: the call ends, the next sync reports it once, and the same call without the fault is right."""
+    import gsvcu
+    c = Q4Case(ty, [q, 0, q], [kv, 5, kv], 4, 2, dim)
+    x = c.rand(c.rows, c.heads, dim)
+    out = torch.empty_like(x)
+    cache, chunks = c.objects()
+    torch.cuda.synchronize()
+    ctx.set_wait_fault(True)
+    try:
+        ctx.op_chunk_attention(cache, chunks, c.layer, x, out)
+        with pytest.raises(gsvcu.GsvcuError) as e:
+            ctx.sync()
+        assert e.value.code == -2 and "gave up" in str(e.value)
+    finally:
+        ctx.set_wait_fault(False)
+    ctx.sync()
+    attend(ctx, c, q=x)
+
+
 # ------------------------------------------------------------------ append: norms and 4 bits
 
 def norm_oracle(x, weight, eps):
