@@ -431,7 +431,9 @@ struct gsvcu_ctx {
     size_t op_split_n = 0;
     int32_t* op_arrived = nullptr;    // its arrival counters, zero between launches
     size_t op_arrived_n = 0;
-    std::vector<void*> op_outgrown;   // what these two outgrew, kept for captured graphs until the context ends
+    void* op_unpacked = nullptr;      // its pages of 4-bit caches as F16
+    size_t op_unpacked_n = 0;
+    std::vector<void*> op_outgrown;   // what these three outgrew, kept for captured graphs until the context ends
     uint64_t op_chunk_ready[2] = {0, 0};   // its kernels whose shared-memory limit is raised
     // set when a bounded wait in a kernel gave up: [0] decode attention in the decode steps (read and
     // cleared with the slot state), [1] gsvcu_op_decode_attention (read and cleared by gsvcu_sync),
@@ -508,6 +510,7 @@ gsvcu_ctx::~gsvcu_ctx() {
     if (op_a16) cudaFree(op_a16);
     if (op_split) cudaFree(op_split);
     if (op_arrived) cudaFree(op_arrived);
+    if (op_unpacked) cudaFree(op_unpacked);
     for (void* p : op_outgrown) cudaFree(p);
     if (att_err) cudaFree(att_err);
     for (cudaStream_t gs : gstream)
@@ -1959,24 +1962,24 @@ int gsvcu_op_chunk_attention(gsvcu_ctx* ctx, const gsvcu_chunk_attention* a) {
     p.fault_extra_tx = ctx->fault_extra_tx;
     p.poll_limit = ctx->fault_poll_limit;
     if (batch->n_rows == 0 || batch->n_seq == 0) return GSVCU_OK;
-    const ChunkAttnPlan plan = chunk_attention_plan(p);
+    ChunkAttnPlan plan = chunk_attention_plan(p);
     if ((int64_t)batch->n_seq * plan.tiles * kv->n_kv_head * plan.n_split > INT32_MAX)
         return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_chunk_attention: batch too large for one launch");
     DeviceGuard g(ctx->device);
     // Scratch at least doubles when it grows, and what it replaces stays until the context ends: captured graphs
     // may hold its address. It does not grow in a capture: the zeros of the counters would only be recorded, and calls
     // outside the graph would find none.
-    auto grow = [&](void** at, size_t* have, size_t need, bool zero) -> int {
+    auto grow = [&](void** at, size_t* have, size_t need, bool zero, size_t most) -> int {   // (4-byte words)
         if (need <= *have) return GSVCU_OK;
         cudaStreamCaptureStatus capture;
         CKC(ctx, cudaStreamIsCapturing(ctx->stream, &capture));
         if (capture != cudaStreamCaptureStatusNone)
             return ctx->fail(GSVCU_ERR_STATE, "gsvcu_op_chunk_attention: run these sizes once before they are captured");
-        const size_t n = std::max(need, 2 * *have);
+        const size_t n = std::max(need, std::min(2 * *have, most));
         void* fresh = nullptr;
         if (cudaMalloc(&fresh, n * 4) != cudaSuccess) {
             cudaGetLastError();
-            return ctx->fail(GSVCU_ERR_OOM, "gsvcu_op_chunk_attention: no memory for the split results");
+            return ctx->fail(GSVCU_ERR_OOM, "gsvcu_op_chunk_attention: no memory for its scratch");
         }
         if (zero) {
             const cudaError_t e = cudaMemsetAsync(fresh, 0, n * 4, ctx->stream);
@@ -1990,10 +1993,15 @@ int gsvcu_op_chunk_attention(gsvcu_ctx* ctx, const gsvcu_chunk_attention* a) {
         *have = n;
         return GSVCU_OK;
     };
-    TRY(grow((void**)&ctx->op_split, &ctx->op_split_n, plan.part_floats, false));
-    TRY(grow((void**)&ctx->op_arrived, &ctx->op_arrived_n, plan.arrivals, true));
+    TRY(grow((void**)&ctx->op_split, &ctx->op_split_n, plan.part_floats, false, SIZE_MAX));
+    TRY(grow((void**)&ctx->op_arrived, &ctx->op_arrived_n, plan.arrivals, true, SIZE_MAX));
+    const int rc = grow(&ctx->op_unpacked, &ctx->op_unpacked_n, plan.unpacked_floats, false, UNPACK_LIMIT / 4);
+    if (rc == GSVCU_ERR_OOM) plan.unpack_pages = 0;   // (the kernel can do without)
+    else if (rc != GSVCU_OK) return rc;
     p.part = ctx->op_split;
     p.arrived = ctx->op_arrived;
+    p.unpacked = ctx->op_unpacked;   // the pages, then their table
+    if (plan.unpack_pages) p.unpacked_table = (int32_t*)ctx->op_unpacked + (plan.unpacked_floats - (size_t)batch->n_seq * plan.unpack_pages);
     const int kernels = launch_chunk_attention(p, plan, ctx->op_chunk_ready, ctx->stream);
     if (kernels == 0) {
         cudaGetLastError();

@@ -78,6 +78,8 @@ struct ChunkAttnParams {
     int32_t* err = nullptr;
     float* part = nullptr;       // scratch of chunk_attention_plan
     int32_t* arrived = nullptr;  // zero between launches
+    void* unpacked = nullptr;    // pages of a 4-bit cache as F16 [n_seq][unpack_pages][K, V][n_head][PAGE][head_dim], their table
+    int32_t* unpacked_table = nullptr;
     // failure-path tests (gsvcu_set_wait_fault): bytes that a pair's barrier expects beyond its copies, polls of its wait (0: the
     // usual limit)
     uint32_t fault_extra_tx = 0, poll_limit = 0;
@@ -91,10 +93,14 @@ struct ChunkAttnPlan {
     int key_tile = 0;      // keys of a tile
     int split_tiles = 0;   // key tiles of a split
     bool join_apart = false;   // the splits are joined by a kernel of its own, not by the last CTA
+    int unpack_pages = 0;      // pages per sequence of a 4-bit cache that are unpacked to F16 first (0: the kernel reads the 4 bits)
+    size_t unpacked_floats = 0;
     size_t part_floats = 0, arrivals = 0;
 };
 ChunkAttnPlan chunk_attention_plan(const ChunkAttnParams& p);
 ChunkAttnPlan chunk_attention_tc_plan(const ChunkAttnParams& p);   // (more than 32 packed rows of a 16-bit type, scale not 0)
+// Bytes that unpacked pages may take.
+constexpr int64_t UNPACK_LIMIT = (int64_t)2 << 30;
 // Kernels launched; 0: none (no tensor map, or no room for the shared memory). `ready`: the caller's record (two words) of
 // the kernels whose shared-memory limit is raised on its device (zero at first; raising the 42 of the first word with the
 // context would add 16 ms to it).

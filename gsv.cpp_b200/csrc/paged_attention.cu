@@ -657,7 +657,7 @@ int launch_chunk_attention(const ChunkAttnParams& p, const ChunkAttnPlan& plan, 
     const size_t size = type_size(ty);
     const bool vec_out = ((uintptr_t)p.out & 15) == 0 && (p.out_stride * (int64_t)size) % 16 == 0;
     if (plan.tensor) {
-        if (!launch_chunk_attention_tc(p, plan, is_q4(p.kv.kv_dtype) ? ready + 1 : ready, s)) return 0;
+        if (!launch_chunk_attention_tc(p, plan, ready, s)) return 0;
     } else if (is_q4(p.kv.kv_dtype)) {
         if (!launch_chunk_attention_q4(p, plan, ready + 1, s)) return 0;
     } else {
@@ -679,11 +679,12 @@ int launch_chunk_attention(const ChunkAttnParams& p, const ChunkAttnPlan& plan, 
         });
         if (!ok) return 0;
     }
-    if (!plan.join_apart) return 1;
+    const int kernels = plan.unpack_pages ? 2 : 1;
+    if (!plan.join_apart) return kernels;
     if (ty == GSVCU_KV_F32) launch_join<float>(p, plan, vec_out, s);
     else if (ty == GSVCU_KV_F16) launch_join<__half>(p, plan, vec_out, s);
     else launch_join<__nv_bfloat16>(p, plan, vec_out, s);
-    return 2;
+    return kernels + 1;
 }
 
 }  // namespace gsvcu

@@ -13,6 +13,8 @@
 // The weights are split into two F16 parts, kept 2^14 up, as in k_chunk_attn.
 #include "paged_q4.cuh"
 
+#include <algorithm>
+
 #include "paged.h"
 #include "paged_join.cuh"
 
@@ -20,6 +22,7 @@ namespace gsvcu {
 namespace {
 
 constexpr int NW = 4;            // warps per CTA
+constexpr int UNPACK_ROWS = 1536;
 constexpr float BIAS = 14.0f;    // weights are 2^BIAS exp(s - maximum)
 __host__ __device__ constexpr int key_tile(int dim) { return dim == 32 ? 64 : 32; }
 
@@ -486,8 +489,19 @@ void pick(int dtype, int dim, int row_tile, F f) {
 ChunkAttnPlan chunk_attention_q4_plan(const ChunkAttnParams& p) {
     const int D = p.kv.head_dim, kt = key_tile(D);
     const int64_t packed = (int64_t)p.batch.max_chunk * (p.n_q_head / p.kv.n_head);
-    if (packed > 32 && p.scale != 0.0f) return chunk_attention_tc_plan(p);
     ChunkAttnPlan c;
+    if (packed > 32 && p.scale != 0.0f) {
+        c = chunk_attention_tc_plan(p);
+        // Many row tiles over the same keys: the keys are unpacked once, by a kernel before it.
+        const int group = p.n_q_head / p.kv.n_head;
+        const int64_t rows = p.window ? std::min(packed, (int64_t)p.window * group) : packed, pages = (p.batch.max_kv + PAGE - 1) / PAGE;
+        const int64_t bytes = p.batch.n_seq * pages * (2 * p.kv.n_head * PAGE * D * 2 + 4);
+        if (rows >= UNPACK_ROWS && bytes <= UNPACK_LIMIT) {
+            c.unpack_pages = (int)pages;
+            c.unpacked_floats = (size_t)(bytes / 4);
+        }
+        return c;
+    }
     c.row_tile = packed >= 32 ? 32 : (int)(packed + 7) / 8 * 8;
     c.tiles = (int)((packed + c.row_tile - 1) / c.row_tile);
     const int64_t units = (int64_t)p.batch.n_seq * c.tiles * p.kv.n_head;

@@ -40,6 +40,8 @@ using namespace tc;
 constexpr int KT = 128;                 // keys per tile
 constexpr int ROWS = 256;               // packed rows per CTA, two row tiles (one of 128 when the call has few CTAs)
 constexpr int THREADS = 384, THREADS_Q4 = 512;   // 4-bit caches: 4 warps more, which unpack the key tiles
+// What the pages hold: elements of the rows' type, 4 bits, or F16 beside BF16 rows (unpacked 4 bits).
+enum Pages { SAME, PACKED_Q4, AS_F16 };
 // Log2 headroom of P above the row's reference maximum, and how far up the weights are kept. F16: TAU 5, 4 or 3 cost
 // about 1 % over TAU 8 on scores of deviation 1, TAU 1 2 to 7 %.
 template <typename T> constexpr float TAU = __is_same(T, __half) ? 4.0f : 8.0f;
@@ -207,11 +209,11 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
                  "r"(bytes), "r"(bar)
                  : "memory");
 }
-// Eight 16-bit elements of T as F16 pairs in the order of the unpacked codes: (0, 4), (1, 5), (2, 6), (3, 7).
-template <typename T>
-__device__ __forceinline__ uint4 as_codes_lie(uint4 u) {
+// Eight 16-bit elements of T as F16, for unpacked codes in their order: (0, 4), (1, 5), (2, 6), (3, 7).
+template <typename T, bool Q4>
+__device__ __forceinline__ uint4 as_f16(uint4 u) {
     const T* x = (const T*)&u;
-    auto two = [&](int k) { return pack2<__half>((float)x[k], (float)x[k + 4]); };
+    auto two = [&](int k) { return Q4 ? pack2<__half>((float)x[k], (float)x[k + 4]) : pack2<__half>((float)x[2 * k], (float)x[2 * k + 1]); };
     return make_uint4(two(0), two(1), two(2), two(3));
 }
 // The unpacking warp's part of a packed tile (two blocks of 64 tokens): 32 of its 128 keys from `first` on, into the
@@ -257,10 +259,11 @@ __device__ __forceinline__ void unpack_tile(const uint8_t* packed, uint8_t* entr
     }
 }
 
-template <typename T, int D, bool Q4>
-__global__ void __launch_bounds__(Q4 ? THREADS_Q4 : THREADS, 1) k_chunk_attn_tc(const __grid_constant__ TcArgs a) {
+template <typename T, int D, Pages PG>
+__global__ void __launch_bounds__(PG == PACKED_Q4 ? THREADS_Q4 : THREADS, 1) k_chunk_attn_tc(const __grid_constant__ TcArgs a) {
+    constexpr bool Q4 = PG == PACKED_Q4;
     using L = Smem<D, Q4>;
-    using CT = typename std::conditional<Q4, __half, T>::type;   // what the products read
+    using CT = typename std::conditional<PG == SAME, T, __half>::type;   // what the products read
     constexpr int NT = Q4 ? THREADS_Q4 : THREADS;
     constexpr int TY = __is_same(CT, __half) ? 0 : 1;
     constexpr uint32_t ID_S = instr(TY, 0, KT), ID_O = instr(TY, 1, D);
@@ -437,7 +440,7 @@ __global__ void __launch_bounds__(Q4 ? THREADS_Q4 : THREADS, 1) k_chunk_attn_tc(
         for (int m = 0; m < 4; m++) {
             const int i = i0 + m * STEP, r = i / (D / 8), pc = i % (D / 8);
             if (r >= 128 * halves) break;
-            if constexpr (Q4) u[m] = as_codes_lie<T>(u[m]);
+            if constexpr (PG != SAME) u[m] = as_f16<T, Q4>(u[m]);
             if (a.negate) { u[m].x ^= 0x80008000u; u[m].y ^= 0x80008000u; u[m].z ^= 0x80008000u; u[m].w ^= 0x80008000u; }
             const int rt = r & 127, atom = D >= 64 ? pc / 8 : 0, ch = D >= 64 ? pc % 8 : pc;
             const int swz = L::RB == 128 ? rt & 7 : (rt >> 1) & 3;
@@ -809,27 +812,76 @@ __global__ void __launch_bounds__(Q4 ? THREADS_Q4 : THREADS, 1) k_chunk_attn_tc(
     }
 }
 
-template <typename T, bool Q4, typename F>
+template <typename T, Pages PG, typename F>
 void pick_tc_dim(int dim, F f) {
-    if (dim == 32) f(k_chunk_attn_tc<T, 32, Q4>, Smem<32, Q4>::SMEM);
-    else if (dim == 64) f(k_chunk_attn_tc<T, 64, Q4>, Smem<64, Q4>::SMEM);
-    else f(k_chunk_attn_tc<T, 128, Q4>, Smem<128, Q4>::SMEM);
+    if (dim == 32) f(k_chunk_attn_tc<T, 32, PG>, Smem<32, PG == PACKED_Q4>::SMEM);
+    else if (dim == 64) f(k_chunk_attn_tc<T, 64, PG>, Smem<64, PG == PACKED_Q4>::SMEM);
+    else f(k_chunk_attn_tc<T, 128, PG>, Smem<128, PG == PACKED_Q4>::SMEM);
 }
 template <typename F>
-void pick_tc(int dtype, int dim, F f) {
-    if (dtype == GSVCU_KV_F16) pick_tc_dim<__half, false>(dim, f);
-    else if (dtype == GSVCU_KV_BF16) pick_tc_dim<__nv_bfloat16, false>(dim, f);
-    else if (dtype == GSVCU_KV_Q4_F16) pick_tc_dim<__half, true>(dim, f);
-    else pick_tc_dim<__nv_bfloat16, true>(dim, f);
+void pick_tc(bool f16, Pages pages, int dim, F f) {
+    if (pages == PACKED_Q4) f16 ? pick_tc_dim<__half, PACKED_Q4>(dim, f) : pick_tc_dim<__nv_bfloat16, PACKED_Q4>(dim, f);
+    else if (f16) pick_tc_dim<__half, SAME>(dim, f);
+    else if (pages == AS_F16) pick_tc_dim<__nv_bfloat16, AS_F16>(dim, f);
+    else pick_tc_dim<__nv_bfloat16, SAME>(dim, f);
+}
+
+// Blocks of 64 tokens of a 4-bit cache as F16, for calls whose keys many row tiles read: a CTA per (sequence, page, K or V
+// and head), a thread per word and token. Page j of sequence s goes to place s * pages + j of p.unpacked, whose table names
+// them (-1: not in the pool); pages that no row of the chunk sees are left out. Bound by HBM and L2: 2 + 9/16 bytes an
+// element.
+template <int D>
+__global__ void __launch_bounds__(256) k_unpack_q4(ChunkAttnParams p, int group, int pages) {
+    using B = Q4Block<D>;
+    griddep_wait();
+    griddep_launch();
+    int id = blockIdx.x;
+    const int h = id % (2 * p.kv.n_head);   // K heads, then V heads
+    id /= 2 * p.kv.n_head;
+    const int j = id % pages, s = id / pages;
+    ChunkRange c;
+    if (!chunk_range(p, s, 0, group, 1 << 30, KT, false, c) || !c.sees(j * PAGE)) return;
+    const int page = p.batch.table[(int64_t)s * p.batch.max_pages + j];
+    const bool held = page >= 0 && page < p.kv.n_page;
+    const int64_t at = (int64_t)s * pages + j;
+    if (h == 0 && threadIdx.x == 0) p.unpacked_table[at] = held ? (int)at : -1;
+    if (!held) return;   // (reported by the attention)
+    const uint8_t* block = (const uint8_t*)p.kv.pool + (((int64_t)page * p.kv.n_layer + p.kv.layer) * 2 * p.kv.n_head + h) * B::BYTES;
+    __half* out = (__half*)p.unpacked + (at * 2 * p.kv.n_head + h) * (PAGE * D);
+#pragma unroll
+    for (int i = threadIdx.x; i < PAGE * D / 8; i += 256) {
+        const int token = i / (D / 8), w = i % (D / 8);
+        const uint32_t x = *(const uint32_t*)(block + token * B::ROW + q4_place<D>(w));
+        const __half2 d = __half2half2(((const __half*)(block + B::OFF_SCALES + token * B::SCALES))[w / 4]);
+        uint32_t v[4];
+        q4_values(x, d, __hmul2(d, __float2half2_rn(-24.0f)), v);
+        *(uint4*)(out + i * 8) = make_uint4(__byte_perm(v[0], v[1], 0x5410), __byte_perm(v[2], v[3], 0x5410),
+                                            __byte_perm(v[0], v[1], 0x7632), __byte_perm(v[2], v[3], 0x7632));
+    }
 }
 
 }  // namespace
 
-bool launch_chunk_attention_tc(const ChunkAttnParams& p, const ChunkAttnPlan& plan, uint64_t* ready, cudaStream_t s) {
+bool launch_chunk_attention_tc(const ChunkAttnParams& given, const ChunkAttnPlan& plan, uint64_t* ready, cudaStream_t s) {
     TcArgs a;
-    a.p = p;
+    a.p = given;
+    const ChunkAttnParams& p = a.p;
+    const int D = p.kv.head_dim, group = p.n_q_head / p.kv.n_head;
+    const bool f16 = row_type(p.kv.kv_dtype) == GSVCU_KV_F16;
+    const Pages pages = !is_q4(p.kv.kv_dtype) ? SAME : plan.unpack_pages ? AS_F16 : PACKED_Q4;
+    if (pages == AS_F16) {
+        const int64_t ctas = (int64_t)p.batch.n_seq * plan.unpack_pages * 2 * p.kv.n_head;
+        launch_pdl(D == 32 ? k_unpack_q4<32> : D == 64 ? k_unpack_q4<64> : k_unpack_q4<128>, dim3((unsigned)ctas), dim3(256), 0, s, p,
+                   group, plan.unpack_pages);
+        a.p.kv.pool = p.unpacked;
+        a.p.kv.n_page = p.batch.n_seq * plan.unpack_pages;
+        a.p.kv.n_layer = 1;
+        a.p.kv.layer = 0;
+        a.p.batch.table = p.unpacked_table;
+        a.p.batch.max_pages = plan.unpack_pages;
+    }
     if (!a.p.poll_limit) a.p.poll_limit = TC_SPIN_LIMIT;
-    a.group = p.n_q_head / p.kv.n_head;
+    a.group = group;
     a.row_tile = plan.row_tile;
     a.tiles = plan.tiles;
     a.n_split = plan.n_split;
@@ -839,25 +891,26 @@ bool launch_chunk_attention_tc(const ChunkAttnParams& p, const ChunkAttnPlan& pl
     a.negate = p.scale < 0.0f;
     a.vec_q = ((uintptr_t)p.q & 15) == 0 && p.q_stride % 8 == 0;
     a.vec_out = ((uintptr_t)p.out & 15) == 0 && p.out_stride % 8 == 0;
-    const int D = p.kv.head_dim;
-    const bool q4 = is_q4(p.kv.kv_dtype);
-    const EncodeTiledFn encode = q4 ? nullptr : encode_fn();
-    if (!q4 && !encode) return false;
-    const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)PAGE, (cuuint64_t)a.n_blocks};
-    const cuuint64_t strides[2] = {(cuuint64_t)D * 2, (cuuint64_t)PAGE * D * 2};
-    const cuuint32_t box[3] = {(cuuint32_t)(D < 64 ? D : 64), (cuuint32_t)PAGE, 1}, step[3] = {1, 1, 1};
-    if (!q4 && encode(&a.map, p.kv.kv_dtype == GSVCU_KV_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
-               p.kv.pool, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-               D >= 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-        return false;
+    if (pages != PACKED_Q4) {
+        const EncodeTiledFn encode = encode_fn();
+        if (!encode) return false;
+        const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)PAGE, (cuuint64_t)a.n_blocks};
+        const cuuint64_t strides[2] = {(cuuint64_t)D * 2, (cuuint64_t)PAGE * D * 2};
+        const cuuint32_t box[3] = {(cuuint32_t)(D < 64 ? D : 64), (cuuint32_t)PAGE, 1}, step[3] = {1, 1, 1};
+        if (encode(&a.map, f16 || pages == AS_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+                   p.kv.pool, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   D >= 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+            return false;
+    }
     const int64_t ctas = (int64_t)p.batch.n_seq * plan.tiles * p.kv.n_head * plan.n_split;
-    const bool f16 = row_type(p.kv.kv_dtype) == GSVCU_KV_F16;
-    const int bit = (q4 ? 24 : 36) + (f16 ? 0 : 3) + D / 64;   // 36 .. 41; 4 bits (their own word): 24 .. 29
+    // a bit of its own for every kernel: of the float caches 36 .. 41 of the first word, others 24 .. 32 of the second
+    const bool same = pages == SAME || (pages == AS_F16 && f16);
+    const int bit = (same ? 36 : pages == PACKED_Q4 ? 24 : 27) + (f16 ? 0 : 3) + D / 64;
     bool ok = false;
-    pick_tc(p.kv.kv_dtype, D, [&](auto k, size_t smem) {
-        ok = raise_smem(k, smem, ready, bit);
-        if (ok) launch_pdl(k, dim3((unsigned)ctas), dim3(q4 ? THREADS_Q4 : THREADS), smem, s, a);
+    pick_tc(f16, pages, D, [&](auto k, size_t smem) {
+        ok = raise_smem(k, smem, same ? ready : ready + 1, bit);
+        if (ok) launch_pdl(k, dim3((unsigned)ctas), dim3(pages == PACKED_Q4 ? THREADS_Q4 : THREADS), smem, s, a);
     });
     return ok;
 }

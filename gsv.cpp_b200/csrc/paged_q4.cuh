@@ -44,8 +44,16 @@ __device__ __forceinline__ __half q4_scale(uint32_t key, float& inv) {
     inv = f != 0.0f ? __fdiv_rn(1.0f, f) : 0.0f;
     return d;
 }
-__device__ __forceinline__ uint32_t q4_code(float x, float inv) {
-    return (uint32_t)(int)fminf(fmaxf(__fadd_rn(__fmul_rn(x, inv), 8.5f), 0.0f), 15.0f);   // (a NaN: 0)
+// Codes of 8 elements as a word. A number of 0 .. 15 added to 2^23, rounded down, ends in its floor; what the 2^23 leave in the
+// word is taken off at the end. (The conversion instruction has a quarter of the rate.)
+__device__ __forceinline__ uint32_t q4_word(const float* x, float inv) {
+    uint32_t word = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const float y = fminf(fmaxf(__fadd_rn(__fmul_rn(x[i], inv), 8.5f), 0.0f), 15.0f);   // (a NaN: 0)
+        word += __float_as_uint(__fadd_rd(y, 8388608.0f)) << (4 * i);
+    }
+    return word - 0xfb000000u;   // 0x4b000000 (1 + 16 + ...), cut to 32 bits
 }
 
 __device__ __forceinline__ uint32_t bits(__half2 h) { return *(const uint32_t*)&h; }

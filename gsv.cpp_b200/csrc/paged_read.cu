@@ -9,39 +9,65 @@
 namespace gsvcu {
 namespace {
 
-// Thread = (row, lane u of D / 8, head lane of the 2 n_head heads of K and V), 8 elements at a time. TC: the cache's
-// element, uint8_t for 4 bits.
+// Thread = (row, lane u, head lane of the 2 n_head heads of K and V): 16 bytes of a row at a time, and NB heads in flight.
+// TC: the cache's element, uint8_t for 4 bits. VEC: rows that 16-byte accesses fit.
 template <typename TC, typename T, int D, bool VEC>
 __global__ void __launch_bounds__(256) k_kv_read(KvReadParams p, int head_lanes) {
-    constexpr int U = D / 8;
     constexpr bool Q4 = sizeof(TC) == 1;
+    constexpr int E = 16 / sizeof(T), U = D / E, NB = 4;   // elements of a thread, threads of a head
     griddep_wait();
     griddep_launch();
     const int per_row = U * head_lanes, rows_per_cta = 256 / per_row;
     const int row = blockIdx.x * rows_per_cta + threadIdx.x / per_row;
     if (row >= p.batch.n_rows) return;   // (warp-uniform: per_row is a multiple of 32)
-    const int t = threadIdx.x % per_row, u = t % U, hl = t / U, lane = threadIdx.x & 31;
+    const int t = threadIdx.x % per_row, e0 = t % U * E, hl = t / U, lane = threadIdx.x & 31;
     const Place w = place_of(p, row, lane, t == 0);
     if (w.block < 0) return;
     const int nk = p.kv.n_head;
-    for (int h = hl; h < 2 * nk; h += head_lanes) {
-        float x[8];
+    for (int h0 = hl; h0 < 2 * nk; h0 += NB * head_lanes) {
+        float x[NB][E];
         if constexpr (Q4) {
             using B = Q4Block<D>;
-            const uint8_t* block = (const uint8_t*)p.kv.pool + (w.block + h) * (int64_t)B::BYTES;
-            const uint32_t word = *(const uint32_t*)(block + w.token * B::ROW + q4_place<D>(u));
-            const float d = __half2float(((const __half*)(block + B::OFF_SCALES + w.token * B::SCALES))[u / 4]);
+            uint32_t code[NB];
+            __half d[NB];
 #pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = (float)((int)(word >> (4 * i) & 15u) - 8) * d;
+            for (int b = 0; b < NB; b++) {
+                const int h = min(h0 + b * head_lanes, 2 * nk - 1);
+                const uint8_t* block = (const uint8_t*)p.kv.pool + (w.block + h) * (int64_t)B::BYTES;
+                const uint8_t* at = block + w.token * B::ROW + q4_place<D>(e0 / 8) + e0 % 8 / 2;
+                code[b] = E == 8 ? *(const uint32_t*)at : *(const uint16_t*)at;
+                d[b] = ((const __half*)(block + B::OFF_SCALES + w.token * B::SCALES))[e0 / 32];
+            }
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int i = 0; i < E; i++) x[b][i] = (float)((int)(code[b] >> (4 * i) & 15u) - 8) * __half2float(d[b]);
         } else {
-            load8((const TC*)p.kv.pool + ((w.block + h) * PAGE + w.token) * D + u * 8, x);
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                const TC* src = (const TC*)p.kv.pool + ((w.block + min(h0 + b * head_lanes, 2 * nk - 1)) * PAGE + w.token) * D + e0;
+                TC y[E];
+#pragma unroll
+                for (int i = 0; i < E; i++) y[i] = src[i];
+#pragma unroll
+                for (int i = 0; i < E; i++) x[b][i] = to_f32(y[i]);
+            }
         }
-        T* dst = (h < nk ? (T*)p.k + row * p.k_stride + h * D : (T*)p.v + row * p.v_stride + (h - nk) * D) + u * 8;
-        if constexpr (VEC) {
-            store8(dst, x);
-        } else {
 #pragma unroll
-            for (int i = 0; i < 8; i++) dst[i] = from_f32<T>(x[i]);
+        for (int b = 0; b < NB; b++) {
+            const int h = h0 + b * head_lanes;
+            if (h >= 2 * nk) break;
+            T* dst = (h < nk ? (T*)p.k + row * p.k_stride + h * D : (T*)p.v + row * p.v_stride + (h - nk) * D) + e0;
+            if constexpr (VEC) {
+                uint4 u;
+                T* y = (T*)&u;
+#pragma unroll
+                for (int i = 0; i < E; i++) y[i] = from_f32<T>(x[b][i]);
+                *(uint4*)dst = u;
+            } else {
+#pragma unroll
+                for (int i = 0; i < E; i++) dst[i] = from_f32<T>(x[b][i]);
+            }
         }
     }
 }
@@ -51,7 +77,7 @@ void launch(const KvReadParams& p, cudaStream_t s) {
     const bool vec = fits16(p.k, p.k_stride, sizeof(T)) && fits16(p.v, p.v_stride, sizeof(T));
     const int per_row = threads_per_row(p.batch.n_rows), rows = 256 / per_row;
     launch_pdl(vec ? k_kv_read<TC, T, D, true> : k_kv_read<TC, T, D, false>, dim3((p.batch.n_rows + rows - 1) / rows),
-               dim3(256), 0, s, p, per_row / (D / 8));
+               dim3(256), 0, s, p, per_row / (D * (int)sizeof(T) / 16));
 }
 template <typename TC, typename T>
 void launch_d(const KvReadParams& p, cudaStream_t s) {

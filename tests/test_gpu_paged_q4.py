@@ -298,6 +298,48 @@ def test_large_and_tiny_groups(ctx, ty, dim, q):  # noqa: F811
     assert float(out.abs().max()) > 100.0
 
 
+@pytest.mark.parametrize("ty,dim,heads,kv_heads,q", [("bf16", 128, 16, 2, 260), ("f16", 64, 8, 1, 300), ("bf16", 32, 16, 1, 130),
+                                                     ("f16", 128, 2, 2, 1700), ("bf16", 64, 9, 1, 500)])
+@pytest.mark.parametrize("window,prefix", [(0, None), (0, [3, 700, 64]), (300, None), (1600, [0, 70, 900])])
+def test_chunks_whose_pages_are_unpacked_first(ctx, ty, dim, heads, kv_heads, q, window, prefix):  # noqa: F811
+    """At least 1536 packed rows in a chunk, beside short ones and single tokens; windows that leave fewer rows to a key."""
+    c = Q4Case(ty, [q, 1, q // 3], [q + 1111, 900, q // 3], heads, kv_heads, dim)
+    attend(ctx, c, window=window, prefix=prefix)
+
+
+def test_pages_are_unpacked_again_for_every_call(ctx):  # noqa: F811
+    """Two caches, two layers and two lengths through the same scratch, captured in a graph too: nothing is kept from one
+    call for the next; a call past the scratch's limit reads the 4 bits themselves."""
+    import gsvcu
+    own = gsvcu.Context(0)
+    a = Q4Case("bf16", [400], [1500], 8, 2, 64, seed=1)
+    b = Q4Case("f16", [410, 3], [700, 90], 8, 2, 64, seed=2, layer=0)
+    x, first, _ = attend(own, a)
+    attend(own, b)
+    _, again, _ = attend(own, a, q=x)
+    assert torch.equal(first, again)
+    cache, chunks = a.objects()
+    out = torch.empty_like(x)
+    stream = torch.cuda.ExternalStream(own.stream_handle())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        own.op_chunk_attention(cache, chunks, a.layer, x, out)
+    attend(own, Q4Case("bf16", [400, 400, 400], [9000, 8000, 7000], 16, 2, 64))   # outgrows the scratch
+    a.set_values(torch.randn(a.pool.shape[0], 2, 2, PAGE, 64, device="cuda"))
+    for _ in range(2):
+        x.normal_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            graph.replay()
+        own.sync()
+        check_attention(a, x, out, None, 0.125)
+    wide = Q4Case("bf16", [400], [1500], 8, 2, 64, seed=1, max_pages=90000)   # (the table's length bounds the scratch)
+    attend(own, wide, q=x)
+    del graph
+    own.close()
+
+
 @pytest.mark.parametrize("ty,dim", [("bf16", 128), ("f16", 64), ("bf16", 32)])
 @pytest.mark.parametrize("rows", [128, 101])
 def test_warps_of_a_row_tile_at_their_own_pace(ctx, ty, dim, rows):  # noqa: F811
@@ -480,6 +522,42 @@ def test_append_in_place_without_queries_and_past_its_keys(ctx):  # noqa: F811
 def test_norms_of_small_and_large_rows(ctx, size, eps, q4):  # noqa: F811
     """Sums of squares far from 1 (1e15: past 2^100; 2^-70: below F32's normal range): summed in 64 bits, rounded once."""
     check_append(ctx, "bf16", "f32", 4, 2, 64, 0, eps=eps, size=min(size, 1e15), q4=q4 and size < 1e4)
+
+
+@pytest.mark.parametrize("off", [0, 1])
+@pytest.mark.parametrize("row_ty,ty", [("f32", "f32"), ("bf16", "bf16"), ("f16", "f16"), ("f32", "f16")])
+def test_norms_of_heads_that_are_not_finite(ctx, row_ty, ty, off):  # noqa: F811
+    """A NaN makes its head NaN; an infinity, or squares that overflow, the rest of its head 0 (an infinity itself NaN); other
+    heads, and values, are as without them. 16-byte accesses and single elements."""
+    import gsvcu
+    n, heads, dim = 9, 3, 64
+    g = torch.Generator(device="cuda")
+    g.manual_seed(5)
+    rows = torch.randn(n, 2 * heads * dim + off, generator=g, device="cuda")
+    x = rows[:, off:].unflatten(1, (2 * heads, dim))
+    x[1, 0, 5], x[2, 1, 63], x[3, 2, 0] = float("nan"), float("inf"), float("-inf")
+    x[4, 0, 7], x[4, 0, 40] = float("inf"), float("nan")
+    if row_ty != "f16":
+        x[5, 1] = 1e30
+    x[6, heads:] = float("nan")   # values
+    rows = rows.to(TYPES[row_ty])
+    x = rows[:, off:].unflatten(1, (2 * heads, dim))
+    k, v = x[:, :heads], x[:, heads:]
+    w = torch.rand(dim, generator=g, device="cuda") + 0.5
+    i32 = dict(dtype=torch.int32, device="cuda")
+    pool = torch.zeros(1, 1, 2, heads, PAGE, dim, dtype=TYPES[ty], device="cuda")
+    chunks = gsvcu.ChunkBatch(torch.tensor([0, n], **i32), torch.tensor([n], **i32), torch.zeros(1, 1, **i32), n, n)
+    out = torch.empty(n, heads, dim, dtype=TYPES[ty], device="cuda")
+    order(ctx).op_kv_append(gsvcu.PagedKV(pool), chunks, 0, k, k, v, out, q_norm=w, k_norm=w)
+    ctx.sync()
+    f = k.float()
+    want = f * (1.0 / (f.square().sum(-1, keepdim=True) / dim + 1e-6).sqrt()) * w
+    for got in (out, pool[0, 0, 0, :, :n].transpose(0, 1)):
+        got = got.float()
+        assert torch.equal(got.isnan(), want.isnan())
+        fine = ~want.isnan()
+        assert ((got - want)[fine].abs() <= ROUND[ty] * want[fine].abs() + 2.0 ** -20).all()
+    assert torch.equal(torch.nan_to_num(pool[0, 0, 1, :, :n].transpose(0, 1).float(), 9.0), torch.nan_to_num(v.to(TYPES[ty]).float(), 9.0))
 
 
 def test_quantiser_borders(ctx):  # noqa: F811
