@@ -93,6 +93,8 @@ struct ChunkAttnPlan {
     int key_tile = 0;      // keys of a tile
     int split_tiles = 0;   // key tiles of a split
     bool join_apart = false;   // the splits are joined by a kernel of its own, not by the last CTA
+    int ctas = 0;              // 4-bit caches, few rows: CTAs, and whether the pages are dealt out to them
+    bool dealt = false;
     int unpack_pages = 0;      // pages per sequence of a 4-bit cache that are unpacked to F16 first (0: the kernel reads the 4 bits)
     size_t unpacked_floats = 0;
     size_t part_floats = 0, arrivals = 0;
@@ -105,10 +107,9 @@ constexpr int64_t UNPACK_LIMIT = (int64_t)2 << 30;
 // the kernels whose shared-memory limit is raised on its device (zero at first; raising the 42 of the first word with the
 // context would add 16 ms to it).
 int launch_chunk_attention(const ChunkAttnParams& p, const ChunkAttnPlan& plan, uint64_t* ready, cudaStream_t s);
-// 4-bit caches: their plan, and their kernel for few rows (false: no room for its shared memory). `ready`: as above, a
-// word of its own.
+// 4-bit caches: their plan, and their kernels for few rows (kernels launched as above). `ready`: as above, a word of its own.
 ChunkAttnPlan chunk_attention_q4_plan(const ChunkAttnParams& p);
-bool launch_chunk_attention_q4(const ChunkAttnParams& p, const ChunkAttnPlan& plan, uint64_t* ready, cudaStream_t s);
+int launch_chunk_attention_q4(const ChunkAttnParams& p, const ChunkAttnPlan& plan, uint64_t* ready, cudaStream_t s);
 bool launch_chunk_attention_tc(const ChunkAttnParams& p, const ChunkAttnPlan& plan, uint64_t* ready, cudaStream_t s);
 template <typename K>
 inline bool raise_smem(K kernel, size_t bytes, uint64_t* ready, int bit) {

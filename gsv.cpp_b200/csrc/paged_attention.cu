@@ -659,7 +659,7 @@ int launch_chunk_attention(const ChunkAttnParams& p, const ChunkAttnPlan& plan, 
     if (plan.tensor) {
         if (!launch_chunk_attention_tc(p, plan, ready, s)) return 0;
     } else if (is_q4(p.kv.kv_dtype)) {
-        if (!launch_chunk_attention_q4(p, plan, ready + 1, s)) return 0;
+        return launch_chunk_attention_q4(p, plan, ready + 1, s);
     } else {
         SplitArgs a;
         a.p = p;

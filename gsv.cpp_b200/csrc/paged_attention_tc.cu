@@ -203,12 +203,6 @@ __device__ __forceinline__ uint64_t ex2_pair(uint64_t x) {
 // Output column of element k of 8: unpacked values lie as (0, 4), (1, 5), (2, 6), (3, 7).
 template <bool Q4>
 constexpr __device__ int column(int k) { return !Q4 ? k : k < 4 ? 2 * k : 2 * k - 7; }
-// Untiled copy of `bytes` (a multiple of 16, both addresses 16-byte aligned) completing on an mbarrier.
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
-                 "r"(bytes), "r"(bar)
-                 : "memory");
-}
 // Eight 16-bit elements of T as F16, for unpacked codes in their order: (0, 4), (1, 5), (2, 6), (3, 7).
 template <typename T, bool Q4>
 __device__ __forceinline__ uint4 as_f16(uint4 u) {

@@ -145,6 +145,22 @@ def test_long_caches_are_split(ctx, ty, dim, heads, kv_heads, q):  # noqa: F811
     attend(ctx, c, q=x, max_kv=0, lse=False)
 
 
+@pytest.mark.parametrize("ty,dim,heads,kv_heads,q", [("f16", 32, 16, 16, 1), ("bf16", 128, 8, 2, 1), ("f16", 64, 16, 4, 1), ("bf16", 128, 8, 2, 5),
+                                                     ("f16", 64, 9, 1, 3), ("bf16", 32, 8, 4, 12), ("f16", 128, 2, 2, 20)])
+@pytest.mark.parametrize("n_seq", [1, 7, 60, 300])
+@pytest.mark.parametrize("window", [0, 200])
+def test_pages_dealt_out_over_ragged_batches(ctx, ty, dim, heads, kv_heads, q, n_seq, window):  # noqa: F811
+    """Lengths from a few keys to thousands, sequences without rows and without keys among them: units that one CTA has to
+    itself, that two or many share, and CTAs with many units. The same result twice, bit for bit, and after a smaller batch."""
+    lens = [(37 * i * i + 11) % 700 + (5000 if i % 50 == 3 else 0) + (9000 if n_seq == 1 else 0) for i in range(n_seq)]
+    rows = [0 if i % 9 == 4 else q if i % 4 else 1 for i in range(n_seq)]
+    c = Q4Case(ty, rows, [max(n, r) if i % 11 else n for i, (n, r) in enumerate(zip(lens, rows))], heads, kv_heads, dim)
+    x, a, la = attend(ctx, c, window=window, prefix=[i % 90 for i in range(n_seq)] if window else None)
+    attend(ctx, Q4Case(ty, [1, 1], [900, 2000], heads, kv_heads, dim))
+    _, b, lb = attend(ctx, c, q=x, window=window, prefix=[i % 90 for i in range(n_seq)] if window else None, max_kv=max(c.kv_len) + 500)
+    assert torch.equal(a, b) and torch.equal(la, lb)
+
+
 @pytest.mark.parametrize("scale", [0.0, 1.7, -0.3])
 @pytest.mark.parametrize("ty,q", [("f16", 1), ("bf16", 140), ("f16", 140)])
 def test_scales(ctx, scale, ty, q):  # noqa: F811
@@ -366,7 +382,7 @@ def test_warps_of_a_row_tile_at_their_own_pace(ctx, ty, dim, rows):  # noqa: F81
 
 
 @pytest.mark.parametrize("ty,dim", [("f16", 64), ("bf16", 128), ("f16", 32)])
-@pytest.mark.parametrize("q,kv", [(60, 60), (60, 900), (300, 300), (300, 2000), (90, 9000)])
+@pytest.mark.parametrize("q,kv", [(1, 700), (1, 9000), (3, 5000), (60, 60), (60, 900), (300, 300), (300, 2000), (90, 9000)])
 def test_page_waits_that_run_out_are_reported(ctx, ty, dim, q, kv):  # noqa: F811
     """Every copy from the second on is expected to bring 16 bytes more than it does (the copies themselves complete) and its
     wait has a short limit: the call ends, the next sync reports it once, and the same call without the fault is right."""
