@@ -1,16 +1,21 @@
 // paged_attention_q4.cu -- attention of few new rows over a 4-bit paged cache (layout and scales: paged_q4.cuh; the
 // operator's formula and the float caches: paged_attention.cu).
 //
-// k_chunk_attn_q4 has the shape of k_chunk_attn: one CTA per (sequence, row tile, kv head, key split), four warps that
-// take the split's key tiles in turn, each with its own cp.async ring, running maximum, sum and output; transposed
-// products (16 keys x 8 query rows), warps joined in order, splits by the last CTA or by k_chunk_join. All products are F16
-// mma.m16n8k16, whatever the rows' type (BF16 queries fit F16 up to 65,504; beyond they count as overflowing):
+// k_chunk_attn_q4: the four warps of a CTA take pages of 64 keys in turn, each with its own copies, running maximum, sum and
+// output; transposed products (16 keys x 8 query rows), warps joined in order, what several CTAs share by the last of them or
+// by k_join_q4, in an order that the sizes alone decide. All products are F16 mma.m16n8k16, whatever the rows' type (BF16
+// queries fit F16 up to 65,504; beyond they count as overflowing):
 //   scores   the codes less 8 are exact in F16, and a group of 32 elements is two products, so a group's sum is multiplied
 //            by its key's scale in f32 afterwards;
 //   values   scale * (code - 8) is exact in F16 too (scales have 8 significant bits) and takes one fused multiply-add per
 //            pair: a code moved to bits 6 .. 9 under the exponent of 16 is the number 16 + code, times the scale less 24
 //            scales.
-// The weights are split into two F16 parts, kept 2^14 up, as in k_chunk_attn.
+// The weights are kept 2^14 up as in k_chunk_attn, for F16 rows in two parts, for BF16 ones in one.
+//
+// What bounds it: unpacking, about 1.5 instructions a value, most of them on the half-rate ALU (shifts, masks, byte permutes)
+// and FP16 pipes; the copies keep up with one block of K and of V per warp. Long caches run at 0.72 of the measured HBM
+// rate (131072 keys, 32/8 heads x 128: 46.4 us, floor 23.4, F16 cache 88); a start, a page per warp and the joins make 8 to 11
+// us. 64 keys at a time need 168 registers at head dim 128 but overlap better than 32 in 128 (46.4 against 52.6 us).
 #include "paged_q4.cuh"
 
 #include <algorithm>
@@ -26,6 +31,9 @@ namespace {
 using namespace tc;
 
 constexpr int NW = 4;            // warps per CTA
+// Packed rows over the same keys from which these are unpacked first (k_unpack_q4) rather than in every CTA. 1024 rows over
+// 16384 keys, 32/8 x 128: 95 us unpacked first, 92 not; 2048: 151 and 170; 4096: 239 and 300; heads of 64: 52 and 50, 79 and 85,
+// 132 and 154.
 constexpr int UNPACK_ROWS = 1536;
 constexpr float BIAS = 14.0f;    // weights are 2^BIAS exp(s - maximum)
 constexpr int KT = PAGE;         // keys of one warp's tile: a block of the cache
@@ -130,7 +138,7 @@ struct SplitArgs {
 // of all units one after the other, so that ragged lengths, windows and units of any number fill the GPU evenly. A unit that
 // several CTAs share is joined from their results; CTA i has at most two such, of its first unit (place 2 i) and of its last
 // when that goes on (place 2 i + 1).
-constexpr int LEAST = 2 * NW;   // pages of a CTA
+constexpr int LEAST = 2 * NW;   // pages of a CTA (fewer and the joins cost more than the pages)
 
 // Pages of a sequence over its row tiles and kv heads; one for a unit that sees none (its rows are written all the same).
 template <int ROWS>
@@ -729,7 +737,7 @@ ChunkAttnPlan chunk_attention_q4_plan(const ChunkAttnParams& p) {
         // Many row tiles over the same keys: the keys are unpacked once, by a kernel before it.
         const int group = p.n_q_head / p.kv.n_head;
         const int64_t rows = p.window ? std::min(packed, (int64_t)p.window * group) : packed, pages = (p.batch.max_kv + PAGE - 1) / PAGE;
-        const int64_t bytes = p.batch.n_seq * pages * (2 * p.kv.n_head * PAGE * D * 2 + 4);
+        const int64_t bytes = p.batch.n_seq * pages * ((int64_t)p.kv.n_head * (4 * PAGE * D) + 4);
         if (rows >= UNPACK_ROWS && bytes <= UNPACK_LIMIT) {
             c.unpack_pages = (int)pages;
             c.unpacked_floats = (size_t)(bytes / 4);
@@ -744,7 +752,9 @@ ChunkAttnPlan chunk_attention_q4_plan(const ChunkAttnParams& p) {
     pick(p.kv.kv_dtype, D, c.row_tile, true, [&](auto, size_t bytes) { smem = bytes; });
     const int64_t slots = 148 * std::min((int64_t)(232448 / (smem + 1024)), (int64_t)resident(D, c.row_tile / 8, true));
     c.key_tile = KT;
-    // Short units: a CTA for each, nothing to join and no lengths to add up first.
+    // Short units: a CTA for each, nothing to join and no lengths to add up first. 64 slots of 600 to 2100 keys, 16 heads x 32:
+    // 31.8 us, 42 dealt out; 4 of 2000 to 4000 keys: 25 and 18; at head dim 128 a page takes longer, and 32 units of 600 to 2100
+    // keys are faster dealt out (17.3, 21.4).
     if (max_tiles <= (D < 128 || units >= slots ? 40 : 16)) {
         c.ctas = (int)units;
         return c;

@@ -2,7 +2,8 @@
 //
 // Row i of a sequence's chunk of n rows is the token at cache position kv_len - n + i (a chunk of kv_len rows: the whole
 // sequence). 4-bit caches: scale * (code - 8), exact in F16 and F32. Every element is read once and written once: bound by
-// HBM, and by the chain row_start -> kv_len -> table -> load for few rows.
+// HBM (102k tokens of 8 heads x 128 from 4 bits to F32: 129.5 us, 6.2 TB/s; 184 with 8 elements a thread, whose F32 stores
+// fill half of a sector each, and one head at a time), and by the chain row_start -> kv_len -> table -> load for few rows.
 #include "paged_q4.cuh"
 #include "paged_rows.cuh"
 

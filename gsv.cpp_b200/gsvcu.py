@@ -258,12 +258,18 @@ def _ints(t, shape, what, device):
     return t.data_ptr()
 
 
+_FLOAT32 = set()   # torch.float32, once met
+
+
 def _floats(t, shape, what, device):
     """Address of a contiguous float32 tensor of this shape on CUDA device `device`."""
+    if t.shape == shape and t.get_device() == device and t.dtype in _FLOAT32 and t.is_contiguous():
+        return t.data_ptr()
     if t.get_device() != device:
         raise ValueError(f"{what}: expected on CUDA device {device}, got {t.device}")
     if t.shape != shape or not t.is_contiguous() or _kv_type(t.dtype, what) != KV_F32:
         raise ValueError(f"{what}: contiguous float32 {list(shape)} expected, got {t.dtype} {list(t.shape)}")
+    _FLOAT32.add(t.dtype)
     return t.data_ptr()
 
 
@@ -276,7 +282,7 @@ def _row_stride(t, shape, what, device):
     row, head, one = t.stride()
     n_rows, heads, head_dim = shape
     width = heads * head_dim
-    if row >= width and head == head_dim and one == 1:
+    if head == head_dim and one == 1 and row >= width:
         return row
     if one != 1 or (head != head_dim and heads > 1):
         raise ValueError(f"{what}: each row's heads must be contiguous")

@@ -282,7 +282,8 @@ int gsvcu_op_prefill_attention(gsvcu_ctx* ctx, const float* qkv_dev, int32_t n_s
  * token. Written by gsvcu_op_kv_append, m being the group's element of the largest magnitude (of both signs the negative
  * one): scale = -m / 8, kept within +- 2720 (elements beyond +- 21,760 saturate), rounded to BF16 and then to F16; code =
  * floor(x * (1 / scale) + 8.5) in F32, kept within 0 .. 15 (scale 0: 8). A group with a NaN or an infinity reads back as NaN.
- * Scales of more than 8 significant bits (a cache written by other means) are read with their products rounded to F16. */
+ * A cache written by other means may have any scales within +- 2720; with more than 8 significant bits the attention reads
+ * it within 1 % of a step (gsvcu_op_kv_read exactly). */
 typedef struct {
     void* pool_dev;
     int32_t kv_dtype, n_page, n_layer, n_kv_head, head_dim;
@@ -353,7 +354,11 @@ int gsvcu_op_kv_read(gsvcu_ctx* ctx, const gsvcu_kv_read* a);
  * lse_dev (may be null) [n_rows][n_q_head] gets the natural logarithm of each row's sum of exp(scale q.k).
  * A row that sees no key gives 0 and -infinity. Scores, softmax and sums are F32, exponentials within 2.7e-6; with more
  * than 32 rows times query heads of a kv head the weights are rounded to the cache's type for the product with the values
- * (F16: 11 bits down to 2^-25 of the row's largest, none below 2^-36). What the pages hold from kv_len on does not
+ * (F16: 11 bits down to 2^-25 of the row's largest, none below 2^-36). 4-bit caches are read exactly and multiplied in F16:
+ * BF16 queries beyond 65,504 count as overflowing, weights have 11 bits (F16 rows of up to 32 22) and none is below 2^-39
+ * (more than 32: 2^-36) of the row's largest. From 1536 rows times query heads of a kv head on, their pages are unpacked into
+ * scratch of the context first, at most 2 GB a call (n_seq * max_kv tokens of all kv heads at 16 bits; what would take more is
+ * read as it is). What the pages hold from kv_len on does not
  * matter, nor do pages that no row sees; in the other pages every key and value has to be finite (a value that is not
  * reaches rows that do not see it, as 0 times infinity) and in F32 below 2^128 - 2^115. A row with a score that is NaN
  * or overflows to infinity is NaN, a score of minus infinity has weight 0 (F32 caches: NaN too); |scale| at most 1e38. */
@@ -535,7 +540,7 @@ int gsvcu_sync(gsvcu_ctx* ctx);
  * next status read of generate / serve (or gsvcu_sync after an op call) returns GSVCU_ERR_CUDA with
  * "staged K/V never arrived", and the context stays usable. Nothing faults: the staged copies all
  * complete, only the expected count is never reached. The same holds for the page waits of gsvcu_op_chunk_attention
- * with many rows (from a block's second pair of copies on, "a bounded wait gave up"). on = 0 (default) restores normal
+ * with many rows, and over 4-bit caches (from the second copies on, "a bounded wait gave up"). on = 0 (default) restores normal
  * operation. */
 int gsvcu_set_wait_fault(gsvcu_ctx* ctx, int32_t on);
 

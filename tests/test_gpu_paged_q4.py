@@ -161,6 +161,18 @@ def test_pages_dealt_out_over_ragged_batches(ctx, ty, dim, heads, kv_heads, q, n
     assert torch.equal(a, b) and torch.equal(la, lb)
 
 
+@pytest.mark.parametrize("ty,dim,heads,kv_heads,q,kv", [("f16", 64, 40, 1, 1, 500), ("bf16", 128, 40, 1, 1, 9000), ("f16", 32, 66, 2, 1, 3000)])
+def test_wide_groups(ctx, ty, dim, heads, kv_heads, q, kv):  # noqa: F811
+    """More than 32 query heads of a kv head: single tokens on the kernel for many rows."""
+    attend(ctx, Q4Case(ty, [q, q], [kv, 70], heads, kv_heads, dim))
+
+
+def test_a_zero_scale_over_a_long_cache(ctx):  # noqa: F811
+    """Many rows on the kernel for few, several row tiles of a sequence, pages dealt out."""
+    attend(ctx, Q4Case("f16", [70, 3, 140], [6000, 90, 3000], 4, 2, 64), scale=0.0)
+    attend(ctx, Q4Case("bf16", [50, 1], [5000, 4000], 8, 2, 128), scale=0.0, window=900)
+
+
 @pytest.mark.parametrize("scale", [0.0, 1.7, -0.3])
 @pytest.mark.parametrize("ty,q", [("f16", 1), ("bf16", 140), ("f16", 140)])
 def test_scales(ctx, scale, ty, q):  # noqa: F811
@@ -898,6 +910,76 @@ def test_bad_device_arrays_are_reported(ctx, q):  # noqa: F811
     expect("position")
 
 
+@pytest.mark.parametrize("group", [1, 5, 7])
+@pytest.mark.parametrize("max_kv", [0, 9000])
+@pytest.mark.parametrize("bounds", [(0, -723922764), (7, -1292124672), (8, -1199745), (0, -1599320890), (3, -2 ** 31),
+                                    (-5, 3), (-2 ** 31, 2 ** 31 - 1), (8, 2 ** 31 - 1), (2 ** 31 - 1, -2 ** 31), (9, 9)])
+def test_row_bounds_far_outside_the_batch(ctx, group, max_kv, bounds):  # noqa: F811
+    """row_start with values whose differences and products pass 32 bits, lengths far off: all three operators report them and
+    write nothing outside their rows and pages. With the wider bound on the lengths the pages are dealt out."""
+    import gsvcu
+    c = Q4Case("f16", [8], [70], 2 * group, 2, 64, max_pages=200 if max_kv else None)
+    c.table.fill_(1)
+    c.row_start.copy_(torch.tensor(bounds, dtype=torch.int32))
+    x, kv = c.rand(8, 2 * group, 64), c.rand(8, 2, 64)
+    guard, back = torch.full((72, 2 * group, 64), 7.0, dtype=c.dtype, device="cuda"), torch.full((72, 2, 64), 7.0, dtype=c.dtype, device="cuda")
+    w = torch.ones(64, device="cuda")
+    cache, chunks = c.objects(max_kv)
+    for lens in (70, 0, -2 ** 31, 2 ** 31 - 1):
+        c.kv.fill_(lens)
+        before = c.pool.clone()
+        for call in (lambda: ctx.op_chunk_attention(cache, chunks, 1, x, guard[32:40]),
+                     lambda: ctx.op_kv_append(cache, chunks, 1, x, kv, kv, guard[32:40], q_norm=w, k_norm=w),
+                     lambda: ctx.op_kv_read(cache, chunks, 1, back[32:40], back[32:40].clone())):
+            order(ctx)
+            call()
+            with pytest.raises(gsvcu.GsvcuError) as e:
+                ctx.sync()
+            assert e.value.code == -1
+        for g in (guard, back):
+            assert (g[:32] == 7.0).all() and (g[40:] == 7.0).all()
+        assert torch.equal(before[:, 0], c.pool[:, 0])   # (the other layer)
+    ctx.sync()
+
+
+@pytest.mark.parametrize("q", [2, 70])
+@pytest.mark.parametrize("kv", [100, 5000])
+def test_the_operators_report_the_same_bounds(ctx, q, kv):  # noqa: F811
+    """Lengths inside the table but outside the given sizes, and rows that no sequence owns, are reported after every operator; a
+    bound on the chunks that is wider than the batch is none of these."""
+    import gsvcu
+    c = Q4Case("f16", [q, q], [q + kv, q + 30], 4, 2, 64, max_pages=90)
+    x, rows = c.rand(2 * q, 4, 64), c.rand(2 * q, 2, 64)
+    out = torch.empty_like(x)
+    cache, _ = c.objects()
+
+    def reported(max_chunk=q, max_kv=q + kv):
+        chunks = gsvcu.ChunkBatch(c.row_start, c.kv, c.table, 2 * q, max_chunk, max_kv)
+        found = []
+        for call in (lambda: ctx.op_kv_append(cache, chunks, 1, x, rows, rows, out), lambda: ctx.op_chunk_attention(cache, chunks, 1, x, out),
+                     lambda: ctx.op_kv_read(cache, chunks, 1, rows.clone(), rows.clone())):
+            order(ctx)
+            call()
+            try:
+                ctx.sync()
+                found.append(None)
+            except gsvcu.GsvcuError as e:
+                assert e.code == -1
+                found.append("kv_len" in str(e))
+        return found
+
+    assert reported() == [None] * 3
+    assert reported(max_chunk=2 * q + 999) == [None] * 3
+    assert reported(max_kv=q + kv - 1) == [True] * 3
+    assert reported(max_chunk=q - 1) == [True] * 3
+    for bounds in ((0, q, 2 * q - 1), (1, q, 2 * q)):
+        c.row_start.copy_(torch.tensor(bounds, dtype=torch.int32))
+        assert reported() == [True] * 3, bounds
+    c.row_start.copy_(torch.tensor([0, q, 2 * q], dtype=torch.int32))
+    c.kv[1] = -1
+    assert reported() == [True] * 3
+
+
 def test_nothing_to_do(ctx):  # noqa: F811
     """No rows: nothing is touched, nothing is launched."""
     c = Q4Case("f16", [0, 0], [5, 70], 4, 2, 64)
@@ -909,3 +991,17 @@ def test_nothing_to_do(ctx):  # noqa: F811
     ctx.op_kv_read(cache, chunks, 0, out[:, :2], out[:, :2].clone())
     ctx.sync()
     assert ctx.kernel_launches() == before
+
+
+def test_example_with_a_4_bit_cache():
+    """examples/chunked_decoder.py over 4 bits. Chunks and whole prompts round their products to BF16 in another order, so a
+    key or value may differ by 2^-8 of itself and, where that crosses a border between codes, by a step s. With elements of up
+    to 8 steps, 3 on average, 2 * 3 * 2^-8 = 2.3 % of the codes cross: 0.15 s over all, and s is at most a quarter of the
+    elements' size: 4 % per layer, under 10 % for both layers' residuals."""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.abspath(__file__)), "..", "examples", "chunked_decoder.py")
+    spec = importlib.util.spec_from_file_location("chunked_decoder", path)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    assert mod.main(lengths=(130, 9, 65), pieces=(50, 1, 64), bits=4) < 0.1
