@@ -335,6 +335,17 @@ def test_chunks_whose_pages_are_unpacked_first(ctx, ty, dim, heads, kv_heads, q,
     attend(ctx, c, window=window, prefix=prefix)
 
 
+@pytest.mark.parametrize("ty,dim,heads,kv_heads,q_len,kv_len,window", [
+    ("bf16", 128, 32, 8, [1300], [9000], 0), ("f16", 64, 16, 4, [900, 700, 5, 1200], [7000, 6500, 9000, 8000], 0),
+    ("bf16", 32, 16, 16, [1500], [9000], 0), ("f16", 128, 8, 8, [3000, 1900], [9500, 1900], 0), ("f16", 64, 16, 4, [1500, 1100], [9000, 9000], 3000)])
+def test_chunks_of_more_than_one_wave(ctx, ty, dim, heads, kv_heads, q_len, kv_len, window):  # noqa: F811
+    """More CTAs than the GPU takes at once, over many keys. Twice the same."""
+    c = Q4Case(ty, q_len, kv_len, heads, kv_heads, dim)
+    x, a, la = attend(ctx, c, window=window)
+    _, b, lb = attend(ctx, c, q=x, window=window)
+    assert torch.equal(a, b) and torch.equal(la, lb)
+
+
 def test_pages_are_unpacked_again_for_every_call(ctx):  # noqa: F811
     """Two caches, two layers and two lengths through the same scratch, captured in a graph too: nothing is kept from one
     call for the next; a call past the scratch's limit reads the 4 bits themselves."""
