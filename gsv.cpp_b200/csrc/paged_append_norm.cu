@@ -204,10 +204,12 @@ __global__ void __launch_bounds__(256, sizeof(TI) == 4 ? 2 : 3) k_kv_append_norm
 // other widths mix them. Adjacent elements: two units.
 bool fits_groups(const KvAppendParams& p) { return p.pairs || p.rot <= 32 || p.rot % 64 == 0; }
 
-// Any alignment and rotation width, element by element: thread = (row, lane u of D / 8, head lane), 8 consecutive elements of
-// a head, whose angles and weights stay in registers over the heads; partners through shared memory.
+// Any alignment and rotation width: thread = (row, lane u of D / 8, head lane), 8 consecutive elements of a head, whose angles
+// and weights stay in registers over the heads; partners through shared memory, rows that 16-byte accesses do not fit element
+// by element. For what is rare: 31k rows of 48 heads x 128 in BF16, 96 rotated, into 4 bits 352 us; 120 rotated, rows at odd
+// addresses, 449 us.
 template <typename TI, typename T, int D, bool Q4>
-__global__ void __launch_bounds__(256) k_kv_append_norm_any(KvAppendParams p, int head_lanes) {
+__global__ void __launch_bounds__(256) k_kv_append_norm_any(KvAppendParams p, int head_lanes, bool aligned) {
     constexpr int U = D / 8;
     __shared__ float turned[256 * 8];
     griddep_wait();
@@ -249,8 +251,12 @@ __global__ void __launch_bounds__(256) k_kv_append_norm_any(KvAppendParams p, in
             const TI* src = is_q ? (const TI*)p.q + row * p.q_stride
                                  : is_v ? (const TI*)p.v + row * p.v_stride : (const TI*)p.k + row * p.k_stride;
             src += hh * D + e0;
+            if (aligned) {
+                load8(src, x);
+            } else {
 #pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = to_f32(src[i]);
+                for (int i = 0; i < 8; i++) x[i] = to_f32(src[i]);
+            }
         }
         if (p.q_norm || p.k_norm) {
             double ss = 0.0;
@@ -296,8 +302,12 @@ __global__ void __launch_bounds__(256) k_kv_append_norm_any(KvAppendParams p, in
             T* dst = is_q ? (T*)p.q_out + row * p.q_out_stride + hh * D
                           : (T*)p.kv.pool + ((w.block + (is_v ? nk : 0) + hh) * PAGE + w.token) * D;
             dst += e0;
+            if (aligned) {
+                store8(dst, x);
+            } else {
 #pragma unroll
-            for (int i = 0; i < 8; i++) dst[i] = from_f32<T>(x[i]);
+                for (int i = 0; i < 8; i++) dst[i] = from_f32<T>(x[i]);
+            }
         } else if (w.block >= 0) {
             using B = Q4Block<D>;
             float inv;
@@ -312,13 +322,13 @@ __global__ void __launch_bounds__(256) k_kv_append_norm_any(KvAppendParams p, in
 template <typename TI, typename T, int D, bool Q4>
 void launch(const KvAppendParams& p, cudaStream_t s) {
     const size_t si = sizeof(TI), so = sizeof(T);
-    const bool vec = p.rot % 16 == 0 && (!Q4 || fits_groups(p)) && fits16(p.q, p.q_stride, si) && fits16(p.k, p.k_stride, si) &&
-                     fits16(p.v, p.v_stride, si) && fits16(p.q_out, p.q_out_stride, so);
+    const bool aligned = fits16(p.q, p.q_stride, si) && fits16(p.k, p.k_stride, si) && fits16(p.v, p.v_stride, si) &&
+                         fits16(p.q_out, p.q_out_stride, so);
+    const bool vec = aligned && p.rot % 16 == 0 && (!Q4 || fits_groups(p));
     const int per_row = threads_per_row(p.batch.n_rows), rows = 256 / per_row;
-    auto go = [&](auto kernel) {
-        launch_pdl(kernel, dim3((p.batch.n_rows + rows - 1) / rows), dim3(256), 0, s, p, per_row / (vec ? D / 16 : D / 8));
-    };
-    if (!vec) go(k_kv_append_norm_any<TI, T, D, Q4>);
+    const dim3 grid((p.batch.n_rows + rows - 1) / rows);
+    auto go = [&](auto kernel) { launch_pdl(kernel, grid, dim3(256), 0, s, p, per_row / (D / 16)); };
+    if (!vec) launch_pdl(k_kv_append_norm_any<TI, T, D, Q4>, grid, dim3(256), 0, s, p, per_row / (D / 8), aligned);
     else if (p.q_norm || p.k_norm) go(k_kv_append_norm<TI, T, D, Q4, true>);
     else if constexpr (Q4) go(k_kv_append_norm<TI, T, D, Q4, false>);   // (float caches without norms: paged_append.cu)
 }

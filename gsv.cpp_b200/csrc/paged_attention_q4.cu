@@ -39,8 +39,8 @@ constexpr float BIAS = 14.0f;    // weights are 2^BIAS exp(s - maximum)
 constexpr int KT = PAGE;         // keys of one warp's tile: a block of the cache
 // Keys whose scores are held at a time.
 __host__ __device__ constexpr int part_keys(int nt) { return nt == 1 ? 64 : 32; }
-// CTAs that the registers of an SM hold (the pages dealt out take a few more). One more or less of them at head dim 128: one
-// sequence of 131072 keys 49.4 us with four, 46.4 with three.
+// CTAs that the registers of an SM hold (pages dealt out take a few more). One sequence of 131072 keys of 8 heads x 128: 49.4 us
+// with four, 46.4 with three.
 __host__ __device__ constexpr int resident(int dim, int nt, bool dealt) {
     return nt > 1 ? 2 : dim == 128 ? 3 : dim == 64 || dealt ? 4 : 5;
 }
@@ -49,7 +49,10 @@ __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)
 template <int N>   // words
 __device__ __forceinline__ void lds(uint32_t a, uint32_t (&x)[N]) {
     if constexpr (N == 4)
-        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(a) : "memory");
+        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                     : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
+                     : "r"(a)
+                     : "memory");
     else if constexpr (N == 2)
         asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(x[0]), "=r"(x[1]) : "r"(a) : "memory");
     else
@@ -95,8 +98,8 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     return y;
 }
 
-// A warp has STAGES blocks of K and of V in shared memory (two are no faster than one): the next K comes while the weights and their product with V are
-// worked on, the next V during the scores.
+// A warp has STAGES blocks of K and of V in shared memory (two are no faster than one): the next K comes while the weights and
+// their product with V are worked on, the next V during the scores.
 template <int D, int NT>
 struct Cfg {
     using B = Q4Block<D>;
@@ -262,424 +265,424 @@ __global__ void __launch_bounds__(NW * 32, resident(D, NT, DEALT)) k_chunk_attn_
     }
 
     for (;;) {   // units
-    ChunkRange c;
-    int v0 = 0, v1, first = 0, n_act = 1;   // this unit's pages here, the CTAs that share it
-    int64_t taken = 0;
-    if constexpr (!DEALT) {
-        if (!chunk_range(p, s, tile, a.group, ROWS, KT, tid == 0 && h == 0 && tile == 0, c)) return;
-        v1 = c.n_tiles;
-    } else {
-        int64_t here = 0;   // pages of a head
-        while (s < p.batch.n_seq) {
-            if (tile < a.tiles && chunk_range(p, s, tile, a.group, ROWS, KT, false, c)) {
-                here = max(1, c.n_tiles);
-                if (off < here * heads) break;
-                off -= here * heads;
-                tile++;
-            } else {
-                s++;
-                tile = 0;
+        ChunkRange c;
+        int v0 = 0, v1, first = 0, n_act = 1;   // this unit's pages here, the CTAs that share it
+        int64_t taken = 0;
+        if constexpr (!DEALT) {
+            if (!chunk_range(p, s, tile, a.group, ROWS, KT, tid == 0 && h == 0 && tile == 0, c)) return;
+            v1 = c.n_tiles;
+        } else {
+            int64_t here = 0;   // pages of a head
+            while (s < p.batch.n_seq) {
+                if (tile < a.tiles && chunk_range(p, s, tile, a.group, ROWS, KT, false, c)) {
+                    here = max(1, c.n_tiles);
+                    if (off < here * heads) break;
+                    off -= here * heads;
+                    tile++;
+                } else {
+                    s++;
+                    tile = 0;
+                }
             }
+            if (s >= p.batch.n_seq) return;   // (not while the lengths stay as they are)
+            h = (int)(off / here);
+            v0 = (int)(off % here);
+            taken = min(here - v0, end - pos);
+            v1 = min(v0 + (int)taken, c.n_tiles);
+            const int64_t start = pos - v0;
+            first = (int)(start / per);
+            n_act = (int)((start + here - 1) / per) - first + 1;
         }
-        if (s >= p.batch.n_seq) return;   // (not while the lengths stay as they are)
-        h = (int)(off / here);
-        v0 = (int)(off % here);
-        taken = min(here - v0, end - pos);
-        v1 = min(v0 + (int)taken, c.n_tiles);
-        const int64_t start = pos - v0;
-        first = (int)(start / per);
-        n_act = (int)((start + here - 1) / per) - first + 1;
-    }
-    const int32_t* tab = p.batch.table + (int64_t)s * p.batch.max_pages;
-    const int row0 = c.row0, n = c.n, total = c.total, len = c.len, r0 = c.r0, rows = c.rows, p0 = c.p0, p1 = c.p1, np = c.np;
-    const int mine = ok && v0 + warp < v1 ? (v1 - v0 - warp + NW - 1) / NW : 0;
-    auto key0 = [&](int i) { return c.tile_of(v0 + warp + i * NW) * KT; };
+        const int32_t* tab = p.batch.table + (int64_t)s * p.batch.max_pages;
+        const int row0 = c.row0, n = c.n, total = c.total, len = c.len, r0 = c.r0, rows = c.rows, p0 = c.p0, p1 = c.p1, np = c.np;
+        const int mine = ok && v0 + warp < v1 ? (v1 - v0 - warp + NW - 1) / NW : 0;
+        auto key0 = [&](int i) { return c.tile_of(v0 + warp + i * NW) * KT; };
 
-    // the page numbers of 32 tiles ahead sit in the warp's lanes
-    int fetched_k = -1, fetched_v = -1;
-    // K (V) of this warp's tile i; called for i, then the same i for V.
-    auto fetch = [&](int i, bool v) {
-        if (i >= mine) return;
-        (v ? fetched_v : fetched_k) = i;
-        if (!v && (i & 31) == 0 && (i || !early)) pages = i + lane < mine ? tab[key0(i + lane) / PAGE] : 0;
-        const int page = __shfl_sync(0xffffffffu, pages, i & 31);
-        const bool held = page >= 0 && page < p.kv.n_page;
-        bad |= !held;
-        if (lane == 0) {
-            const uint32_t st = 2 * ((phase + i) % ST) + v, bar = bars + 8 * st;
-            bar_expect_tx(bar, (held ? B::BYTES : 0) + (phase + i > 0 ? p.fault_extra_tx : 0u));
-            const int64_t block = ((int64_t)page * p.kv.n_layer + p.kv.layer) * 2 * p.kv.n_head + h + (v ? p.kv.n_head : 0);
-            if (held) bulk_load(ring + st * B::BYTES, (const uint8_t*)p.kv.pool + block * B::BYTES, B::BYTES, bar);
-        }
-    };
-    auto arrived = [&](int i, bool v) {   // bounded
-        const uint32_t bar = bars + 8 * (2 * ((phase + i) % ST) + v), parity = (phase + i) / ST & 1u;
-        for (uint32_t it = 0; it < p.poll_limit; it++)
-            if (__any_sync(0xffffffffu, bar_try_short(bar, parity))) return true;
-        return false;
-    };
-#pragma unroll
-    for (int i = 0; i < ST; i++) {
-        fetch(i, false);
-        fetch(i, true);
-    }
-    // queries into shared memory, zero past the tile's rows (after the first copies are under way)
-    uint8_t* sq = sm + C::OFF_Q;
-    for (int i = tid; i < ROWS * (D / 8); i += NW * 32) {
-        const int r = i / (D / 8), pc = i % (D / 8);
-        __half x[8];
-#pragma unroll
-        for (int k = 0; k < 8; k++) x[k] = __float2half_rn(0.0f);
-        if (r < rows) {
-            const int tok = (r0 + r) / a.group, j = (r0 + r) % a.group;
-            const T* src = (const T*)p.q + (int64_t)(row0 + tok) * p.q_stride + (int64_t)(h * a.group + j) * D + pc * 8;
-            uint4 u;
-            if (a.vec_q) {
-                u = *(const uint4*)src;
-            } else {
-                T* y = (T*)&u;
-#pragma unroll
-                for (int k = 0; k < 8; k++) y[k] = src[k];
+        // the page numbers of 32 tiles ahead sit in the warp's lanes
+        int fetched_k = -1, fetched_v = -1;
+        // K (V) of this warp's tile i; called for i, then the same i for V.
+        auto fetch = [&](int i, bool v) {
+            if (i >= mine) return;
+            (v ? fetched_v : fetched_k) = i;
+            if (!v && (i & 31) == 0 && (i || !early)) pages = i + lane < mine ? tab[key0(i + lane) / PAGE] : 0;
+            const int page = __shfl_sync(0xffffffffu, pages, i & 31);
+            const bool held = page >= 0 && page < p.kv.n_page;
+            bad |= !held;
+            if (lane == 0) {
+                const uint32_t st = 2 * ((phase + i) % ST) + v, bar = bars + 8 * st;
+                bar_expect_tx(bar, (held ? B::BYTES : 0) + (phase + i > 0 ? p.fault_extra_tx : 0u));
+                const int64_t block = ((int64_t)page * p.kv.n_layer + p.kv.layer) * 2 * p.kv.n_head + h + (v ? p.kv.n_head : 0);
+                if (held) bulk_load(ring + st * B::BYTES, (const uint8_t*)p.kv.pool + block * B::BYTES, B::BYTES, bar);
             }
+        };
+        auto arrived = [&](int i, bool v) {   // bounded
+            const uint32_t bar = bars + 8 * (2 * ((phase + i) % ST) + v), parity = (phase + i) / ST & 1u;
+            for (uint32_t it = 0; it < p.poll_limit; it++)
+                if (__any_sync(0xffffffffu, bar_try_short(bar, parity))) return true;
+            return false;
+        };
 #pragma unroll
-            for (int k = 0; k < 8; k++) {
-                if constexpr (__is_same(T, __half)) x[k] = ((const T*)&u)[k];
-                else x[k] = __float2half_rn(__bfloat162float(((const T*)&u)[k]));
-            }
+        for (int i = 0; i < ST; i++) {
+            fetch(i, false);
+            fetch(i, true);
         }
-        auto two = [&](int k) { return bits(__halves2half2(x[k], x[k + 4])) ^ a.flip; };
-        *(uint4*)(sq + query_at<D>(r, pc)) = make_uint4(two(0), two(1), two(2), two(3));
-    }
-    __syncthreads();   // queries
+        // queries into shared memory, zero past the tile's rows (after the first copies are under way)
+        uint8_t* sq = sm + C::OFF_Q;
+        for (int i = tid; i < ROWS * (D / 8); i += NW * 32) {
+            const int r = i / (D / 8), pc = i % (D / 8);
+            __half x[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++) x[k] = __float2half_rn(0.0f);
+            if (r < rows) {
+                const int tok = (r0 + r) / a.group, j = (r0 + r) % a.group;
+                const T* src = (const T*)p.q + (int64_t)(row0 + tok) * p.q_stride + (int64_t)(h * a.group + j) * D + pc * 8;
+                uint4 u;
+                if (a.vec_q) {
+                    u = *(const uint4*)src;
+                } else {
+                    T* y = (T*)&u;
+#pragma unroll
+                    for (int k = 0; k < 8; k++) y[k] = src[k];
+                }
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    if constexpr (__is_same(T, __half)) x[k] = ((const T*)&u)[k];
+                    else x[k] = __float2half_rn(__bfloat162float(((const T*)&u)[k]));
+                }
+            }
+            auto two = [&](int k) { return bits(__halves2half2(x[k], x[k + 4])) ^ a.flip; };
+            *(uint4*)(sq + query_at<D>(r, pc)) = make_uint4(two(0), two(1), two(2), two(3));
+        }
+        __syncthreads();   // queries
 
-    // this lane's rows: 2 of every 8 (fragment columns 2 (lane % 4) and the next)
-    const int t4 = lane & 3, col = t4 * 2, kr = lane >> 2;   // kr: the lane's key (or dims) in a fragment
-    int see_lo[NT][2], see_hi[NT][2];
-#pragma unroll
-    for (int b = 0; b < NT; b++)
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-            const int pos = total - n + (r0 + min(rows - 1, b * 8 + col + e)) / a.group;
-            see_hi[b][e] = min(len, pos + 1);
-            see_lo[b][e] = p.window ? pos - p.window + 1 : 0;
-        }
-    float m[NT][2], o[NT][D / 16][4];
-    uint64_t l[NT];   // sums of the weights of two rows
-#pragma unroll
-    for (int b = 0; b < NT; b++) {
-        m[b][0] = m[b][1] = NEG_INF;
-        l[b] = 0;
-#pragma unroll
-        for (int d = 0; d < D / 16; d++) o[b][d][0] = o[b][d][1] = o[b][d][2] = o[b][d][3] = 0.0f;
-    }
-    const uint32_t sqa = smem_addr(sq);
-    // query fragments: in registers where they are few, else read again for every tile
-    constexpr bool QREG = NT * D <= 256;
-    uint32_t qr[QREG ? NT : 1][QREG ? G : 1][4];
-    if constexpr (QREG) {
+        // this lane's rows: 2 of every 8 (fragment columns 2 (lane % 4) and the next)
+        const int t4 = lane & 3, col = t4 * 2, kr = lane >> 2;   // kr: the lane's key (or dims) in a fragment
+        int see_lo[NT][2], see_hi[NT][2];
 #pragma unroll
         for (int b = 0; b < NT; b++)
 #pragma unroll
-            for (int g = 0; g < G; g++) lds<4>(sqa + query_at<D>(b * 8 + kr, g * 4 + t4), qr[b][g]);
-    }
+            for (int e = 0; e < 2; e++) {
+                const int pos = total - n + (r0 + min(rows - 1, b * 8 + col + e)) / a.group;
+                see_hi[b][e] = min(len, pos + 1);
+                see_lo[b][e] = p.window ? pos - p.window + 1 : 0;
+            }
+        float m[NT][2], o[NT][D / 16][4];
+        uint64_t l[NT];   // sums of the weights of two rows
+#pragma unroll
+        for (int b = 0; b < NT; b++) {
+            m[b][0] = m[b][1] = NEG_INF;
+            l[b] = 0;
+#pragma unroll
+            for (int d = 0; d < D / 16; d++) o[b][d][0] = o[b][d][1] = o[b][d][2] = o[b][d][3] = 0.0f;
+        }
+        const uint32_t sqa = smem_addr(sq);
+        // query fragments: in registers where they are few, else read again for every tile
+        constexpr bool QREG = NT * D <= 256;
+        uint32_t qr[QREG ? NT : 1][QREG ? G : 1][4];
+        if constexpr (QREG) {
+#pragma unroll
+            for (int b = 0; b < NT; b++)
+#pragma unroll
+                for (int g = 0; g < G; g++) lds<4>(sqa + query_at<D>(b * 8 + kr, g * 4 + t4), qr[b][g]);
+        }
 
-    for (int i = 0; i < mine; i++) {
-        const int first = key0(i);
-        ok = arrived(i, false);
-        if (!ok) break;
-        const uint32_t kt = ring + 2 * ((phase + i) % ST) * B::BYTES, vt = kt + B::BYTES;
-        const uint32_t ks = kt + B::OFF_SCALES, vs = vt + B::OFF_SCALES;
+        for (int i = 0; i < mine; i++) {
+            const int first = key0(i);
+            ok = arrived(i, false);
+            if (!ok) break;
+            const uint32_t kt = ring + 2 * ((phase + i) % ST) * B::BYTES, vt = kt + B::BYTES;
+            const uint32_t ks = kt + B::OFF_SCALES, vs = vt + B::OFF_SCALES;
 #pragma unroll 1
-        for (int part = 0; part < KT; part += PK) {
-            float sc[NT][PK / 16][4];   // [key kr, + 8][row col, + 1]
+            for (int part = 0; part < KT; part += PK) {
+                float sc[NT][PK / 16][4];   // [key kr, + 8][row col, + 1]
 #pragma unroll
-            for (int j = 0; j < PK / 16; j++) {
-                uint32_t w[2][G];
-                float d[2][G];
+                for (int j = 0; j < PK / 16; j++) {
+                    uint32_t w[2][G];
+                    float d[2][G];
 #pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    const int key = part + j * 16 + kr + 8 * e;
-                    lds<G>(kt + key * B::ROW + t4 * (4 * G), w[e]);
-                    if constexpr (G == 1) {
-                        d[e][0] = __half2float(__ushort_as_half((unsigned short)lds16(ks + key * 2)));
-                    } else {
-                        uint32_t x[G / 2];
-                        lds<G / 2>(ks + key * B::SCALES, x);
-#pragma unroll
-                        for (int g = 0; g < G; g += 2) {
-                            d[e][g] = __low2float(half2_of(x[g / 2]));
-                            d[e][g + 1] = __high2float(half2_of(x[g / 2]));
-                        }
-                    }
-                }
-#pragma unroll
-                for (int g = 0; g < G; g++) {
-                    uint32_t x[4], y[4];
-                    codes(w[0][g], x);
-                    codes(w[1][g], y);
-                    const uint32_t f0[4] = {x[0], y[0], x[1], y[1]}, f1[4] = {x[2], y[2], x[3], y[3]};
-#pragma unroll
-                    for (int b = 0; b < NT; b++) {
-                        uint32_t q[4];
-                        if constexpr (QREG) {
-#pragma unroll
-                            for (int k = 0; k < 4; k++) q[k] = qr[b][g][k];
+                    for (int e = 0; e < 2; e++) {
+                        const int key = part + j * 16 + kr + 8 * e;
+                        lds<G>(kt + key * B::ROW + t4 * (4 * G), w[e]);
+                        if constexpr (G == 1) {
+                            d[e][0] = __half2float(__ushort_as_half((unsigned short)lds16(ks + key * 2)));
                         } else {
-                            lds<4>(sqa + query_at<D>(b * 8 + kr, g * 4 + t4), q);
-                        }
-                        float z[4];
-                        mma0(z, f0, q[0], q[1]);
-                        mma(z, f1, q[2], q[3]);
+                            uint32_t x[G / 2];
+                            lds<G / 2>(ks + key * B::SCALES, x);
 #pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            sc[b][j][e] = g == 0 ? z[e] * d[e >> 1][g] : fmaf(z[e], d[e >> 1][g], sc[b][j][e]);
+                            for (int g = 0; g < G; g += 2) {
+                                d[e][g] = __low2float(half2_of(x[g / 2]));
+                                d[e][g + 1] = __high2float(half2_of(x[g / 2]));
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int g = 0; g < G; g++) {
+                        uint32_t x[4], y[4];
+                        codes(w[0][g], x);
+                        codes(w[1][g], y);
+                        const uint32_t f0[4] = {x[0], y[0], x[1], y[1]}, f1[4] = {x[2], y[2], x[3], y[3]};
+#pragma unroll
+                        for (int b = 0; b < NT; b++) {
+                            uint32_t q[4];
+                            if constexpr (QREG) {
+#pragma unroll
+                                for (int k = 0; k < 4; k++) q[k] = qr[b][g][k];
+                            } else {
+                                lds<4>(sqa + query_at<D>(b * 8 + kr, g * 4 + t4), q);
+                            }
+                            float z[4];
+                            mma0(z, f0, q[0], q[1]);
+                            mma(z, f1, q[2], q[3]);
+#pragma unroll
+                            for (int e = 0; e < 4; e++)
+                                sc[b][j][e] = g == 0 ? z[e] * d[e >> 1][g] : fmaf(z[e], d[e >> 1][g], sc[b][j][e]);
+                        }
                     }
                 }
-            }
-            if (part + PK == KT) {
-                __syncwarp();   // every lane is done with K
-                fetch(i + ST, false);
-            }
-            // keys that a row must not see to -infinity
-            const int k0 = first + part;
-            const bool whole = k0 + PK <= np || (k0 + PK <= min(len, p0 + 1) && (!p.window || k0 > p1 - p.window));
-            if (!whole) {
+                if (part + PK == KT) {
+                    __syncwarp();   // every lane is done with K
+                    fetch(i + ST, false);
+                }
+                // keys that a row must not see to -infinity
+                const int k0 = first + part;
+                const bool whole = k0 + PK <= np || (k0 + PK <= min(len, p0 + 1) && (!p.window || k0 > p1 - p.window));
+                if (!whole) {
 #pragma unroll
-                for (int b = 0; b < NT; b++)
+                    for (int b = 0; b < NT; b++)
+#pragma unroll
+                        for (int j = 0; j < PK / 16; j++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                const int key = k0 + j * 16 + kr + 8 * (e >> 1);
+                                if (!(key < np || (key < see_hi[b][e & 1] && key >= see_lo[b][e & 1]))) sc[b][j][e] = NEG_INF;
+                            }
+                    asm volatile("" ::: "memory");   // keeps the tests out of the tiles that need none
+                }
+#pragma unroll
+                for (int b = 0; b < NT; b++) {
+                    float ref[2];
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        float top = fmaxf(sc[b][0][e], sc[b][0][e + 2]);
+#pragma unroll
+                        for (int j = 1; j < PK / 16; j++) top = fmaxf(top, fmaxf(sc[b][j][e], sc[b][j][e + 2]));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16)) * a.c;   // (log2 units)
+                        if (top > m[b][e]) {
+                            const float f = ex2(m[b][e] - top);
+                            l[b] = fmul2(l[b], e == 0 ? f2pack(f, 1.0f) : f2pack(1.0f, f));
+#pragma unroll
+                            for (int d = 0; d < D / 16; d++) {
+                                o[b][d][e] *= f;
+                                o[b][d][e + 2] *= f;
+                            }
+                            m[b][e] = top;
+                        }
+                        ref[e] = m[b][e] == NEG_INF ? 0.0f : BIAS - m[b][e];
+                    }
+                    const uint64_t c2 = f2pack(a.c, a.c), r2 = f2pack(ref[0], ref[1]);
 #pragma unroll
                     for (int j = 0; j < PK / 16; j++)
 #pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            const int key = k0 + j * 16 + kr + 8 * (e >> 1);
-                            if (!(key < np || (key < see_hi[b][e & 1] && key >= see_lo[b][e & 1]))) sc[b][j][e] = NEG_INF;
+                        for (int g = 0; g < 4; g += 2) {
+                            const uint64_t x = ffma2(f2pack(sc[b][j][g], sc[b][j][g + 1]), c2, r2);
+                            const uint64_t w = f2pack(ex2(f2lo(x)), ex2(f2hi(x)));
+                            sc[b][j][g] = f2lo(w);
+                            sc[b][j][g + 1] = f2hi(w);
+                            l[b] = fadd2(l[b], w);
                         }
-                asm volatile("" ::: "memory");   // keeps the tests out of the tiles that need none
-            }
-#pragma unroll
-            for (int b = 0; b < NT; b++) {
-                float ref[2];
-#pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    float top = fmaxf(sc[b][0][e], sc[b][0][e + 2]);
-#pragma unroll
-                    for (int j = 1; j < PK / 16; j++) top = fmaxf(top, fmaxf(sc[b][j][e], sc[b][j][e + 2]));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16)) * a.c;   // (log2 units)
-                    if (top > m[b][e]) {
-                        const float f = ex2(m[b][e] - top);
-                        l[b] = fmul2(l[b], e == 0 ? f2pack(f, 1.0f) : f2pack(1.0f, f));
-#pragma unroll
-                        for (int d = 0; d < D / 16; d++) {
-                            o[b][d][e] *= f;
-                            o[b][d][e + 2] *= f;
-                        }
-                        m[b][e] = top;
-                    }
-                    ref[e] = m[b][e] == NEG_INF ? 0.0f : BIAS - m[b][e];
                 }
-                const uint64_t c2 = f2pack(a.c, a.c), r2 = f2pack(ref[0], ref[1]);
-#pragma unroll
-                for (int j = 0; j < PK / 16; j++)
-#pragma unroll
-                    for (int g = 0; g < 4; g += 2) {
-                        const uint64_t x = ffma2(f2pack(sc[b][j][g], sc[b][j][g + 1]), c2, r2);
-                        const uint64_t w = f2pack(ex2(f2lo(x)), ex2(f2hi(x)));
-                        sc[b][j][g] = f2lo(w);
-                        sc[b][j][g + 1] = f2hi(w);
-                        l[b] = fadd2(l[b], w);
+                if (part == 0) {
+                    ok = arrived(i, true);
+                    if (!ok) break;
+                    if (first + KT > len) {   // values past the last key become 0 by their scales
+                        for (int x = max(0, len - first) * G + lane; x < KT * G; x += 32)
+                            asm volatile("st.shared.u16 [%0], %1;" ::"r"(vs + x * 2), "h"((uint16_t)0) : "memory");
+                        __syncwarp();
                     }
-            }
-            if (part == 0) {
-                ok = arrived(i, true);
-                if (!ok) break;
-                if (first + KT > len) {   // values past the last key become 0 by their scales
-                    for (int x = max(0, len - first) * G + lane; x < KT * G; x += 32)
-                        asm volatile("st.shared.u16 [%0], %1;" ::"r"(vs + x * 2), "h"((uint16_t)0) : "memory");
-                    __syncwarp();
                 }
-            }
 #pragma unroll
-            for (int j = 0; j < PK / 16; j++) {
-                uint32_t wh[NT][2], wl[NT][2];
+                for (int j = 0; j < PK / 16; j++) {
+                    uint32_t wh[NT][2], wl[NT][2];
 #pragma unroll
-                for (int b = 0; b < NT; b++)
-#pragma unroll
-                    for (int g = 0; g < 2; g++) {
-                        if constexpr (SPLIT) {
-                            uint32_t rest;
-                            wh[b][g] = transpose8(pack_split(sc[b][j][2 * g], sc[b][j][2 * g + 1], rest));
-                            wl[b][g] = transpose8(rest);
-                        } else {
-                            wh[b][g] = transpose8(bits(__floats2half2_rn(sc[b][j][2 * g], sc[b][j][2 * g + 1])));
-                        }
-                    }
-                // values of the lane's D / 8 dims: [key pair: col, col + 8][dim] halves (key, key + 1)
-                uint32_t v[2][D / 8];
-#pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    const int key = part + j * 16 + col + 8 * e;
-                    if constexpr (D == 128) {
-                        uint32_t x[2], y[2], dx[1], dy[1];
-                        lds<2>(vt + key * B::ROW + kr * 8, x);
-                        lds<2>(vt + (key + 1) * B::ROW + kr * 8, y);
-                        lds<1>(vs + key * B::SCALES + (kr & 1) * 4, dx);
-                        lds<1>(vs + (key + 1) * B::SCALES + (kr & 1) * 4, dy);
+                    for (int b = 0; b < NT; b++)
 #pragma unroll
                         for (int g = 0; g < 2; g++) {
-                            const __half2 dd = half2_of(__byte_perm(dx[0], dy[0], g ? 0x7632 : 0x5410));
-                            const __half2 off = __hmul2(dd, __float2half2_rn(-24.0f));
-                            uint32_t lo[4], hi[4];
-                            q4_values(__byte_perm(x[g], y[g], 0x5410), dd, off, lo);
-                            q4_values(__byte_perm(x[g], y[g], 0x7632), dd, off, hi);
-#pragma unroll
-                            for (int k = 0; k < 4; k++) { v[e][g * 8 + k] = lo[k]; v[e][g * 8 + 4 + k] = hi[k]; }
+                            if constexpr (SPLIT) {
+                                uint32_t rest;
+                                wh[b][g] = transpose8(pack_split(sc[b][j][2 * g], sc[b][j][2 * g + 1], rest));
+                                wl[b][g] = transpose8(rest);
+                            } else {
+                                wh[b][g] = transpose8(bits(__floats2half2_rn(sc[b][j][2 * g], sc[b][j][2 * g + 1])));
+                            }
                         }
-                    } else if constexpr (D == 64) {
-                        uint32_t x[1], y[1];
-                        lds<1>(vt + key * B::ROW + kr * 4, x);
-                        lds<1>(vt + (key + 1) * B::ROW + kr * 4, y);
-                        const uint32_t dx = lds16(vs + key * B::SCALES + (kr & 1) * 2);
-                        const uint32_t dy = lds16(vs + (key + 1) * B::SCALES + (kr & 1) * 2);
-                        const __half2 dd = half2_of(dx | dy << 16), off = __hmul2(dd, __float2half2_rn(-24.0f));
-                        uint32_t lo[4], hi[4];
-                        q4_values(__byte_perm(x[0], y[0], 0x5410), dd, off, lo);
-                        q4_values(__byte_perm(x[0], y[0], 0x7632), dd, off, hi);
+                    // values of the lane's D / 8 dims: [key pair: col, col + 8][dim] halves (key, key + 1)
+                    uint32_t v[2][D / 8];
 #pragma unroll
-                        for (int k = 0; k < 4; k++) { v[e][k] = lo[k]; v[e][4 + k] = hi[k]; }
-                    } else {
-                        const uint32_t x = lds16(vt + key * B::ROW + kr * 2), y = lds16(vt + (key + 1) * B::ROW + kr * 2);
-                        uint32_t dx[1], lo[4];
-                        lds<1>(vs + key * B::SCALES, dx);   // (key is even)
-                        const __half2 dd = half2_of(dx[0]), off = __hmul2(dd, __float2half2_rn(-24.0f));
-                        q4_values(x | y << 16, dd, off, lo);
+                    for (int e = 0; e < 2; e++) {
+                        const int key = part + j * 16 + col + 8 * e;
+                        if constexpr (D == 128) {
+                            uint32_t x[2], y[2], dx[1], dy[1];
+                            lds<2>(vt + key * B::ROW + kr * 8, x);
+                            lds<2>(vt + (key + 1) * B::ROW + kr * 8, y);
+                            lds<1>(vs + key * B::SCALES + (kr & 1) * 4, dx);
+                            lds<1>(vs + (key + 1) * B::SCALES + (kr & 1) * 4, dy);
 #pragma unroll
-                        for (int k = 0; k < 4; k++) v[e][k] = lo[k];
+                            for (int g = 0; g < 2; g++) {
+                                const __half2 dd = half2_of(__byte_perm(dx[0], dy[0], g ? 0x7632 : 0x5410));
+                                const __half2 off = __hmul2(dd, __float2half2_rn(-24.0f));
+                                uint32_t lo[4], hi[4];
+                                q4_values(__byte_perm(x[g], y[g], 0x5410), dd, off, lo);
+                                q4_values(__byte_perm(x[g], y[g], 0x7632), dd, off, hi);
+#pragma unroll
+                                for (int k = 0; k < 4; k++) { v[e][g * 8 + k] = lo[k]; v[e][g * 8 + 4 + k] = hi[k]; }
+                            }
+                        } else if constexpr (D == 64) {
+                            uint32_t x[1], y[1];
+                            lds<1>(vt + key * B::ROW + kr * 4, x);
+                            lds<1>(vt + (key + 1) * B::ROW + kr * 4, y);
+                            const uint32_t dx = lds16(vs + key * B::SCALES + (kr & 1) * 2);
+                            const uint32_t dy = lds16(vs + (key + 1) * B::SCALES + (kr & 1) * 2);
+                            const __half2 dd = half2_of(dx | dy << 16), off = __hmul2(dd, __float2half2_rn(-24.0f));
+                            uint32_t lo[4], hi[4];
+                            q4_values(__byte_perm(x[0], y[0], 0x5410), dd, off, lo);
+                            q4_values(__byte_perm(x[0], y[0], 0x7632), dd, off, hi);
+#pragma unroll
+                            for (int k = 0; k < 4; k++) { v[e][k] = lo[k]; v[e][4 + k] = hi[k]; }
+                        } else {
+                            const uint32_t x = lds16(vt + key * B::ROW + kr * 2), y = lds16(vt + (key + 1) * B::ROW + kr * 2);
+                            uint32_t dx[1], lo[4];
+                            lds<1>(vs + key * B::SCALES, dx);   // (key is even)
+                            const __half2 dd = half2_of(dx[0]), off = __hmul2(dd, __float2half2_rn(-24.0f));
+                            q4_values(x | y << 16, dd, off, lo);
+#pragma unroll
+                            for (int k = 0; k < 4; k++) v[e][k] = lo[k];
+                        }
                     }
+#pragma unroll
+                    for (int d = 0; d < D / 16; d++) {
+                        const uint32_t va[4] = {v[0][2 * d], v[0][2 * d + 1], v[1][2 * d], v[1][2 * d + 1]};
+#pragma unroll
+                        for (int b = 0; b < NT; b++) {
+                            if constexpr (SPLIT) mma(o[b][d], va, wl[b][0], wl[b][1]);
+                            mma(o[b][d], va, wh[b][0], wh[b][1]);
+                        }
+                    }
+                }
+            }
+            if (!ok) break;
+            __syncwarp();   // every lane is done with V
+            fetch(i + ST, true);
+        }
+        if (!ok) {   // whatever is on its way lands before the CTA goes on
+            if (lane == 0) atomicOr(p.err, PAGED_WAIT);
+            for (int k = max(0, fetched_k - ST + 1); k <= fetched_k; k++) arrived(k, false);
+            for (int k = max(0, fetched_v - ST + 1); k <= fetched_v; k++) arrived(k, true);
+        }
+        phase += (uint32_t)mine;
+        if (bad && lane == 0) atomicOr(p.err, PAGED_BAD_PAGE);
+        bad = false;
+
+        // join the warps
+        float* ml = (float*)(sm + C::OFF_ML);   // [NW][ROWS] {m, l}
+        float* so = (float*)sm;                 // [NW][ROWS][OSTR]
+        __syncthreads();
+#pragma unroll
+        for (int b = 0; b < NT; b++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                float x = e ? f2hi(l[b]) : f2lo(l[b]);
+                x += __shfl_xor_sync(0xffffffffu, x, 4);
+                x += __shfl_xor_sync(0xffffffffu, x, 8);
+                x += __shfl_xor_sync(0xffffffffu, x, 16);
+                const int r = warp * ROWS + b * 8 + col + e;
+                if (lane < 4) {
+                    ml[2 * r] = m[b][e] - BIAS;   // (what the weights refer to)
+                    ml[2 * r + 1] = x;
                 }
 #pragma unroll
                 for (int d = 0; d < D / 16; d++) {
-                    const uint32_t va[4] = {v[0][2 * d], v[0][2 * d + 1], v[1][2 * d], v[1][2 * d + 1]};
-#pragma unroll
-                    for (int b = 0; b < NT; b++) {
-                        if constexpr (SPLIT) mma(o[b][d], va, wl[b][0], wl[b][1]);
-                        mma(o[b][d], va, wh[b][0], wh[b][1]);
-                    }
+                    so[r * C::OSTR + dim_of<D>(kr, 2 * d)] = o[b][d][e];
+                    so[r * C::OSTR + dim_of<D>(kr, 2 * d + 1)] = o[b][d][e + 2];
                 }
             }
-        }
-        if (!ok) break;
-        __syncwarp();   // every lane is done with V
-        fetch(i + ST, true);
-    }
-    if (!ok) {   // whatever is on its way lands before the CTA goes on
-        if (lane == 0) atomicOr(p.err, PAGED_WAIT);
-        for (int k = max(0, fetched_k - ST + 1); k <= fetched_k; k++) arrived(k, false);
-        for (int k = max(0, fetched_v - ST + 1); k <= fetched_v; k++) arrived(k, true);
-    }
-    phase += (uint32_t)mine;
-    if (bad && lane == 0) atomicOr(p.err, PAGED_BAD_PAGE);
-    bad = false;
-
-    // join the warps
-    float* ml = (float*)(sm + C::OFF_ML);   // [NW][ROWS] {m, l}
-    float* so = (float*)sm;                 // [NW][ROWS][OSTR]
-    __syncthreads();
+        __syncthreads();
+        const int64_t unit = ((int64_t)s * a.tiles + tile) * heads + h;
+        float* part = p.part + (2 * (int64_t)blockIdx.x + ((int)blockIdx.x == first)) * (ROWS * (D + 2));   // [ROWS][D], {m, l}
+        for (int i = tid; i < rows * (D / 4); i += NW * 32) {
+            const int r = i / (D / 4), d = i % (D / 4) * 4;
+            float top = NEG_INF;
 #pragma unroll
-    for (int b = 0; b < NT; b++)
+            for (int w = 0; w < NW; w++) top = fmaxf(top, ml[2 * (w * ROWS + r)]);
+            const float ref = top == NEG_INF ? 0.0f : top;
+            float sum = 0.0f, x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int e = 0; e < 2; e++) {
-            float x = e ? f2hi(l[b]) : f2lo(l[b]);
-            x += __shfl_xor_sync(0xffffffffu, x, 4);
-            x += __shfl_xor_sync(0xffffffffu, x, 8);
-            x += __shfl_xor_sync(0xffffffffu, x, 16);
-            const int r = warp * ROWS + b * 8 + col + e;
-            if (lane < 4) {
-                ml[2 * r] = m[b][e] - BIAS;   // (what the weights refer to)
-                ml[2 * r + 1] = x;
+            for (int w = 0; w < NW; w++) {
+                const float f = ex2(ml[2 * (w * ROWS + r)] - ref);
+                sum = fmaf(f, ml[2 * (w * ROWS + r) + 1], sum);
+                const float4 v = *(const float4*)(so + (w * ROWS + r) * C::OSTR + d);
+                x[0] = fmaf(f, v.x, x[0]); x[1] = fmaf(f, v.y, x[1]);
+                x[2] = fmaf(f, v.z, x[2]); x[3] = fmaf(f, v.w, x[3]);
             }
-#pragma unroll
-            for (int d = 0; d < D / 16; d++) {
-                so[r * C::OSTR + dim_of<D>(kr, 2 * d)] = o[b][d][e];
-                so[r * C::OSTR + dim_of<D>(kr, 2 * d + 1)] = o[b][d][e + 2];
+            if (!DEALT || n_act == 1) {
+                finish<T, D>(p, c, a.vec_out, a.group, h, r, d, top, sum, x);
+            } else {
+                *(float4*)(part + r * D + d) = make_float4(x[0], x[1], x[2], x[3]);
+                if (d == 0) *(float2*)(part + ROWS * D + 2 * r) = make_float2(top, sum);
             }
         }
-    __syncthreads();
-    const int64_t unit = ((int64_t)s * a.tiles + tile) * heads + h;
-    float* part = p.part + (2 * (int64_t)blockIdx.x + ((int)blockIdx.x == first ? 1 : 0)) * (ROWS * (D + 2));   // [ROWS][D], [ROWS] {m, l}
-    for (int i = tid; i < rows * (D / 4); i += NW * 32) {
-        const int r = i / (D / 4), d = i % (D / 4) * 4;
-        float top = NEG_INF;
-#pragma unroll
-        for (int w = 0; w < NW; w++) top = fmaxf(top, ml[2 * (w * ROWS + r)]);
-        const float ref = top == NEG_INF ? 0.0f : top;
-        float sum = 0.0f, x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int w = 0; w < NW; w++) {
-            const float f = ex2(ml[2 * (w * ROWS + r)] - ref);
-            sum = fmaf(f, ml[2 * (w * ROWS + r) + 1], sum);
-            const float4 v = *(const float4*)(so + (w * ROWS + r) * C::OSTR + d);
-            x[0] = fmaf(f, v.x, x[0]); x[1] = fmaf(f, v.y, x[1]);
-            x[2] = fmaf(f, v.z, x[2]); x[3] = fmaf(f, v.w, x[3]);
-        }
-        if (!DEALT || n_act == 1) {
-            finish<T, D>(p, c, a.vec_out, a.group, h, r, d, top, sum, x);
-        } else {
-            *(float4*)(part + r * D + d) = make_float4(x[0], x[1], x[2], x[3]);
-            if (d == 0) *(float2*)(part + ROWS * D + 2 * r) = make_float2(top, sum);
-        }
-    }
-    if (DEALT && ROWS > 8 && v0 == 0 && tid == 0) a.meta[unit] = make_int2(first, n_act);   // (joined by k_join_q4)
-    if (DEALT && ROWS == 8 && n_act > 1) {
-        // The CTA that arrives last joins the unit and clears its counter.
-        __threadfence();
-        __syncthreads();
-        if (tid == 0) last = atomicAdd(p.arrived + unit, 1) == n_act - 1;
-        __syncthreads();
-        if (last) {
+        if (DEALT && ROWS > 8 && v0 == 0 && tid == 0) a.meta[unit] = make_int2(first, n_act);   // (joined by k_join_q4)
+        if (DEALT && ROWS == 8 && n_act > 1) {
+            // The CTA that arrives last joins the unit and clears its counter.
             __threadfence();
-            if (tid == 0) p.arrived[unit] = 0;
-            // thread = four outputs of a row over every ways-th result; where rows and outputs are fewer than the threads, ways
-            // of them share a row's results
-            float* buf = (float*)sm;
-            const int items = rows * (D / 4);
-            int ways = 1;
-            while (ways * 2 * items <= NW * 32 && ways * 2 <= n_act) ways *= 2;
-            for (int i = tid; i < items * ways; i += NW * 32) {
-                const int item = i % items, g = i / items, r = item / (D / 4), d = item % (D / 4) * 4;
-                float top, sum, x[4];
-                sum_parts<D, ROWS>(p.part, first, n_act, g, ways, r, d, top, sum, x);
-                if (ways > 1) {
-                    *(float4*)(buf + 8 * i) = make_float4(x[0], x[1], x[2], x[3]);
-                    *(float2*)(buf + 8 * i + 4) = make_float2(top, sum);
-                } else {
-                    finish<T, D>(p, c, a.vec_out, a.group, h, r, d, top, sum, x);
-                }
-            }
-            if (ways > 1) {   // (items * ways <= the threads)
-                __syncthreads();
-                if (tid < items) {
-                    float top = NEG_INF, sum = 0.0f, x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                    for (int g = 0; g < ways; g++) top = fmaxf(top, buf[8 * (g * items + tid) + 4]);
-                    const float ref = top == NEG_INF ? 0.0f : top;
-                    for (int g = 0; g < ways; g++) {
-                        const float* y = buf + 8 * (g * items + tid);
-                        const float f = ex2(y[4] - ref);
-                        sum = fmaf(f, y[5], sum);
-#pragma unroll
-                        for (int k = 0; k < 4; k++) x[k] = fmaf(f, y[k], x[k]);
+            __syncthreads();
+            if (tid == 0) last = atomicAdd(p.arrived + unit, 1) == n_act - 1;
+            __syncthreads();
+            if (last) {
+                __threadfence();
+                if (tid == 0) p.arrived[unit] = 0;
+                // thread = four outputs of a row over every ways-th result; where rows and outputs are fewer than the threads, ways
+                // of them share a row's results
+                float* buf = (float*)sm;
+                const int items = rows * (D / 4);
+                int ways = 1;
+                while (ways * 2 * items <= NW * 32 && ways * 2 <= n_act) ways *= 2;
+                for (int i = tid; i < items * ways; i += NW * 32) {
+                    const int item = i % items, g = i / items, r = item / (D / 4), d = item % (D / 4) * 4;
+                    float top, sum, x[4];
+                    sum_parts<D, ROWS>(p.part, first, n_act, g, ways, r, d, top, sum, x);
+                    if (ways > 1) {
+                        *(float4*)(buf + 8 * i) = make_float4(x[0], x[1], x[2], x[3]);
+                        *(float2*)(buf + 8 * i + 4) = make_float2(top, sum);
+                    } else {
+                        finish<T, D>(p, c, a.vec_out, a.group, h, r, d, top, sum, x);
                     }
-                    finish<T, D>(p, c, a.vec_out, a.group, h, tid / (D / 4), tid % (D / 4) * 4, top, sum, x);
+                }
+                if (ways > 1) {   // (items * ways <= the threads)
+                    __syncthreads();
+                    if (tid < items) {
+                        float top = NEG_INF, sum = 0.0f, x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        for (int g = 0; g < ways; g++) top = fmaxf(top, buf[8 * (g * items + tid) + 4]);
+                        const float ref = top == NEG_INF ? 0.0f : top;
+                        for (int g = 0; g < ways; g++) {
+                            const float* y = buf + 8 * (g * items + tid);
+                            const float f = ex2(y[4] - ref);
+                            sum = fmaf(f, y[5], sum);
+#pragma unroll
+                            for (int k = 0; k < 4; k++) x[k] = fmaf(f, y[k], x[k]);
+                        }
+                        finish<T, D>(p, c, a.vec_out, a.group, h, tid / (D / 4), tid % (D / 4) * 4, top, sum, x);
+                    }
                 }
             }
         }
-    }
-    if (!DEALT) return;
-    pos += taken;
-    off += taken;
-    if (pos >= end) return;
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // what follows is copied over what was written here
-    __syncthreads();
+        if (!DEALT) return;
+        pos += taken;
+        off += taken;
+        if (pos >= end) return;
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // what follows is copied over what was written here
+        __syncthreads();
     }
 }
 

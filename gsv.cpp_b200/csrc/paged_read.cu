@@ -47,11 +47,10 @@ __global__ void __launch_bounds__(256) k_kv_read(KvReadParams p, int head_lanes)
 #pragma unroll
             for (int b = 0; b < NB; b++) {
                 const TC* src = (const TC*)p.kv.pool + ((w.block + min(h0 + b * head_lanes, 2 * nk - 1)) * PAGE + w.token) * D + e0;
-                TC y[E];
+                struct alignas(E * sizeof(TC)) Run { TC v[E]; };
+                const Run y = *(const Run*)src;
 #pragma unroll
-                for (int i = 0; i < E; i++) y[i] = src[i];
-#pragma unroll
-                for (int i = 0; i < E; i++) x[b][i] = to_f32(y[i]);
+                for (int i = 0; i < E; i++) x[b][i] = to_f32(y.v[i]);
             }
         }
 #pragma unroll
