@@ -739,7 +739,8 @@ ChunkAttnPlan chunk_attention_q4_plan(const ChunkAttnParams& p) {
         c = chunk_attention_tc_plan(p);
         // Many row tiles over the same keys: the keys are unpacked once, by a kernel before it.
         const int group = p.n_q_head / p.kv.n_head;
-        const int64_t rows = p.window ? std::min(packed, (int64_t)p.window * group) : packed, pages = (p.batch.max_kv + PAGE - 1) / PAGE;
+        const int64_t rows = p.window ? std::min(packed, (int64_t)p.window * group) : packed;
+        const int64_t pages = (p.batch.max_kv + PAGE - 1) / PAGE;
         const int64_t bytes = p.batch.n_seq * pages * ((int64_t)p.kv.n_head * (4 * PAGE * D) + 4);
         if (rows >= UNPACK_ROWS && bytes <= UNPACK_LIMIT) {
             c.unpack_pages = (int)pages;

@@ -214,7 +214,9 @@ constexpr __device__ int column(int k) { return !Q4 ? k : k < 4 ? 2 * k : 2 * k 
 template <typename T, bool Q4>
 __device__ __forceinline__ uint4 as_f16(uint4 u) {
     const T* x = (const T*)&u;
-    auto two = [&](int k) { return Q4 ? pack2<__half>((float)x[k], (float)x[k + 4]) : pack2<__half>((float)x[2 * k], (float)x[2 * k + 1]); };
+    auto two = [&](int k) {
+        return Q4 ? pack2<__half>((float)x[k], (float)x[k + 4]) : pack2<__half>((float)x[2 * k], (float)x[2 * k + 1]);
+    };
     return make_uint4(two(0), two(1), two(2), two(3));
 }
 // The unpacking warp's part of a packed tile (two blocks of 64 tokens): 32 of its 128 keys from `first` on, into the

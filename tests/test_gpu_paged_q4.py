@@ -292,7 +292,7 @@ def test_pages_behind_the_window_may_be_gone(ctx, ty, dim, q, prefix):  # noqa: 
     check_attention(c, x, out, None, dim ** -0.5, window, None if prefix is None else [prefix] * 2)
 
 
-@pytest.mark.parametrize("ty,dim,q", [("f16", 32, 1), ("bf16", 128, 5), ("f16", 64, 60), ("bf16", 128, 300)])
+@pytest.mark.parametrize("ty,dim,q", [("f16", 32, 1), ("bf16", 128, 5), ("f16", 64, 60), ("bf16", 128, 300), ("bf16", 64, 800), ("f16", 32, 800)])
 @pytest.mark.parametrize("kv", [70, 5000])
 @pytest.mark.parametrize("bad", [float("nan"), 1e30])
 def test_a_query_of_nan_or_past_the_range_makes_its_row_nan(ctx, ty, dim, q, kv, bad):  # noqa: F811
