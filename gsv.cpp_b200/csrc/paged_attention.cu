@@ -79,11 +79,15 @@ __device__ __forceinline__ void mma8(float (&d)[4], const uint32_t (&a)[4], uint
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 // Two 16-bit values of the type, x in the low half, and what their rounding left over.
+// F16: a score past 2^25 (log2 units) less BIAS is rounded to steps of 4 to 16, and the maximum's weight may then be 2^16:
+// that is 65504, F16's largest, and 32 left over.
 __device__ __forceinline__ uint32_t pack_split(__half, float x, float y, uint32_t& rest) {
-    const __half2 h = __floats2half2_rn(x, y);
+    uint32_t u;
+    asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(u) : "f"(y), "f"(x));
+    const __half2 h = *(const __half2*)&u;
     const __half2 r = __floats2half2_rn(x - __low2float(h), y - __high2float(h));
     rest = *(const uint32_t*)&r;
-    return *(const uint32_t*)&h;
+    return u;
 }
 __device__ __forceinline__ uint32_t pack_split(__nv_bfloat16, float x, float y, uint32_t& rest) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);

@@ -35,7 +35,9 @@ constexpr int NW = 4;            // warps per CTA
 // 16384 keys, 32/8 x 128: 95 us unpacked first, 92 not; 2048: 151 and 170; 4096: 239 and 300; heads of 64: 52 and 50, 79 and 85,
 // 132 and 154.
 constexpr int UNPACK_ROWS = 1536;
-constexpr float BIAS = 14.0f;    // weights are 2^BIAS exp(s - maximum)
+// Weights are 2^BIAS exp(s - maximum). The maximum is taken off first, then the difference scaled: in one step a score past 2^24
+// would be off from its own maximum by whole steps of F32, its weight infinite in F16, or 0.
+constexpr float BIAS = 14.0f;
 constexpr int KT = PAGE;         // keys of one warp's tile: a block of the cache
 // Keys whose scores are held at a time.
 __host__ __device__ constexpr int part_keys(int nt) { return nt == 1 ? 64 : 32; }
@@ -468,9 +470,9 @@ __global__ void __launch_bounds__(NW * 32, resident(D, NT, DEALT)) k_chunk_attn_
                         for (int j = 1; j < PK / 16; j++) top = fmaxf(top, fmaxf(sc[b][j][e], sc[b][j][e + 2]));
                         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
                         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16)) * a.c;   // (log2 units)
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
                         if (top > m[b][e]) {
-                            const float f = ex2(m[b][e] - top);
+                            const float f = ex2((m[b][e] - top) * a.c);
                             l[b] = fmul2(l[b], e == 0 ? f2pack(f, 1.0f) : f2pack(1.0f, f));
 #pragma unroll
                             for (int d = 0; d < D / 16; d++) {
@@ -479,14 +481,14 @@ __global__ void __launch_bounds__(NW * 32, resident(D, NT, DEALT)) k_chunk_attn_
                             }
                             m[b][e] = top;
                         }
-                        ref[e] = m[b][e] == NEG_INF ? 0.0f : BIAS - m[b][e];
+                        ref[e] = m[b][e] == NEG_INF ? 0.0f : -m[b][e];
                     }
-                    const uint64_t c2 = f2pack(a.c, a.c), r2 = f2pack(ref[0], ref[1]);
+                    const uint64_t c2 = f2pack(a.c, a.c), r2 = f2pack(ref[0], ref[1]), up = f2pack(BIAS, BIAS);
 #pragma unroll
                     for (int j = 0; j < PK / 16; j++)
 #pragma unroll
                         for (int g = 0; g < 4; g += 2) {
-                            const uint64_t x = ffma2(f2pack(sc[b][j][g], sc[b][j][g + 1]), c2, r2);
+                            const uint64_t x = ffma2(fadd2(f2pack(sc[b][j][g], sc[b][j][g + 1]), r2), c2, up);
                             const uint64_t w = f2pack(ex2(f2lo(x)), ex2(f2hi(x)));
                             sc[b][j][g] = f2lo(w);
                             sc[b][j][g + 1] = f2hi(w);
@@ -598,7 +600,7 @@ __global__ void __launch_bounds__(NW * 32, resident(D, NT, DEALT)) k_chunk_attn_
                 x += __shfl_xor_sync(0xffffffffu, x, 16);
                 const int r = warp * ROWS + b * 8 + col + e;
                 if (lane < 4) {
-                    ml[2 * r] = m[b][e] - BIAS;   // (what the weights refer to)
+                    ml[2 * r] = m[b][e] * a.c - BIAS;   // (what the weights refer to)
                     ml[2 * r + 1] = x;
                 }
 #pragma unroll

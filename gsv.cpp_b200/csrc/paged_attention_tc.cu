@@ -53,6 +53,10 @@ enum Pages { SAME, PACKED_Q4, AS_F16 };
 // about 1 % over TAU 8 on scores of deviation 1, TAU 1 2 to 7 %.
 template <typename T> constexpr float TAU = __is_same(T, __half) ? 4.0f : 8.0f;
 template <typename T> constexpr float BIAS = __is_same(T, __half) ? 11.0f : 0.0f;
+// References (log2 units) beyond which scores are scaled and rounded, as their maximum was, before the reference is taken off:
+// in one step a score that F32 holds in steps of 2^-7 and more is off from its own maximum, and from 2^27 on its weight could
+// be infinite in F16, or 0.
+constexpr float COARSE = 65536.0f;
 
 template <int D, bool Q4>
 struct Smem {
@@ -670,11 +674,11 @@ __global__ void __launch_bounds__(PG == PACKED_Q4 ? THREADS_Q4 : THREADS, 1) k_c
                     mx[k] = max2(mx[k], __uint_as_float(x[k][31]));
                 }
                 const float top = max2(max2(mx[0], mx[1]), max2(mx[2], mx[3])) * a.c;
-                // Raise the reference maximum of the warp's rows when one of them needs it. A score that is NaN or has
-                // overflowed makes the row's reference NaN, and with it all that the row gives: the polynomial would take the
-                // exponent of such a score for a small one.
-                if (__any_sync(0xffffffffu, !(top <= mref + (TAU<CT> + BIAS<CT>)))) {
-                    float up = max2(mref, top - BIAS<CT>);
+                // Raise the reference maximum of the warp's rows when one of them needs it (rounded so that no weight passes
+                // 2^(TAU + BIAS)). A score that is NaN or has overflowed makes the row's reference NaN, and with it all that the
+                // row gives: the polynomial would take the exponent of such a score for a small one.
+                if (__any_sync(0xffffffffu, !(top <= __fadd_rd(mref, TAU<CT> + BIAS<CT>)))) {
+                    float up = max2(mref, __fsub_ru(top, BIAS<CT>));
                     if (up == -NEG_INF) up = __int_as_float(0x7fffffff);
                     if (j > 0) {
                         // O must be at rest. With two row tiles it is: these scores were issued after the product before
@@ -700,7 +704,16 @@ __global__ void __launch_bounds__(PG == PACKED_Q4 ? THREADS_Q4 : THREADS, 1) k_c
                     mref = up;
                 }
                 const float ref = mref == NEG_INF ? 0.0f : -mref;
-                const uint64_t c2 = f2pack(a.c, a.c), ref2 = f2pack(ref, ref);
+                uint64_t c2 = f2pack(a.c, a.c), ref2 = f2pack(ref, ref);
+                if (__any_sync(0xffffffffu, fabsf(ref) > COARSE)) {
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+#pragma unroll
+                        for (int i = 0; i < 32; i++)
+                            x[k][i] = __float_as_uint(__fadd_rn(__fmul_rn(__uint_as_float(x[k][i]), a.c), ref));
+                    c2 = f2pack(1.0f, 1.0f);
+                    ref2 = 0;
+                }
                 uint64_t sum = 0;   // two partial sums
                 auto weights = [&](auto tested) {
 #pragma unroll

@@ -1,0 +1,67 @@
+"""Chunk attention at the ends of its range, over float and 4-bit caches: scores far above the steps of F32 and queries far
+below those of F16.
+
+Tolerances, set before the first run. u: unit roundoff of the rows' type.
+  large scores   two keys with the same score, all others so far below that their weight is 0: the output is the mean of the
+                 two values, off by a rounding of each weight to the type's bits (u, of the values' magnitudes), one of the
+                 output (u) and F32's sums and quotient (2^-20). The log-sum-exp S + log 2 has a rounding of the scale's
+                 factor, the product, the reference, its sum with the logarithm and the factor log 2: 5 times 2^-24 of S,
+                 rounded up to 2^-21, and 1 for the logarithm.
+"""
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+from test_gpu_paged import PAGE, ROUND, Case, ctx, order  # noqa: E402,F401
+from test_gpu_paged_q4 import Q4Case  # noqa: E402
+
+
+def case(ty, q4, *args, **kw):
+    return (Q4Case if q4 else Case)(ty, *args, **kw)
+
+
+def set_layer(c, v):
+    """The layer's keys and values [page][2][kv head][64][dim]."""
+    if isinstance(c, Q4Case):
+        c.set_values(v)
+    else:
+        c.pool[:, c.layer] = v.to(c.dtype)
+
+
+# ------------------------------------------------------------------ large scores
+
+TYPES = [("f16", False), ("bf16", False), ("f32", False), ("f16", True), ("bf16", True)]
+
+
+@pytest.mark.parametrize("ty,q4", TYPES)
+@pytest.mark.parametrize("dim", [32, 64, 128])
+@pytest.mark.parametrize("q,kv", [(1, 700), (1, 9000), (7, 5000), (14, 70), (60, 900), (60, 9000), (800, 2000)])
+@pytest.mark.parametrize("scale", [1.0, 37.0, 1e12])
+def test_finite_scores_of_any_size(ctx, ty, q4, dim, q, kv, scale):  # noqa: F811
+    """Scores of 2^24 to 2^70, in few rows, in chunks, split and with their pages unpacked first: two keys share the weight,
+    in every row as its own query decides how large they are."""
+    c = case(ty, q4, [q], [kv + q], 2, 1, dim)
+    a, b = 5, kv - 9
+    v = torch.zeros(c.pool.shape[0], 2, 1, PAGE, dim, device="cuda")
+    v[:, 1].normal_(generator=c.gen)
+    for key in (a, b):
+        v[int(c.table[0, key // PAGE]), 0, 0, key % PAGE, 0] = -16384.0
+    set_layer(c, v)
+    x = torch.zeros(q, 2, dim, device="cuda")
+    x[..., 0] = -1024.0 * 2.0 ** (5.0 * torch.rand(q, 2, generator=c.gen, device="cuda"))
+    x = x.bfloat16().to(c.dtype)   # (8 bits: the products are exact in every type)
+    out, lse = torch.empty_like(x), torch.empty(q, 2, device="cuda")
+    cache, chunks = c.objects()
+    order(ctx).op_chunk_attention(cache, chunks, c.layer, x, out, scale=scale, lse=lse)
+    ctx.sync()
+    values = c.keys(0, 0, 1)
+    va, vb = values[a], values[b]
+    u = ROUND[ty]
+    tol = u * ((va + vb) / 2).abs() + (u + 2.0 ** -20) * (va.abs() + vb.abs()) / 2 + (2.0 ** -25 if ty == "f16" else 0.0)
+    score = x[..., 0].double() * -16384.0 * scale
+    assert torch.isfinite(out).all(), (~torch.isfinite(out[..., 0])).sum()
+    err = (out.double() - (va + vb) / 2).abs()
+    assert (err <= tol).all(), float((err / tol).max())
+    assert ((lse.double() - score).abs() <= 2.0 ** -21 * score + 1.0).all()
