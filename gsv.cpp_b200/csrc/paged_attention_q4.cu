@@ -4,7 +4,7 @@
 // k_chunk_attn_q4: the four warps of a CTA take pages of 64 keys in turn, each with its own copies, running maximum, sum and
 // output; transposed products (16 keys x 8 query rows), warps joined in order, what several CTAs share by the last of them or
 // by k_join_q4, in an order that the sizes alone decide. All products are F16 mma.m16n8k16, whatever the rows' type (BF16
-// queries fit F16 up to 65,504; beyond they count as overflowing):
+// queries fit F16 up to 65,504; beyond they count as overflowing; small rows enter scaled by a power of two):
 //   scores   the codes less 8 are exact in F16, and a group of 32 elements is two products, so a group's sum is multiplied
 //            by its key's scale in f32 afterwards;
 //   values   scale * (code - 8) is exact in F16 too (scales have 8 significant bits) and takes one fused multiply-add per
@@ -196,6 +196,7 @@ __global__ void __launch_bounds__(NW * 32, resident(D, NT, DEALT)) k_chunk_attn_
     using C = Cfg<D, NT>;
     using B = Q4Block<D>;
     constexpr int ROWS = C::ROWS, G = D / 32, PK = part_keys(NT), ST = C::STAGES;
+    constexpr bool SCALED = !__is_same(T, __half);   // rows may have a factor of their own
     constexpr bool SPLIT = __is_same(T, __half);   // weights in two F16 parts; BF16 outputs have 8 bits, one part has 11
     extern __shared__ __align__(128) uint8_t sm[];
     __shared__ int64_t sums[NW], found[2];
@@ -330,15 +331,13 @@ __global__ void __launch_bounds__(NW * 32, resident(D, NT, DEALT)) k_chunk_attn_
         }
         // queries into shared memory, zero past the tile's rows (after the first copies are under way)
         uint8_t* sq = sm + C::OFF_Q;
+        float* row_c = (float*)(sm + C::OFF_ML);   // factors of the rows' scores, until the warps are joined
         for (int i = tid; i < ROWS * (D / 8); i += NW * 32) {
             const int r = i / (D / 8), pc = i % (D / 8);
-            __half x[8];
-#pragma unroll
-            for (int k = 0; k < 8; k++) x[k] = __float2half_rn(0.0f);
+            uint4 u = make_uint4(0, 0, 0, 0);
             if (r < rows) {
                 const int tok = (r0 + r) / a.group, j = (r0 + r) % a.group;
                 const T* src = (const T*)p.q + (int64_t)(row0 + tok) * p.q_stride + (int64_t)(h * a.group + j) * D + pc * 8;
-                uint4 u;
                 if (a.vec_q) {
                     u = *(const uint4*)src;
                 } else {
@@ -346,11 +345,21 @@ __global__ void __launch_bounds__(NW * 32, resident(D, NT, DEALT)) k_chunk_attn_
 #pragma unroll
                     for (int k = 0; k < 8; k++) y[k] = src[k];
                 }
-#pragma unroll
-                for (int k = 0; k < 8; k++) {
-                    if constexpr (__is_same(T, __half)) x[k] = ((const T*)&u)[k];
-                    else x[k] = __float2half_rn(__bfloat162float(((const T*)&u)[k]));
+            }
+            __half x[8];
+            if constexpr (SCALED) {   // (every lane of the warp is here: a tile's pieces are a multiple of 32)
+                int up = 0;
+                float f = 1.0f, own = a.c;
+                if (small_queries<D / 8>(u, up)) {
+                    f = power_of_two(up);
+                    own = fmaxf(own * power_of_two(-up), FLT_MIN);
                 }
+                if (pc == 0) row_c[r] = own;
+#pragma unroll
+                for (int k = 0; k < 8; k++) x[k] = __float2half_rn(__bfloat162float(((const T*)&u)[k]) * f);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; k++) x[k] = ((const T*)&u)[k];
             }
             auto two = [&](int k) { return bits(__halves2half2(x[k], x[k + 4])) ^ a.flip; };
             *(uint4*)(sq + query_at<D>(r, pc)) = make_uint4(two(0), two(1), two(2), two(3));
@@ -377,6 +386,11 @@ __global__ void __launch_bounds__(NW * 32, resident(D, NT, DEALT)) k_chunk_attn_
 #pragma unroll
             for (int d = 0; d < D / 16; d++) o[b][d][0] = o[b][d][1] = o[b][d][2] = o[b][d][3] = 0.0f;
         }
+        float cr[NT][2];
+#pragma unroll
+        for (int b = 0; b < NT; b++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) cr[b][e] = SCALED ? row_c[b * 8 + col + e] : a.c;
         const uint32_t sqa = smem_addr(sq);
         // query fragments: in registers where they are few, else read again for every tile
         constexpr bool QREG = NT * D <= 256;
@@ -472,7 +486,7 @@ __global__ void __launch_bounds__(NW * 32, resident(D, NT, DEALT)) k_chunk_attn_
                         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
                         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
                         if (top > m[b][e]) {
-                            const float f = ex2((m[b][e] - top) * a.c);
+                            const float f = ex2((m[b][e] - top) * cr[b][e]);
                             l[b] = fmul2(l[b], e == 0 ? f2pack(f, 1.0f) : f2pack(1.0f, f));
 #pragma unroll
                             for (int d = 0; d < D / 16; d++) {
@@ -483,7 +497,7 @@ __global__ void __launch_bounds__(NW * 32, resident(D, NT, DEALT)) k_chunk_attn_
                         }
                         ref[e] = m[b][e] == NEG_INF ? 0.0f : -m[b][e];
                     }
-                    const uint64_t c2 = f2pack(a.c, a.c), r2 = f2pack(ref[0], ref[1]), up = f2pack(BIAS, BIAS);
+                    const uint64_t c2 = f2pack(cr[b][0], cr[b][1]), r2 = f2pack(ref[0], ref[1]), up = f2pack(BIAS, BIAS);
 #pragma unroll
                     for (int j = 0; j < PK / 16; j++)
 #pragma unroll
@@ -600,7 +614,7 @@ __global__ void __launch_bounds__(NW * 32, resident(D, NT, DEALT)) k_chunk_attn_
                 x += __shfl_xor_sync(0xffffffffu, x, 16);
                 const int r = warp * ROWS + b * 8 + col + e;
                 if (lane < 4) {
-                    ml[2 * r] = m[b][e] * a.c - BIAS;   // (what the weights refer to)
+                    ml[2 * r] = m[b][e] * cr[b][e] - BIAS;   // (what the weights refer to)
                     ml[2 * r + 1] = x;
                 }
 #pragma unroll

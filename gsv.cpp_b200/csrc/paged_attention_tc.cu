@@ -26,12 +26,14 @@
 //
 // 4-bit caches (paged_q4.cuh): the products read F16 (values are exact in it), whatever the rows' type. With many row tiles
 // over the same keys the pages are unpacked to F16 once, by k_unpack_q4, and read as above (2048 rows over 16384 keys, 32/8 x
-// 128 BF16: 442 us, 560 without, the F16 cache 430). Else warp 0 copies the blocks as they lie and warps 12-15 unpack them into
+// 128 BF16: 442 us, 560 without, the F16 cache 430). Small BF16 rows enter scaled by a power of two (paged_q4.cuh), so that a row's
+// scores have a factor of its own, which costs 1 to 2 %. Else warp 0 copies the blocks as they lie and warps 12-15 unpack them into
 // the operand ring, a word of 8 codes to a 16-byte piece; they take issue slots from the softmax, which costs 10 to 30 % (512
 // rows over 8192 keys, 16/4 x 128: 65 us, 57 from F16), but the keys cross HBM at 4.5 bits. A piece's elements lie in the order
 // of the codes; queries are stored in that order, outputs put back.
 #include <cuda_bf16.h>
 
+#include <cfloat>
 #include <type_traits>
 
 #include "paged.h"
@@ -76,7 +78,8 @@ struct Smem {
     // full, empty [NP], S full [2], P full [2][2 halves], PV done [2] (one per row tile; with one row tile, for its key
     // tiles in turn), V landed, V cleared, drain; 4 bits: packed tile landed, unpacked [NS]
     static constexpr int NBAR = 2 * NP + 11 + 2 * NS;
-    static constexpr size_t SMEM = OFF_BAR + NBAR * 8 + 16 + 4 * NS + 1024;
+    static constexpr size_t OFF_C = OFF_BAR + NBAR * 8 + 16 + 4 * NS;   // factors of the rows' scores
+    static constexpr size_t SMEM = OFF_C + 4 * ROWS + 1024;
 };
 
 struct TcArgs {
@@ -214,12 +217,13 @@ __device__ __forceinline__ uint64_t ex2_pair(uint64_t x) {
 // Output column of element k of 8: unpacked values lie as (0, 4), (1, 5), (2, 6), (3, 7).
 template <bool Q4>
 constexpr __device__ int column(int k) { return !Q4 ? k : k < 4 ? 2 * k : 2 * k - 7; }
-// Eight 16-bit elements of T as F16, for unpacked codes in their order: (0, 4), (1, 5), (2, 6), (3, 7).
+// Eight 16-bit elements of T times a power of two as F16, for unpacked codes in their order: (0, 4), (1, 5), (2, 6), (3, 7).
 template <typename T, bool Q4>
-__device__ __forceinline__ uint4 as_f16(uint4 u) {
+__device__ __forceinline__ uint4 as_f16(uint4 u, float f) {
     const T* x = (const T*)&u;
     auto two = [&](int k) {
-        return Q4 ? pack2<__half>((float)x[k], (float)x[k + 4]) : pack2<__half>((float)x[2 * k], (float)x[2 * k + 1]);
+        const int i = Q4 ? k : 2 * k, j = Q4 ? k + 4 : 2 * k + 1;
+        return pack2<__half>((float)x[i] * f, (float)x[j] * f);
     };
     return make_uint4(two(0), two(1), two(2), two(3));
 }
@@ -271,6 +275,7 @@ __global__ void __launch_bounds__(PG == PACKED_Q4 ? THREADS_Q4 : THREADS, 1) k_c
     constexpr bool Q4 = PG == PACKED_Q4;
     using L = Smem<D, Q4>;
     using CT = typename std::conditional<PG == SAME, T, __half>::type;   // what the products read
+    constexpr bool SCALED = !__is_same(T, CT);   // BF16 rows over F16 products: each may have a factor of its own
     constexpr int NT = Q4 ? THREADS_Q4 : THREADS;
     constexpr int TY = __is_same(CT, __half) ? 0 : 1;
     constexpr uint32_t ID_S = instr(TY, 0, KT), ID_O = instr(TY, 1, D);
@@ -290,6 +295,7 @@ __global__ void __launch_bounds__(PG == PACKED_Q4 ? THREADS_Q4 : THREADS, 1) k_c
     uint32_t* tmem_slot = (uint32_t*)(sm + L::OFF_BAR + L::NBAR * 8);
     volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
     int* held_mask = (int*)(tmem_slot + 4);   // [NS] which blocks of a packed tile are there
+    float* row_c = (float*)(sm + L::OFF_C);
 
     int id = blockIdx.x;
     const int sp = id % a.n_split;
@@ -447,7 +453,19 @@ __global__ void __launch_bounds__(PG == PACKED_Q4 ? THREADS_Q4 : THREADS, 1) k_c
         for (int m = 0; m < 4; m++) {
             const int i = i0 + m * STEP, r = i / (D / 8), pc = i % (D / 8);
             if (r >= 128 * halves) break;
-            if constexpr (PG != SAME) u[m] = as_f16<T, Q4>(u[m]);
+            if constexpr (SCALED) {   // (a warp's pieces are of whole rows)
+                int up = 0;
+                float own = a.c;
+                if (small_queries<D / 8>(u[m], up)) {
+                    u[m] = as_f16<T, Q4>(u[m], power_of_two(up));
+                    own = fmaxf(own * power_of_two(-up), FLT_MIN);
+                } else {
+                    u[m] = as_f16<T, Q4>(u[m], 1.0f);
+                }
+                if (pc == 0) row_c[r] = own;
+            } else if constexpr (PG != SAME) {
+                u[m] = as_f16<T, Q4>(u[m], 1.0f);
+            }
             if (a.negate) { u[m].x ^= 0x80008000u; u[m].y ^= 0x80008000u; u[m].z ^= 0x80008000u; u[m].w ^= 0x80008000u; }
             const int rt = r & 127, atom = D >= 64 ? pc / 8 : 0, ch = D >= 64 ? pc % 8 : pc;
             const int swz = L::RB == 128 ? rt & 7 : (rt >> 1) & 3;
@@ -644,6 +662,7 @@ __global__ void __launch_bounds__(PG == PACKED_Q4 ? THREADS_Q4 : THREADS, 1) k_c
                     break;
                 }
                 tc_fence_after();
+                const float cr = SCALED ? ((volatile float*)row_c)[r] : a.c;   // (read for every tile: registers are short)
                 uint32_t x[4][32];
 #pragma unroll
                 for (int k = 0; k < 4; k++) tmem_ld32(ts + 32u * k, x[k]);
@@ -673,7 +692,7 @@ __global__ void __launch_bounds__(PG == PACKED_Q4 ? THREADS_Q4 : THREADS, 1) k_c
                     for (int i = 1; i < 31; i += 2) mx[k] = max3(mx[k], __uint_as_float(x[k][i]), __uint_as_float(x[k][i + 1]));
                     mx[k] = max2(mx[k], __uint_as_float(x[k][31]));
                 }
-                const float top = max2(max2(mx[0], mx[1]), max2(mx[2], mx[3])) * a.c;
+                const float top = max2(max2(mx[0], mx[1]), max2(mx[2], mx[3])) * cr;
                 // Raise the reference maximum of the warp's rows when one of them needs it (rounded so that no weight passes
                 // 2^(TAU + BIAS)). A score that is NaN or has overflowed makes the row's reference NaN, and with it all that the
                 // row gives: the polynomial would take the exponent of such a score for a small one.
@@ -704,13 +723,13 @@ __global__ void __launch_bounds__(PG == PACKED_Q4 ? THREADS_Q4 : THREADS, 1) k_c
                     mref = up;
                 }
                 const float ref = mref == NEG_INF ? 0.0f : -mref;
-                uint64_t c2 = f2pack(a.c, a.c), ref2 = f2pack(ref, ref);
+                uint64_t c2 = f2pack(cr, cr), ref2 = f2pack(ref, ref);
                 if (__any_sync(0xffffffffu, fabsf(ref) > COARSE)) {
 #pragma unroll
                     for (int k = 0; k < 4; k++)
 #pragma unroll
                         for (int i = 0; i < 32; i++)
-                            x[k][i] = __float_as_uint(__fadd_rn(__fmul_rn(__uint_as_float(x[k][i]), a.c), ref));
+                            x[k][i] = __float_as_uint(__fadd_rn(__fmul_rn(__uint_as_float(x[k][i]), cr), ref));
                     c2 = f2pack(1.0f, 1.0f);
                     ref2 = 0;
                 }

@@ -56,6 +56,29 @@ __device__ __forceinline__ uint32_t q4_word(const float* x, float inv) {
     return word - 0xfb000000u;   // 0x4b000000 (1 + 16 + ...), cut to 32 bits
 }
 
+// BF16 query rows whose largest element is below 1/4 enter F16 products times a power of two, which the factor of their scores is
+// divided by: the largest comes to 2^14 .. 2^15, so that elements keep their 8 bits down to 2^-31 of it. As they are they would
+// lose them below 2^-17 and vanish below 2^-25 (2^-23 of the largest in the rows that are left so, the rule).
+// `row`: 8 elements of a row that this lane and its PIECES - 1 neighbours have; all lanes of the warp take part. False: none of the
+// warp's rows is scaled; else `up` is this row's exponent, 0 .. 126.
+template <int PIECES>
+__device__ __forceinline__ bool small_queries(uint4 row, int& up) {
+    constexpr uint32_t QUARTER = 0x3e80u;
+    auto larger = [](uint32_t x, uint32_t y) {   // of each half
+        uint32_t z;
+        asm("max.u16x2 %0, %1, %2;" : "=r"(z) : "r"(x & 0x7fff7fffu), "r"(y & 0x7fff7fffu));
+        return z;
+    };
+    const uint32_t two = larger(larger(row.x, row.y), larger(row.z, row.w));
+    uint32_t m = max(two & 0xffffu, two >> 16);
+    if (!__any_sync(0xffffffffu, m > 0 && m < QUARTER)) return false;
+#pragma unroll
+    for (int o = 1; o < PIECES; o *= 2) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    up = m == 0 || m >= QUARTER ? 0 : min(126, 141 - (int)(m >> 7));   // (bits from 7 on: the exponent, 127 for 2^0)
+    return true;
+}
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }   // -126 .. 127
+
 __device__ __forceinline__ uint32_t bits(__half2 h) { return *(const uint32_t*)&h; }
 __device__ __forceinline__ __half2 half2_of(uint32_t u) { return *(const __half2*)&u; }
 // (x & mask) | bits

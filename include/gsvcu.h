@@ -355,7 +355,7 @@ int gsvcu_op_kv_read(gsvcu_ctx* ctx, const gsvcu_kv_read* a);
  * A row that sees no key gives 0 and -infinity. Scores, softmax and sums are F32, exponentials within 2.7e-6; with more
  * than 32 rows times query heads of a kv head the weights are rounded to the cache's type for the product with the values
  * (F16: 11 bits down to 2^-25 of the row's largest, none below 2^-36). 4-bit caches are read exactly and multiplied in F16:
- * BF16 queries beyond 65,504 count as overflowing, weights have 11 bits (F16 rows of up to 32 22) and none is below 2^-39
+ * BF16 queries beyond 65,504 count as overflowing, elements below 2^-23 of their row's largest as 0; weights have 11 bits (F16 rows of up to 32 22) and none is below 2^-39
  * (more than 32: 2^-36) of the row's largest. From 1536 rows times query heads of a kv head on, their pages are unpacked into
  * scratch of the context first, at most 2 GB a call (n_seq * max_kv tokens of all kv heads at 16 bits; what would take more is
  * read as it is). What the pages hold from kv_len on does not

@@ -15,7 +15,7 @@ pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
 
 from test_gpu_paged import PAGE, ROUND, Case, ctx, order  # noqa: E402,F401
-from test_gpu_paged_q4 import Q4Case  # noqa: E402
+from test_gpu_paged_q4 import Q4Case, attend  # noqa: E402
 
 
 def case(ty, q4, *args, **kw):
@@ -65,3 +65,32 @@ def test_finite_scores_of_any_size(ctx, ty, q4, dim, q, kv, scale):  # noqa: F81
     err = (out.double() - (va + vb) / 2).abs()
     assert (err <= tol).all(), float((err / tol).max())
     assert ((lse.double() - score).abs() <= 2.0 ** -21 * score + 1.0).all()
+
+
+# ------------------------------------------------------------------ small queries
+
+@pytest.mark.parametrize("dim", [32, 64, 128])
+@pytest.mark.parametrize("heads,kv_heads,q,kv", [(16, 4, 1, 900), (8, 1, 1, 9000), (8, 2, 4, 700), (8, 2, 40, 900), (8, 1, 130, 300), (8, 1, 260, 900)])
+@pytest.mark.parametrize("size", [2.0 ** -20, 2.0 ** -40, 2.0 ** -126, 2.0 ** -132, 1.0])
+def test_bf16_queries_of_any_size(ctx, dim, heads, kv_heads, q, kv, size):  # noqa: F811
+    """BF16 queries below F16's range with a scale that makes up for them, over 4 bits: in few rows, in chunks and with the
+    pages unpacked first. Rows of one tile differ by 2^10, one is 0, and one has an element that outweighs its others by
+    2^12. The tolerances are the usual ones: nothing of a query is lost."""
+    c = Q4Case("bf16", [q, 1, q], [kv + q, 90, kv + 3], heads, kv_heads, dim)
+    x = torch.randn(c.rows, heads, dim, generator=c.gen, device="cuda")
+    x *= 2.0 ** -(torch.arange(c.rows * heads, device="cuda") % 11).float().view(c.rows, heads, 1)
+    x[c.rows // 2, heads // 2] = 0.0
+    x[0, heads - 1, 1:] *= 2.0 ** -12
+    x = (x.bfloat16().double() * size).bfloat16()
+    cut = 126 if size < 2.0 ** -126 else 0   # (the scale is at most 1e38)
+    attend(ctx, c, q=x, scale=(1.0 / size if not cut else 2.0 ** cut) * dim ** -0.5)
+
+
+@pytest.mark.parametrize("q", [1, 9, 60, 800])
+def test_bf16_queries_of_any_size_with_a_negative_scale_and_masks(ctx, q):  # noqa: F811
+    c = Q4Case("bf16", [q, 3], [q + 900, 70], 2, 1, 64)
+    x = (c.rand(c.rows, 2, 64).double() * 2.0 ** -50).bfloat16()
+    attend(ctx, c, q=x, scale=-0.125 * 2.0 ** 50)
+    attend(ctx, c, q=x, scale=0.125 * 2.0 ** 50, window=100, prefix=[70, 3])
+    attend(ctx, c, q=x, scale=0.0)
+    attend(ctx, c, q=x, scale=1e-38)   # (scores far below 1: every key weighs the same)
