@@ -433,6 +433,7 @@ struct gsvcu_ctx {
     size_t op_arrived_n = 0;
     void* op_unpacked = nullptr;      // its pages of 4-bit caches as F16
     size_t op_unpacked_n = 0;
+    size_t op_unpacked_denied = SIZE_MAX;   // the size from which there was no memory for it
     std::vector<void*> op_outgrown;   // what these three outgrew, kept for captured graphs until the context ends
     uint64_t op_chunk_ready[2] = {0, 0};   // its kernels whose shared-memory limit is raised
     // set when a bounded wait in a kernel gave up: [0] decode attention in the decode steps (read and
@@ -442,6 +443,7 @@ struct gsvcu_ctx {
     int32_t* att_err = nullptr;
     // test-only fault injection (gsvcu_set_wait_fault): extra bytes each K/V page wait expects, poll limit
     uint32_t fault_extra_tx = 0, fault_poll_limit = 0;
+    bool fault_memory = false;   // (gsvcu_set_memory_fault) chunk attention finds no memory for scratch
     // prefill GEMMs of Q8_0 matrices on the tcgen05 tensor cores (gemm_tc.cu) from TC_MIN_ROWS rows on
     // (gsvcu_set_prefill_gemm; the default: measured on B200 1.4x faster than the mma.sync tiles at 4096
     // rows); a16: the scratch of its activation side
@@ -1969,17 +1971,22 @@ int gsvcu_op_chunk_attention(gsvcu_ctx* ctx, const gsvcu_chunk_attention* a) {
     // Scratch at least doubles when it grows, and what it replaces stays until the context ends: captured graphs
     // may hold its address. It does not grow in a capture: the zeros of the counters would only be recorded, and calls
     // outside the graph would find none.
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
     auto grow = [&](void** at, size_t* have, size_t need, bool zero, size_t most) -> int {   // (4-byte words)
         if (need <= *have) return GSVCU_OK;
-        cudaStreamCaptureStatus capture;
         CKC(ctx, cudaStreamIsCapturing(ctx->stream, &capture));
         if (capture != cudaStreamCaptureStatusNone)
             return ctx->fail(GSVCU_ERR_STATE, "gsvcu_op_chunk_attention: run these sizes once before they are captured");
-        const size_t n = std::max(need, std::min(2 * *have, most));
+        size_t n = std::max(need, std::min(2 * *have, most));
         void* fresh = nullptr;
-        if (cudaMalloc(&fresh, n * 4) != cudaSuccess) {
+        auto allocate = [&] { return !ctx->fault_memory && cudaMalloc(&fresh, n * 4) == cudaSuccess; };
+        if (!allocate()) {
             cudaGetLastError();
-            return ctx->fail(GSVCU_ERR_OOM, "gsvcu_op_chunk_attention: no memory for its scratch");
+            n = need;
+            if (!allocate()) {
+                cudaGetLastError();
+                return ctx->fail(GSVCU_ERR_OOM, "gsvcu_op_chunk_attention: no memory for its scratch");
+            }
         }
         if (zero) {
             const cudaError_t e = cudaMemsetAsync(fresh, 0, n * 4, ctx->stream);
@@ -1995,9 +2002,18 @@ int gsvcu_op_chunk_attention(gsvcu_ctx* ctx, const gsvcu_chunk_attention* a) {
     };
     TRY(grow((void**)&ctx->op_split, &ctx->op_split_n, plan.part_floats, false, SIZE_MAX));
     TRY(grow((void**)&ctx->op_arrived, &ctx->op_arrived_n, plan.arrivals, true, SIZE_MAX));
-    const int rc = grow(&ctx->op_unpacked, &ctx->op_unpacked_n, plan.unpacked_floats, false, UNPACK_LIMIT / 4);
-    if (rc == GSVCU_ERR_OOM) plan.unpack_pages = 0;   // (the kernel can do without)
-    else if (rc != GSVCU_OK) return rc;
+    // The kernel can do without unpacked pages. Sizes that found no memory for them do from then on, so that a call is not tried
+    // again and again, can be captured once it has run, and sums in one order.
+    if (plan.unpacked_floats >= ctx->op_unpacked_denied) plan.unpack_pages = 0;
+    if (plan.unpack_pages) {
+        const int rc = grow(&ctx->op_unpacked, &ctx->op_unpacked_n, plan.unpacked_floats, false, UNPACK_LIMIT / 4);
+        if (rc == GSVCU_ERR_OOM) {
+            ctx->op_unpacked_denied = plan.unpacked_floats;
+            plan.unpack_pages = 0;
+        } else if (rc != GSVCU_OK) {
+            return rc;
+        }
+    }
     p.part = ctx->op_split;
     p.arrived = ctx->op_arrived;
     p.unpacked = ctx->op_unpacked;   // the pages, then their table
@@ -2192,6 +2208,12 @@ int gsvcu_set_wait_fault(gsvcu_ctx* ctx, int32_t on) {
     ctx->drop_graphs();   // captured steps hold the launch parameters
     ctx->fault_extra_tx = on ? 16u : 0u;
     ctx->fault_poll_limit = on ? 4096u : 0u;
+    return GSVCU_OK;
+}
+
+int gsvcu_set_memory_fault(gsvcu_ctx* ctx, int32_t on) {
+    if (!ctx || on < 0 || on > 1) return GSVCU_ERR_ARG;
+    ctx->fault_memory = on != 0;
     return GSVCU_OK;
 }
 

@@ -128,6 +128,7 @@ SIGNATURES = {
     "gsvcu_set_serve_lookahead": ([_P, _I], C.c_int),
     "gsvcu_fused_decode": ([_P], C.c_int),
     "gsvcu_set_wait_fault": ([_P, _I], C.c_int),
+    "gsvcu_set_memory_fault": ([_P, _I], C.c_int),
     "gsvcu_set_prefill_gemm": ([_P, _I], C.c_int),
     "gsvcu_op_q8_gemm_tc": ([_P, _P, _P, _I, _P, _P, _I, _I, _P, _P, _I, _P, _P, _P], C.c_int),
     "gsvcu_op_kv_append": ([_P, C.POINTER(KvAppendArgs)], C.c_int),
@@ -501,6 +502,10 @@ class Context:
     def set_wait_fault(self, on):
         """Test-only: make this context's decode- and chunk-attention page waits run out (gsvcu_set_wait_fault)."""
         self._check(self.lib.gsvcu_set_wait_fault(self.h, 1 if on else 0))
+
+    def set_memory_fault(self, on):
+        """Test-only: make chunk attention find no memory for new scratch (gsvcu_set_memory_fault)."""
+        self._check(self.lib.gsvcu_set_memory_fault(self.h, 1 if on else 0))
 
     def stream_handle(self):
         return int(self.lib.gsvcu_stream(self.h) or 0)

@@ -355,13 +355,14 @@ int gsvcu_op_kv_read(gsvcu_ctx* ctx, const gsvcu_kv_read* a);
  * A row that sees no key gives 0 and -infinity. Scores, softmax and sums are F32, exponentials within 2.7e-6; with more
  * than 32 rows times query heads of a kv head the weights are rounded to the cache's type for the product with the values
  * (F16: 11 bits down to 2^-25 of the row's largest, none below 2^-36). 4-bit caches are read exactly and multiplied in F16:
- * BF16 queries beyond 65,504 count as overflowing, elements below 2^-23 of their row's largest as 0; weights have 11 bits (F16 rows of up to 32 22) and none is below 2^-39
- * (more than 32: 2^-36) of the row's largest. From 1536 rows times query heads of a kv head on, their pages are unpacked into
- * scratch of the context first, at most 2 GB a call (n_seq * max_kv tokens of all kv heads at 16 bits; what would take more is
- * read as it is). What the pages hold from kv_len on does not
- * matter, nor do pages that no row sees; in the other pages every key and value has to be finite (a value that is not
- * reaches rows that do not see it, as 0 times infinity) and in F32 below 2^128 - 2^115. A row with a score that is NaN
- * or overflows to infinity is NaN, a score of minus infinity has weight 0 (F32 caches: NaN too); |scale| at most 1e38. */
+ * BF16 queries beyond 65,504 count as overflowing, elements below 2^-23 of their row's largest as 0; weights have 11 bits
+ * (F16 rows of up to 32 22) and none is below 2^-39 (more than 32: 2^-36) of the row's largest. From 1536 rows times query
+ * heads of a kv head on, their pages are unpacked into scratch of the context first, at most 2 GB a call (n_seq * max_kv
+ * tokens of all kv heads at 16 bits). What would take more is read as it is; so is, from then on, what found no memory and
+ * all that would take as much. What the pages hold from kv_len on does not matter, nor do pages that no row sees; in the
+ * other pages every key and value has to be finite (a value that is not reaches rows that do not see it, as 0 times infinity)
+ * and in F32 below 2^128 - 2^115. A row with a score that is NaN or overflows to infinity is NaN, a score of minus infinity
+ * has weight 0 (F32 caches: NaN too); |scale| at most 1e38. */
 typedef struct {
     const gsvcu_paged_kv* kv;
     const gsvcu_chunk_batch* batch;
@@ -543,6 +544,9 @@ int gsvcu_sync(gsvcu_ctx* ctx);
  * with many rows, and over 4-bit caches (from the second copies on, "a bounded wait gave up"). on = 0 (default) restores normal
  * operation. */
 int gsvcu_set_wait_fault(gsvcu_ctx* ctx, int32_t on);
+/* The same for memory: with on = 1 gsvcu_op_chunk_attention finds no device memory for scratch that it does not have yet.
+ * It returns GSVCU_ERR_OOM and does nothing, or reads a 4-bit cache as it is. on = 0 (default): normal operation. */
+int gsvcu_set_memory_fault(gsvcu_ctx* ctx, int32_t on);
 
 #ifdef __cplusplus
 }

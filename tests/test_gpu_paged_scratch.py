@@ -1,0 +1,83 @@
+"""The scratch of chunk attention when memory is short: a call that needs it says so, one that can do without it does, from then
+on in the same way, and can be captured."""
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+import test_gpu_paged as floats  # noqa: E402
+from test_gpu_paged import Case, order  # noqa: E402
+from test_gpu_paged_q4 import Q4Case, attend, check_attention  # noqa: E402
+
+
+@pytest.fixture()
+def own():
+    import gsvcu
+    c = gsvcu.Context(0)
+    yield c
+    c.close()
+
+
+@pytest.mark.parametrize("ty", ["f16", "bf16"])
+def test_without_memory_for_unpacked_pages_the_4_bits_are_read(own, ty):
+    """Long chunks whose pages would be unpacked first: right without the memory for it, the same bits every time, in a captured
+    graph too, and also after there is memory again; smaller calls are unpacked then."""
+    import gsvcu
+    c = Q4Case(ty, [400] * 12, [1500] * 12, 16, 4, 64)   # (336 CTAs: no splits, so the unpacked pages are all the scratch)
+    other = gsvcu.Context(0)
+    x, unpacked, _ = attend(other, c)
+    kernels = [0, 0]
+    for i, ctx in enumerate((own, other)):
+        if ctx is own:
+            own.set_memory_fault(True)
+        before = ctx.kernel_launches()
+        _, first, _ = attend(ctx, c, q=x)
+        kernels[i] = ctx.kernel_launches() - before
+        if ctx is own:
+            a = first
+    assert kernels == [1, 2]
+    assert torch.equal(attend(own, c, q=x)[1], a)
+    cache, chunks = c.objects()
+    out = torch.empty_like(x)
+    stream = torch.cuda.ExternalStream(own.stream_handle())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        own.op_chunk_attention(cache, chunks, c.layer, x, out)
+    own.set_memory_fault(False)
+    for _ in range(2):
+        out.fill_(float("nan"))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            graph.replay()
+        own.sync()
+        assert torch.equal(out, a)
+    check_attention(c, x, out, None, 0.125)
+    assert torch.equal(attend(own, c, q=x)[1], a)
+    small = Q4Case(ty, [400] * 8, [900] * 8, 16, 4, 64, seed=1)
+    before = own.kernel_launches()
+    y, b, _ = attend(own, small)
+    assert own.kernel_launches() - before == 2
+    assert torch.equal(attend(other, small, q=y)[1], b)
+    del graph
+    other.close()
+
+
+@pytest.mark.parametrize("q4", [False, True])
+@pytest.mark.parametrize("q", [1, 60])
+def test_split_results_without_memory_are_refused(own, q4, q):
+    import gsvcu
+    c = (Q4Case if q4 else Case)("f16", [q], [9000 + q], 8, 2, 64)
+    x = c.rand(q, 8, 64)
+    out = torch.full_like(x, 7.0)
+    cache, chunks = c.objects()
+    own.set_memory_fault(True)
+    for _ in range(2):
+        with pytest.raises(gsvcu.GsvcuError) as e:
+            order(own).op_chunk_attention(cache, chunks, c.layer, x, out)
+        assert e.value.code == -3 and "memory" in str(e.value)
+    own.sync()
+    assert (out == 7.0).all()
+    own.set_memory_fault(False)
+    (attend if q4 else floats.attend)(own, c, q=x)
