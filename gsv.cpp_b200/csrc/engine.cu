@@ -433,6 +433,7 @@ struct gsvcu_ctx {
     size_t op_arrived_n = 0;
     void* op_unpacked = nullptr;      // its pages of 4-bit caches as F16
     size_t op_unpacked_n = 0;
+    bool op_unpacked_captured = false;   // a captured graph may hold its address
     size_t op_unpacked_denied = SIZE_MAX;   // the size from which there was no memory for it
     std::vector<void*> op_outgrown;   // what these three outgrew, kept for captured graphs until the context ends
     uint64_t op_chunk_ready[2] = {0, 0};   // its kernels whose shared-memory limit is raised
@@ -1969,10 +1970,10 @@ int gsvcu_op_chunk_attention(gsvcu_ctx* ctx, const gsvcu_chunk_attention* a) {
         return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_chunk_attention: batch too large for one launch");
     DeviceGuard g(ctx->device);
     // Scratch at least doubles when it grows, and what it replaces stays until the context ends: captured graphs
-    // may hold its address. It does not grow in a capture: the zeros of the counters would only be recorded, and calls
+    // may hold its address (unpacked pages, which are large, go when no capture has seen them). It does not grow in a capture: the zeros of the counters would only be recorded, and calls
     // outside the graph would find none.
     cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
-    auto grow = [&](void** at, size_t* have, size_t need, bool zero, size_t most) -> int {   // (4-byte words)
+    auto grow = [&](void** at, size_t* have, size_t need, bool zero, size_t most, bool keep) -> int {   // (4-byte words)
         if (need <= *have) return GSVCU_OK;
         CKC(ctx, cudaStreamIsCapturing(ctx->stream, &capture));
         if (capture != cudaStreamCaptureStatusNone)
@@ -1995,23 +1996,38 @@ int gsvcu_op_chunk_attention(gsvcu_ctx* ctx, const gsvcu_chunk_attention* a) {
                 return ctx->fail(GSVCU_ERR_CUDA, cudaGetErrorString(e));
             }
         }
-        if (*at) ctx->op_outgrown.push_back(*at);
+        if (*at && keep) {
+            ctx->op_outgrown.push_back(*at);
+        } else if (*at) {
+            const cudaError_t e = cudaStreamSynchronize(ctx->stream);
+            if (e != cudaSuccess) {
+                cudaFree(fresh);
+                return ctx->fail(GSVCU_ERR_CUDA, cudaGetErrorString(e));
+            }
+            cudaFree(*at);
+        }
         *at = fresh;
         *have = n;
         return GSVCU_OK;
     };
-    TRY(grow((void**)&ctx->op_split, &ctx->op_split_n, plan.part_floats, false, SIZE_MAX));
-    TRY(grow((void**)&ctx->op_arrived, &ctx->op_arrived_n, plan.arrivals, true, SIZE_MAX));
+    TRY(grow((void**)&ctx->op_split, &ctx->op_split_n, plan.part_floats, false, SIZE_MAX, true));
+    TRY(grow((void**)&ctx->op_arrived, &ctx->op_arrived_n, plan.arrivals, true, SIZE_MAX, true));
     // The kernel can do without unpacked pages. Sizes that found no memory for them do from then on, so that a call is not tried
     // again and again, can be captured once it has run, and sums in one order.
     if (plan.unpacked_floats >= ctx->op_unpacked_denied) plan.unpack_pages = 0;
     if (plan.unpack_pages) {
-        const int rc = grow(&ctx->op_unpacked, &ctx->op_unpacked_n, plan.unpacked_floats, false, UNPACK_LIMIT / 4);
+        const void* before = ctx->op_unpacked;
+        const int rc = grow(&ctx->op_unpacked, &ctx->op_unpacked_n, plan.unpacked_floats, false, UNPACK_LIMIT / 4,
+                            ctx->op_unpacked_captured);
+        if (ctx->op_unpacked != before) ctx->op_unpacked_captured = false;
         if (rc == GSVCU_ERR_OOM) {
             ctx->op_unpacked_denied = plan.unpacked_floats;
             plan.unpack_pages = 0;
         } else if (rc != GSVCU_OK) {
             return rc;
+        } else {
+            CKC(ctx, cudaStreamIsCapturing(ctx->stream, &capture));
+            ctx->op_unpacked_captured |= capture != cudaStreamCaptureStatusNone;
         }
     }
     p.part = ctx->op_split;

@@ -7,7 +7,7 @@ pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
 
 import test_gpu_paged as floats  # noqa: E402
-from test_gpu_paged import Case, order  # noqa: E402
+from test_gpu_paged import PAGE, Case, order  # noqa: E402
 from test_gpu_paged_q4 import Q4Case, attend, check_attention  # noqa: E402
 
 
@@ -81,3 +81,38 @@ def test_split_results_without_memory_are_refused(own, q4, q):
     assert (out == 7.0).all()
     own.set_memory_fault(False)
     (attend if q4 else floats.attend)(own, c, q=x)
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_outgrown_unpacked_pages_are_freed_unless_a_graph_may_use_them(own, captured):
+    """Calls that need 105, 236 and 524 MB for unpacked pages (the table's length bounds it) hold what the last one needs, and
+    before that only what a graph was captured with, whose replays stay right."""
+    c = Q4Case("bf16", [400], [1500], 32, 8, 128, max_pages=400)
+    table = c.table.clone()
+    x, first, _ = attend(own, c)
+    cache, chunks = c.objects()
+    out = torch.empty_like(x)
+    stream = torch.cuda.ExternalStream(own.stream_handle())
+    torch.cuda.synchronize()
+    if captured:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            own.op_chunk_attention(cache, chunks, c.layer, x, out)
+    free, reserved = torch.cuda.mem_get_info()[0], torch.cuda.memory_reserved()
+    for pages in (900, 2000):
+        c.table = torch.full((1, pages), 2 ** 30, dtype=torch.int32, device="cuda")
+        c.table[:, :400] = table
+        attend(own, c, q=x)
+        attend(own, c, q=x)
+    grown = free - torch.cuda.mem_get_info()[0] - (torch.cuda.memory_reserved() - reserved)
+    block = 400 * 8 * 4 * PAGE * 128   # bytes of the first
+    want = block * 5 - (0 if captured else block)
+    assert abs(grown - want) < block // 2, (grown, want)   # (splits: up to 40 MB)
+    if captured:
+        out.fill_(float("nan"))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            graph.replay()
+        own.sync()
+        assert torch.equal(out, first)
+        del graph
