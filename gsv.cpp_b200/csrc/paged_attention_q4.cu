@@ -35,6 +35,9 @@ constexpr int NW = 4;            // warps per CTA
 // 16384 keys, 32/8 x 128: 95 us unpacked first, 92 not; 2048: 151 and 170; 4096: 239 and 300; heads of 64: 52 and 50, 79 and 85,
 // 132 and 154.
 constexpr int UNPACK_ROWS = 1536;
+// And the mean over the sequences of a call. 32/8 x 128, 8192 keys each, unpacked first and not: a chunk of 512 tokens and 32
+// single ones 555 and 422 us; 512 and 4: 170 and 160; 512 and 2: 152 and 158; 512, 100, 100, 100: 168 and 168; 1024 and 8: 283 and 297.
+constexpr int UNPACK_MEAN = 512;
 // Weights are 2^BIAS exp(s - maximum). The maximum is taken off first, then the difference scaled: in one step a score past 2^24
 // would be off from its own maximum by whole steps of F32, its weight infinite in F16, or 0.
 constexpr float BIAS = 14.0f;
@@ -753,12 +756,14 @@ ChunkAttnPlan chunk_attention_q4_plan(const ChunkAttnParams& p) {
     ChunkAttnPlan c;
     if (packed > 32 && p.scale != 0.0f) {
         c = chunk_attention_tc_plan(p);
-        // Many row tiles over the same keys: the keys are unpacked once, by a kernel before it.
+        // Many row tiles over the same keys: the keys are unpacked once, by a kernel before it. All sequences' keys are, so it
+        // takes some rows of each that has any (at most 1 + n_rows - max_chunk beside idle ones).
         const int group = p.n_q_head / p.kv.n_head;
-        const int64_t rows = p.window ? std::min(packed, (int64_t)p.window * group) : packed;
+        const int64_t active = std::min<int64_t>(p.batch.n_seq, 1 + p.batch.n_rows - p.batch.max_chunk);
+        auto rows = [&](int64_t tokens) { return group * (p.window ? std::min<int64_t>(tokens, p.window) : tokens); };
         const int64_t pages = (p.batch.max_kv + PAGE - 1) / PAGE;
         const int64_t bytes = p.batch.n_seq * pages * ((int64_t)p.kv.n_head * (4 * PAGE * D) + 4);
-        if (rows >= UNPACK_ROWS && bytes <= UNPACK_LIMIT) {
+        if (rows(p.batch.max_chunk) >= UNPACK_ROWS && rows(p.batch.n_rows / active) >= UNPACK_MEAN && bytes <= UNPACK_LIMIT) {
             c.unpack_pages = (int)pages;
             c.unpacked_floats = (size_t)(bytes / 4);
         }

@@ -356,14 +356,14 @@ int gsvcu_op_kv_read(gsvcu_ctx* ctx, const gsvcu_kv_read* a);
  * than 32 rows times query heads of a kv head the weights are rounded to the cache's type for the product with the values
  * (F16: 11 bits down to 2^-25 of the row's largest, none below 2^-36). 4-bit caches are read exactly and multiplied in F16:
  * BF16 queries beyond 65,504 count as overflowing, elements below 2^-23 of their row's largest as 0; weights have 11 bits
- * (F16 rows of up to 32 22) and none is below 2^-39 (more than 32: 2^-36) of the row's largest. From 1536 rows times query
- * heads of a kv head on, their pages are unpacked into scratch of the context first, at most 2 GB a call (n_seq * max_kv
- * tokens of all kv heads at 16 bits). What would take more is read as it is; so is, from then on, what found no memory and
- * all that would take as much. The scratch stays with the context; outgrown, it is freed unless a graph was captured
- * with it. What the pages hold from kv_len on does not matter, nor do pages that no row sees; in the
- * other pages every key and value has to be finite (a value that is not reaches rows that do not see it, as 0 times infinity)
- * and in F32 below 2^128 - 2^115. A row with a score that is NaN or overflows to infinity is NaN, a score of minus infinity
- * has weight 0 (F32 caches: NaN too); |scale| at most 1e38. */
+ * (F16 rows of up to 32 22) and none is below 2^-39 (more than 32: 2^-36) of the row's largest. Where the longest chunk has
+ * 1536 rows times query heads of a kv head or more, and the sequences with rows 512 on average, all their pages are unpacked
+ * into scratch of the context first, at most 2 GB a call (n_seq * max_kv tokens of all kv heads at 16 bits). What would take
+ * more is read as it is; so is, from then on, what found no memory and all that would take as much. The scratch stays with
+ * the context; outgrown, it is freed unless a graph was captured with it. What the pages hold from kv_len on does not matter,
+ * nor do pages that no row sees; in the other pages every key and value has to be finite (a value that is not reaches rows
+ * that do not see it, as 0 times infinity) and in F32 below 2^128 - 2^115. A row with a score that is NaN or overflows to
+ * infinity is NaN, a score of minus infinity has weight 0 (F32 caches: NaN too); |scale| at most 1e38. */
 typedef struct {
     const gsvcu_paged_kv* kv;
     const gsvcu_chunk_batch* batch;

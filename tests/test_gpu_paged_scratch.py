@@ -116,3 +116,14 @@ def test_outgrown_unpacked_pages_are_freed_unless_a_graph_may_use_them(own, capt
         own.sync()
         assert torch.equal(out, first)
         del graph
+
+
+@pytest.mark.parametrize("ty,dim,heads,kv_heads", [("bf16", 128, 32, 8), ("f16", 64, 16, 4)])
+@pytest.mark.parametrize("window", [0, 1000])
+def test_a_long_chunk_beside_many_single_tokens(own, ty, dim, heads, kv_heads, window):
+    """The slots' pages are not unpacked for the chunk's sake; without slots, or with idle ones, its own are."""
+    for q_len, kernels in (([512] + [1] * 32, 1), ([512] + [0] * 11, 2)):
+        c = Q4Case(ty, q_len, [1900] + [700 + 31 * s for s in range(1, len(q_len))], heads, kv_heads, dim)
+        before = own.kernel_launches()
+        attend(own, c, window=window)
+        assert own.kernel_launches() - before == kernels   # (enough CTAs: the keys are not split)

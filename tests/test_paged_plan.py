@@ -1,0 +1,40 @@
+"""How a call of chunk attention over the paged cache is cut up, from its sizes alone: no GPU."""
+import json
+import os
+import subprocess
+
+import pytest
+
+HERE = os.path.dirname(os.path.abspath(__file__))
+EXE = os.path.join(HERE, "cpp", "bin", "paged_plan")
+F16, F32, BF16, Q4_F16, Q4_BF16 = range(5)
+
+
+def plan(kv_dtype=Q4_BF16, head_dim=128, kv_heads=8, heads=32, n_seq=1, n_rows=1, max_chunk=None, max_kv=8192, window=0,
+         scale=0.125):
+    assert os.path.exists(EXE), "build with `make -C tests/cpp`"
+    chunk = n_rows if max_chunk is None else max_chunk
+    args = [kv_dtype, head_dim, kv_heads, heads, n_seq, -(-max_kv // 64), n_rows, chunk, max_kv, window, scale]
+    out = subprocess.run([EXE] + [str(a) for a in args], capture_output=True, text=True, check=True, timeout=60)
+    return json.loads(out.stdout)
+
+
+@pytest.mark.parametrize("sizes,unpacked", [
+    (dict(n_rows=384), True), (dict(n_rows=383), False),                       # 1536 rows times query heads of a kv head
+    (dict(n_seq=8, n_rows=8 * 128, max_chunk=384), True), (dict(n_seq=8, n_rows=8 * 128 - 1, max_chunk=384), False),
+    (dict(n_seq=33, n_rows=512 + 32, max_chunk=512), False),                   # one chunk beside 32 decoding slots
+    (dict(n_seq=33, n_rows=4096, max_chunk=4096), True),                       # the slots are idle
+    (dict(n_seq=33, n_rows=4096 + 1, max_chunk=4096), True),                   # one of them decodes
+    (dict(n_seq=33, n_rows=4096 + 1, max_chunk=2048), False), (dict(n_seq=32, n_rows=4096 + 1, max_chunk=2048), True),
+    (dict(n_seq=2, n_rows=4096, max_chunk=2048), True),
+    (dict(n_rows=2048, window=384), True), (dict(n_rows=2048, window=383), False),
+    (dict(n_seq=9, n_rows=2048 + 8, max_chunk=2048, window=400), True),
+    (dict(n_seq=17, n_rows=2048 + 16, max_chunk=2048, window=400), False),
+    (dict(n_rows=2048, kv_dtype=BF16), False), (dict(n_rows=2048, scale=0.0), False),
+    (dict(n_rows=2048, n_seq=1, max_kv=1 << 20), False),                       # more than 2 GB
+])
+def test_pages_are_unpacked_for_many_rows_of_every_sequence(sizes, unpacked):
+    """The pages of every sequence in the call are: that pays where the longest chunk has 1536 rows times query heads of a kv
+    head and the others not too few (512 on average), not for one chunk beside many single tokens."""
+    c = plan(**sizes)
+    assert (c["unpack_pages"] > 0) == unpacked, c
