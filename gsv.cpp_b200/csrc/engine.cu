@@ -1966,7 +1966,7 @@ int gsvcu_op_chunk_attention(gsvcu_ctx* ctx, const gsvcu_chunk_attention* a) {
     p.poll_limit = ctx->fault_poll_limit;
     if (batch->n_rows == 0 || batch->n_seq == 0) return GSVCU_OK;
     ChunkAttnPlan plan = chunk_attention_plan(p);
-    if ((int64_t)batch->n_seq * plan.tiles * kv->n_kv_head * (plan.dealt ? 4 : plan.n_split) > INT32_MAX)   // (the join's CTAs)
+    if (chunk_attention_ctas(p, plan) > INT32_MAX)
         return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_chunk_attention: batch too large for one launch");
     DeviceGuard g(ctx->device);
     // Scratch at least doubles when it grows, and what it replaces stays until the context ends: captured graphs

@@ -89,17 +89,21 @@ struct ChunkAttnPlan {
     bool tensor = false;   // the tcgen05 kernel (paged_attention_tc.cu)
     int row_tile = 0;      // packed rows (token x query head of one kv head) of a CTA
     int tiles = 0;         // row tiles per sequence (bound)
-    int n_split = 0;       // key splits (bound)
+    int n_split = 1;       // key splits (bound)
     int key_tile = 0;      // keys of a tile
     int split_tiles = 0;   // key tiles of a split
     bool join_apart = false;   // the splits are joined by a kernel of its own, not by the last CTA
-    int ctas = 0;              // 4-bit caches, few rows: CTAs, and whether the pages are dealt out to them
+    int64_t ctas = 0;          // 4-bit caches, few rows: CTAs, and whether the pages are dealt out to them
     bool dealt = false;
     int unpack_pages = 0;      // pages per sequence of a 4-bit cache that are unpacked to F16 first (0: the kernel reads the 4 bits)
     size_t unpacked_floats = 0;
     size_t part_floats = 0, arrivals = 0;
 };
 ChunkAttnPlan chunk_attention_plan(const ChunkAttnParams& p);
+// CTAs of the plan's largest launch (pages dealt out: at most 4 join a unit). A grid takes INT32_MAX.
+inline int64_t chunk_attention_ctas(const ChunkAttnParams& p, const ChunkAttnPlan& c) {
+    return (int64_t)p.batch.n_seq * c.tiles * p.kv.n_head * (c.dealt ? 4 : c.n_split);
+}
 ChunkAttnPlan chunk_attention_tc_plan(const ChunkAttnParams& p);   // (more than 32 packed rows of a 16-bit type, scale not 0)
 // Bytes that unpacked pages may take.
 constexpr int64_t UNPACK_LIMIT = (int64_t)2 << 30;

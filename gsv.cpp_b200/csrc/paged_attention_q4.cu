@@ -782,10 +782,10 @@ ChunkAttnPlan chunk_attention_q4_plan(const ChunkAttnParams& p) {
     // keys are faster dealt out (17.3, 21.4). Many units even out by themselves: 3200 of 2000 to 4000 keys, heads of 32, 140 us,
     // dealt out 163.
     if (max_tiles <= (units >= 4 * slots ? 64 : D < 128 || units >= slots ? 40 : 16)) {
-        c.ctas = (int)units;
+        c.ctas = units;
         return c;
     }
-    c.ctas = (int)std::min(slots, (units * std::max(max_tiles, 1) + LEAST - 1) / LEAST);
+    c.ctas = std::min(slots, (units * std::max(max_tiles, 1) + LEAST - 1) / LEAST);
     c.dealt = true;
     c.join_apart = c.row_tile > 8;   // (as chunk_attention_plan)
     c.part_floats = (size_t)2 * c.ctas * c.row_tile * (D + 2) + (c.join_apart ? 2 * units : 0);

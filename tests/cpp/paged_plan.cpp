@@ -20,7 +20,7 @@ int main(int argc, char** argv) {
     p.window = atoi(argv[10]);
     p.scale = (float)atof(argv[11]);
     const gsvcu::ChunkAttnPlan c = gsvcu::chunk_attention_plan(p);
-    printf("{\"tensor\": %d, \"row_tile\": %d, \"tiles\": %d, \"n_split\": %d, \"dealt\": %d, \"unpack_pages\": %d}\n", c.tensor,
-           c.row_tile, c.tiles, c.n_split, c.dealt, c.unpack_pages);
+    printf("{\"tensor\": %d, \"row_tile\": %d, \"tiles\": %d, \"n_split\": %d, \"dealt\": %d, \"unpack_pages\": %d, \"ctas\": %lld}\n",
+           c.tensor, c.row_tile, c.tiles, c.n_split, c.dealt, c.unpack_pages, (long long)gsvcu::chunk_attention_ctas(p, c));
     return 0;
 }

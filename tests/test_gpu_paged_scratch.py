@@ -127,3 +127,23 @@ def test_a_long_chunk_beside_many_single_tokens(own, ty, dim, heads, kv_heads, w
         before = own.kernel_launches()
         attend(own, c, window=window)
         assert own.kernel_launches() - before == kernels   # (enough CTAs: the keys are not split)
+
+
+@pytest.mark.parametrize("q4", [False, True])
+@pytest.mark.parametrize("max_kv", [64, 1 << 20])
+def test_batches_too_large_for_one_launch_are_refused(own, q4, max_kv):
+    """2^16 sequences times 2^15 row tiles: refused from the sizes, on the host."""
+    import ctypes as C
+
+    import gsvcu
+    c = (Q4Case if q4 else Case)("f16", [1], [5], 1, 1, 32)
+    cache, _ = c.objects()
+    x, out = c.rand(1, 1, 32), torch.full((1, 1, 32), 7.0, dtype=torch.float16, device="cuda")
+    batch = gsvcu.ChunkBatchDesc(c.row_start.data_ptr(), c.kv.data_ptr(), c.table.data_ptr(), 1 << 16, max_kv // PAGE, 1 << 20,
+                                 1 << 20, max_kv)
+    args = gsvcu.ChunkAttentionArgs(cache.addr, C.addressof(batch), x.data_ptr(), out.data_ptr(), None, None, 32, 32, c.layer, 1, 0, 0.0)
+    before = own.kernel_launches()
+    assert order(own).lib.gsvcu_op_chunk_attention(own.h, C.byref(args)) == -1
+    assert own.kernel_launches() == before
+    own.sync()
+    assert (out == 7.0).all()

@@ -38,3 +38,18 @@ def test_pages_are_unpacked_for_many_rows_of_every_sequence(sizes, unpacked):
     head and the others not too few (512 on average), not for one chunk beside many single tokens."""
     c = plan(**sizes)
     assert (c["unpack_pages"] > 0) == unpacked, c
+
+
+@pytest.mark.parametrize("kv_dtype", [F16, F32, BF16, Q4_F16, Q4_BF16])
+@pytest.mark.parametrize("head_dim", [32, 128])
+@pytest.mark.parametrize("sizes,least", [
+    (dict(kv_heads=1, heads=1, n_seq=1 << 16, n_rows=1 << 20, scale=0.0, max_kv=64), 1 << 31),      # row tiles of 32 rows
+    (dict(kv_heads=1, heads=1, n_seq=1 << 16, n_rows=1 << 20, scale=0.0, max_kv=1 << 20), 1 << 31),
+    (dict(kv_heads=1 << 10, heads=1 << 10, n_seq=1 << 21, n_rows=1 << 20, max_chunk=1, max_kv=64), 1 << 31),
+    (dict(kv_heads=1 << 10, heads=1 << 10, n_seq=(1 << 31) - 1, n_rows=1 << 20, max_chunk=1, max_kv=1 << 20), 1 << 40),
+    (dict(kv_heads=1 << 10, heads=1 << 10, n_seq=1 << 20, n_rows=1 << 20, max_chunk=1, max_kv=64), 1 << 30),   # (fits)
+    (dict(kv_heads=8, heads=8, n_seq=64, n_rows=64, max_chunk=1, max_kv=2048), 512),
+])
+def test_the_blocks_of_a_launch_are_counted_in_64_bits(kv_dtype, head_dim, sizes, least):
+    """What a call compares with the largest grid: a CTA at least for every sequence, row tile and kv head, whichever kernel."""
+    assert plan(kv_dtype, head_dim, **sizes)["ctas"] >= least
