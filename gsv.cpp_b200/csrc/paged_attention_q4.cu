@@ -779,8 +779,8 @@ ChunkAttnPlan chunk_attention_q4_plan(const ChunkAttnParams& p) {
     c.key_tile = KT;
     // Short units: a CTA for each, nothing to join and no lengths to add up first. 64 slots of 600 to 2100 keys, 16 heads x 32:
     // 31.8 us, 42 dealt out; 4 of 2000 to 4000 keys: 25 and 18; at head dim 128 a page takes longer, and 32 units of 600 to 2100
-    // keys are faster dealt out (17.3, 21.4). Many units even out by themselves: 3200 of 2000 to 4000 keys, heads of 32, 140 us,
-    // dealt out 163.
+    // keys are faster dealt out (17.3, 21.4). Many units even out by themselves: 3200 of 2000 to 4000 keys, heads of 32, 141 us,
+    // dealt out 164; of 64 187 and 211, of 128 311 and 338; with 32 rows of 32 545 and 591, of 128 1005 and 1100.
     if (max_tiles <= (units >= 4 * slots ? 64 : D < 128 || units >= slots ? 40 : 16)) {
         c.ctas = units;
         return c;

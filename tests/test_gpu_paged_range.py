@@ -94,3 +94,19 @@ def test_bf16_queries_of_any_size_with_a_negative_scale_and_masks(ctx, q):  # no
     attend(ctx, c, q=x, scale=0.125 * 2.0 ** 50, window=100, prefix=[70, 3])
     attend(ctx, c, q=x, scale=0.0)
     attend(ctx, c, q=x, scale=1e-38)   # (scores far below 1: every key weighs the same)
+
+
+# ------------------------------------------------------------------ many units
+
+@pytest.mark.parametrize("ty,dim,heads,kv_heads,q,n_seq", [("bf16", 128, 8, 8, 1, 230), ("bf16", 128, 32, 8, 8, 150), ("f16", 32, 16, 16, 1, 190)])
+@pytest.mark.parametrize("longest", [4096, 4097])
+def test_many_units_at_the_border_of_64_pages(ctx, ty, dim, heads, kv_heads, q, n_seq, longest):  # noqa: F811
+    """A block for each unit, or the pages dealt out. Twice the same."""
+    lens = [q + 37 * s % 600 for s in range(n_seq - 2)] + [longest, 4000]
+    c = Q4Case(ty, [q] * n_seq, lens, heads, kv_heads, dim)
+    x, a, la = attend(ctx, c, max_kv=longest)
+    cache, chunks = c.objects(longest)
+    b, lb = torch.empty_like(a), torch.empty_like(la)
+    order(ctx).op_chunk_attention(cache, chunks, c.layer, x, b, lse=lb)
+    ctx.sync()
+    assert torch.equal(a, b) and torch.equal(la, lb)

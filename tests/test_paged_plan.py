@@ -53,3 +53,14 @@ def test_pages_are_unpacked_for_many_rows_of_every_sequence(sizes, unpacked):
 def test_the_blocks_of_a_launch_are_counted_in_64_bits(kv_dtype, head_dim, sizes, least):
     """What a call compares with the largest grid: a CTA at least for every sequence, row tile and kv head, whichever kernel."""
     assert plan(kv_dtype, head_dim, **sizes)["ctas"] >= least
+
+
+@pytest.mark.parametrize("head_dim", [32, 64, 128])
+@pytest.mark.parametrize("group,chunk", [(1, 1), (4, 5), (4, 8)])
+def test_short_units_have_a_block_of_their_own(head_dim, group, chunk):
+    """4-bit caches, few rows: up to 64 pages when there are many units, up to 40 (heads of 128 when there are few: 16) else."""
+    many, some, few = ((n, dict(kv_heads=8, heads=8 * group, n_seq=n, n_rows=n * chunk, max_chunk=chunk)) for n in (1000, 75, 4))
+    for (n, sizes), pages in ((many, 64), (some, 40), (few, 16 if head_dim == 128 else 40)):
+        c = plan(Q4_BF16, head_dim, max_kv=64 * pages, **sizes)
+        assert not c["dealt"] and c["ctas"] == n * 8 * -(-group * chunk // 32)
+        assert plan(Q4_BF16, head_dim, max_kv=64 * pages + 1, **sizes)["dealt"]
