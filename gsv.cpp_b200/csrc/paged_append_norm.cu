@@ -2,15 +2,15 @@
 // caches (paged_append.cu has the float caches without norms).
 //
 // Per head of a query or key row, D elements x: y = x * r * w with r = 1 / sqrt(mean(x^2) + eps) in f32; the squares are
-// summed in 64 bits and rounded once, so that r, and with it every code next to a border, does not depend on the order of
-// the sum. Then the rotation (a' = a cos - b sin, b' = a sin + b cos, each operation rounded) and the rounding to the
-// cache's type, or the quantiser of paged_q4.cuh: the largest magnitude over the lanes of a group, one word of codes per 8
-// elements.
+// summed in 64 bits and rounded once, so that r, and with it every code next to a border, is the same in both kernels below
+// whatever the order of the sum. Then the rotation (a' = a cos - b sin, b' = a sin + b cos, each operation rounded) and the
+// rounding to the cache's type, or the quantiser of paged_q4.cuh: the largest magnitude over the lanes of a group, one word of
+// codes per 8 elements.
 // Every element is read once and written once: HBM bounds it on prompts, the chain row_start -> kv_len -> table -> store on
 // single tokens (64 rows of 48 heads x 32: 2.9 us). 31k rows of 48 heads x 128: normalised, rotated, BF16 to BF16 149 to 157 us
 // (5.0 to 5.3 TB/s; without norms 131: the sums of squares take a third of the instructions), F32 to F32 268 us (5.7 TB/s);
-// into 4 bits 134 to 139 us without norms, 173 with (5.1 and 3.9 TB/s). One element per lane and step less (8 instead of 16)
-// was 290 us, the conversion to F64 by its instruction 200.
+// into 4 bits 134 to 139 us without norms, 173 with (5.1 and 3.9 TB/s). With 8 elements a lane instead of 16 the first
+// was 290 us, with the instruction that converts to F64 200.
 #include "paged_q4.cuh"
 #include "paged_rows.cuh"
 

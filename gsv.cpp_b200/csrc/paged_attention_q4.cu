@@ -13,9 +13,9 @@
 // The weights are kept 2^14 up as in k_chunk_attn, for F16 rows in two parts, for BF16 ones in one.
 //
 // What bounds it: unpacking, about 1.5 instructions a value, most of them on the half-rate ALU (shifts, masks, byte permutes)
-// and FP16 pipes; the copies keep up with one block of K and of V per warp. Long caches run at 0.72 of the measured HBM
-// rate (131072 keys, 32/8 heads x 128: 46.4 us, floor 23.4, F16 cache 88); a start, a page per warp and the joins make 8 to 11
-// us. 64 keys at a time need 168 registers at head dim 128 but overlap better than 32 in 128 (46.4 against 52.6 us).
+// and FP16 pipes; the copies keep up with one block of K and of V per warp. 131072 keys, 32/8 heads x 128: 46.6 us, 0.50 of the
+// measured HBM rate (floor 23.4, F16 cache 88); 262144: 77.0, so 0.23 us per 1000 keys (0.77 of the rate) and 16 us that do not
+// grow: a start, a page per warp, the joins. 64 keys at a time need 168 registers at head dim 128 but overlap better than 32 in 128 (46.4 against 52.6 us).
 #include "paged_q4.cuh"
 
 #include <algorithm>
@@ -80,7 +80,7 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// Codes 0 .. 7 of a word, less 8, as the pairs (0, 4), (1, 5), (2, 6), (3, 7): under the exponent of 1024 a code in bits 0
+// Codes 0 .. 7 of a word, less 8, as the pairs (0, 4), (1, 5), (2, 6), (3, 7), by the usual way of widening nibbles: under the exponent of 1024 a code in bits 0
 // .. 3 is 1024 + code, one in bits 4 .. 7 is 1024 + 16 code.
 __device__ __forceinline__ void codes(uint32_t w, uint32_t (&x)[4]) {
     const __half2 low = __float2half2_rn(-1032.0f), up = __float2half2_rn(0.0625f), high = __float2half2_rn(-72.0f);

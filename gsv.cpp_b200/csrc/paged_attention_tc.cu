@@ -26,7 +26,7 @@
 //
 // 4-bit caches (paged_q4.cuh): the products read F16 (values are exact in it), whatever the rows' type. With many row tiles
 // over the same keys the pages are unpacked to F16 once, by k_unpack_q4, and read as above (2048 rows over 16384 keys, 32/8 x
-// 128 BF16: 442 us, 560 without, the F16 cache 430). Small BF16 rows enter scaled by a power of two (paged_q4.cuh), so that a row's
+// 128 BF16: 442 us in single blocks, 560 without, the F16 cache 430; in a long run under the power cap 515). Small BF16 rows enter scaled by a power of two (paged_q4.cuh), so that a row's
 // scores have a factor of its own, which costs 1 to 2 %. Else warp 0 copies the blocks as they lie and warps 12-15 unpack them into
 // the operand ring, a word of 8 codes to a 16-byte piece; they take issue slots from the softmax, which costs 10 to 30 % (512
 // rows over 8192 keys, 16/4 x 128: 65 us, 57 from F16), but the keys cross HBM at 4.5 bits. A piece's elements lie in the order

@@ -327,7 +327,8 @@ int gsvcu_op_kv_append(gsvcu_ctx* ctx, const gsvcu_kv_append* a);
 
 /* The same with a norm for each head before the rotation: y = x / sqrt(mean(x^2) + eps) * weight over the head's
  * elements, q heads with q_weight_dev, k heads with k_weight_dev ([head_dim] F32; null: those heads are not normalised),
- * in F32 with the sum of the squares in 64 bits. eps finite, not negative. norm null: gsvcu_op_kv_append. */
+ * in F32 with the sum of the squares in 64 bits (rounded to F32: past its range the head's finite elements become 0). eps
+ * finite, not negative. norm null: gsvcu_op_kv_append. */
 typedef struct {
     const float *q_weight_dev, *k_weight_dev;
     float eps;
