@@ -1970,8 +1970,8 @@ int gsvcu_op_chunk_attention(gsvcu_ctx* ctx, const gsvcu_chunk_attention* a) {
         return ctx->fail(GSVCU_ERR_ARG, "gsvcu_op_chunk_attention: batch too large for one launch");
     DeviceGuard g(ctx->device);
     // Scratch at least doubles when it grows, and what it replaces stays until the context ends: captured graphs
-    // may hold its address (unpacked pages, which are large, go when no capture has seen them). It does not grow in a capture: the zeros of the counters would only be recorded, and calls
-    // outside the graph would find none.
+    // may hold its address (unpacked pages, which are large, go when no capture has seen them). It does not grow in a
+    // capture: the zeros of the counters would only be recorded, and calls outside the graph would find none.
     cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
     auto grow = [&](void** at, size_t* have, size_t need, bool zero, size_t most, bool keep) -> int {   // (4-byte words)
         if (need <= *have) return GSVCU_OK;
@@ -2012,8 +2012,8 @@ int gsvcu_op_chunk_attention(gsvcu_ctx* ctx, const gsvcu_chunk_attention* a) {
     };
     TRY(grow((void**)&ctx->op_split, &ctx->op_split_n, plan.part_floats, false, SIZE_MAX, true));
     TRY(grow((void**)&ctx->op_arrived, &ctx->op_arrived_n, plan.arrivals, true, SIZE_MAX, true));
-    // The kernel can do without unpacked pages. Sizes that found no memory for them do from then on, so that a call is not tried
-    // again and again, can be captured once it has run, and sums in one order.
+    // The kernel can do without unpacked pages. Sizes that found no memory for them do from then on, so that memory is not
+    // asked for in every call, a call can be captured once it has run, and it sums in one order.
     if (plan.unpacked_floats >= ctx->op_unpacked_denied) plan.unpack_pages = 0;
     if (plan.unpack_pages) {
         const void* before = ctx->op_unpacked;

@@ -15,7 +15,8 @@
 // What bounds it: unpacking, about 1.5 instructions a value, most of them on the half-rate ALU (shifts, masks, byte permutes)
 // and FP16 pipes; the copies keep up with one block of K and of V per warp. 131072 keys, 32/8 heads x 128: 46.6 us, 0.50 of the
 // measured HBM rate (floor 23.4, F16 cache 88); 262144: 77.0, so 0.23 us per 1000 keys (0.77 of the rate) and 16 us that do not
-// grow: a start, a page per warp, the joins. 64 keys at a time need 168 registers at head dim 128 but overlap better than 32 in 128 (46.4 against 52.6 us).
+// grow: a start, a page per warp, the joins. 64 keys at a time need 168 registers at head dim 128 but overlap better than 32 in
+// 128 (46.4 against 52.6 us).
 #include "paged_q4.cuh"
 
 #include <algorithm>
@@ -36,10 +37,11 @@ constexpr int NW = 4;            // warps per CTA
 // 132 and 154.
 constexpr int UNPACK_ROWS = 1536;
 // And the mean over the sequences of a call. 32/8 x 128, 8192 keys each, unpacked first and not: a chunk of 512 tokens and 32
-// single ones 555 and 422 us; 512 and 4: 170 and 160; 512 and 2: 152 and 158; 512, 100, 100, 100: 168 and 168; 1024 and 8: 283 and 297.
+// single ones 555 and 422 us; 512 and 4: 170 and 160; 512 and 2: 152 and 158; 512, 100, 100, 100: 168 and 168; 1024 and 8: 283
+// and 297.
 constexpr int UNPACK_MEAN = 512;
-// Weights are 2^BIAS exp(s - maximum). The maximum is taken off first, then the difference scaled: in one step a score past 2^24
-// would be off from its own maximum by whole steps of F32, its weight infinite in F16, or 0.
+// Weights are 2^BIAS exp(s - maximum). The maximum is taken off first, then the difference scaled: in one step a score past
+// 2^24 would be off from its own maximum by whole steps of F32, its weight infinite in F16, or 0.
 constexpr float BIAS = 14.0f;
 constexpr int KT = PAGE;         // keys of one warp's tile: a block of the cache
 // Keys whose scores are held at a time.
@@ -80,8 +82,8 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// Codes 0 .. 7 of a word, less 8, as the pairs (0, 4), (1, 5), (2, 6), (3, 7), by the usual way of widening nibbles: under the exponent of 1024 a code in bits 0
-// .. 3 is 1024 + code, one in bits 4 .. 7 is 1024 + 16 code.
+// Codes 0 .. 7 of a word, less 8, as the pairs (0, 4), (1, 5), (2, 6), (3, 7), by the usual way of widening nibbles: under the
+// exponent of 1024 a code in bits 0 .. 3 is 1024 + code, one in bits 4 .. 7 is 1024 + 16 code.
 __device__ __forceinline__ void codes(uint32_t w, uint32_t (&x)[4]) {
     const __half2 low = __float2half2_rn(-1032.0f), up = __float2half2_rn(0.0625f), high = __float2half2_rn(-72.0f);
     const uint32_t v = w >> 8;

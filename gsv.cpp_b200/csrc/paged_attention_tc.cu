@@ -26,11 +26,11 @@
 //
 // 4-bit caches (paged_q4.cuh): the products read F16 (values are exact in it), whatever the rows' type. With many row tiles
 // over the same keys the pages are unpacked to F16 once, by k_unpack_q4, and read as above (2048 rows over 16384 keys, 32/8 x
-// 128 BF16: 442 us in single blocks, 560 without, the F16 cache 430; in a long run under the power cap 515). Small BF16 rows enter scaled by a power of two (paged_q4.cuh), so that a row's
-// scores have a factor of its own, which costs 1 to 2 %. Else warp 0 copies the blocks as they lie and warps 12-15 unpack them into
-// the operand ring, a word of 8 codes to a 16-byte piece; they take issue slots from the softmax, which costs 10 to 30 % (512
-// rows over 8192 keys, 16/4 x 128: 65 us, 57 from F16), but the keys cross HBM at 4.5 bits. A piece's elements lie in the order
-// of the codes; queries are stored in that order, outputs put back.
+// 128 BF16: 442 us in single blocks, 560 without, the F16 cache 430; in a long run under the power cap 515). Else warp 0 copies
+// the blocks as they lie and warps 12-15 unpack them into the operand ring, a word of 8 codes to a 16-byte piece; they take
+// issue slots from the softmax, which costs 10 to 30 % (512 rows over 8192 keys, 16/4 x 128: 65 us; 57 from F16), but the keys
+// cross HBM at 4.5 bits. A piece's elements lie in the order of the codes; queries are stored in that order, outputs put back.
+// Small BF16 rows enter scaled by a power of two, so that a row's scores have a factor of its own, which costs 1 to 2 %.
 #include <cuda_bf16.h>
 
 #include <cfloat>
@@ -55,8 +55,8 @@ enum Pages { SAME, PACKED_Q4, AS_F16 };
 // about 1 % over TAU 8 on scores of deviation 1, TAU 1 2 to 7 %.
 template <typename T> constexpr float TAU = __is_same(T, __half) ? 4.0f : 8.0f;
 template <typename T> constexpr float BIAS = __is_same(T, __half) ? 11.0f : 0.0f;
-// References (log2 units) beyond which scores are scaled and rounded, as their maximum was, before the reference is taken off:
-// in one step a score that F32 holds in steps of 2^-7 and more is off from its own maximum, and from 2^27 on its weight could
+// References (log2 units) beyond which scores are scaled and rounded, as their maximum was, before the reference is taken off.
+// In one step a score that F32 holds in steps of 2^-7 and more is off from its own maximum, and from 2^27 on its weight could
 // be infinite in F16, or 0.
 constexpr float COARSE = 65536.0f;
 

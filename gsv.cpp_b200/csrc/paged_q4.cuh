@@ -56,11 +56,11 @@ __device__ __forceinline__ uint32_t q4_word(const float* x, float inv) {
     return word - 0xfb000000u;   // 0x4b000000 (1 + 16 + ...), cut to 32 bits
 }
 
-// BF16 query rows whose largest element is below 1/4 enter F16 products times a power of two, which the factor of their scores is
-// divided by: the largest comes to 2^14 .. 2^15, so that elements keep their 8 bits down to 2^-31 of it. As they are they would
-// lose them below 2^-17 and vanish below 2^-25 (2^-23 of the largest in the rows that are left so, the rule).
-// `row`: 8 elements of a row that this lane and its PIECES - 1 neighbours have; all lanes of the warp take part. False: none of the
-// warp's rows is scaled; else `up` is this row's exponent, 0 .. 126.
+// BF16 query rows whose largest element is below 1/4 enter F16 products times a power of two, which the factor of their scores
+// is divided by: the largest comes to 2^14 .. 2^15, so that elements keep their 8 bits down to 2^-31 of it. As they are they
+// would lose them below 2^-17 and vanish below 2^-25 (2^-23 of the largest in the rows that are left so, the rule).
+// `row`: 8 elements of a row that this lane and its PIECES - 1 neighbours have; all lanes of the warp take part. False: none of
+// the warp's rows is scaled; else `up` is this row's exponent, 0 .. 126.
 template <int PIECES>
 __device__ __forceinline__ bool small_queries(uint4 row, int& up) {
     constexpr uint32_t QUARTER = 0x3e80u;

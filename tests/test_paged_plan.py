@@ -5,6 +5,8 @@ import subprocess
 
 import pytest
 
+import gsvcu
+
 HERE = os.path.dirname(os.path.abspath(__file__))
 EXE = os.path.join(HERE, "cpp", "bin", "paged_plan")
 F16, F32, BF16, Q4_F16, Q4_BF16 = range(5)
@@ -64,3 +66,7 @@ def test_short_units_have_a_block_of_their_own(head_dim, group, chunk):
         c = plan(Q4_BF16, head_dim, max_kv=64 * pages, **sizes)
         assert not c["dealt"] and c["ctas"] == n * 8 * -(-group * chunk // 32)
         assert plan(Q4_BF16, head_dim, max_kv=64 * pages + 1, **sizes)["dealt"]
+
+
+def test_the_switch_for_missing_memory_takes_a_context():
+    assert gsvcu.load_library().gsvcu_set_memory_fault(None, 1) == -1
